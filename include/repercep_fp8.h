@@ -492,6 +492,112 @@ int rp_fp8_gemm_rowwise(const uint8_t* a8, const uint8_t* b8, int b_layout, void
 int rp_fp8_transpose(const uint8_t* src, uint8_t* dst, int64_t R, int64_t C,
                      int64_t lds, int64_t ldd, void* stream);
 
+/* ------------------------------------------------- paged key-value cache
+ * A decoder's cache of K and V rows in pages, with no counterpart in the
+ * reference.  Position j of sequence b lies in row j % page_size of page
+ * block_table[b][j / page_size], for every kv head.
+ *
+ *   k, v      (num_pages, heads, page_size, head_dim), unit stride along
+ *             head_dim, the other strides in elements and the same for both;
+ *             rows 16-byte aligned
+ *   dtype     RP_CACHE_BF16, RP_CACHE_F16, or RP_CACHE_E4M3: codes under one
+ *             dequant scale per row (the row-wise quantizer's)
+ *   k_scale, v_scale   float (num_pages, heads, page_size) contiguous for
+ *             RP_CACHE_E4M3, else NULL
+ *   block_table   int32, `table_stride` elements between sequences, max_pages
+ *             entries each
+ * page_size is a power of two up to 65536; head_dim is 32, 64, 128 or 256.
+ *
+ * What the device reads from the caller's memory is checked there: a
+ * position past max_pages * page_size, or in a page whose id is outside
+ * [0, num_pages), holds no row (it is not written, attended to or moved),
+ * and a negative length counts as zero. */
+#define RP_CACHE_BF16 0
+#define RP_CACHE_F16 1
+#define RP_CACHE_E4M3 2
+typedef struct rp_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* block_table;
+  int64_t num_pages, heads, page_size, head_dim;
+  int64_t stride_page, stride_head, stride_row;
+  int64_t table_stride, max_pages;
+  int64_t dtype;
+} rp_paged_cache;
+
+/* Writes new rows: row i of k and v ((B, heads, S, head_dim) with element
+ * strides sb, sh, ss, bf16 or fp16) goes to position start[b] + i of sequence
+ * b, for i < lengths[b] (NULL: all S).  A 16-bit cache takes rows of its own
+ * type as they are; RP_CACHE_E4M3 takes the codes and dequant scale that
+ * rp_fp8_rowwise_quantize gives a row of head_dim elements.  A page that is
+ * written belongs to one sequence. */
+int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int64_t B, int64_t S,
+                       int64_t ksb, int64_t ksh, int64_t kss, int64_t vsb, int64_t vsh,
+                       int64_t vss, const rp_paged_cache* cache, const int32_t* start,
+                       const int32_t* lengths, void* stream);
+
+/* Attention of one new token per sequence over its first seq_lens[b] rows:
+ *   s_j = sm_scale * q . k_j,  out = sum_j softmax(s)_j v_j,
+ *   lse = log(sum_j exp(s_j))                        (lse NULL: not written)
+ * q (B, H, head_dim) bf16 or fp16 with strides qsb, qsh; out of the same type
+ * with strides osb, osh; lse float (B, H).  A 16-bit cache has q's type.
+ * Query head h reads kv head h / (H / heads).  Products are exact in fp32
+ * sums, weights enter the second product with 16 bits or more, out is
+ * rounded once.  A sequence that sees no row gets zeros and lse -inf.
+ * key_weights, if not NULL: float (B, heads, >= max_pages * page_size), strides
+ * wsb, wsh and 1; each seen key's softmax weights, summed over its kv head's
+ * query heads, are added to it (in a fixed order: equal calls give equal bits).
+ * max_seq_len (0: unknown) is where the lengths are expected to end: it sets
+ * how the work is split, not what is computed.
+ * workspace: rp_paged_attn_workspace_bytes of the same arguments, 256-byte
+ * aligned (may be NULL where that is 0). */
+size_t rp_paged_attn_workspace_bytes(int64_t B, int64_t H, const rp_paged_cache* cache,
+                                     int64_t max_seq_len, int with_key_weights);
+int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64_t qsb,
+                         int64_t qsh, const rp_paged_cache* cache, const int32_t* seq_lens,
+                         float sm_scale, void* out, int64_t osb, int64_t osh, float* lse,
+                         float* key_weights, int64_t wsb, int64_t wsh, int64_t max_seq_len,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Cuts each sequence longer than `budget` rows to `budget`, per kv head: the
+ * last `recent` (<= budget) rows stay, and of the others those with the
+ * largest weights, the lower position where weights are equal (-0 equals 0; a
+ * NaN counts as larger than any number).  The kept rows, with their scales,
+ * move in place to positions 0, 1, ... in their order; rows behind them are
+ * left as they were.  weights float (B, heads, >= max_pages * page_size),
+ * strides wsb, wsh and 1, is only read; new_weights, (B, heads, W)
+ * contiguous with W >= max_pages * page_size, gets the kept rows' weights and
+ * zeros behind them; new_lens[b] = min(seq_lens[b], budget).  Sequences within
+ * the budget keep their rows and weights.  The sequences' pages are their own
+ * (none is shared).  workspace: rp_paged_evict_workspace_bytes, 256-byte
+ * aligned. */
+size_t rp_paged_evict_workspace_bytes(int64_t B, const rp_paged_cache* cache, int64_t budget);
+int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq_lens, int64_t B,
+                      const float* weights, int64_t wsb, int64_t wsh, int64_t budget,
+                      int64_t recent, int32_t* new_lens, float* new_weights, int64_t W,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------- token log probabilities
+ * For each of N rows of V logits (row stride ld elements; RP_OUT_BF16,
+ * RP_OUT_F16 or RP_OUT_F32 by logits_dtype), z = x / temperature:
+ *   logprobs[i]  log softmax(z)[tokens[i]]; 0 for a negative token (padding),
+ *                NaN for one >= V
+ *   entropy[i]   -sum p log p                            (NULL: not written)
+ *   top_logprobs, top_ids (N, top): the `top` (0..32, <= V) largest log
+ *                probabilities and their tokens, largest first, the lower
+ *                token first where logits are equal
+ * A row of -inf only gives log probabilities of -inf and entropy 0; a row
+ * with a NaN or +inf gives NaN, its NaNs taken as the largest logits.
+ * No counterpart in the reference. */
+#define RP_LOGPROB_MAX_TOP 32
+size_t rp_token_logprobs_workspace_bytes(int64_t N, int64_t V, int logits_dtype, int top);
+int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N, int64_t V, int64_t ld,
+                      const int64_t* tokens, float temperature, int top, float* logprobs,
+                      float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------- self-test
  * Device routines exposed so the tests can pin them exhaustively against
  * the CPU oracle.  They run the same device functions the kernels above use.
@@ -502,13 +608,17 @@ int rp_fp8_transpose(const uint8_t* src, uint8_t* dst, int64_t R, int64_t C,
  * `groups` groups of up to `elems` (<= 65536) elements and `tiles` (<= 8) V^T
  * tiles of 128 x 64 takes one launch.
  * rp_selftest_rope_block (host only): the row range and the chunk of heads of
- * block `block` of the prologue's rotary passes, of ranges * chunks blocks. */
+ * block `block` of the prologue's rotary passes, of ranges * chunks blocks.
+ * rp_selftest_paged_row (host only): the element offset at which the paged
+ * kernels look for position `pos` of head `head`, -1 where there is no row
+ * (block_table: one sequence's entries, in host memory). */
 int rp_selftest_e4m3(const float* x, uint8_t* out, int64_t n, void* stream);
 int rp_selftest_scale(const uint16_t* amax_bits, int x_dtype, float* dequant, float* qmul, int64_t n,
                       void* stream);
 int rp_selftest_quant_one_launch(int64_t groups, int64_t elems, int64_t tiles, int capturing);
 int rp_selftest_rope_block(int64_t ranges, int64_t chunks, int64_t block, int64_t* range,
                            int64_t* chunk);
+int64_t rp_selftest_paged_row(const rp_paged_cache* cache, int64_t head, int64_t pos);
 
 #ifdef __cplusplus
 }

@@ -34,6 +34,10 @@ RP_QKV_NOALLOC_SCRATCH_BYTES = 1 << 20
 RP_B_NK = 0
 RP_B_KN = 1
 RP_GEMM_BALANCED_WORKSPACE_BYTES = 256
+RP_CACHE_BF16 = 0
+RP_CACHE_F16 = 1
+RP_CACHE_E4M3 = 2
+RP_LOGPROB_MAX_TOP = 32
 
 #: Every function include/repercep_fp8.h declares.
 EXPORTS = (
@@ -55,8 +59,11 @@ EXPORTS = (
     "rp_fp8_transpose",
     "rp_fp8_gemm_rowwise", "rp_fp8_rowwise_quantize", "rp_transpose16",
     "rp_fp8_softmax_rowwise_quantize",
+    "rp_paged_kv_append", "rp_paged_attn_workspace_bytes", "rp_paged_attn_decode",
+    "rp_paged_evict_workspace_bytes", "rp_paged_kv_evict",
+    "rp_token_logprobs_workspace_bytes", "rp_token_logprobs",
     "rp_selftest_e4m3", "rp_selftest_scale", "rp_selftest_quant_one_launch",
-    "rp_selftest_rope_block",
+    "rp_selftest_rope_block", "rp_selftest_paged_row",
 )
 
 
@@ -72,6 +79,15 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
+
+
+class PagedCache(ctypes.Structure):
+    """``rp_paged_cache``."""
+
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "block_table")]
+                + [(n, _i64) for n in ("num_pages", "heads", "page_size", "head_dim",
+                                       "stride_page", "stride_head", "stride_row",
+                                       "table_stride", "max_pages", "dtype")])
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -164,6 +180,26 @@ def _declare(L: ctypes.CDLL) -> None:
     L.rp_fp8_softmax_rowwise_quantize.restype = _int
     L.rp_fp8_softmax_rowwise_quantize.argtypes = [_vp, _i64, _i64, _i64, _i64, _int, _f32, _vp,
                                                   _vp, _i64, _vp]
+    cache = ctypes.POINTER(PagedCache)
+    L.rp_paged_kv_append.restype = _int
+    L.rp_paged_kv_append.argtypes = [_vp, _vp, _int] + [_i64] * 8 + [cache, _vp, _vp, _vp]
+    L.rp_paged_attn_workspace_bytes.restype = _sz
+    L.rp_paged_attn_workspace_bytes.argtypes = [_i64, _i64, cache, _i64, _int]
+    L.rp_paged_attn_decode.restype = _int
+    L.rp_paged_attn_decode.argtypes = ([_vp, _int] + [_i64] * 4 + [cache, _vp, _f32, _vp, _i64,
+                                       _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp])
+    L.rp_paged_evict_workspace_bytes.restype = _sz
+    L.rp_paged_evict_workspace_bytes.argtypes = [_i64, cache, _i64]
+    L.rp_paged_kv_evict.restype = _int
+    L.rp_paged_kv_evict.argtypes = [cache, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64,
+                                    _vp, _sz, _vp]
+    L.rp_token_logprobs_workspace_bytes.restype = _sz
+    L.rp_token_logprobs_workspace_bytes.argtypes = [_i64, _i64, _int, _int]
+    L.rp_token_logprobs.restype = _int
+    L.rp_token_logprobs.argtypes = ([_vp, _int, _i64, _i64, _i64, _vp, _f32, _int]
+                                    + [_vp] * 5 + [_sz, _vp])
+    L.rp_selftest_paged_row.restype = _i64
+    L.rp_selftest_paged_row.argtypes = [cache, _i64, _i64]
     L.rp_fp8_transpose.restype = _int
     L.rp_fp8_transpose.argtypes = [_vp, _vp, _i64, _i64, _i64, _i64, _vp]
     L.rp_selftest_e4m3.restype = _int

@@ -40,7 +40,7 @@ COMMON = [
     "-Wno-inline-asm",
 ]
 SOURCES = ["rp_api.hip", "rp_quant.hip", "rp_prologue.hip", "rp_attn.hip", "rp_gemm.hip",
-           "rp_rowwise.hip"]
+           "rp_rowwise.hip", "rp_paged.hip", "rp_paged_attn.hip", "rp_logprob.hip"]
 # Per-source flags.  The attention kernel schedules better under the
 # memory-clause strategy: C3 self 54.60-54.77 ms against 55.31-55.49 ms, C2
 # 24.23-24.25 against 24.50-24.54 ms, alternating on one box.  The same flag

@@ -1,0 +1,376 @@
+// A paged key-value cache's writer and its eviction by attention weight.
+//
+// * append_kernel: new K and V rows to their pages, as they are or through
+//   the row-wise e4m3fn quantizer (rp_rowwise_dev.h).  D / 8 lanes hold one
+//   row, a 16-byte vector each, so a row is read once, its maximum found by a
+//   butterfly and its codes written once.
+// * evict_select_kernel: which rows of one (sequence, kv head) stay: the
+//   budget-th largest weight by a radix select over order-preserving integer
+//   keys, then one ordered pass that ranks the kept rows and writes their
+//   positions and weights.
+// * evict_move_kernel: the kept rows moved to the front, in place.
+
+#include "rp_paged_dev.h"
+#include "rp_rowwise_dev.h"
+
+namespace rp {
+namespace {
+
+constexpr int kPThreads = 256;
+
+struct AppendArgs {
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t ksb, ksh, kss, vsb, vsh, vss;
+  const int32_t* start;
+  const int32_t* lengths;
+  int32_t S;
+};
+
+// One row of K or V from registers to its place.
+template <int DT, bool FP8, int TPR>
+__device__ __forceinline__ void append_row(const u32x4r& x, char* cache, float* scale, int64_t row,
+                                           int64_t srow, int t) {
+  if constexpr (FP8) {
+    uint32_t m = absmax8(x);
+#pragma unroll
+    for (int o = TPR / 2; o >= 1; o >>= 1) m = umax32(m, (uint32_t)__shfl_xor((int)m, o, kWave));
+    float qm, dq;
+    rowwise_scales<DT>(m, &qm, &dq);
+    if (row >= 0) {
+      *reinterpret_cast<uint2*>(cache + row + 8 * t) = quant8<DT>(x, qm);
+      if (t == 0) scale[srow] = dq;
+    }
+  } else if (row >= 0) {
+    *reinterpret_cast<u32x4r*>(cache + 2 * row + 16 * t) = x;
+  }
+}
+
+template <int DT, bool FP8, int TPR>
+__global__ __launch_bounds__(kPThreads) void append_kernel(AppendArgs a, PagedView c) {
+  constexpr int RPB = kPThreads / TPR;
+  const int b = blockIdx.y;
+  const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const int n = a.lengths ? min(a.lengths[b], a.S) : a.S;
+  const int i = (int)(r / c.heads), h = (int)(r % c.heads);
+  const bool live = i < n;
+  const int64_t pos = (int64_t)a.start[b] + i;
+  const int32_t page = live ? paged_page(c, c.table + b * c.table_stride, pos) : -1;
+  u32x4r x{0u, 0u, 0u, 0u}, y{0u, 0u, 0u, 0u};
+  if (page >= 0) {
+    x = *reinterpret_cast<const u32x4r*>(a.k + b * a.ksb + h * a.ksh + i * a.kss + 8 * t);
+    y = *reinterpret_cast<const u32x4r*>(a.v + b * a.vsb + h * a.vsh + i * a.vss + 8 * t);
+  }
+  const int64_t row = page >= 0 ? paged_row(c, page, h, pos) : -1;
+  const int64_t srow = FP8 && page >= 0 ? paged_scale(c, page, h, pos) : 0;
+  append_row<DT, FP8, TPR>(x, c.k, c.ks, row, srow, t);
+  append_row<DT, FP8, TPR>(y, c.v, c.vs, row, srow, t);
+}
+
+template <int DT, bool FP8>
+void launch_append(const AppendArgs& a, const PagedView& c, int64_t B, int64_t D, hipStream_t st) {
+  const int64_t rows = (int64_t)a.S * c.heads;
+  auto go = [&](auto kernel, int64_t tpr) {
+    const int64_t rpb = kPThreads / tpr;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + rpb - 1) / rpb), (unsigned)B),
+                       dim3(kPThreads), 0, st, a, c);
+  };
+  if (D == 32) go(append_kernel<DT, FP8, 4>, 4);
+  else if (D == 64) go(append_kernel<DT, FP8, 8>, 8);
+  else if (D == 128) go(append_kernel<DT, FP8, 16>, 16);
+  else go(append_kernel<DT, FP8, 32>, 32);
+}
+
+// ------------------------------------------------------------------ eviction
+
+constexpr int kSelThreads = 1024;
+
+// fp32 -> an unsigned key in the same order; -0 as 0, NaN above everything.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  const uint32_t u = __float_as_uint(w);
+  if (w != w) return 0xffffffffu;
+  if (w == 0.0f) return 0x80000000u;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct EvictArgs {
+  const int32_t* lens;
+  const float* weights;
+  int64_t wsb, wsh;
+  int32_t budget, recent;
+  int32_t* new_lens;
+  float* new_weights;
+  int64_t W;
+  int32_t* src;        // (B, heads, budget): the position each kept row comes from
+  int32_t* first;      // (B, heads): ranks below it are their own positions
+};
+
+__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, PagedView c) {
+  constexpr int kWaves = kSelThreads / kWave;
+  __shared__ uint32_t hist[256];
+  __shared__ uint32_t pick[2];
+  __shared__ uint32_t wave_sum[2][kWaves];
+  __shared__ int first;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int64_t g = (int64_t)b * c.heads + h;
+  const int n = (int)paged_len(c, a.lens[b]);
+  const float* w = a.weights + b * a.wsb + h * a.wsh;
+  float* out = a.new_weights + g * a.W;
+  if (tid == 0 && h == 0) a.new_lens[b] = min(n, a.budget);
+  if (n <= a.budget) {
+    for (int64_t i = tid; i < a.W; i += kSelThreads) out[i] = i < n ? w[i] : 0.0f;
+    if (tid == 0) a.first[g] = a.budget;
+    return;
+  }
+  const int old = n - a.recent;
+  uint32_t need = (uint32_t)(a.budget - a.recent);   // of the first `old`; < old
+  // the need-th largest key: digit by digit, counting the keys that share
+  // the digits found so far
+  uint32_t key = 0xffffffffu;
+  uint32_t ties = 0;                // of the rows with that key, how many stay
+  if (need > 0) {
+    key = 0;
+    for (int d = 24; d >= 0; d -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      const uint32_t mask = d == 24 ? 0u : 0xffffffffu << (d + 8);
+      for (int i = tid; i < old; i += kSelThreads) {
+        const uint32_t u = weight_key(w[i]);
+        if ((u & mask) == key) atomicAdd(&hist[(u >> d) & 255u], 1u);
+      }
+      __syncthreads();
+      if (tid == 0) {
+        uint32_t above = 0;
+        int v = 255;
+        while (v > 0 && above + hist[v] < need) above += hist[v--];
+        pick[0] = (uint32_t)v;
+        pick[1] = above;
+      }
+      __syncthreads();
+      key |= pick[0] << d;
+      need -= pick[1];
+    }
+    ties = need;
+  }
+  // rank the kept rows in their order
+  const int lane = tid & (kWave - 1), wave = tid / kWave;
+  int32_t* src = a.src + g * a.budget;
+  if (tid == 0) first = a.budget;
+  uint32_t over0 = 0, tie0 = 0;     // rows above the border, rows on it, before this tile
+  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
+    const int i = i0 + tid;
+    const float x = i < n ? w[i] : 0.0f;
+    const uint32_t u = weight_key(x);
+    const bool over = i < n && (i >= old || (a.budget > a.recent && u > key));
+    const bool tie = i < old && a.budget > a.recent && u == key;
+    const uint64_t mo = __ballot(over), mt = __ballot(tie);
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    uint32_t ro = over0 + __popcll(mo & below), rt = tie0 + __popcll(mt & below);
+    __syncthreads();
+    if (lane == 0) {
+      wave_sum[0][wave] = __popcll(mo);
+      wave_sum[1][wave] = __popcll(mt);
+    }
+    __syncthreads();
+    for (int q = 0; q < kWaves; ++q) {
+      if (q < wave) {
+        ro += wave_sum[0][q];
+        rt += wave_sum[1][q];
+      }
+      over0 += wave_sum[0][q];
+      tie0 += wave_sum[1][q];
+    }
+    if (over || (tie && rt < ties)) {
+      const uint32_t rank = ro + min(rt, ties);
+      src[rank] = i;
+      out[rank] = x;
+    } else if (i < n) {
+      atomicMin(&first, i);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) a.first[g] = first;
+  for (int64_t i = a.budget + tid; i < a.W; i += kSelThreads) out[i] = 0.0f;
+}
+
+// Moves the kept rows of one (sequence, kv head) to their ranks, one slice of
+// 16-byte columns of K or of V (or the row scales) per workgroup.  A row only
+// moves down and ranks rise with positions, so tiles of rows in order need no
+// second buffer: every row that a tile overwrites is one that this tile or an
+// earlier one has read, or one that goes.
+constexpr int kMoveUnroll = 8;
+
+__global__ __launch_bounds__(kPThreads) void evict_move_kernel(EvictArgs a, PagedView c,
+                                                               int slices, int lanes,
+                                                               int row_bytes) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t g = (int64_t)b * c.heads + h;
+  const int begin = a.first[g];
+  if (begin >= a.budget) return;
+  const int32_t* src = a.src + g * a.budget;
+  const int32_t* table = c.table + b * c.table_stride;
+  const int kind = blockIdx.x / slices;     // 0: K, 1: V, 2: the scales
+  if (kind == 2) {
+    // four bytes a row: K's in the first half of the threads, V's in the second
+    float* s = threadIdx.x < kPThreads / 2 ? c.ks : c.vs;
+    for (int r0 = begin; r0 < a.budget; r0 += kPThreads / 2) {
+      const int r = r0 + (threadIdx.x & (kPThreads / 2 - 1));
+      float x = 0.0f;
+      int64_t to = -1;
+      if (r < a.budget) {
+        const int32_t from = src[r];
+        const int32_t pf = paged_page(c, table, from), pt = paged_page(c, table, r);
+        if (pf >= 0 && pt >= 0) {
+          x = s[paged_scale(c, pf, h, from)];
+          to = paged_scale(c, pt, h, r);
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(x)::"memory");
+      __syncthreads();
+      if (to >= 0) s[to] = x;
+    }
+    return;
+  }
+  char* base = kind == 0 ? c.k : c.v;
+  const int eb = c.ks ? 1 : 2;
+  const int col = ((blockIdx.x % slices) * lanes + threadIdx.x % lanes) * 16;
+  const int rows = kPThreads / lanes;
+  for (int r0 = begin; r0 < a.budget; r0 += rows * kMoveUnroll) {
+    u32x4r x[kMoveUnroll];
+    int64_t to[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int r = r0 + u * rows + threadIdx.x / lanes;
+      to[u] = -1;
+      x[u] = u32x4r{0u, 0u, 0u, 0u};
+      if (r < a.budget && col < row_bytes) {
+        const int32_t from = src[r];
+        const int32_t pf = paged_page(c, table, from), pt = paged_page(c, table, r);
+        if (pf >= 0 && pt >= 0) {
+          x[u] = *reinterpret_cast<const u32x4r*>(base + paged_row(c, pf, h, from) * eb + col);
+          to[u] = paged_row(c, pt, h, r) * eb + col;
+        }
+      }
+    }
+    // every load of the tile has to be back before any store of it
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) asm volatile("" : "+v"(x[u]));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u)
+      if (to[u] >= 0) *reinterpret_cast<u32x4r*>(base + to[u]) = x[u];
+  }
+}
+
+}  // namespace
+}  // namespace rp
+
+using namespace rp;
+
+extern "C" int64_t rp_selftest_paged_row(const rp_paged_cache* cache, int64_t head, int64_t pos) {
+  PagedView c;
+  if (paged_view("selftest_paged_row", cache, &c) != RP_OK || head < 0 || head >= c.heads)
+    return -1;
+  const int32_t page = paged_page(c, c.table, pos);
+  return page < 0 ? -1 : paged_row(c, page, head, pos);
+}
+
+extern "C" int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int64_t B, int64_t S,
+                                  int64_t ksb, int64_t ksh, int64_t kss, int64_t vsb, int64_t vsh,
+                                  int64_t vss, const rp_paged_cache* cache, const int32_t* start,
+                                  const int32_t* lengths, void* stream) {
+  if (!k || !v || !start) {
+    rp_set_error("paged_kv_append: null pointer");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  PagedView c;
+  const int rc = paged_view("paged_kv_append", cache, &c);
+  if (rc != RP_OK) return rc;
+  if (x_dtype != RP_DTYPE_BF16 && x_dtype != RP_DTYPE_F16) {
+    rp_set_error("paged_kv_append: unknown input dtype %d", x_dtype);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  const bool fp8 = cache->dtype == RP_CACHE_E4M3;
+  if (!fp8 && (cache->dtype == RP_CACHE_F16) != (x_dtype == RP_DTYPE_F16)) {
+    rp_set_error("paged_kv_append: a 16-bit cache takes rows of its own dtype");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  if (B <= 0 || S <= 0) {
+    rp_set_error("paged_kv_append: non-positive size B=%lld S=%lld", (long long)B, (long long)S);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  if (B > 65535 || S > 0x7fffffff / cache->heads) {
+    rp_set_error("paged_kv_append: too many sequences or rows");
+    return RP_ERR_UNSUPPORTED;
+  }
+  if (((ksb | ksh | kss | vsb | vsh | vss) & 7) != 0 ||
+      ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) {
+    rp_set_error("paged_kv_append: new rows must be 16-byte aligned");
+    return RP_ERR_UNSUPPORTED;
+  }
+  const AppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                     ksb, ksh, kss, vsb, vsh, vss, start, lengths, (int32_t)S};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t D = cache->head_dim;
+  if (!fp8) launch_append<kInBf16, false>(a, c, B, D, st);
+  else if (x_dtype == RP_DTYPE_F16) launch_append<kInF16, true>(a, c, B, D, st);
+  else launch_append<kInBf16, true>(a, c, B, D, st);
+  return paged_launched("paged_kv_append");
+}
+
+extern "C" size_t rp_paged_evict_workspace_bytes(int64_t B, const rp_paged_cache* cache,
+                                                 int64_t budget) {
+  if (!cache || B <= 0 || budget <= 0 || cache->heads <= 0) return 0;
+  return (size_t)((B * cache->heads * 4 + 255) / 256 * 256 + B * cache->heads * budget * 4);
+}
+
+extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq_lens, int64_t B,
+                                 const float* weights, int64_t wsb, int64_t wsh, int64_t budget,
+                                 int64_t recent, int32_t* new_lens, float* new_weights, int64_t W,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  if (!seq_lens || !weights || !new_lens || !new_weights) {
+    rp_set_error("paged_kv_evict: null pointer");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  PagedView c;
+  const int rc = paged_view("paged_kv_evict", cache, &c);
+  if (rc != RP_OK) return rc;
+  if (B <= 0 || budget <= 0 || recent < 0 || recent > budget) {
+    rp_set_error("paged_kv_evict: needs B > 0 and 0 <= recent <= budget, budget > 0 (B=%lld "
+                 "budget=%lld recent=%lld)", (long long)B, (long long)budget, (long long)recent);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  if (B > 65535) {
+    rp_set_error("paged_kv_evict: too many sequences");
+    return RP_ERR_UNSUPPORTED;
+  }
+  if (wsb < 0 || wsh < 0 || W < c.capacity()) {
+    rp_set_error("paged_kv_evict: weights need a place for each of %lld positions (got %lld)",
+                 (long long)c.capacity(), (long long)W);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  // a budget past the table's end cuts nothing: the workspace need not hold it
+  budget = budget < c.capacity() ? budget : c.capacity();
+  recent = recent < budget ? recent : budget;
+  const size_t want = rp_paged_evict_workspace_bytes(B, cache, budget);
+  if (!workspace || workspace_bytes < want || (reinterpret_cast<uintptr_t>(workspace) & 255)) {
+    rp_set_error("paged_kv_evict: workspace of %zu bytes, 256-byte aligned, needed", want);
+    return RP_ERR_WORKSPACE;
+  }
+  int32_t* first = static_cast<int32_t*>(workspace);
+  int32_t* src = first + (B * c.heads * 4 + 255) / 256 * 64;
+  const EvictArgs a{seq_lens, weights, wsb, wsh, (int32_t)budget, (int32_t)recent, new_lens,
+                    new_weights, W, src, first};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)c.heads, (unsigned)B), dim3(kSelThreads),
+                     0, st, a, c);
+  const int row_bytes = (int)cache->head_dim * cache_elem_bytes(cache->dtype);
+  const int lanes = row_bytes >= 64 ? 4 : row_bytes / 16;
+  const int slices = row_bytes / (16 * lanes);
+  hipLaunchKernelGGL(evict_move_kernel,
+                     dim3((unsigned)(2 * slices + (c.ks ? 1 : 0)), (unsigned)c.heads, (unsigned)B),
+                     dim3(kPThreads), 0, st, a, c, slices, lanes, row_bytes);
+  return paged_launched("paged_kv_evict");
+}

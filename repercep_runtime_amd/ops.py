@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import functools
 import math
-from typing import Callable, Literal
+from typing import Callable, Literal, NamedTuple
 
 import torch
 
@@ -50,6 +50,8 @@ _GRAN = {"bh": C.RP_SCALE_PER_BH, "tensor": C.RP_SCALE_PER_TENSOR}
 _IN_DTYPES = {torch.bfloat16: C.RP_DTYPE_BF16, torch.float16: C.RP_DTYPE_F16}
 _OUT_DTYPES = {torch.bfloat16: C.RP_OUT_BF16, torch.float16: C.RP_OUT_F16,
                torch.float32: C.RP_OUT_F32}
+_CACHE_DTYPES = {torch.bfloat16: C.RP_CACHE_BF16, torch.float16: C.RP_CACHE_F16,
+                 torch.float8_e4m3fn: C.RP_CACHE_E4M3}
 
 
 # torch's accessor of the current stream's raw handle (what its own kernels
@@ -1038,6 +1040,280 @@ def fp8_scaled_mm_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
     vs, vt8 = rowwise_quantize(vt)
     out = gemm_rowwise(p8.view(torch.uint8), vt8.view(torch.uint8), ps, vs)
     return out.reshape(b, h, sq, d).to(q.dtype)
+
+
+# ------------------------------------------------------ paged key-value cache
+# A decoder's step: new keys and values into a cache of pages, one new token's
+# attention over it, its eviction by attention weight, and the scores of the
+# chosen tokens.  The reference decodes through HF generate on bf16 SDPA and
+# has no counterpart of these.
+
+def _int32_vector(name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous int32 ({n},) vector "
+                         f"(got {t.dtype} {tuple(t.shape)})")
+
+
+def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, B: int,
+                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> C.PagedCache:
+    """The C descriptor of a cache, its tensors checked against each other."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache and v_cache must share one (pages, Hkv, page_size, D) shape "
+                         f"(got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
+    P, Hkv, page, D = k_cache.shape
+    dt = _CACHE_DTYPES.get(k_cache.dtype)
+    if dt is None or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"k_cache and v_cache must both be bfloat16, float16 or float8_e4m3fn "
+                        f"(got {k_cache.dtype}, {v_cache.dtype})")
+    strides = k_cache.stride()
+    if v_cache.stride() != strides or strides[3] != 1:
+        raise ValueError("k_cache and v_cache must share their strides, with a unit stride on D")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B \
+            or block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be int32 ({B}, max_pages) with contiguous rows "
+                         f"(got {block_table.dtype} {tuple(block_table.shape)})")
+    ks = vs = None
+    if dt == C.RP_CACHE_E4M3:
+        if k_scale is None or v_scale is None:
+            raise ValueError("an e4m3fn cache needs k_scale and v_scale")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32 or t.shape != (P, Hkv, page) or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous float32 ({P}, {Hkv}, {page})")
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("only an e4m3fn cache has scales")
+    _on_device_of(k_cache, v_cache=v_cache, block_table=block_table, k_scale=k_scale,
+                  v_scale=v_scale, k_cache=k_cache)
+    # a dimension of one has no stride of its own
+    return C.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, block_table.data_ptr(),
+                        P, Hkv, page, D, strides[0] if P > 1 else 0, strides[1] if Hkv > 1 else 0,
+                        strides[2] if page > 1 else D,
+                        block_table.stride(0) if B > 1 else 0, block_table.shape[1], dt)
+
+
+def _unit_stride(name: str, t: torch.Tensor) -> None:
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def _strides(t: torch.Tensor, dims: int) -> tuple[int, ...]:
+    """The first strides of ``t``, 0 for a dimension of one (whose stride means nothing)."""
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(dims))
+
+
+def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
+                    lengths: torch.Tensor | None = None, *, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None) -> None:
+    """Write new keys and values into a paged cache, in place.
+
+    ``k``, ``v``: (B, Hkv, S, D) bf16 or fp16 with a unit stride on D (a
+    prompt, or S = 1 for a decoder's step).  Row i of sequence b goes to
+    position ``start[b] + i``, for i < ``lengths[b]`` (int32; None: all S), and
+    position j lies in row ``j % page_size`` of page ``block_table[b, j //
+    page_size]``.  ``k_cache``, ``v_cache``: (pages, Hkv, page_size, D) views
+    of one layout, of the rows' dtype or float8_e4m3fn; the latter takes each
+    row's codes and dequant scale as ``rowwise_quantize`` gives them, the
+    scales in ``k_scale``, ``v_scale`` (pages, Hkv, page_size) fp32.
+
+    Positions past the table, and pages whose id is not in [0, pages), are
+    left out.  A page that is written belongs to one sequence."""
+    if k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"k and v must share one (B, Hkv, S, D) shape (got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)})")
+    B, Hkv, S, D = k.shape
+    if k_cache.dim() != 4 or k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+        raise ValueError(f"cache {tuple(k_cache.shape)} does not hold rows of {tuple(k.shape)}")
+    dt = _IN_DTYPES.get(k.dtype)
+    if dt is None or v.dtype != k.dtype:
+        raise TypeError(f"k and v must both be bfloat16 or float16 (got {k.dtype}, {v.dtype})")
+    if k_cache.element_size() == 2 and k_cache.dtype != k.dtype:
+        raise TypeError(f"a {k_cache.dtype} cache takes no {k.dtype} rows")
+    _unit_stride("k", k)
+    _unit_stride("v", v)
+    _int32_vector("start", start, B)
+    if lengths is not None:
+        _int32_vector("lengths", lengths, B)
+    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    _on_device_of(k_cache, k=k, v=v, start=start, lengths=lengths)
+    if B == 0 or S == 0:
+        return
+    C.check(C.lib().rp_paged_kv_append(
+        k.data_ptr(), v.data_ptr(), dt, B, S, *_strides(k, 3), *_strides(v, 3), cache,
+        start.data_ptr(), lengths.data_ptr() if lengths is not None else None, _stream(k)),
+        "rp_paged_kv_append")
+
+
+def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           block_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                           scale: float | None = None, k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None, max_seq_len: int | None = None,
+                           key_weights: torch.Tensor | None = None, return_lse: bool = False,
+                           out: torch.Tensor | None = None
+                           ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of one new token per sequence over a paged cache.
+
+    ``q``: (B, H, 1, D) bf16 or fp16, H a multiple of the cache's Hkv (query
+    head h reads kv head h // (H / Hkv)); the cache as ``paged_kv_append``
+    fills it, of q's dtype or float8_e4m3fn with its scales; ``seq_lens`` (B,)
+    int32, the rows of each sequence that are attended to.  Returns out (B, H,
+    1, D) in q's dtype, or (out, lse) with ``return_lse``, lse (B, H) fp32 the
+    log of the sum of exponentials.  A sequence without rows gives zeros and
+    -inf.  Pages may be shared between sequences, as the candidates of one
+    prompt share its pages.
+
+    ``key_weights`` (B, Hkv, at least max_pages * page_size) fp32: each
+    attended key's weight, summed over the query heads of its kv head, is
+    added to it in place, the totals that ``paged_kv_evict`` goes by.
+    ``max_seq_len`` says where the lengths are expected to end (default: the
+    table's end) and sets how the keys are split, not the result."""
+    if q.dim() != 4 or q.shape[2] != 1:
+        raise ValueError(f"q must be (B, H, 1, D), got {tuple(q.shape)}")
+    B, H, _, D = q.shape
+    if k_cache.dim() != 4 or k_cache.shape[3] != D or k_cache.shape[1] == 0 \
+            or H % k_cache.shape[1] != 0:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {tuple(k_cache.shape)}")
+    dt = _IN_DTYPES.get(q.dtype)
+    if dt is None:
+        raise TypeError(f"q must be bfloat16 or float16 (got {q.dtype})")
+    if k_cache.element_size() == 2 and k_cache.dtype != q.dtype:
+        raise TypeError(f"a {k_cache.dtype} cache is not read with {q.dtype} queries")
+    if D not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"head_dim {D} not in compiled tile shapes {sorted(SUPPORTED_HEAD_DIMS)}")
+    _unit_stride("q", q)
+    _int32_vector("seq_lens", seq_lens, B)
+    if out is not None:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
+        _unit_stride("out", out)
+    w_ptr, wsb, wsh = None, 0, 0
+    if key_weights is not None:
+        slots = block_table.shape[-1] * k_cache.shape[2]
+        if key_weights.dtype != torch.float32 or key_weights.dim() != 3 \
+                or key_weights.shape[:2] != (B, k_cache.shape[1]) or key_weights.shape[2] < slots:
+            raise ValueError(f"key_weights must be float32 ({B}, {k_cache.shape[1]}, >= {slots}), "
+                             f"got {key_weights.dtype} {tuple(key_weights.shape)}")
+        _unit_stride("key_weights", key_weights)
+        w_ptr, (wsb, wsh) = key_weights.data_ptr(), _strides(key_weights, 2)
+    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    _on_device_of(k_cache, q=q, seq_lens=seq_lens, key_weights=key_weights, out=out)
+    if out is None:
+        out = torch.empty((B, H, 1, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
+    if B > 0:
+        hint = max_seq_len if max_seq_len is not None else 0
+        n = C.lib().rp_paged_attn_workspace_bytes(B, H, cache, hint, w_ptr is not None)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        C.check(C.lib().rp_paged_attn_decode(
+            q.data_ptr(), dt, B, H, *_strides(q, 2), cache, seq_lens.data_ptr(),
+            1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(),
+            *_strides(out, 2), lse.data_ptr() if return_lse else None, w_ptr, wsb, wsh, hint,
+            ws.data_ptr() if n else None, n, _stream(q)), "rp_paged_attn_decode")
+    return (out, lse) if return_lse else out
+
+
+def paged_kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, key_weights: torch.Tensor, *, budget: int,
+                   recent: int, k_scale: torch.Tensor | None = None,
+                   v_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cut each sequence longer than ``budget`` rows to ``budget``, per kv head.
+
+    The last ``recent`` rows stay, and of the others those with the largest
+    ``key_weights`` (the totals of ``paged_attention_decode``), the lower
+    position where weights are equal (a NaN counts as the largest).  The kept rows move to
+    positions 0, 1, ... of the cache in their order, in place, scales
+    included; what lies behind them is left as it was.  Returns (new lengths
+    (B,) int32, new key_weights: the kept rows' weights and zeros behind them);
+    the inputs ``seq_lens`` and ``key_weights`` keep their values.  Sequences
+    within the budget stay as they are.  The sequences' pages are their own:
+    a page that several share is copied first."""
+    B = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    if B < 0:
+        raise ValueError(f"seq_lens must be a vector, got {tuple(seq_lens.shape)}")
+    _int32_vector("seq_lens", seq_lens, B)
+    if not 0 <= recent <= budget or budget < 1:
+        raise ValueError(f"needs 0 <= recent <= budget and budget >= 1 (got recent={recent}, "
+                         f"budget={budget})")
+    if k_cache.dim() != 4 or k_cache.shape[3] not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"cache {tuple(k_cache.shape)}: head_dim not in compiled tile shapes "
+                         f"{sorted(SUPPORTED_HEAD_DIMS)}")
+    slots = block_table.shape[-1] * k_cache.shape[2]
+    if key_weights.dtype != torch.float32 or key_weights.dim() != 3 \
+            or key_weights.shape[:2] != (B, k_cache.shape[1]) or key_weights.shape[2] < slots:
+        raise ValueError(f"key_weights must be float32 ({B}, {k_cache.shape[1]}, >= {slots}), "
+                         f"got {key_weights.dtype} {tuple(key_weights.shape)}")
+    _unit_stride("key_weights", key_weights)
+    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    _on_device_of(k_cache, seq_lens=seq_lens, key_weights=key_weights)
+    new_lens = torch.empty_like(seq_lens)
+    kept = torch.empty(key_weights.shape, dtype=torch.float32, device=key_weights.device)
+    if B == 0:
+        return new_lens, kept
+    budget = min(budget, slots)
+    n = C.lib().rp_paged_evict_workspace_bytes(B, cache, budget)
+    ws = torch.empty(n, dtype=torch.uint8, device=k_cache.device)
+    C.check(C.lib().rp_paged_kv_evict(
+        cache, seq_lens.data_ptr(), B, key_weights.data_ptr(), *_strides(key_weights, 2), budget,
+        min(recent, budget), new_lens.data_ptr(), kept.data_ptr(), kept.shape[2], ws.data_ptr(), n,
+        _stream(k_cache)), "rp_paged_kv_evict")
+    return new_lens, kept
+
+
+class TokenLogprobs(NamedTuple):
+    """``token_logprobs``' answer; the last two are None without ``top``."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
+                   temperature: float = 1.0) -> TokenLogprobs:
+    """Log probabilities of given tokens, with entropy and best alternatives.
+
+    ``logits`` (..., V) bf16, fp16 or fp32 with a unit stride on V and rows
+    that flatten to one row stride; ``tokens`` (...) int64.  Under softmax(logits
+    / temperature), in fp32: ``logprobs`` (...) of the tokens (0 for a negative
+    token, the padding of a ragged batch; NaN for one >= V), ``entropy`` (...)
+    in nats, and with ``top`` <= 32 the largest log probabilities
+    ``top_logprobs`` (..., top) and their tokens ``top_ids`` (..., top) int64,
+    the lower token first where logits are equal.  Logits of -inf have
+    probability 0; a row of nothing else gives -inf and entropy 0."""
+    if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens {tuple(tokens.shape)} must have the leading shape of logits "
+                         f"{tuple(logits.shape)}")
+    V = logits.shape[-1]
+    dt = _OUT_DTYPES.get(logits.dtype)
+    if dt is None:
+        raise TypeError(f"logits must be bfloat16, float16 or float32 (got {logits.dtype})")
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"tokens must be int64 (got {tokens.dtype})")
+    if V < 1 or not 0 <= top <= min(C.RP_LOGPROB_MAX_TOP, V):
+        raise ValueError(f"top must lie in [0, min({C.RP_LOGPROB_MAX_TOP}, V)] (got {top}, V={V})")
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive and finite (got {temperature})")
+    _unit_stride("logits", logits)
+    _on_device_of(logits, tokens=tokens, logits=logits)
+    lead = logits.shape[:-1]
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    t = tokens.reshape(-1)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    N = x.shape[0]
+    f32 = torch.empty((2 + top) * N, dtype=torch.float32, device=x.device)
+    ids = torch.empty((*lead, top), dtype=torch.int64, device=x.device) if top else None
+    if N > 0:
+        ld = x.stride(0) if N > 1 else V
+        n = C.lib().rp_token_logprobs_workspace_bytes(N, V, dt, top)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        base = f32.data_ptr()
+        C.check(C.lib().rp_token_logprobs(
+            x.data_ptr(), dt, N, V, ld, t.data_ptr(), temperature, top, base, base + 4 * N,
+            base + 8 * N if top else None, ids.data_ptr() if top else None,
+            ws.data_ptr() if n else None, n, _stream(x)), "rp_token_logprobs")
+    return TokenLogprobs(f32[:N].view(lead), f32[N:2 * N].view(lead),
+                         f32[2 * N:].view(*lead, top) if top else None, ids)
 
 
 def selftest_e4m3(x: torch.Tensor) -> torch.Tensor:

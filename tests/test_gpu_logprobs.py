@@ -1,0 +1,198 @@
+"""Token log probabilities, entropy and best alternatives on the GPU against 64 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from repercep_runtime_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+U = 2.0 ** -24
+NAN, INF = float("nan"), float("inf")
+
+
+def reference(x: torch.Tensor, tokens: torch.Tensor, top: int, T: float) -> tuple:
+    """(logprobs, entropy, top values, top ids) in 64 bits; ids by (value, lower id)."""
+    z = x.double() / T
+    lp = torch.log_softmax(z, dim=-1)
+    p = torch.exp(lp)
+    plogp = torch.where(p > 0, p * lp, torch.zeros_like(p))
+    ids = torch.sort(x.double(), dim=-1, descending=True, stable=True).indices[:, :top]
+    return lp.gather(1, tokens.unsqueeze(1)).squeeze(1), -plogp.sum(-1), lp.gather(1, ids), ids
+
+
+def check(gpu, x: torch.Tensor, top: int, T: float = 1.0, seed: int = 0) -> None:
+    """A shifted logit z = x / T - m is off by two roundings at |x| / T and one
+    at |z| (R below); an exponential by R |z|'s share plus its own 2 u, a sum
+    of V of them by V u more, its logarithm by that and 2 u; the entropy's
+    second sum by as much of sum p |z|."""
+    N, V = x.shape
+    tokens = torch.randint(0, V, (N,), generator=torch.Generator().manual_seed(seed))
+    lp, ent, tv, ti = reference(x, tokens, top, T)
+    r = ops.token_logprobs(x.to(gpu), tokens.to(gpu), top=top, temperature=T)
+    z = x.double() / T
+    big = torch.where(torch.isfinite(z), z.abs(), torch.zeros_like(z)).amax(-1)
+    R = 6 * U * big + 4 * U
+    tol = 2 * R + (min(V, 4096) + 16) * U        # sums of up to 4096 terms in a row, then trees
+    zz = torch.where(torch.isfinite(z), z - z.amax(-1, keepdim=True), torch.zeros_like(z))
+    spread = (torch.softmax(z, -1) * zz.abs()).sum(-1)
+    got = r.logprobs.cpu().double()
+    fin = torch.isfinite(lp)
+    assert torch.equal(torch.isfinite(got), fin) and torch.equal(got[~fin], lp[~fin])
+    assert ((got - lp).abs()[fin] <= (tol + 2 * U * lp.abs())[fin]).all()
+    assert ((r.entropy.cpu().double() - ent).abs() <= 2 * tol * (1 + spread)).all()
+    if not top:
+        assert r.top_ids is None and r.top_logprobs is None
+        return
+    assert torch.equal(r.top_ids.cpu(), ti)
+    fin = torch.isfinite(tv)
+    got = r.top_logprobs.cpu().double()
+    assert torch.equal(torch.isfinite(got), fin) and torch.equal(got[~fin], tv[~fin])
+    assert ((got - tv).abs()[fin] <= (tol.unsqueeze(1) + 2 * U * tv.abs())[fin]).all()
+
+
+def logits(N: int, V: int, dt: str, seed: int, std: float = 2.5) -> torch.Tensor:
+    return (torch.randn(N, V, generator=torch.Generator().manual_seed(seed)) * std).to(DTYPES[dt])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,V", [(1, 1), (3, 2), (1, 7), (5, 63), (4, 64), (2, 65), (3, 1000),
+                                 (2, 1023), (1, 4097), (7, 8192), (1, 8193), (2, 16385),
+                                 (1, 32000), (3, 32769), (1, 65537), (2, 100003), (1, 152064)])
+@pytest.mark.parametrize("top", [0, 1, 20, 32])
+def test_scores(gpu, dt, N, V, top) -> None:
+    check(gpu, logits(N, V, dt, N * V), min(top, V), seed=V)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("N", [130, 600, 1500])
+def test_many_rows(gpu, dt, N) -> None:
+    check(gpu, logits(N, 4100, dt, N), 5)
+
+
+@pytest.mark.parametrize("T", [0.25, 0.7, 3.0])
+def test_temperature(gpu, T) -> None:
+    check(gpu, logits(4, 5000, "bf16", 1), 8, T)
+
+
+@pytest.mark.parametrize("shift", [-3e4, 1e3, 3e4])
+def test_large_logits(gpu, shift) -> None:
+    """Logits far from zero: only their differences count."""
+    check(gpu, (logits(3, 3001, "fp32", 2) + shift).float(), 8)
+
+
+def test_wide_spread(gpu) -> None:
+    """One token takes all; the others' probabilities leave the type's range."""
+    check(gpu, logits(3, 5000, "fp32", 3, std=200.0), 32)
+    x = torch.full((2, 3000), -1e4)
+    x[:, 1234] = 1e4
+    check(gpu, x, 4)
+
+
+@pytest.mark.parametrize("V", [50, 3000, 40000, 140000])
+def test_ties_go_to_the_lower_token(gpu, V) -> None:
+    """All equal, two values, few values, zeros of both signs: ids by (value, lower id)."""
+    g = torch.Generator().manual_seed(V)
+    few = torch.tensor([0.0, 1.0, 2.0])[torch.randint(0, 3, (V,), generator=g)]
+    signs = torch.tensor([0.0, -0.0])[torch.randint(0, 2, (V,), generator=g)]
+    one = torch.zeros(V)
+    one[V // 2] = 1.0
+    check(gpu, torch.stack([torch.full((V,), 1.5), few, signs, one]).to(torch.bfloat16), 32)
+
+
+@pytest.mark.parametrize("V", [300, 9000, 140000])
+def test_sorted_rows(gpu, V) -> None:
+    """The best logits next to each other, at either end or in the middle."""
+    up = torch.arange(V, dtype=torch.float32) * 1e-3
+    check(gpu, torch.stack([up, -up, up.roll(V // 3), -(up - up[V // 2]).abs()]), 32)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [100, 33000])
+def test_masked_logits(gpu, dt, V) -> None:
+    """-inf at most places (fewer left than asked for among them), the type's
+    lowest value at most places, and a single one left."""
+    x = logits(4, V, dt, V)
+    g = torch.Generator().manual_seed(1)
+    x[0][torch.rand(V, generator=g) < 0.7] = -INF
+    x[1, 10:] = -INF
+    x[2, :V - 3] = torch.finfo(x.dtype).min
+    x[3, :] = -INF
+    x[3, V // 2] = 0.5
+    check(gpu, x, 32)
+
+
+@pytest.mark.parametrize("V", [70, 50000])
+def test_rows_without_a_distribution(gpu, V) -> None:
+    """Nothing but -inf: -inf and 0; a NaN or +inf anywhere: NaN, in that row only."""
+    x = logits(4, V, "bf16", 4)
+    x[0] = -INF
+    x[1, V - 1] = NAN
+    x[2, 3] = INF
+    tokens = torch.tensor([1, 2, 3, 4])
+    r = ops.token_logprobs(x.to(gpu), tokens.to(gpu), top=3)
+    assert r.logprobs[0] == -INF and r.entropy[0] == 0
+    assert torch.isneginf(r.top_logprobs[0]).all() and r.top_ids[0].tolist() == [0, 1, 2]
+    for i in (1, 2):
+        assert r.logprobs[i].isnan() and r.entropy[i].isnan() and r.top_logprobs[i].isnan().all()
+    assert int(r.top_ids[1, 0]) == V - 1 and int(r.top_ids[2, 0]) == 3
+    want = ops.token_logprobs(x[3:].to(gpu), tokens[3:].to(gpu), top=3)
+    assert torch.equal(r.logprobs[3:], want.logprobs)
+    assert torch.equal(r.top_ids[3:], want.top_ids)
+
+
+def test_padding_and_foreign_tokens(gpu) -> None:
+    x = logits(4, 50, "bf16", 5).to(gpu)
+    r = ops.token_logprobs(x, torch.tensor([-100, 50, 49, -1], device=gpu))
+    assert r.logprobs[0] == 0 and r.logprobs[3] == 0 and r.logprobs[1].isnan()
+    assert torch.isfinite(r.logprobs[2]) and torch.isfinite(r.entropy).all()
+    assert r.top_ids is None
+
+
+def test_views_and_leading_shapes(gpu) -> None:
+    """(B, S, V) logits, rows at an odd stride and address, one row, none."""
+    x = logits(12, 5003, "bf16", 6)
+    wide = torch.full((12, 5010), 99.0, dtype=torch.bfloat16, device=gpu)
+    wide[:, 3:5006] = x.to(gpu)
+    t = torch.arange(12, device=gpu)
+    want = ops.token_logprobs(x.to(gpu), t, top=4)
+    got = ops.token_logprobs(wide[:, 3:5006], t, top=4)
+    for a, b in zip(want[:3], got[:3]):
+        assert torch.allclose(a, b, rtol=0, atol=64 * U * 8)
+    assert torch.equal(want.top_ids, got.top_ids)
+    r = ops.token_logprobs(x.to(gpu).view(3, 4, 5003), t.view(3, 4), top=4)
+    assert r.logprobs.shape == (3, 4) and r.top_ids.shape == (3, 4, 4)
+    assert torch.equal(r.top_ids.view(12, 4), want.top_ids)
+    one = ops.token_logprobs(x[2].to(gpu), t[2], top=4)
+    assert one.logprobs.shape == () and torch.equal(one.top_ids, want.top_ids[2])
+    none = ops.token_logprobs(x[:0].to(gpu), t[:0], top=4)
+    assert none.logprobs.shape == (0,) and none.top_ids.shape == (0, 4)
+
+
+def test_rows_past_32_bit_offsets(gpu) -> None:
+    V, N = 1 << 20, (1 << 12) + 3
+    free, _ = torch.cuda.mem_get_info(gpu)
+    if free < 12 << 30:
+        pytest.skip("needs 12 GB of GPU memory")
+    x = torch.zeros((N, V), dtype=torch.bfloat16, device=gpu)
+    x[N - 1, 777] = 20.0
+    t = torch.full((N,), 777, device=gpu)
+    r = ops.token_logprobs(x, t, top=1)
+    # the other V - 1 weigh e^-20 each: V e^-20 = 0.00216
+    assert abs(float(r.logprobs[N - 1]) + math.log1p((V - 1) * math.exp(-20))) < 1e-5
+    assert int(r.top_ids[N - 1, 0]) == 777 and int(r.top_ids[N - 2, 0]) == 0
+    assert abs(float(r.logprobs[0]) + math.log(V)) < 1e-4
+
+
+def test_equal_calls_give_equal_bits(gpu) -> None:
+    for N, V in ((1, 32000), (300, 32000), (2, 150000)):
+        x = logits(N, V, "bf16", 9).to(gpu)
+        t = torch.zeros(N, dtype=torch.int64, device=gpu)
+        a = ops.token_logprobs(x, t, top=20)
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(a, ops.token_logprobs(x, t, top=20)))
