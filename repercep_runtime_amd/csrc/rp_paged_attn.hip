@@ -1,136 +1,589 @@
 // Attention of one new token per sequence over a paged key-value cache.
 //
-// One workgroup per (sequence, query head): its waves take the keys in turn,
-// a wave's lanes share a key's head dim, and each wave keeps a running
-// maximum, sum and output, joined at the end.
+// A call reads every attended row of K and V once per kv head and does
+// 4 * (H / Hkv) * D operations with a row's pair, so its floor is the cache's
+// bytes; the kernel is built to keep loads in flight.
+//
+// * Products run on the matrix cores (16x16x32) although a decoder has few
+//   query heads per kv head: the 16 columns are the query heads of one kv
+//   head, unused ones idle, and 32 keys take D / 32 * 2 + D / 16 * 2
+//   instructions, far below what their bytes take to arrive.  In S^T = K Q^T
+//   a lane ends up with the scores of one head (its column) and the eight keys
+//   4 g + 0..3 and 16 + 4 g + 0..3 of a step's 32 (g = lane / 16).  O^T = V^T P^T
+//   sums over those same keys if lane group g brings V's rows in that order, so
+//   P goes from the first product to the second inside its lane: nothing
+//   passes through LDS in the loop.
+// * V's operand needs eight keys of one column in a register quad.  A lane
+//   loads D / 16 columns of each of its eight rows and transposes them with
+//   byte permutes (v_perm_b32), one per pair of values.
+// * P enters the second product as the sum of two 16-bit numbers, the rounded
+//   weight and the rounded rest (16 bits of it or more), so the output keeps
+//   the accuracy of an fp32 weight; the products are idle otherwise.
+// * The running maximum is lazy: a lane's scores are weighed against its
+//   column's base, and only when one exceeds it by 2^8 (kSlack) does the wave
+//   agree on a new base and rescale.  Every lane of a column holds the same
+//   base, and the final sums are exact about any base.
+// * K rows of step i + 1 are requested as soon as step i's first product has
+//   read its registers, V rows after the second one, so a wave always has a
+//   step's K or V on its way.
+//
+// The keys of a (sequence, kv head) are split into chunks of equal size over
+// workgroups, a chunk over a workgroup's waves; waves join through LDS,
+// chunks through fp32 partial sums and join_kernel.  A sequence longer than
+// expected takes several rounds of its workgroups.
 
 #include "rp_paged_dev.h"
 
 namespace rp {
 namespace {
 
-constexpr int kDThreads = 256;
+constexpr int kDWaves = 4;
+constexpr int kDThreads = kDWaves * kWave;
+constexpr int kStep = 32;                       // keys per step of a wave
+constexpr int kMaxChunk = kDWaves * 1024;       // a wave holds 64 tiles' pages in one register
+constexpr int kJThreads = 256;
+constexpr float kSlack = 8.0f;                  // powers of two
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.693147180559945309f;
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct DecodeArgs {
   const uint16_t* q;
   int64_t qsb, qsh;
   const int32_t* lens;
-  float scale;
+  float c;                       // sm_scale * log2(e)
   uint16_t* out;
   int64_t osb, osh;
   float* lse;
   float* weights;
   int64_t wsb, wsh;
-  int32_t H, group;
+  int32_t H, group, tiles;       // query heads, per kv head, 16-head tiles per kv head
+  int32_t splits, chunk;
+  float* part;                   // (B, H, splits, D): sums about the part's base
+  float2* ml;                    // (B, H, splits): base (in powers of two), sum of weights
+  float* scores;                 // (B, H, score_ld): scores in powers of two, for the key weights
+  int64_t score_ld;
 };
 
-__device__ __forceinline__ float e4m3_to_f32(uint32_t code) {
-  return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+template <bool F16>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Element d of cache row `row` (element offset).
-template <int CT>
-__device__ __forceinline__ float cache_elem(const char* p, int64_t row, int d) {
-  if constexpr (CT == RP_CACHE_E4M3) return e4m3_to_f32(reinterpret_cast<const uint8_t*>(p)[row + d]);
-  else return in_to_f32<CT>(reinterpret_cast<const uint16_t*>(p)[row + d]);
+// Two e4m3fn codes of a dword (its low or high half) as a pair of 16-bit
+// floats, exact: e4m3fn is a subset of both.
+template <bool F16, bool HI>
+__device__ __forceinline__ uint32_t codes_to_16(uint32_t w) {
+  if constexpr (F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 
-template <int QT, int CT, int D>
-__global__ __launch_bounds__(kDThreads) void decode_kernel(DecodeArgs a, PagedView c) {
-  constexpr int E = (D + kWave - 1) / kWave, kWaves = kDThreads / kWave;
-  __shared__ float sm[kWaves], sl[kWaves], so[kWaves][D];
-  const int h = blockIdx.x, b = blockIdx.y, kv = h / a.group;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+// Weights a, b as packed 16-bit numbers `hi` and the rest `lo`.
+template <bool F16>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo) {
+  if constexpr (F16) {
+    // toward zero: the rest is exact in fp32 and keeps 10 more bits
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    *hi = __builtin_bit_cast(uint32_t, h);
+    *lo = __builtin_bit_cast(uint32_t,
+                             __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+  } else {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    *hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+    const float ra = a - __uint_as_float(*hi << 16), rb = b - __uint_as_float(*hi & 0xffff0000u);
+    *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{ra, rb}, bf16x2_t));
+  }
+}
+
+// One wave's state over its keys.  PG16: pages hold 16 rows or more, so each
+// half of a step lies in one page.
+template <int QT, int CT, int D, bool PG16>
+struct Wave {
+  static constexpr bool FP8 = CT == RP_CACHE_E4M3;
+  static constexpr bool QF16 = QT == kInF16;          // the first product's type
+  static constexpr bool PF16 = QF16 && !FP8;          // the second's: a scaled weight fits bf16 only
+  static constexpr int EB = FP8 ? 1 : 2;
+  static constexpr int NT = D / 32;                   // first products per 16 keys
+  static constexpr int DPL = D / 16;                  // V columns per lane
+  static constexpr int KL = FP8 ? (D + 63) / 64 : NT; // 16-byte K loads per 16 keys (8 at D = 32, fp8)
+  static constexpr int VB = DPL * EB;                 // V bytes per lane and row
+  static constexpr int VW = VB < 4 ? 1 : VB / 4;
+  // fp16 weights: a lift of 2^14 keeps them off the subnormals (2^8 of slack fits)
+  static constexpr float kLift = PF16 ? 6.0f : 0.0f;
+
+  const PagedView& c;
+  const DecodeArgs& a;
+  int lane, m, g, n;
+  int64_t head;                  // kv head
+  const int32_t* table;
+  int32_t pages;                 // lane i: page of 16-key tile i of this wave's range (PG16)
+  int k0;
+  uint32_t koff, voff[4];        // byte offsets of a lane's rows within a tile (PG16)
+  u32x4 q[NT];
+  u32x4 kr[2][KL];
+  uint32_t vr[8][VW];
+  f32x4 kscale[2], vscale[2];
+  int32_t vpage[8];              // !PG16: pages of the lane's eight rows of the loaded step's V
+  int32_t kvalid;                // !PG16: of the step whose K is loaded, the keys that exist
+  f32x4 acc[DPL];
+  float base, sum;
+  float* score_row;
+
+  __device__ __forceinline__ Wave(const DecodeArgs& a_, const PagedView& c_) : c(c_), a(a_) {}
+
+  __device__ __forceinline__ void load_q(const uint16_t* src, bool live) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int d = FP8 && D >= 64 ? 64 * (t / 2) + 16 * g + 8 * (t % 2) : 32 * t + 8 * g;
+      q[t] = live ? *reinterpret_cast<const u32x4*>(src + d) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+
+  __device__ __forceinline__ void begin(int from) {
+    k0 = from;
+    if constexpr (PG16) pages = paged_page(c, table, (int64_t)from + 16 * lane);
+  }
+
+  __device__ __forceinline__ int key(int k, int e) const {
+    return k + 4 * g + (e < 4 ? e : 12 + e);
+  }
+
+  __device__ __forceinline__ int32_t tile_page(int k, int half) const {
+    return __builtin_amdgcn_readlane(pages, ((k - k0) >> 4) + half);
+  }
+
+  __device__ __forceinline__ void k_row(const char* p, int half) {
+    if constexpr (FP8 && D == 32) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p + 8 * g);
+      kr[half][0] = u32x4{x[0], x[1], 0u, 0u};
+    } else {
+#pragma unroll
+      for (int t = 0; t < KL; ++t)
+        kr[half][t] = *reinterpret_cast<const u32x4*>(p + 64 * t + 16 * g);
+    }
+  }
+
+  __device__ __forceinline__ void v_row(const char* p, int e) {
+    if constexpr (VB == 2) {
+      vr[e][0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if constexpr (VB == 4) {
+      vr[e][0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (VB == 8) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      vr[e][0] = x[0];
+      vr[e][1] = x[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VB / 16; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 256 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vr[e][4 * i + j] = x[j];
+      }
+    }
+  }
+
+  // Bytes of a lane's first column, and the column of its value j.
+  __device__ __forceinline__ int v_col() const { return m * (VB > 16 ? 16 : VB); }
+  __device__ __forceinline__ static int column(int mm, int j) {
+    if constexpr (VB > 16) return (j < 8 ? 0 : 128) + 8 * mm + j % 8;
+    else return mm * DPL + j;
+  }
+
+  __device__ __forceinline__ void load_k(int k) {
+    if constexpr (PG16) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // a page that is none is read as page 0 and masked
+        const int32_t p = max(tile_page(k, half), 0);
+        const char* tile = c.k + paged_row(c, p, head, k + 16 * half) * EB;
+        k_row(tile + koff, half);
+        if constexpr (FP8)
+          kscale[half] = *reinterpret_cast<const f32x4*>(c.ks + paged_scale(c, p, head, k + 16 * half) + 4 * g);
+      }
+    } else {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int j = k + 16 * half + m;
+        const int32_t p = max(paged_page(c, table, j), 0);
+        k_row(c.k + paged_row(c, p, head, j) * EB, half);
+      }
+      if constexpr (FP8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int32_t p = max(paged_page(c, table, key(k, e)), 0);
+          kscale[e / 4][e % 4] = c.ks[paged_scale(c, p, head, key(k, e))];
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load_v(int k) {
+    if constexpr (PG16) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int32_t p = max(tile_page(k, half), 0);
+        const char* tile = c.v + paged_row(c, p, head, k + 16 * half) * EB;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v_row(tile + voff[r], 4 * half + r);
+        if constexpr (FP8)
+          vscale[half] = *reinterpret_cast<const f32x4*>(c.vs + paged_scale(c, p, head, k + 16 * half) + 4 * g);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int32_t p = max(paged_page(c, table, key(k, e)), 0);
+        v_row(c.v + paged_row(c, p, head, key(k, e)) * EB + v_col(), e);
+        if constexpr (FP8) vscale[e / 4][e % 4] = c.vs[paged_scale(c, p, head, key(k, e))];
+      }
+    }
+  }
+
+  // Which of the lane's eight keys exist.
+  __device__ __forceinline__ uint32_t present(int k, int end) const {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = PG16 ? tile_page(k, e / 4) >= 0 : paged_page(c, table, key(k, e)) >= 0;
+      if (in && key(k, e) < end) mask |= 1u << e;
+    }
+    return mask;
+  }
+
+  // Operand words of K's fragment t of a half step.
+  __device__ __forceinline__ u32x4 k_frag(int half, int t) const {
+    if constexpr (!FP8) {
+      return kr[half][t];
+    } else {
+      const u32x4& x = kr[half][t / 2];
+      const uint32_t w0 = t % 2 ? x[2] : x[0], w1 = t % 2 ? x[3] : x[1];
+      return u32x4{codes_to_16<QF16, false>(w0), codes_to_16<QF16, true>(w0),
+                   codes_to_16<QF16, false>(w1), codes_to_16<QF16, true>(w1)};
+    }
+  }
+
+  // Keys [k, k + 32) of which those below `end` exist; `more`: another step follows.
+  template <bool MORE>
+  __device__ __forceinline__ void step(int k, int end) {
+    f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) s[half] = mma<QF16>(k_frag(half, t), q[t], s[half]);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = s[e / 4][e % 4] * a.c;
+      if constexpr (FP8) x[e] *= kscale[e / 4][e % 4];
+    }
+    bool whole;
+    if constexpr (PG16)
+      whole = k + kStep <= end && tile_page(k, 0) >= 0 && tile_page(k, 1) >= 0;
+    else
+      whole = false;
+    uint32_t mask = 0xffu;
+    if (!whole) {
+      mask = present(k, end);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = mask >> e & 1 ? x[e] : neg_inf();
+    }
+    if constexpr (MORE) load_k(k + kStep);
+    if (score_row) {
+      *reinterpret_cast<f32x4*>(score_row + k + 4 * g) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4*>(score_row + k + 16 + 4 * g) = f32x4{x[4], x[5], x[6], x[7]};
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                      fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__any(top > base + (kSlack + kLift))) {
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float next = fmaxf(base, top - kLift);
+      const float r = next == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(base - next);
+      sum *= r;
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) acc[j] *= r;
+      base = next;
+    }
+    // a column that has seen no score yet weighs about 0: exp2(-inf) is 0
+    const float b = base == neg_inf() ? 0.0f : base;
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - b);
+    sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    if constexpr (FP8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] *= vscale[e / 4][e % 4];
+    }
+    if (!whole) {
+      // what is no row may hold anything: neither it nor its scale takes part
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = mask >> e & 1;
+        p[e] = in ? p[e] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) vr[e][i] = in ? vr[e][i] : 0u;
+      }
+    }
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h, l;
+      split_pair<PF16>(p[2 * i], p[2 * i + 1], &h, &l);
+      hi[i] = h;
+      lo[i] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < DPL; j += 2) {
+      // the pair of columns j, j + 1 of each row as 16-bit values
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (!FP8) w[e] = vr[e][j / 2];
+        else w[e] = j % 4 ? codes_to_16<PF16, true>(vr[e][j / 4]) : codes_to_16<PF16, false>(vr[e][j / 4]);
+      }
+      u32x4 f0, f1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f0[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+        f1[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+      }
+      acc[j] = mma<PF16>(f0, hi, acc[j]);
+      acc[j + 1] = mma<PF16>(f1, hi, acc[j + 1]);
+      acc[j] = mma<PF16>(f0, lo, acc[j]);
+      acc[j + 1] = mma<PF16>(f1, lo, acc[j + 1]);
+    }
+    if constexpr (MORE) load_v(k + kStep);
+  }
+};
+
+template <int QT, int CT, int D, bool PG16>
+__global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedView c) {
+  typedef Wave<QT, CT, D, PG16> W;
+  __shared__ f32x4 sacc[kDWaves / 2][W::DPL][kWave];
+  __shared__ float sbase[kDWaves][16], ssum[kDWaves][16];
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int kv = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = (int)paged_len(c, a.lens[b]);
-  const int32_t* table = c.table + b * c.table_stride;
-  float q[E], o[E];
+  // a part beyond the sequence's end has nothing to say, and join_kernel does
+  // not ask it; the first part always answers
+  if (split > 0 && (int64_t)split * a.chunk >= n) return;
+  W w(a, c);
+  w.lane = threadIdx.x & (kWave - 1);
+  w.m = w.lane & 15;
+  w.g = w.lane >> 4;
+  w.head = kv;
+  w.table = c.table + b * c.table_stride;
+  const int first = tile * 16;                         // of the group's query heads
+  const bool live = first + w.m < a.group;
+  const int h = kv * a.group + first + w.m;
+  w.load_q(a.q + b * a.qsb + (int64_t)h * a.qsh, live);
+  w.koff = (uint32_t)(w.m * c.sr * W::EB);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int d = lane + e * kWave;
-    q[e] = d < D ? in_to_f32<QT>(a.q[b * a.qsb + h * a.qsh + d]) * a.scale : 0.0f;
-    o[e] = 0.0f;
+  for (int r = 0; r < 4; ++r) w.voff[r] = (uint32_t)((4 * w.g + r) * c.sr * W::EB) + w.v_col();
+  w.base = neg_inf();
+  w.sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < W::DPL; ++j) w.acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  w.score_row = a.scores && live ? a.scores + ((int64_t)b * a.H + h) * a.score_ld : nullptr;
+
+  for (int64_t c0 = (int64_t)split * a.chunk; c0 < n; c0 += (int64_t)a.splits * a.chunk) {
+    const int rem = (int)min((int64_t)a.chunk, n - c0);
+    const int per = ((rem + kDWaves - 1) / kDWaves + kStep - 1) / kStep * kStep;
+    const int from = (int)c0 + wave * per, end = min(from + per, (int)c0 + rem);
+    if (from >= end) continue;
+    w.begin(from);
+    w.load_k(from);
+    w.load_v(from);
+    int k = from;
+    for (; k + kStep < end; k += kStep) w.template step<true>(k, end);
+    w.template step<false>(k, end);
   }
-  float m = -__builtin_inff(), l = 0.0f;
-  for (int j = wave; j < n; j += kWaves) {
-    const int32_t page = paged_page(c, table, j);
-    if (page < 0) continue;
-    const int64_t row = paged_row(c, page, kv, j);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + e * kWave;
-      if (d < D) s += q[e] * cache_elem<CT>(c.k, row, d);
-    }
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x, kWave);
-    float vs = 1.0f;
-    if constexpr (CT == RP_CACHE_E4M3) {
-      s *= c.ks[paged_scale(c, page, kv, j)];
-      vs = c.vs[paged_scale(c, page, kv, j)];
-    }
-    const float mn = fmaxf(m, s), base = mn == -__builtin_inff() ? 0.0f : mn;
-    const float r = expf(m - base), p = expf(s - base);
-    l = l * r + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + e * kWave;
-      if (d < D) o[e] = o[e] * r + p * (vs * cache_elem<CT>(c.v, row, d));
-    }
-    m = mn;
+
+  // the waves' parts about one base
+  w.sum += __shfl_xor(w.sum, 16, kWave);
+  w.sum += __shfl_xor(w.sum, 32, kWave);
+  if (w.g == 0) {
+    sbase[wave][w.m] = w.base;
+    ssum[wave][w.m] = w.sum;
   }
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (lane + e * kWave < D) so[wave][lane + e * kWave] = o[e];
   __syncthreads();
-  float mt = sm[0], lt = 0.0f;
-  for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, sm[w]);
-  const float base = mt == -__builtin_inff() ? 0.0f : mt;
-  for (int w = 0; w < kWaves; ++w) lt += sl[w] * expf(sm[w] - base);
-  for (int d = threadIdx.x; d < D; d += kDThreads) {
-    float x = 0.0f;
-    for (int w = 0; w < kWaves; ++w) x += so[w][d] * expf(sm[w] - base);
-    x = lt == 0.0f ? 0.0f : x / lt;
-    a.out[b * a.osb + h * a.osh + d] =
-        QT == kInF16 ? __builtin_bit_cast(uint16_t, (_Float16)x) : (uint16_t)f32_to_bf16_bits(x);
+  float base = sbase[0][w.m];
+#pragma unroll
+  for (int i = 1; i < kDWaves; ++i) base = fmaxf(base, sbase[i][w.m]);
+  const float b0 = base == neg_inf() ? 0.0f : base;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kDWaves; ++i) sum += ssum[i][w.m] * __builtin_amdgcn_exp2f(sbase[i][w.m] - b0);
+  const float r = __builtin_amdgcn_exp2f(w.base - b0);
+#pragma unroll
+  for (int j = 0; j < W::DPL; ++j) w.acc[j] *= r;
+#pragma unroll
+  for (int half = kDWaves / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < W::DPL; ++j) sacc[wave - half][j][w.lane] = w.acc[j];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int j = 0; j < W::DPL; ++j) w.acc[j] += sacc[wave][j][w.lane];
+    }
+    __syncthreads();
   }
-  if (threadIdx.x == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = lt == 0.0f ? -__builtin_inff() : base + logf(lt);
+  if (wave != 0 || !live) return;
+  const int64_t bh = (int64_t)b * a.H + h;
+  if (a.splits > 1) {
+    float* part = a.part + (bh * a.splits + split) * D;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < W::DPL; ++j) part[W::column(4 * w.g + i, j)] = w.acc[j][i];
+    if (w.g == 0) a.ml[bh * a.splits + split] = float2{base, sum};
+    return;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t* out = a.out + b * a.osb + h * a.osh;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < W::DPL; ++j) {
+      const float x = sum == 0.0f ? 0.0f : w.acc[j][i] * inv;
+      out[W::column(4 * w.g + i, j)] = QT == kInF16
+          ? __builtin_bit_cast(uint16_t, (_Float16)x) : (uint16_t)f32_to_bf16_bits(x);
+    }
+  if (w.g == 0) {
+    if (a.lse) a.lse[bh] = sum == 0.0f ? neg_inf() : (base + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (a.ml) a.ml[bh] = float2{base, sum};
+  }
 }
 
-// Adds each seen key's weights: a thread per key.
-template <int QT, int CT, int D>
-__global__ __launch_bounds__(kDThreads) void decode_weights_kernel(DecodeArgs a, PagedView c) {
-  const int kv = blockIdx.y, b = blockIdx.z;
-  const int j = blockIdx.x * kDThreads + threadIdx.x;
-  if (j >= (int)paged_len(c, a.lens[b])) return;
-  const int32_t page = paged_page(c, c.table + b * c.table_stride, j);
-  if (page < 0) return;
-  const int64_t row = paged_row(c, page, kv, j);
-  float w = 0.0f;
-  for (int i = 0; i < a.group; ++i) {
-    const int h = kv * a.group + i;
-    float s = 0.0f;
-    for (int d = 0; d < D; ++d)
-      s += in_to_f32<QT>(a.q[b * a.qsb + h * a.qsh + d]) * a.scale * cache_elem<CT>(c.k, row, d);
-    if constexpr (CT == RP_CACHE_E4M3) s *= c.ks[paged_scale(c, page, kv, j)];
-    const float lse = a.lse[(int64_t)b * a.H + h];
-    w += lse == -__builtin_inff() ? 0.0f : expf(s - lse);
+// The base and sum of a head's parts together.
+__device__ __forceinline__ float2 join_parts(const float2* ml, int parts) {
+  float base = neg_inf();
+  for (int i = 0; i < parts; ++i) base = fmaxf(base, ml[i].x);
+  const float b0 = base == neg_inf() ? 0.0f : base;
+  float sum = 0.0f;
+  for (int i = 0; i < parts; ++i) sum += ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - b0);
+  return float2{b0, sum};
+}
+
+// Joins the parts of each (sequence, query head), D threads' worth of columns
+// at a time (blocks with blockIdx.x < H), and adds the key weights from the
+// stored scores (the others, a block per 1024 keys of a kv head).
+template <int QT, int D>
+__global__ __launch_bounds__(kJThreads) void join_kernel(DecodeArgs a, PagedView c, int heads_x) {
+  const int b = blockIdx.y;
+  const int n = (int)paged_len(c, a.lens[b]);
+  const int parts = max(1, min(a.splits, (n + a.chunk - 1) / a.chunk));
+  if ((int)blockIdx.x < heads_x) {
+    constexpr int COLS = D < kJThreads ? D : kJThreads, GR = kJThreads / COLS;
+    __shared__ float part_sum[GR][COLS];
+    const int h = blockIdx.x;
+    const int64_t bh = (int64_t)b * a.H + h;
+    const float2* ml = a.ml + bh * a.splits;
+    const float2 t = join_parts(ml, parts);
+    const int d = threadIdx.x % COLS, gr = threadIdx.x / COLS;
+    float x = 0.0f;
+    for (int i = gr; i < parts; i += GR)
+      x += a.part[(bh * a.splits + i) * D + d] * __builtin_amdgcn_exp2f(ml[i].x - t.x);
+    part_sum[gr][d] = x;
+    __syncthreads();
+    if (gr != 0) return;
+    for (int i = 1; i < GR; ++i) x += part_sum[i][d];
+    x = t.y == 0.0f ? 0.0f : x / t.y;
+    a.out[b * a.osb + h * a.osh + d] = QT == kInF16
+        ? __builtin_bit_cast(uint16_t, (_Float16)x) : (uint16_t)f32_to_bf16_bits(x);
+    if (threadIdx.x == 0 && a.lse)
+      a.lse[bh] = t.y == 0.0f ? neg_inf() : (t.x + __builtin_amdgcn_logf(t.y)) * kLn2;
+    return;
   }
-  a.weights[b * a.wsb + kv * a.wsh + j] += w;
+  const int blocks = (gridDim.x - heads_x) / c.heads;
+  const int kv = (blockIdx.x - heads_x) / blocks, part = (blockIdx.x - heads_x) % blocks;
+  const int j = (part * kJThreads + threadIdx.x) * 4;
+  if (part * kJThreads * 4 >= n) return;
+  float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < a.group; ++i) {
+    const int64_t bh = (int64_t)b * a.H + kv * a.group + i;
+    const float2 t = join_parts(a.ml + bh * a.splits, parts);
+    if (j >= n || t.y == 0.0f) continue;
+    const float inv = 1.0f / t.y;
+    const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + bh * a.score_ld + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(s[e] - t.x) * inv;
+  }
+  float* to = a.weights + b * a.wsb + kv * a.wsh + j;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < n) to[e] += w[e];
+}
+
+// How a call's keys are split: chunks of `chunk` keys, `splits` of them at
+// most (the last ones empty for shorter sequences).
+struct Plan {
+  int32_t splits, chunk;
+};
+
+inline Plan decode_plan(int64_t groups, int64_t keys) {
+  constexpr int64_t kWant = 1024;                  // workgroups
+  constexpr int64_t kUnit = kDWaves * kStep;
+  int64_t splits = (kWant + groups - 1) / groups;
+  const int64_t most = (keys + kUnit - 1) / kUnit;
+  if (splits > most) splits = most;
+  int64_t chunk = ((keys + splits - 1) / splits + kUnit - 1) / kUnit * kUnit;
+  if (chunk > kMaxChunk) chunk = kMaxChunk;
+  splits = (keys + chunk - 1) / chunk;
+  return Plan{(int32_t)splits, (int32_t)chunk};
+}
+
+struct Layout {
+  Plan plan;
+  int64_t score_ld;
+  size_t ml, part, scores, total;      // byte offsets
+};
+
+inline Layout decode_layout(int64_t B, int64_t H, const rp_paged_cache* c, int64_t max_seq_len,
+                            bool weights) {
+  const int64_t cap = c->max_pages * c->page_size, group = H / c->heads;
+  const int64_t keys = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
+  Layout l;
+  l.plan = decode_plan(B * c->heads * ((group + 15) / 16), keys);
+  auto up = [](int64_t x) { return (size_t)((x + 255) / 256 * 256); };
+  const bool split = l.plan.splits > 1;
+  // whole steps are written, the last one past the capacity
+  l.score_ld = (cap + kStep - 1) / kStep * kStep;
+  l.ml = 0;
+  l.part = l.ml + (split || weights ? up(B * H * l.plan.splits * 8) : 0);
+  l.scores = l.part + (split ? up(B * H * l.plan.splits * c->head_dim * 4) : 0);
+  l.total = l.scores + (weights ? up(B * H * l.score_ld * 4) : 0);
+  return l;
 }
 
 template <int QT, int CT, int D>
 void launch_decode_d(const DecodeArgs& a, const PagedView& c, int64_t B, hipStream_t st) {
-  hipLaunchKernelGGL((decode_kernel<QT, CT, D>), dim3((unsigned)a.H, (unsigned)B), dim3(kDThreads),
-                     0, st, a, c);
-  if (a.weights)
-    hipLaunchKernelGGL((decode_weights_kernel<QT, CT, D>),
-                       dim3((unsigned)((c.capacity() + kDThreads - 1) / kDThreads),
-                            (unsigned)c.heads, (unsigned)B),
-                       dim3(kDThreads), 0, st, a, c);
+  const dim3 grid((unsigned)a.splits, (unsigned)(c.heads * a.tiles), (unsigned)B);
+  if (c.shift >= 4)
+    hipLaunchKernelGGL((attend_kernel<QT, CT, D, true>), grid, dim3(kDThreads), 0, st, a, c);
+  else
+    hipLaunchKernelGGL((attend_kernel<QT, CT, D, false>), grid, dim3(kDThreads), 0, st, a, c);
+  const int heads_x = a.splits > 1 ? a.H : 0;
+  const int64_t blocks = a.weights ? (c.capacity() + 4 * kJThreads - 1) / (4 * kJThreads) : 0;
+  if (heads_x + blocks > 0)
+    hipLaunchKernelGGL((join_kernel<QT, D>), dim3((unsigned)(heads_x + blocks * c.heads), (unsigned)B),
+                       dim3(kJThreads), 0, st, a, c, heads_x);
 }
 
 template <int QT, int CT>
@@ -148,9 +601,10 @@ using namespace rp;
 
 extern "C" size_t rp_paged_attn_workspace_bytes(int64_t B, int64_t H, const rp_paged_cache* cache,
                                                 int64_t max_seq_len, int with_key_weights) {
-  (void)max_seq_len;
-  if (!cache || B <= 0 || H <= 0) return 0;
-  return with_key_weights ? (size_t)(B * H * 4) : 0;
+  if (!cache || B <= 0 || H <= 0 || cache->heads <= 0 || cache->max_pages <= 0 ||
+      cache->page_size <= 0 || cache->head_dim <= 0)
+    return 0;
+  return decode_layout(B, H, cache, max_seq_len, with_key_weights != 0).total;
 }
 
 extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64_t qsb,
@@ -185,8 +639,12 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_decode: sm_scale must be finite");
     return RP_ERR_INVALID_ARGUMENT;
   }
-  if (B > 65535 || H > 65535) {
-    rp_set_error("paged_attn_decode: too many sequences or heads");
+  if (B > 65535 || H > 65535 || cache->stride_row > (1 << 25)) {
+    rp_set_error("paged_attn_decode: too many sequences or heads, or rows too far apart");
+    return RP_ERR_UNSUPPORTED;
+  }
+  if (fp8 && ((reinterpret_cast<uintptr_t>(c.ks) | reinterpret_cast<uintptr_t>(c.vs)) & 15) != 0) {
+    rp_set_error("paged_attn_decode: scales must be 16-byte aligned");
     return RP_ERR_UNSUPPORTED;
   }
   if (((qsb | qsh) & 7) != 0 || ((osb | osh) & 3) != 0 ||
@@ -198,16 +656,41 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_decode: bad key_weights strides");
     return RP_ERR_INVALID_ARGUMENT;
   }
-  const size_t want = rp_paged_attn_workspace_bytes(B, H, cache, max_seq_len, key_weights != nullptr);
-  if (want > 0 && (!workspace || workspace_bytes < want ||
-                   (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) {
-    rp_set_error("paged_attn_decode: workspace of %zu bytes, 256-byte aligned, needed", want);
+  const int64_t tiles = (H / cache->heads + 15) / 16;
+  if (cache->heads * tiles > 65535 ||
+      H + (c.capacity() / (4 * kJThreads) + 1) * cache->heads > 0x7fffffff) {
+    rp_set_error("paged_attn_decode: too many heads or positions");
+    return RP_ERR_UNSUPPORTED;
+  }
+  const Layout l = decode_layout(B, H, cache, max_seq_len, key_weights != nullptr);
+  if (l.total > 0 && (!workspace || workspace_bytes < l.total ||
+                      (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) {
+    rp_set_error("paged_attn_decode: workspace of %zu bytes, 256-byte aligned, needed", l.total);
     return RP_ERR_WORKSPACE;
   }
-  if (!lse && key_weights) lse = static_cast<float*>(workspace);
-  const DecodeArgs a{static_cast<const uint16_t*>(q), qsb, qsh, seq_lens, sm_scale,
-                     static_cast<uint16_t*>(out), osb, osh, lse, key_weights, wsb, wsh,
-                     (int32_t)H, (int32_t)(H / cache->heads)};
+  char* ws = static_cast<char*>(workspace);
+  DecodeArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.qsb = qsb;
+  a.qsh = qsh;
+  a.lens = seq_lens;
+  a.c = sm_scale * kLog2e;
+  a.out = static_cast<uint16_t*>(out);
+  a.osb = osb;
+  a.osh = osh;
+  a.lse = lse;
+  a.weights = key_weights;
+  a.wsb = wsb;
+  a.wsh = wsh;
+  a.H = (int32_t)H;
+  a.group = (int32_t)(H / cache->heads);
+  a.tiles = (int32_t)tiles;
+  a.splits = l.plan.splits;
+  a.chunk = l.plan.chunk;
+  a.ml = l.part > l.ml ? reinterpret_cast<float2*>(ws + l.ml) : nullptr;
+  a.part = l.scores > l.part ? reinterpret_cast<float*>(ws + l.part) : nullptr;
+  a.scores = key_weights ? reinterpret_cast<float*>(ws + l.scores) : nullptr;
+  a.score_ld = l.score_ld;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t D = cache->head_dim;
   if (q_dtype == RP_DTYPE_F16) {

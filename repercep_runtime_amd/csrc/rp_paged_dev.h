@@ -78,7 +78,7 @@ inline int paged_view(const char* what, const rp_paged_cache* c, PagedView* v) {
                  (long long)c->page_size);
     return RP_ERR_UNSUPPORTED;
   }
-  if (c->num_pages > 0x7fffffff || c->max_pages > 0x7fffffff / c->page_size ||
+  if (c->num_pages > 0x7fffffff || c->max_pages > (1 << 30) / c->page_size ||
       c->heads > 65535) {
     rp_set_error("%s: too many pages, positions or heads", what);
     return RP_ERR_UNSUPPORTED;
