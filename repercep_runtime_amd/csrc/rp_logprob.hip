@@ -1,33 +1,52 @@
 // Token log probabilities, entropy and the best alternatives of rows of logits.
 //
-// One workgroup per row: the maximum, then the sums over exp(z - max), then
-// the best logits one after another.
+// The floor is one read of the logits, and 5 TB/s of 16-bit logits leave the
+// VALU about 15 lane operations each, so a row is read once, into registers,
+// and everything is computed from there:
+//   M = max x,  t = (x - M) c  (c = log2(e) / temperature),
+//   s = sum 2^t,  u = sum 2^t t,
+//   log p(x) = ln 2 (t - log2 s),  entropy = ln 2 (log2 s - u / s).
+// Subtracting first keeps logits far from zero exact; t below -200 (2^t = 0)
+// is held there, so a masked logit adds 0 and not 0 * inf.
+//
+// The best `top` logits cost no pass of their own.  The threads' maxima,
+// folded to 64 groups, give M and, as their top-th largest, a bound that at
+// least `top` logits reach; the few that do are collected in LDS and ranked
+// by counting, on keys of the logit and its token so that no two are equal.
+// Should more reach it than the buffer holds (a row of equal logits, a sorted
+// one), or a NaN or infinity upset the order, the best are taken one by one.
+//
+// A workgroup holds up to 64 logits a thread.  Longer rows are split over
+// workgroups; join_kernel merges their sums and their best.
+
+#include <type_traits>
 
 #include "rp_common.h"
 
 namespace rp {
 namespace {
 
-constexpr int kLThreads = 256;
-constexpr int kLWaves = kLThreads / kWave;
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxThreads = 512;
+constexpr int kCap = 1024;                     // keys collected per workgroup
+constexpr int kMaxParts = 68;
+constexpr int kJoinThreads = 64;
+constexpr double kLn2 = 0.693147180559945309417;
 
 struct LogprobArgs {
-  const void* x;
+  const char* x;
   int64_t ld;
-  int32_t V, top;
+  int32_t V, top, parts, chunk;
+  float c;
   const int64_t* tokens;
-  float temperature;
   float* logprobs;
   float* entropy;
   float* top_logprobs;
   int64_t* top_ids;
+  f32x4* sums;              // (N, parts): M, s, u of each part
+  uint64_t* keys;           // (N, parts, top)
 };
-
-template <int DT>
-__device__ __forceinline__ float logit(const void* x, int64_t i) {
-  if constexpr (DT == RP_OUT_F32) return static_cast<const float*>(x)[i];
-  else return in_to_f32<DT == RP_OUT_F16 ? kInF16 : kInBf16>(static_cast<const uint16_t*>(x)[i]);
-}
 
 // fp32 -> an unsigned key in the same order; -0 as 0, NaN above everything.
 __device__ __forceinline__ uint32_t logit_key(float x) {
@@ -36,75 +55,299 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
   if (x == 0.0f) return 0x80000000u;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);   // NaN's key is a NaN's bits
+}
+constexpr uint32_t kKeyNegInf = 0x007fffffu;
+
+__device__ __forceinline__ uint64_t full_key(float x, int32_t id) {
+  return ((uint64_t)logit_key(x) << 32) | (0xffffffffu - (uint32_t)id);
+}
 
 template <int DT>
-__global__ __launch_bounds__(kLThreads) void logprob_kernel(LogprobArgs a) {
-  __shared__ float red[3][kLWaves];
-  __shared__ uint64_t redk[kLWaves];
-  const int64_t row = blockIdx.x;
-  const int64_t base = row * a.ld;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  float m = -__builtin_inff();
-  for (int i = threadIdx.x; i < a.V; i += kLThreads) m = fmaxf(m, logit<DT>(a.x, base + i) / a.temperature);
-  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-  if (lane == 0) red[0][wave] = m;
-  __syncthreads();
-  for (int w = 0; w < kLWaves; ++w) m = fmaxf(m, red[0][w]);
-  if (m == -__builtin_inff()) m = 0.0f;   // no logit above -inf: every weight is 0
-  float s = 0.0f, sz = 0.0f;
-  for (int i = threadIdx.x; i < a.V; i += kLThreads) {
-    const float z = __builtin_elementwise_maximum(logit<DT>(a.x, base + i) / a.temperature - m, -200.0f);
-    const float e = expf(z);
-    s += e;
-    sz += e * z;
+__device__ __forceinline__ float logit_at(const char* row, int64_t i) {
+  if constexpr (DT == RP_OUT_F32) return reinterpret_cast<const float*>(row)[i];
+  else return in_to_f32<DT == RP_OUT_F16 ? kInF16 : kInBf16>(reinterpret_cast<const uint16_t*>(row)[i]);
+}
+
+// What one (M, s, u) says of a row: written for its token, entropy and best.
+struct Row {
+  float m, s, u, c;
+  __device__ __forceinline__ float logprob(float x) const {
+    if (s == 0.0f) return -__builtin_inff();
+    // in 64 bits: a lowest value's log probability is finite
+    return (float)((((double)x - (double)m) * (double)c - (double)__builtin_amdgcn_logf(s)) * kLn2);
   }
+  __device__ __forceinline__ float entropy() const {
+    return s == 0.0f ? 0.0f : (float)(((double)__builtin_amdgcn_logf(s) - (double)u / (double)s) * kLn2);
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ float token_logit(const LogprobArgs& a, const char* row, int64_t t) {
+  return t >= 0 && t < a.V ? logit_at<DT>(row, t) : 0.0f;
+}
+__device__ __forceinline__ void write_row(const LogprobArgs& a, const Row& r, int64_t row,
+                                          int64_t token, float x) {
+  a.logprobs[row] = token < 0 ? 0.0f : token >= a.V ? __builtin_nanf("") : r.logprob(x);
+  if (a.entropy) a.entropy[row] = r.entropy();
+}
+__device__ __forceinline__ void write_top(const LogprobArgs& a, const Row& r, int64_t row, int rank,
+                                          uint64_t key) {
+  a.top_ids[row * a.top + rank] = 0xffffffffu - (uint32_t)key;
+  a.top_logprobs[row * a.top + rank] = r.logprob(key_logit((uint32_t)(key >> 32)));
+}
+
+// max that propagates NaN (v_maximum3_f32)
+__device__ __forceinline__ float nmax(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
+// One part of one row.  T threads, NV 16-byte vectors each.
+template <int DT, int T, int NV>
+__global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
+  constexpr int EB = DT == RP_OUT_F32 ? 4 : 2, EPV = 16 / EB, WAVES = T / kWave;
+  constexpr int GROUP = T / kWave;                  // threads per group: 64 groups
+  __shared__ float group_max[kWave];
+  __shared__ float wave_sum[2][WAVES];
+  __shared__ uint64_t found[kCap];
+  __shared__ uint64_t wave_best[WAVES];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const char* xr = a.x + row * a.ld * EB;
+  const int c0 = part * a.chunk, c1 = min(a.V, c0 + a.chunk);
+  // vector v of the part: elements first + v * EPV + 0..EPV-1, 16-byte aligned
+  const int first = c0 - (int)((reinterpret_cast<uintptr_t>(xr + (int64_t)c0 * EB) & 15) / EB);
+  const int64_t token = a.tokens[row];
+  const float xt = tid == 0 && a.parts == 1 ? token_logit<DT>(a, xr, token) : 0.0f;
+  if (tid == 0) count = 0;
+
+  constexpr uint32_t kFill = DT == RP_OUT_F32 ? 0xff800000u : DT == RP_OUT_F16 ? 0xfc00fc00u : 0xff80ff80u;
+  u32x4 raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = first + (tid + v * T) * EPV;
+    raw[v] = u32x4{kFill, kFill, kFill, kFill};
+    if (i >= c0 && i + EPV <= c1) {
+      raw[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(xr + (int64_t)i * EB));
+    } else if (i < c1 && i + EPV > c0) {
+      // the part's ends, off a vector's border
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) {
+        if (i + e < c0 || i + e >= c1) continue;
+        if constexpr (EB == 4) {
+          raw[v][e] = reinterpret_cast<const uint32_t*>(xr)[i + e];
+        } else {
+          const uint32_t h = reinterpret_cast<const uint16_t*>(xr)[i + e];
+          raw[v][e / 2] = e & 1 ? (raw[v][e / 2] & 0xffffu) | h << 16 : (raw[v][e / 2] & 0xffff0000u) | h;
+        }
+      }
+    }
+  }
+  auto value = [&](int v, int e) -> float {
+    if constexpr (EB == 4) return __uint_as_float(raw[v][e]);
+    else if constexpr (DT == RP_OUT_F16) return f16_to_f32(e & 1 ? raw[v][e / 2] >> 16 : raw[v][e / 2] & 0xffffu);
+    else return __uint_as_float(e & 1 ? raw[v][e / 2] & 0xffff0000u : raw[v][e / 2] << 16);
+  };
+
+  float mine = -__builtin_inff();
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) mine = nmax(mine, value(v, e));
+  float gm = mine;
+#pragma unroll
+  for (int o = 1; o < GROUP; o *= 2) gm = nmax(gm, __shfl_xor(gm, o, kWave));
+  if (tid % GROUP == 0) group_max[tid / GROUP] = gm;
+  __syncthreads();
+  gm = group_max[lane];
+  float m = gm;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = nmax(m, __shfl_xor(m, o, kWave));
+  const bool odd = !(m < __builtin_inff());         // a NaN or +inf: no distribution
+  const float m0 = m == -__builtin_inff() ? 0.0f : m;
+
+  // the bound: the top-th largest group maximum, its low bits dropped
+  float bound = __builtin_inff();
+  if (a.top > 0) {
+    const uint32_t k = logit_key(gm);
+    uint32_t b = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t cand = b | 1u << bit;
+      if (__popcll(__ballot(k >= cand)) >= a.top) b = cand;
+    }
+    bound = key_logit(b < kKeyNegInf ? kKeyNegInf : b);
+  }
+
+  float s = 0.0f, u = 0.0f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    float s1 = 0.0f, u1 = 0.0f;                     // short sums, then theirs
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) {
+      const float t = fmaxf((value(v, e) - m0) * a.c, -200.0f);
+      const float p = __builtin_amdgcn_exp2f(t);
+      s1 += p;
+      u1 = __builtin_fmaf(p, t, u1);
+    }
+    s += s1;
+    u += u1;
+  }
+  if (mine >= bound && !odd) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) {
+        const int i = first + (tid + v * T) * EPV + e;
+        if (value(v, e) >= bound && i >= c0 && i < c1) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kCap) found[at] = full_key(value(v, e), i);
+        }
+      }
+  }
+#pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     s += __shfl_xor(s, o, kWave);
-    sz += __shfl_xor(sz, o, kWave);
+    u += __shfl_xor(u, o, kWave);
   }
   if (lane == 0) {
-    red[1][wave] = s;
-    red[2][wave] = sz;
+    wave_sum[0][wave] = s;
+    wave_sum[1][wave] = u;
   }
   __syncthreads();
-  s = sz = 0.0f;
-  for (int w = 0; w < kLWaves; ++w) {
-    s += red[1][w];
-    sz += red[2][w];
+  s = u = 0.0f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    s += wave_sum[0][w];
+    u += wave_sum[1][w];
   }
-  const bool none = s == 0.0f;
-  const float lg = logf(s);
-  if (threadIdx.x == 0) {
-    const int64_t t = a.tokens[row];
-    float lp = 0.0f;
-    if (t >= a.V) lp = __builtin_nanf("");
-    else if (t >= 0) lp = none ? -__builtin_inff() : logit<DT>(a.x, base + t) / a.temperature - m - lg;
-    a.logprobs[row] = lp;
-    if (a.entropy) a.entropy[row] = none ? 0.0f : lg - sz / s;
+  if (odd) s = u = __builtin_nanf("");
+  const Row r{m0, s, u, a.c};
+  if (tid == 0) {
+    if (a.parts == 1) write_row(a, r, row, token, xt);
+    else a.sums[row * a.parts + part] = f32x4{m0, s, u, 0.0f};
+  }
+  if (a.top == 0) return;
+  uint64_t* keys = a.keys + (row * a.parts + part) * a.top;
+  const int n = count;
+  if (!odd && n <= kCap) {
+    for (int i = tid; i < n; i += T) {
+      const uint64_t key = found[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += found[j] > key;
+      if (rank < a.top) {
+        if (a.parts == 1) write_top(a, r, row, rank, key);
+        else keys[rank] = key;
+      }
+    }
+    // a part shorter than `top` leaves the rest to the other parts
+    if (a.parts > 1)
+      for (int i = n + tid; i < a.top; i += T) keys[i] = 0;
+    return;
   }
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top; ++k) {
     uint64_t best = 0;
-    for (int i = threadIdx.x; i < a.V; i += kLThreads) {
-      const uint64_t key = ((uint64_t)logit_key(logit<DT>(a.x, base + i)) << 32) | (0xffffffffu - (uint32_t)i);
-      if (key < last && key > best) best = key;
-    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) {
+        const int i = first + (tid + v * T) * EPV + e;
+        const uint64_t key = i >= c0 && i < c1 ? full_key(value(v, e), i) : 0;
+        if (key < last && key > best) best = key;
+      }
+#pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
       const uint64_t other = __shfl_xor((unsigned long long)best, o, kWave);
       best = other > best ? other : best;
     }
     __syncthreads();
-    if (lane == 0) redk[wave] = best;
+    if (lane == 0) wave_best[wave] = best;
     __syncthreads();
-    for (int w = 0; w < kLWaves; ++w) best = redk[w] > best ? redk[w] : best;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) best = wave_best[w] > best ? wave_best[w] : best;
     last = best;
-    if (threadIdx.x == 0) {
-      const int64_t id = 0xffffffffu - (uint32_t)best;
-      a.top_ids[row * a.top + k] = id;
-      a.top_logprobs[row * a.top + k] =
-          none ? -__builtin_inff() : logit<DT>(a.x, base + id) / a.temperature - m - lg;
+    if (tid == 0) {
+      if (a.parts > 1) keys[k] = best;
+      else if (best) write_top(a, r, row, k, best);
     }
   }
+}
+
+// Merges a row's parts.
+template <int DT>
+__global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs a) {
+  __shared__ uint64_t keys[kMaxParts * RP_LOGPROB_MAX_TOP];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t token = a.tokens[row];
+  const float xt = tid == 0 ? token_logit<DT>(a, a.x + row * a.ld * (DT == RP_OUT_F32 ? 4 : 2), token) : 0.0f;
+  const int n = a.parts * a.top;
+  for (int i = tid; i < n; i += kJoinThreads) keys[i] = a.keys[row * n + i];
+  float m = -__builtin_inff(), s = 0.0f, u = 0.0f;
+  for (int i = 0; i < a.parts; ++i) {
+    const f32x4 p = a.sums[row * a.parts + i];
+    if (p[1] != 0.0f) m = nmax(m, p[0]);             // a part of nothing but -inf has no maximum
+  }
+  for (int i = 0; i < a.parts; ++i) {
+    const f32x4 p = a.sums[row * a.parts + i];
+    if (p[1] == 0.0f) continue;
+    const float t = fmaxf((p[0] - m) * a.c, -200.0f), f = __builtin_amdgcn_exp2f(t);
+    s += p[1] * f;
+    u += f * __builtin_fmaf(p[1], t, p[2]);
+  }
+  const Row r{m, s, u, a.c};
+  if (tid == 0) write_row(a, r, row, token, xt);
+  __syncthreads();
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const uint64_t key = keys[i];
+    if (key == 0) continue;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += keys[j] > key;
+    if (rank < a.top) write_top(a, r, row, rank, key);
+  }
+}
+
+// Threads, vectors a thread and logits a part, by the row's length: enough
+// threads to hold a row where 512 of 64 logits do, one wave a SIMD at least.
+struct LogprobPlan {
+  int threads, vectors, parts, chunk;
+};
+
+inline LogprobPlan logprob_plan(int64_t V, int dtype, bool aligned) {
+  const int epv = dtype == RP_OUT_F32 ? 4 : 8, per = 64 / epv;
+  const int64_t off = aligned ? 0 : epv;       // a part off the border needs a vector more
+  LogprobPlan p;
+  p.threads = V + off > 256 * 64 ? 512 : 256;
+  p.vectors = V + off > 256 * 32 ? per : V + off > 256 * 8 ? per / 2 : per / 8;
+  const int64_t most = (int64_t)p.threads * p.vectors * epv - off;
+  p.parts = (int)((V + most - 1) / most);
+  p.chunk = (int)(((V + p.parts - 1) / p.parts + epv - 1) / epv * epv);
+  p.parts = (int)((V + p.chunk - 1) / p.chunk);
+  return p;
+}
+
+inline size_t logprob_sums_bytes(int64_t N, int parts) {
+  return (size_t)((N * parts * 16 + 255) / 256 * 256);
+}
+
+template <int DT>
+void launch_logprob(const LogprobArgs& a, const LogprobPlan& p, int64_t N, hipStream_t st) {
+  constexpr int P = DT == RP_OUT_F32 ? 16 : 8;       // vectors of 64 logits
+  auto go = [&](auto t, auto nv) {
+    hipLaunchKernelGGL((logprob_kernel<DT, decltype(t)::value, decltype(nv)::value>),
+                       dim3((unsigned)(N * p.parts)), dim3(p.threads), 0, st, a);
+  };
+  using std::integral_constant;
+  if (p.threads == 512) go(integral_constant<int, 512>{}, integral_constant<int, P>{});
+  else if (p.vectors == P) go(integral_constant<int, 256>{}, integral_constant<int, P>{});
+  else if (p.vectors == P / 2) go(integral_constant<int, 256>{}, integral_constant<int, P / 2>{});
+  else go(integral_constant<int, 256>{}, integral_constant<int, P / 8>{});
+  if (p.parts > 1)
+    hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)N), dim3(kJoinThreads), 0, st, a);
 }
 
 }  // namespace
@@ -114,8 +357,10 @@ using namespace rp;
 
 extern "C" size_t rp_token_logprobs_workspace_bytes(int64_t N, int64_t V, int logits_dtype,
                                                     int top) {
-  (void)N; (void)V; (void)logits_dtype; (void)top;
-  return 0;
+  if (N <= 0 || V <= 0 || top < 0) return 0;
+  // the split of rows off 16 bytes, which may have a part more
+  const LogprobPlan p = logprob_plan(V, logits_dtype, false);
+  return p.parts == 1 ? 0 : logprob_sums_bytes(N, p.parts) + (size_t)(N * p.parts * top * 8);
 }
 
 extern "C" int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N, int64_t V,
@@ -144,18 +389,37 @@ extern "C" int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N
     rp_set_error("token_logprobs: temperature must be positive and finite");
     return RP_ERR_INVALID_ARGUMENT;
   }
-  if (N > 0x7fffffff || V > 0x7fffff00) {
+  const float c = (float)(1.4426950408889634 / (double)temperature);
+  if (!(c - c == 0.0f)) {
+    rp_set_error("token_logprobs: temperature too small");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  if (V > (1 << 21) || N > 0x7fffffff / kMaxParts) {
     rp_set_error("token_logprobs: too many rows or logits");
     return RP_ERR_UNSUPPORTED;
   }
-  (void)workspace; (void)workspace_bytes;
-  const LogprobArgs a{logits, ld, (int32_t)V, top, tokens, temperature, logprobs, entropy,
-                      top_logprobs, top_ids};
+  const int eb = logits_dtype == RP_OUT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % eb != 0) {
+    rp_set_error("token_logprobs: logits must be aligned to their type");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (N == 1 || ld * eb % 16 == 0);
+  const LogprobPlan p = logprob_plan(V, logits_dtype, aligned);
+  const size_t sums = logprob_sums_bytes(N, p.parts);
+  const size_t want = p.parts == 1 ? 0 : sums + (size_t)(N * p.parts * top * 8);
+  if (want > 0 && (!workspace || workspace_bytes < want ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) {
+    rp_set_error("token_logprobs: workspace of %zu bytes, 256-byte aligned, needed", want);
+    return RP_ERR_WORKSPACE;
+  }
+  char* ws = static_cast<char*>(workspace);
+  const LogprobArgs a{static_cast<const char*>(logits), ld, (int32_t)V, top, p.parts, p.chunk, c,
+                      tokens, logprobs, entropy, top_logprobs, top_ids,
+                      reinterpret_cast<f32x4*>(ws), reinterpret_cast<uint64_t*>(ws + (want ? sums : 0))};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 g((unsigned)N), t(kLThreads);
-  if (logits_dtype == RP_OUT_F32) hipLaunchKernelGGL(logprob_kernel<RP_OUT_F32>, g, t, 0, st, a);
-  else if (logits_dtype == RP_OUT_F16) hipLaunchKernelGGL(logprob_kernel<RP_OUT_F16>, g, t, 0, st, a);
-  else hipLaunchKernelGGL(logprob_kernel<RP_OUT_BF16>, g, t, 0, st, a);
+  if (logits_dtype == RP_OUT_F32) launch_logprob<RP_OUT_F32>(a, p, N, st);
+  else if (logits_dtype == RP_OUT_F16) launch_logprob<RP_OUT_F16>(a, p, N, st);
+  else launch_logprob<RP_OUT_BF16>(a, p, N, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     rp_set_error("token_logprobs: launch failed: %s", hipGetErrorString(e));

@@ -141,8 +141,12 @@ def test_rows_without_a_distribution(gpu, V) -> None:
     for i in (1, 2):
         assert r.logprobs[i].isnan() and r.entropy[i].isnan() and r.top_logprobs[i].isnan().all()
     assert int(r.top_ids[1, 0]) == V - 1 and int(r.top_ids[2, 0]) == 3
+    # row 3 alone lies at another offset from a 16-byte border, so its sums run
+    # in another order: both sides are within check()'s bound of 64 bits, |x| < 12
     want = ops.token_logprobs(x[3:].to(gpu), tokens[3:].to(gpu), top=3)
-    assert torch.equal(r.logprobs[3:], want.logprobs)
+    tol = 2 * (6 * 12 + 4) * U + (min(V, 4096) + 16) * U + 2 * U * 24
+    assert float(x[3].abs().max()) < 12
+    assert abs(float(r.logprobs[3] - want.logprobs[0])) <= 2 * tol
     assert torch.equal(r.top_ids[3:], want.top_ids)
 
 
