@@ -3,10 +3,10 @@
 // The floor is one read of the logits, and 5 TB/s of 16-bit logits leave the
 // VALU about 15 lane operations each, so a row is read once, into registers,
 // and everything is computed from there:
-//   M = max x,  t = (x - M) c  (c = log2(e) / temperature),
+//   M = max x,  t = x c - M c  (c = log2(e) / temperature),
 //   s = sum 2^t,  u = sum 2^t t,
 //   log p(x) = ln 2 (t - log2 s),  entropy = ln 2 (log2 s - u / s).
-// Subtracting first keeps logits far from zero exact; t below -200 (2^t = 0)
+// t is one fma, so logits far from zero lose nothing; t below -200 (2^t = 0)
 // is held there, so a masked logit adds 0 and not 0 * inf.
 //
 // The best `top` logits cost no pass of their own.  The threads' maxima,
@@ -29,9 +29,9 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxThreads = 512;
-constexpr int kCap = 1024;                     // keys collected per workgroup
-constexpr int kMaxParts = 68;
-constexpr int kJoinThreads = 64;
+constexpr int kHits = 128;                     // vectors collected per workgroup
+constexpr int kMaxParts = 64;                  // of 2^21 logits
+constexpr int kJoinRows = 4, kJoinThreads = kJoinRows * kWave;
 constexpr double kLn2 = 0.693147180559945309417;
 
 struct LogprobArgs {
@@ -70,13 +70,21 @@ __device__ __forceinline__ float logit_at(const char* row, int64_t i) {
   else return in_to_f32<DT == RP_OUT_F16 ? kInF16 : kInBf16>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
-// What one (M, s, u) says of a row: written for its token, entropy and best.
+// Whether M c is far from fp32's range: then t is one fma about B = fp32(M c),
+// an exact base like any other; a row of lowest values takes (x - M) c.
+__device__ __forceinline__ bool near(float m, float c) { return fabsf(m * c) < 0x1p100f; }
+
+// What one (M, s, u) says of a row: its log probabilities and entropy.
 struct Row {
-  float m, s, u, c;
+  double base;
+  float s, u, c;
+  __device__ __forceinline__ Row(float m, float s_, float u_, float c_) : s(s_), u(u_), c(c_) {
+    base = near(m, c) ? (double)(m * c) : (double)m * (double)c;
+  }
   __device__ __forceinline__ float logprob(float x) const {
     if (s == 0.0f) return -__builtin_inff();
     // in 64 bits: a lowest value's log probability is finite
-    return (float)((((double)x - (double)m) * (double)c - (double)__builtin_amdgcn_logf(s)) * kLn2);
+    return (float)(((double)x * (double)c - base - (double)__builtin_amdgcn_logf(s)) * kLn2);
   }
   __device__ __forceinline__ float entropy() const {
     return s == 0.0f ? 0.0f : (float)(((double)__builtin_amdgcn_logf(s) - (double)u / (double)s) * kLn2);
@@ -103,70 +111,132 @@ __device__ __forceinline__ float nmax(float a, float b) {
   return __builtin_elementwise_maximum(a, b);
 }
 
-// One part of one row.  T threads, NV 16-byte vectors each.
+__device__ __forceinline__ uint32_t pk_max_i16(uint32_t a, uint32_t b) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(i16x2, a),
+                                                                __builtin_bit_cast(i16x2, b)));
+}
+// The larger of two 16-bit logits as signed integers, as a float.
+template <int DT>
+__device__ __forceinline__ float half_max(uint32_t w) {
+  const int lo = (int16_t)(w & 0xffffu), hi = (int)w >> 16;
+  const uint32_t x = (uint32_t)(lo > hi ? lo : hi) & 0xffffu;
+  return DT == RP_OUT_F16 ? f16_to_f32(x) : bf16_to_f32(x);
+}
+// 16-bit logits whose t may leave fp32's range: -2^100 and below, fp16's -inf
+template <int DT>
+constexpr uint32_t kLow16 = DT == RP_OUT_F16 ? 0xfc00u : 0xf180u;
+
+// One part of one row.  T threads, NV 16-byte vectors each, and a logit more
+// for what lies before the part's first 16-byte border and behind its last.
 template <int DT, int T, int NV>
 __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   constexpr int EB = DT == RP_OUT_F32 ? 4 : 2, EPV = 16 / EB, WAVES = T / kWave;
   constexpr int GROUP = T / kWave;                  // threads per group: 64 groups
+  constexpr bool PACKED = EB == 2;
   __shared__ float group_max[kWave];
   __shared__ float wave_sum[2][WAVES];
-  __shared__ uint64_t found[kCap];
+  __shared__ u32x4 hit[kHits];                      // vectors that reach the bound
+  __shared__ int32_t hit_at[kHits];                 // their first logits
+  __shared__ uint64_t found[kHits * EPV + 2 * EPV];
   __shared__ uint64_t wave_best[WAVES];
-  __shared__ int count;
+  __shared__ int hits, count;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
   const char* xr = a.x + row * a.ld * EB;
   const int c0 = part * a.chunk, c1 = min(a.V, c0 + a.chunk);
-  // vector v of the part: elements first + v * EPV + 0..EPV-1, 16-byte aligned
-  const int first = c0 - (int)((reinterpret_cast<uintptr_t>(xr + (int64_t)c0 * EB) & 15) / EB);
-  const int64_t token = a.tokens[row];
-  const float xt = tid == 0 && a.parts == 1 ? token_logit<DT>(a, xr, token) : 0.0f;
-  if (tid == 0) count = 0;
+  const int skew = (int)((reinterpret_cast<uintptr_t>(xr + (int64_t)c0 * EB) & 15) / EB);
+  const int a0 = min(c1, c0 + (skew ? EPV - skew : 0));     // the vectors' logits: [a0, a1)
+  const int a1 = a0 + (c1 - a0) / EPV * EPV;
+  if (tid == 0) hits = count = 0;
 
+  const u32x4* src = reinterpret_cast<const u32x4*>(xr + (int64_t)a0 * EB);
+  const int nvec = (a1 - a0) / EPV;
   constexpr uint32_t kFill = DT == RP_OUT_F32 ? 0xff800000u : DT == RP_OUT_F16 ? 0xfc00fc00u : 0xff80ff80u;
   u32x4 raw[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int i = first + (tid + v * T) * EPV;
     raw[v] = u32x4{kFill, kFill, kFill, kFill};
-    if (i >= c0 && i + EPV <= c1) {
-      raw[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(xr + (int64_t)i * EB));
-    } else if (i < c1 && i + EPV > c0) {
-      // the part's ends, off a vector's border
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) {
-        if (i + e < c0 || i + e >= c1) continue;
-        if constexpr (EB == 4) {
-          raw[v][e] = reinterpret_cast<const uint32_t*>(xr)[i + e];
-        } else {
-          const uint32_t h = reinterpret_cast<const uint16_t*>(xr)[i + e];
-          raw[v][e / 2] = e & 1 ? (raw[v][e / 2] & 0xffffu) | h << 16 : (raw[v][e / 2] & 0xffff0000u) | h;
-        }
-      }
-    }
+    if (tid + v * T < nvec) raw[v] = __builtin_nontemporal_load(src + tid + v * T);
   }
+  // threads 0 .. EPV-1: the part's head, EPV .. 2 EPV-1: its tail
+  const int edge = tid < EPV ? c0 + tid : a1 + tid - EPV;
+  const bool has_edge = tid < EPV ? edge < a0 : tid < 2 * EPV && edge < c1;
+  const float extra = has_edge ? logit_at<DT>(xr, edge) : -__builtin_inff();
+  const int64_t token = a.tokens[row];
+  const float xt = tid == 0 && a.parts == 1 ? token_logit<DT>(a, xr, token) : 0.0f;
+
   auto value = [&](int v, int e) -> float {
     if constexpr (EB == 4) return __uint_as_float(raw[v][e]);
     else if constexpr (DT == RP_OUT_F16) return f16_to_f32(e & 1 ? raw[v][e / 2] >> 16 : raw[v][e / 2] & 0xffffu);
     else return __uint_as_float(e & 1 ? raw[v][e / 2] & 0xffff0000u : raw[v][e / 2] << 16);
   };
+  // The logits are unpacked anew in each phase: kept unpacked they would take
+  // the registers of another workgroup, whose loads hide this one's arithmetic.
+  auto forget = [&](int v) { asm volatile("" : "+v"(raw[v])); };
+  auto phase = [&]() {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) forget(v);
+  };
 
-  float mine = -__builtin_inff();
+  // Maxima of each vector and of the thread.  Of 16-bit logits, two at a time
+  // as signed integers: right where any is at or above 0, and else some
+  // logit of the thread (the lowest), which shows as a negative part maximum
+  // and sends the part through the exact loop below.  As unsigned integers
+  // the largest is the most negative logit (or a NaN of that sign).
+  uint32_t vec16[NV], low16 = 0;
+  float vec_max[NV], mine = -__builtin_inff();
+  if constexpr (PACKED) {
+    uint32_t top16 = kFill;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      vec16[v] = pk_max_i16(pk_max_i16(raw[v][0], raw[v][1]), pk_max_i16(raw[v][2], raw[v][3]));
+      top16 = v == 0 ? vec16[0] : pk_max_i16(top16, vec16[v]);
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) mine = nmax(mine, value(v, e));
-  float gm = mine;
+      for (int i = 0; i < 4; ++i) low16 = pk_max_u16(low16, raw[v][i]);
+    }
+    mine = half_max<DT>(top16);
+    low16 = umax32(low16 & 0xffffu, low16 >> 16);
+  } else {
 #pragma unroll
-  for (int o = 1; o < GROUP; o *= 2) gm = nmax(gm, __shfl_xor(gm, o, kWave));
-  if (tid % GROUP == 0) group_max[tid / GROUP] = gm;
-  __syncthreads();
-  gm = group_max[lane];
-  float m = gm;
+    for (int v = 0; v < NV; ++v) {
+      vec_max[v] = value(v, 0);
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) m = nmax(m, __shfl_xor(m, o, kWave));
-  const bool odd = !(m < __builtin_inff());         // a NaN or +inf: no distribution
+      for (int e = 1; e < EPV; ++e) vec_max[v] = nmax(vec_max[v], value(v, e));
+      mine = nmax(mine, vec_max[v]);
+    }
+  }
+  mine = nmax(mine, extra);
+  float gm, m;
+  auto exchange = [&]() {
+    gm = mine;
+#pragma unroll
+    for (int o = 1; o < GROUP; o *= 2) gm = nmax(gm, __shfl_xor(gm, o, kWave));
+    if (tid % GROUP == 0) group_max[tid / GROUP] = gm;
+    __syncthreads();
+    gm = group_max[lane];
+    m = gm;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = nmax(m, __shfl_xor(m, o, kWave));
+  };
+  exchange();
+  phase();
+  if constexpr (PACKED) {
+    if (m < 0.0f) {                                 // the same in every thread
+      __syncthreads();
+      mine = extra;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        forget(v);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) mine = nmax(mine, value(v, e));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      exchange();
+    }
+    phase();
+  }
   const float m0 = m == -__builtin_inff() ? 0.0f : m;
 
   // the bound: the top-th largest group maximum, its low bits dropped
@@ -181,32 +251,57 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
     }
     bound = key_logit(b < kKeyNegInf ? kKeyNegInf : b);
   }
+  if (mine >= bound) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if constexpr (PACKED) {
+        if (bound >= 0.0f && half_max<DT>(vec16[v]) < bound) continue;
+      } else {
+        if (vec_max[v] < bound) continue;
+      }
+      if (tid + v * T >= nvec) continue;             // the fill reaches a bound of -inf
+      const int at = atomicAdd(&hits, 1);
+      if (at < kHits) {
+        hit[at] = raw[v];
+        hit_at[at] = a0 + (tid + v * T) * EPV;
+      }
+    }
+    if (has_edge && extra >= bound) found[atomicAdd(&count, 1)] = full_key(extra, edge);
+  }
+  phase();
 
   float s = 0.0f, u = 0.0f;
+  auto weigh = [&](auto power) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    float s1 = 0.0f, u1 = 0.0f;                     // short sums, then theirs
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      const float t = fmaxf((value(v, e) - m0) * a.c, -200.0f);
-      const float p = __builtin_amdgcn_exp2f(t);
-      s1 += p;
-      u1 = __builtin_fmaf(p, t, u1);
-    }
-    s += s1;
-    u += u1;
-  }
-  if (mine >= bound && !odd) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      forget(v);                                      // or the branches' common unpacking moves up
+      float s1 = 0.0f, u1 = 0.0f;                     // short sums, then theirs
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
-        const int i = first + (tid + v * T) * EPV + e;
-        if (value(v, e) >= bound && i >= c0 && i < c1) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kCap) found[at] = full_key(value(v, e), i);
-        }
+        const float t = power(value(v, e));
+        const float p = __builtin_amdgcn_exp2f(t);
+        s1 += p;
+        u1 = __builtin_fmaf(p, t, u1);
       }
+      s += s1;
+      u += u1;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const float base = m0 * a.c;
+  const bool fma = near(m0, a.c);
+  if (!fma) {
+    weigh([&](float x) { return nmax((x - m0) * a.c, -200.0f); });
+  } else if (!PACKED || __any(low16 >= kLow16<DT>)) {
+    weigh([&](float x) { return nmax(__builtin_fmaf(x, a.c, -base), -200.0f); });
+  } else {
+    weigh([&](float x) { return __builtin_fmaf(x, a.c, -base); });
+  }
+  if (wave == 0) {                                    // the edges are in its first 16 lanes
+    const float t = nmax(fma ? __builtin_fmaf(extra, a.c, -base) : (extra - m0) * a.c, -200.0f);
+    const float p = __builtin_amdgcn_exp2f(t);
+    s += p;
+    u = __builtin_fmaf(p, t, u);
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
@@ -224,19 +319,28 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
     s += wave_sum[0][w];
     u += wave_sum[1][w];
   }
-  if (odd) s = u = __builtin_nanf("");
-  const Row r{m0, s, u, a.c};
+  const bool odd = s != s;                            // a NaN or +inf: no distribution
+  const Row r(m0, s, u, a.c);
   if (tid == 0) {
     if (a.parts == 1) write_row(a, r, row, token, xt);
     else a.sums[row * a.parts + part] = f32x4{m0, s, u, 0.0f};
   }
   if (a.top == 0) return;
   uint64_t* keys = a.keys + (row * a.parts + part) * a.top;
-  const int n = count;
-  if (!odd && n <= kCap) {
+  if (!odd && hits <= kHits) {
+    for (int i = tid; i < hits * EPV; i += T) {
+      const int v = i / EPV, e = i % EPV;
+      float x;
+      if constexpr (EB == 4) x = reinterpret_cast<const float*>(hit)[i];
+      else x = in_to_f32<DT == RP_OUT_F16 ? kInF16 : kInBf16>(reinterpret_cast<const uint16_t*>(hit)[i]);
+      if (x >= bound) found[atomicAdd(&count, 1)] = full_key(x, hit_at[v] + e);
+    }
+    __syncthreads();
+    const int n = count;
     for (int i = tid; i < n; i += T) {
       const uint64_t key = found[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) rank += found[j] > key;
       if (rank < a.top) {
         if (a.parts == 1) write_top(a, r, row, rank, key);
@@ -251,14 +355,10 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top; ++k) {
     uint64_t best = 0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) {
-        const int i = first + (tid + v * T) * EPV + e;
-        const uint64_t key = i >= c0 && i < c1 ? full_key(value(v, e), i) : 0;
-        if (key < last && key > best) best = key;
-      }
+    for (int i = c0 + tid; i < c1; i += T) {        // from memory: this path is rare
+      const uint64_t key = full_key(logit_at<DT>(xr, i), i);
+      if (key < last && key > best) best = key;
+    }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
       const uint64_t other = __shfl_xor((unsigned long long)best, o, kWave);
@@ -277,38 +377,57 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   }
 }
 
-// Merges a row's parts.
+// Merges the parts of a row, a wave each.
 template <int DT>
-__global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs a) {
-  __shared__ uint64_t keys[kMaxParts * RP_LOGPROB_MAX_TOP];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int64_t token = a.tokens[row];
-  const float xt = tid == 0 ? token_logit<DT>(a, a.x + row * a.ld * (DT == RP_OUT_F32 ? 4 : 2), token) : 0.0f;
+__global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs a, int64_t rows) {
+  extern __shared__ uint64_t join_keys[];          // kJoinRows * parts * top
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t row = (int64_t)blockIdx.x * kJoinRows + wave;
   const int n = a.parts * a.top;
-  for (int i = tid; i < n; i += kJoinThreads) keys[i] = a.keys[row * n + i];
-  float m = -__builtin_inff(), s = 0.0f, u = 0.0f;
-  for (int i = 0; i < a.parts; ++i) {
-    const f32x4 p = a.sums[row * a.parts + i];
-    if (p[1] != 0.0f) m = nmax(m, p[0]);             // a part of nothing but -inf has no maximum
-  }
-  for (int i = 0; i < a.parts; ++i) {
-    const f32x4 p = a.sums[row * a.parts + i];
-    if (p[1] == 0.0f) continue;
-    const float t = fmaxf((p[0] - m) * a.c, -200.0f), f = __builtin_amdgcn_exp2f(t);
-    s += p[1] * f;
-    u += f * __builtin_fmaf(p[1], t, p[2]);
-  }
-  const Row r{m, s, u, a.c};
-  if (tid == 0) write_row(a, r, row, token, xt);
+  uint64_t* keys = join_keys + wave * n;
+  if (row < rows)
+    for (int i = lane; i < n; i += kWave) keys[i] = a.keys[row * n + i];
   __syncthreads();
-  for (int i = tid; i < n; i += kJoinThreads) {
+  if (row >= rows) return;
+  const int64_t token = a.tokens[row];
+  const float xt = lane == 0 ? token_logit<DT>(a, a.x + row * a.ld * (DT == RP_OUT_F32 ? 4 : 2), token) : 0.0f;
+  // a part a lane; one of nothing but -inf has no maximum
+  static_assert(kMaxParts <= kWave, "a row's parts fit a wave");
+  const f32x4 p = lane < a.parts ? a.sums[row * a.parts + lane] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const bool some = p[1] != 0.0f;
+  float m = some ? p[0] : -__builtin_inff();
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = nmax(m, __shfl_xor(m, o, kWave));
+  const double base = Row(m, 0.0f, 0.0f, a.c).base;
+  float s = 0.0f, u = 0.0f;
+  if (some) {
+    const float t = nmax((float)(Row(p[0], 0.0f, 0.0f, a.c).base - base), -200.0f);
+    const float f = __builtin_amdgcn_exp2f(t);
+    s = p[1] * f;
+    u = f * __builtin_fmaf(p[1], t, p[2]);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    s += __shfl_xor(s, o, kWave);
+    u += __shfl_xor(u, o, kWave);
+  }
+  const Row r(m, s, u, a.c);
+  for (int i = lane; i < n; i += kWave) {
     const uint64_t key = keys[i];
     if (key == 0) continue;
+    // a part's keys fall: how many of each are above this one, by bisection
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += keys[j] > key;
+    for (int q = 0; q < a.parts && rank < a.top; ++q) {
+      const uint64_t* part = keys + q * a.top;
+      int above = 0;
+#pragma unroll
+      for (int step = RP_LOGPROB_MAX_TOP; step >= 1; step /= 2)
+        if (above + step <= a.top && part[above + step - 1] > key) above += step;
+      rank += above;
+    }
     if (rank < a.top) write_top(a, r, row, rank, key);
   }
+  if (lane == 0) write_row(a, r, row, token, xt);
 }
 
 // Threads, vectors a thread and logits a part, by the row's length: enough
@@ -317,13 +436,12 @@ struct LogprobPlan {
   int threads, vectors, parts, chunk;
 };
 
-inline LogprobPlan logprob_plan(int64_t V, int dtype, bool aligned) {
+inline LogprobPlan logprob_plan(int64_t V, int dtype) {
   const int epv = dtype == RP_OUT_F32 ? 4 : 8, per = 64 / epv;
-  const int64_t off = aligned ? 0 : epv;       // a part off the border needs a vector more
   LogprobPlan p;
-  p.threads = V + off > 256 * 64 ? 512 : 256;
-  p.vectors = V + off > 256 * 32 ? per : V + off > 256 * 8 ? per / 2 : per / 8;
-  const int64_t most = (int64_t)p.threads * p.vectors * epv - off;
+  p.threads = V > 256 * 64 ? 512 : 256;
+  p.vectors = V > 256 * 32 ? per : V > 256 * 8 ? per / 2 : per / 8;
+  const int64_t most = (int64_t)p.threads * p.vectors * epv;
   p.parts = (int)((V + most - 1) / most);
   p.chunk = (int)(((V + p.parts - 1) / p.parts + epv - 1) / epv * epv);
   p.parts = (int)((V + p.chunk - 1) / p.chunk);
@@ -347,7 +465,8 @@ void launch_logprob(const LogprobArgs& a, const LogprobPlan& p, int64_t N, hipSt
   else if (p.vectors == P / 2) go(integral_constant<int, 256>{}, integral_constant<int, P / 2>{});
   else go(integral_constant<int, 256>{}, integral_constant<int, P / 8>{});
   if (p.parts > 1)
-    hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)N), dim3(kJoinThreads), 0, st, a);
+    hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)((N + kJoinRows - 1) / kJoinRows)),
+                       dim3(kJoinThreads), (size_t)(kJoinRows * p.parts * a.top * 8), st, a, N);
 }
 
 }  // namespace
@@ -358,8 +477,7 @@ using namespace rp;
 extern "C" size_t rp_token_logprobs_workspace_bytes(int64_t N, int64_t V, int logits_dtype,
                                                     int top) {
   if (N <= 0 || V <= 0 || top < 0) return 0;
-  // the split of rows off 16 bytes, which may have a part more
-  const LogprobPlan p = logprob_plan(V, logits_dtype, false);
+  const LogprobPlan p = logprob_plan(V, logits_dtype);
   return p.parts == 1 ? 0 : logprob_sums_bytes(N, p.parts) + (size_t)(N * p.parts * top * 8);
 }
 
@@ -403,8 +521,7 @@ extern "C" int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N
     rp_set_error("token_logprobs: logits must be aligned to their type");
     return RP_ERR_INVALID_ARGUMENT;
   }
-  const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (N == 1 || ld * eb % 16 == 0);
-  const LogprobPlan p = logprob_plan(V, logits_dtype, aligned);
+  const LogprobPlan p = logprob_plan(V, logits_dtype);
   const size_t sums = logprob_sums_bytes(N, p.parts);
   const size_t want = p.parts == 1 ? 0 : sums + (size_t)(N * p.parts * top * 8);
   if (want > 0 && (!workspace || workspace_bytes < want ||
