@@ -42,6 +42,7 @@ constexpr int kDThreads = kDWaves * kWave;
 constexpr int kStep = 32;                       // keys per step of a wave
 constexpr int kMaxChunk = kDWaves * 1024;       // a wave holds 64 tiles' pages in one register
 constexpr int kJThreads = 256;
+constexpr int kMaxSplits = 1024;
 constexpr float kSlack = 8.0f;                  // powers of two
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.693147180559945309f;
@@ -471,57 +472,100 @@ __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedVi
   }
 }
 
-// The base and sum of a head's parts together.
-__device__ __forceinline__ float2 join_parts(const float2* ml, int parts) {
+// Joins the parts of a (sequence, query head), or adds the key weights.
+//
+// Blocks with blockIdx.x < heads_x join: the parts' bases and sums are read a
+// part a thread and turned into factors, then D / 4 threads take a part's
+// columns and the block 1024 / D parts at a time.  The others add the key
+// weights of up to 1024 keys of a kv head from the stored scores.
+struct JoinShared {
+  float factor[kMaxSplits];
+  float red[2][kJThreads / kWave];
+};
+
+// The parts' joint base, and with `factors` what each part's sums are
+// multiplied by; the joint sum.  Called by the whole block.
+__device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinShared& sh,
+                                             bool factors) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  constexpr int PER = kMaxSplits / kJThreads;
+  float2 p[PER];
   float base = neg_inf();
-  for (int i = 0; i < parts; ++i) base = fmaxf(base, ml[i].x);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = threadIdx.x + i * kJThreads;
+    p[i] = at < parts ? ml[at] : float2{neg_inf(), 0.0f};
+    base = fmaxf(base, p[i].x);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) base = fmaxf(base, __shfl_xor(base, o, kWave));
+  if (lane == 0) sh.red[0][wave] = base;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJThreads / kWave; ++w) base = fmaxf(base, sh.red[0][w]);
   const float b0 = base == neg_inf() ? 0.0f : base;
   float sum = 0.0f;
-  for (int i = 0; i < parts; ++i) sum += ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - b0);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = threadIdx.x + i * kJThreads;
+    const float f = __builtin_amdgcn_exp2f(p[i].x - b0);
+    if (factors && at < parts) sh.factor[at] = f;
+    sum += p[i].y * f;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+  if (lane == 0) sh.red[1][wave] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJThreads / kWave; ++w) sum += sh.red[1][w];
   return float2{b0, sum};
 }
 
-// Joins the parts of each (sequence, query head), D threads' worth of columns
-// at a time (blocks with blockIdx.x < H), and adds the key weights from the
-// stored scores (the others, a block per 1024 keys of a kv head).
 template <int QT, int D>
 __global__ __launch_bounds__(kJThreads) void join_kernel(DecodeArgs a, PagedView c, int heads_x) {
+  __shared__ JoinShared sh;
   const int b = blockIdx.y;
   const int n = (int)paged_len(c, a.lens[b]);
-  const int parts = max(1, min(a.splits, (n + a.chunk - 1) / a.chunk));
+  const int parts = (int)max((int64_t)1, min((int64_t)a.splits, ((int64_t)n + a.chunk - 1) / a.chunk));
   if ((int)blockIdx.x < heads_x) {
-    constexpr int COLS = D < kJThreads ? D : kJThreads, GR = kJThreads / COLS;
-    __shared__ float part_sum[GR][COLS];
+    constexpr int COLS = D / 4, GR = kJThreads / COLS;
+    __shared__ f32x4 group_sum[GR][COLS];
     const int h = blockIdx.x;
     const int64_t bh = (int64_t)b * a.H + h;
-    const float2* ml = a.ml + bh * a.splits;
-    const float2 t = join_parts(ml, parts);
+    const float2 t = join_parts(a.ml + bh * a.splits, parts, sh, true);
     const int d = threadIdx.x % COLS, gr = threadIdx.x / COLS;
-    float x = 0.0f;
-    for (int i = gr; i < parts; i += GR)
-      x += a.part[(bh * a.splits + i) * D + d] * __builtin_amdgcn_exp2f(ml[i].x - t.x);
-    part_sum[gr][d] = x;
+    const f32x4* part = reinterpret_cast<const f32x4*>(a.part + bh * a.splits * D) + d;
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = gr; i < parts; i += GR) x += part[(int64_t)i * COLS] * sh.factor[i];
+    group_sum[gr][d] = x;
     __syncthreads();
     if (gr != 0) return;
-    for (int i = 1; i < GR; ++i) x += part_sum[i][d];
-    x = t.y == 0.0f ? 0.0f : x / t.y;
-    a.out[b * a.osb + h * a.osh + d] = QT == kInF16
-        ? __builtin_bit_cast(uint16_t, (_Float16)x) : (uint16_t)f32_to_bf16_bits(x);
+#pragma unroll
+    for (int i = 1; i < GR; ++i) x += group_sum[i][d];
+    uint16_t* out = a.out + b * a.osb + h * a.osh + 4 * d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = t.y == 0.0f ? 0.0f : x[e] / t.y;
+      out[e] = QT == kInF16 ? __builtin_bit_cast(uint16_t, (_Float16)y) : (uint16_t)f32_to_bf16_bits(y);
+    }
     if (threadIdx.x == 0 && a.lse)
       a.lse[bh] = t.y == 0.0f ? neg_inf() : (t.x + __builtin_amdgcn_logf(t.y)) * kLn2;
     return;
   }
   const int blocks = (gridDim.x - heads_x) / c.heads;
-  const int kv = (blockIdx.x - heads_x) / blocks, part = (blockIdx.x - heads_x) % blocks;
-  const int j = (part * kJThreads + threadIdx.x) * 4;
-  if (part * kJThreads * 4 >= n) return;
+  const int kv = (blockIdx.x - heads_x) / blocks, block = (blockIdx.x - heads_x) % blocks;
+  const int64_t j = ((int64_t)block * kJThreads + threadIdx.x) * 4;
+  if ((int64_t)block * kJThreads * 4 >= n) return;
   float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int i = 0; i < a.group; ++i) {
     const int64_t bh = (int64_t)b * a.H + kv * a.group + i;
-    const float2 t = join_parts(a.ml + bh * a.splits, parts);
-    if (j >= n || t.y == 0.0f) continue;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (j < n) s = *reinterpret_cast<const f32x4*>(a.scores + bh * a.score_ld + j);
+    const float2 t = join_parts(a.ml + bh * a.splits, parts, sh, false);
+    if (t.y == 0.0f) continue;                      // the same in every thread
     const float inv = 1.0f / t.y;
-    const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + bh * a.score_ld + j);
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(s[e] - t.x) * inv;
   }
@@ -543,9 +587,10 @@ inline Plan decode_plan(int64_t groups, int64_t keys) {
   int64_t splits = (kWant + groups - 1) / groups;
   const int64_t most = (keys + kUnit - 1) / kUnit;
   if (splits > most) splits = most;
+  if (splits > kMaxSplits) splits = kMaxSplits;
   int64_t chunk = ((keys + splits - 1) / splits + kUnit - 1) / kUnit * kUnit;
-  if (chunk > kMaxChunk) chunk = kMaxChunk;
-  splits = (keys + chunk - 1) / chunk;
+  if (chunk > kMaxChunk) chunk = kMaxChunk;        // a workgroup takes several chunks
+  splits = min(splits, (keys + chunk - 1) / chunk);
   return Plan{(int32_t)splits, (int32_t)chunk};
 }
 
