@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "librepercep_fp8.so"
@@ -88,6 +89,16 @@ class PagedCache(ctypes.Structure):
                 + [(n, _i64) for n in ("num_pages", "heads", "page_size", "head_dim",
                                        "stride_page", "stride_head", "stride_row",
                                        "table_stride", "max_pages", "dtype")])
+
+    @property
+    def _as_parameter_(self) -> object:
+        return ctypes.byref(self)
+
+
+#: The bytes of an ``rp_paged_cache``, its fields in order (a null pointer as
+#: 0): quicker than building the structure.
+pack_paged_cache = struct.Struct("5P10q").pack
+assert struct.calcsize("5P10q") == ctypes.sizeof(PagedCache)
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -180,7 +191,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.rp_fp8_softmax_rowwise_quantize.restype = _int
     L.rp_fp8_softmax_rowwise_quantize.argtypes = [_vp, _i64, _i64, _i64, _i64, _int, _f32, _vp,
                                                   _vp, _i64, _vp]
-    cache = ctypes.POINTER(PagedCache)
+    cache = _vp     # a PagedCache or pack_paged_cache's bytes
     L.rp_paged_kv_append.restype = _int
     L.rp_paged_kv_append.argtypes = [_vp, _vp, _int] + [_i64] * 8 + [cache, _vp, _vp, _vp]
     L.rp_paged_attn_workspace_bytes.restype = _sz

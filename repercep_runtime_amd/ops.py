@@ -1049,46 +1049,52 @@ def fp8_scaled_mm_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
 # has no counterpart of these.
 
 def _int32_vector(name: str, t: torch.Tensor, n: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a contiguous int32 ({n},) vector "
                          f"(got {t.dtype} {tuple(t.shape)})")
 
 
 def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, B: int,
-                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> C.PagedCache:
+                 k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> bytes:
     """The C descriptor of a cache, its tensors checked against each other."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"k_cache and v_cache must share one (pages, Hkv, page_size, D) shape "
                          f"(got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
-    P, Hkv, page, D = k_cache.shape
-    dt = _CACHE_DTYPES.get(k_cache.dtype)
-    if dt is None or v_cache.dtype != k_cache.dtype:
+    P, Hkv, page, D = shape
+    dtype = k_cache.dtype
+    dt = _CACHE_DTYPES.get(dtype)
+    if dt is None or v_cache.dtype != dtype:
         raise TypeError(f"k_cache and v_cache must both be bfloat16, float16 or float8_e4m3fn "
                         f"(got {k_cache.dtype}, {v_cache.dtype})")
     strides = k_cache.stride()
     if v_cache.stride() != strides or strides[3] != 1:
         raise ValueError("k_cache and v_cache must share their strides, with a unit stride on D")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B \
+    table = block_table.shape
+    if len(table) != 2 or table[0] != B or block_table.dtype != torch.int32 \
             or block_table.stride(1) != 1:
         raise ValueError(f"block_table must be int32 ({B}, max_pages) with contiguous rows "
                          f"(got {block_table.dtype} {tuple(block_table.shape)})")
-    ks = vs = None
+    dev = k_cache.get_device()
+    ks = vs = 0
     if dt == C.RP_CACHE_E4M3:
         if k_scale is None or v_scale is None:
             raise ValueError("an e4m3fn cache needs k_scale and v_scale")
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             if t.dtype != torch.float32 or t.shape != (P, Hkv, page) or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float32 ({P}, {Hkv}, {page})")
+        if dev < 0 or k_scale.get_device() != dev or v_scale.get_device() != dev:
+            _on_device_of(k_cache, k_cache=k_cache, k_scale=k_scale, v_scale=v_scale)
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
     elif k_scale is not None or v_scale is not None:
         raise ValueError("only an e4m3fn cache has scales")
-    _on_device_of(k_cache, v_cache=v_cache, block_table=block_table, k_scale=k_scale,
-                  v_scale=v_scale, k_cache=k_cache)
+    if dev < 0 or v_cache.get_device() != dev or block_table.get_device() != dev:
+        _on_device_of(k_cache, k_cache=k_cache, v_cache=v_cache, block_table=block_table)
     # a dimension of one has no stride of its own
-    return C.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, block_table.data_ptr(),
-                        P, Hkv, page, D, strides[0] if P > 1 else 0, strides[1] if Hkv > 1 else 0,
-                        strides[2] if page > 1 else D,
-                        block_table.stride(0) if B > 1 else 0, block_table.shape[1], dt)
+    return C.pack_paged_cache(
+        k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, block_table.data_ptr(), P, Hkv, page, D,
+        strides[0] if P > 1 else 0, strides[1] if Hkv > 1 else 0, strides[2] if page > 1 else D,
+        block_table.stride(0) if B > 1 else 0, table[1], dt)
 
 
 def _unit_stride(name: str, t: torch.Tensor) -> None:
@@ -1096,9 +1102,9 @@ def _unit_stride(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
-def _strides(t: torch.Tensor, dims: int) -> tuple[int, ...]:
+def _strides(t: torch.Tensor, dims: int) -> list[int]:
     """The first strides of ``t``, 0 for a dimension of one (whose stride means nothing)."""
-    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(dims))
+    return [st if n > 1 else 0 for st, n in zip(t.stride()[:dims], t.shape)]
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
@@ -1135,7 +1141,10 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     if lengths is not None:
         _int32_vector("lengths", lengths, B)
     cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
-    _on_device_of(k_cache, k=k, v=v, start=start, lengths=lengths)
+    dev = k_cache.get_device()
+    if k.get_device() != dev or v.get_device() != dev or start.get_device() != dev or \
+            (lengths is not None and lengths.get_device() != dev):
+        _on_device_of(k_cache, k=k, v=v, start=start, lengths=lengths)
     if B == 0 or S == 0:
         return
     C.check(C.lib().rp_paged_kv_append(
@@ -1196,19 +1205,24 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         _unit_stride("key_weights", key_weights)
         w_ptr, (wsb, wsh) = key_weights.data_ptr(), _strides(key_weights, 2)
     cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
-    _on_device_of(k_cache, q=q, seq_lens=seq_lens, key_weights=key_weights, out=out)
+    dev = k_cache.get_device()
+    if q.get_device() != dev or seq_lens.get_device() != dev or \
+            (key_weights is not None and key_weights.get_device() != dev) or \
+            (out is not None and out.get_device() != dev):
+        _on_device_of(k_cache, q=q, seq_lens=seq_lens, key_weights=key_weights, out=out)
     if out is None:
-        out = torch.empty((B, H, 1, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
     if B > 0:
         hint = max_seq_len if max_seq_len is not None else 0
         n = C.lib().rp_paged_attn_workspace_bytes(B, H, cache, hint, w_ptr is not None)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        C.check(C.lib().rp_paged_attn_decode(
+        ws = q.new_empty(n, dtype=torch.uint8) if n else None
+        rc = C.lib().rp_paged_attn_decode(
             q.data_ptr(), dt, B, H, *_strides(q, 2), cache, seq_lens.data_ptr(),
             1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(),
             *_strides(out, 2), lse.data_ptr() if return_lse else None, w_ptr, wsb, wsh, hint,
-            ws.data_ptr() if n else None, n, _stream(q)), "rp_paged_attn_decode")
+            ws.data_ptr() if n else None, n, _stream(q))
+        C.check(rc, "rp_paged_attn_decode")
     return (out, lse) if return_lse else out
 
 
@@ -1244,14 +1258,16 @@ def paged_kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: to
                          f"got {key_weights.dtype} {tuple(key_weights.shape)}")
     _unit_stride("key_weights", key_weights)
     cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
-    _on_device_of(k_cache, seq_lens=seq_lens, key_weights=key_weights)
+    dev = k_cache.get_device()
+    if seq_lens.get_device() != dev or key_weights.get_device() != dev:
+        _on_device_of(k_cache, seq_lens=seq_lens, key_weights=key_weights)
     new_lens = torch.empty_like(seq_lens)
-    kept = torch.empty(key_weights.shape, dtype=torch.float32, device=key_weights.device)
+    kept = torch.empty_like(key_weights, memory_format=torch.contiguous_format)
     if B == 0:
         return new_lens, kept
     budget = min(budget, slots)
     n = C.lib().rp_paged_evict_workspace_bytes(B, cache, budget)
-    ws = torch.empty(n, dtype=torch.uint8, device=k_cache.device)
+    ws = kept.new_empty(n, dtype=torch.uint8)
     C.check(C.lib().rp_paged_kv_evict(
         cache, seq_lens.data_ptr(), B, key_weights.data_ptr(), *_strides(key_weights, 2), budget,
         min(recent, budget), new_lens.data_ptr(), kept.data_ptr(), kept.shape[2], ws.data_ptr(), n,
@@ -1294,26 +1310,26 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError(f"temperature must be positive and finite (got {temperature})")
     _unit_stride("logits", logits)
-    _on_device_of(logits, tokens=tokens, logits=logits)
-    lead = logits.shape[:-1]
+    dev = logits.get_device()
+    if dev < 0 or tokens.get_device() != dev:
+        _on_device_of(logits, tokens=tokens, logits=logits)
+    lead = tokens.shape
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    t = tokens.reshape(-1)
-    if not t.is_contiguous():
-        t = t.contiguous()
+    t = tokens if tokens.is_contiguous() else tokens.contiguous()
     N = x.shape[0]
-    f32 = torch.empty((2 + top) * N, dtype=torch.float32, device=x.device)
-    ids = torch.empty((*lead, top), dtype=torch.int64, device=x.device) if top else None
+    logprobs = logits.new_empty(lead, dtype=torch.float32)
+    entropy = torch.empty_like(logprobs)
+    top_lp = logprobs.new_empty((*lead, top)) if top else None
+    ids = t.new_empty((*lead, top)) if top else None
     if N > 0:
-        ld = x.stride(0) if N > 1 else V
         n = C.lib().rp_token_logprobs_workspace_bytes(N, V, dt, top)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        base = f32.data_ptr()
-        C.check(C.lib().rp_token_logprobs(
-            x.data_ptr(), dt, N, V, ld, t.data_ptr(), temperature, top, base, base + 4 * N,
-            base + 8 * N if top else None, ids.data_ptr() if top else None,
-            ws.data_ptr() if n else None, n, _stream(x)), "rp_token_logprobs")
-    return TokenLogprobs(f32[:N].view(lead), f32[N:2 * N].view(lead),
-                         f32[2 * N:].view(*lead, top) if top else None, ids)
+        ws = logprobs.new_empty(n, dtype=torch.uint8) if n else None
+        rc = C.lib().rp_token_logprobs(
+            x.data_ptr(), dt, N, V, x.stride(0) if N > 1 else V, t.data_ptr(), temperature, top,
+            logprobs.data_ptr(), entropy.data_ptr(), top_lp.data_ptr() if top else None,
+            ids.data_ptr() if top else None, ws.data_ptr() if n else None, n, _stream(x))
+        C.check(rc, "rp_token_logprobs")
+    return TokenLogprobs(logprobs, entropy, top_lp, ids)
 
 
 def selftest_e4m3(x: torch.Tensor) -> torch.Tensor:
