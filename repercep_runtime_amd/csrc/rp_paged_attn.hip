@@ -581,10 +581,18 @@ struct Plan {
   int32_t splits, chunk;
 };
 
-inline Plan decode_plan(int64_t groups, int64_t keys) {
-  constexpr int64_t kWant = 1024;                  // workgroups
+// * Key weights need join_kernel anyway, so their calls split down to 1024
+//   workgroups, four a CU, which evens out ragged lengths (8 sequences of 1 to
+//   4100 keys: 22 us, 25.6 us at 512).
+// * Else a second launch is worth its 4 us where a workgroup's keys take
+//   longer than that: not up to 384 KB of them (640 keys of 128: 12.5 us a call
+//   unsplit, 16.9 in five parts), nor with two workgroups a CU already (16
+//   sequences x 32 heads: 17 us unsplit, 23 in two parts); 131071 keys in 8
+//   heads take 55 us on 512 workgroups, 58 on 1024, 64 on 2048.
+inline Plan decode_plan(int64_t groups, int64_t keys, int64_t key_bytes, bool weights) {
   constexpr int64_t kUnit = kDWaves * kStep;
-  int64_t splits = (kWant + groups - 1) / groups;
+  const int64_t want = weights ? 1024 : keys * key_bytes <= 384 << 10 ? 1 : 512;
+  int64_t splits = (want + groups - 1) / groups;
   const int64_t most = (keys + kUnit - 1) / kUnit;
   if (splits > most) splits = most;
   if (splits > kMaxSplits) splits = kMaxSplits;
@@ -605,7 +613,8 @@ inline Layout decode_layout(int64_t B, int64_t H, const rp_paged_cache* c, int64
   const int64_t cap = c->max_pages * c->page_size, group = H / c->heads;
   const int64_t keys = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
   Layout l;
-  l.plan = decode_plan(B * c->heads * ((group + 15) / 16), keys);
+  l.plan = decode_plan(B * c->heads * ((group + 15) / 16), keys,
+                       2 * c->head_dim * cache_elem_bytes(c->dtype), weights);
   auto up = [](int64_t x) { return (size_t)((x + 255) / 256 * 256); };
   const bool split = l.plan.splits > 1;
   // whole steps are written, the last one past the capacity
