@@ -483,10 +483,9 @@ struct JoinShared {
   float red[2][kJThreads / kWave];
 };
 
-// The parts' joint base, and with `factors` what each part's sums are
-// multiplied by; the joint sum.  Called by the whole block.
-__device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinShared& sh,
-                                             bool factors) {
+// The parts' joint base and sum, and in sh.factor what each part's sums are
+// multiplied by.  Called by the whole block.
+__device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinShared& sh) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   constexpr int PER = kMaxSplits / kJThreads;
   float2 p[PER];
@@ -509,7 +508,7 @@ __device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinSh
   for (int i = 0; i < PER; ++i) {
     const int at = threadIdx.x + i * kJThreads;
     const float f = __builtin_amdgcn_exp2f(p[i].x - b0);
-    if (factors && at < parts) sh.factor[at] = f;
+    if (at < parts) sh.factor[at] = f;
     sum += p[i].y * f;
   }
 #pragma unroll
@@ -519,6 +518,19 @@ __device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinSh
   sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < kJThreads / kWave; ++w) sum += sh.red[1][w];
+  return float2{b0, sum};
+}
+
+// The same by one wave: base and sum.
+__device__ __forceinline__ float2 wave_parts(const float2* ml, int parts, int lane) {
+  float base = neg_inf(), sum = 0.0f;
+  for (int i = lane; i < parts; i += kWave) base = fmaxf(base, ml[i].x);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) base = fmaxf(base, __shfl_xor(base, o, kWave));
+  const float b0 = base == neg_inf() ? 0.0f : base;
+  for (int i = lane; i < parts; i += kWave) sum += ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - b0);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, kWave);
   return float2{b0, sum};
 }
 
@@ -533,7 +545,7 @@ __global__ __launch_bounds__(kJThreads) void join_kernel(DecodeArgs a, PagedView
     __shared__ f32x4 group_sum[GR][COLS];
     const int h = blockIdx.x;
     const int64_t bh = (int64_t)b * a.H + h;
-    const float2 t = join_parts(a.ml + bh * a.splits, parts, sh, true);
+    const float2 t = join_parts(a.ml + bh * a.splits, parts, sh);
     const int d = threadIdx.x % COLS, gr = threadIdx.x / COLS;
     const f32x4* part = reinterpret_cast<const f32x4*>(a.part + bh * a.splits * D) + d;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -558,16 +570,30 @@ __global__ __launch_bounds__(kJThreads) void join_kernel(DecodeArgs a, PagedView
   const int kv = (blockIdx.x - heads_x) / blocks, block = (blockIdx.x - heads_x) % blocks;
   const int64_t j = ((int64_t)block * kJThreads + threadIdx.x) * 4;
   if ((int64_t)block * kJThreads * 4 >= n) return;
+  // sixteen heads at a time: a wave finds the base and sum of every fourth
+  // one, then every thread weighs its four keys under each
+  float2* stat = reinterpret_cast<float2*>(sh.factor);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t bh0 = (int64_t)b * a.H + kv * a.group;
   float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = 0; i < a.group; ++i) {
-    const int64_t bh = (int64_t)b * a.H + kv * a.group + i;
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (j < n) s = *reinterpret_cast<const f32x4*>(a.scores + bh * a.score_ld + j);
-    const float2 t = join_parts(a.ml + bh * a.splits, parts, sh, false);
-    if (t.y == 0.0f) continue;                      // the same in every thread
-    const float inv = 1.0f / t.y;
+  for (int i0 = 0; i0 < a.group; i0 += 16) {
+    const int heads = min(16, a.group - i0);
+    __syncthreads();
+    for (int i = wave; i < heads; i += kJThreads / kWave) {
+      const float2 t = wave_parts(a.ml + (bh0 + i0 + i) * a.splits, parts, lane);
+      if (lane == 0) stat[i] = float2{t.x, t.y == 0.0f ? 0.0f : 1.0f / t.y};
+    }
+    __syncthreads();
+    if (j < n) {
+      const float* s = a.scores + (bh0 + i0) * a.score_ld + j;
+#pragma unroll 4
+      for (int i = 0; i < heads; ++i) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(s + (int64_t)i * a.score_ld);
+        const float2 t = stat[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(s[e] - t.x) * inv;
+        for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(x[e] - t.x) * t.y;
+      }
+    }
   }
   float* to = a.weights + b * a.wsb + kv * a.wsh + j;
 #pragma unroll
