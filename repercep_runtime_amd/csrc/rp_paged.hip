@@ -85,6 +85,8 @@ void launch_append(const AppendArgs& a, const PagedView& c, int64_t B, int64_t D
 // ------------------------------------------------------------------ eviction
 
 constexpr int kSelThreads = 1024;
+constexpr int kSelKeep = 8;
+constexpr int kBins = 2048;
 
 // fp32 -> an unsigned key in the same order; -0 as 0, NaN above everything.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -106,13 +108,25 @@ struct EvictArgs {
   int32_t* first;      // (B, heads): ranks below it are their own positions
 };
 
+struct SelectShared {
+  uint32_t hist[kBins];
+  uint32_t pick[2];                // the digit, the keys above it
+  uint32_t wave_count[kSelThreads / kWave];
+  uint64_t wave_rank[kSelThreads / kWave];
+  int first;
+};
+
+// One workgroup per (sequence, kv head).  Each thread owns `per` consecutive
+// positions (REG: at most kSelKeep, held in registers; else read again in each
+// pass).  The border key is found eleven bits at a time: a histogram of the
+// digit among the keys that share the digits found so far, and the bin in
+// which the count from above passes `need`.  A scan of each thread's rows above
+// and on the border then ranks the kept rows in one go.
+template <bool REG>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, PagedView c) {
-  constexpr int kWaves = kSelThreads / kWave;
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t pick[2];
-  __shared__ uint32_t wave_sum[2][kWaves];
-  __shared__ int first;
+  __shared__ SelectShared sh;
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t g = (int64_t)b * c.heads + h;
   const int n = (int)paged_len(c, a.lens[b]);
   const float* w = a.weights + b * a.wsb + h * a.wsh;
@@ -123,87 +137,162 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, 
     if (tid == 0) a.first[g] = a.budget;
     return;
   }
+  for (int64_t i = a.budget + tid; i < a.W; i += kSelThreads) out[i] = 0.0f;
+  const int per = (n + kSelThreads - 1) / kSelThreads;
+  const int from = min((int64_t)n, (int64_t)tid * per), to = min(n, from + per);
+  float x[kSelKeep];
+  if constexpr (REG) {
+#pragma unroll
+    for (int i = 0; i < kSelKeep; ++i) x[i] = from + i < to ? w[from + i] : 0.0f;
+  }
+  // calls f(position, weight) for each of the thread's rows, in order
+  auto each = [&](auto f) {
+    if constexpr (REG) {
+#pragma unroll
+      for (int i = 0; i < kSelKeep; ++i)
+        if (from + i < to) f(from + i, x[i]);
+    } else {
+      for (int i = from; i < to; ++i) f(i, w[i]);
+    }
+  };
+
   const int old = n - a.recent;
   uint32_t need = (uint32_t)(a.budget - a.recent);   // of the first `old`; < old
-  // the need-th largest key: digit by digit, counting the keys that share
-  // the digits found so far
-  uint32_t key = 0xffffffffu;
-  uint32_t ties = 0;                // of the rows with that key, how many stay
-  if (need > 0) {
-    key = 0;
-    for (int d = 24; d >= 0; d -= 8) {
-      if (tid < 256) hist[tid] = 0;
+  const bool choose = need > 0;
+  uint32_t key = 0;
+  if (choose) {
+    constexpr int kLow[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      const int low = kLow[d];
+      const uint32_t bins = 1u << kWidth[d], digit = bins - 1;
+      for (int i = tid; i < kBins; i += kSelThreads) sh.hist[i] = 0;
       __syncthreads();
-      const uint32_t mask = d == 24 ? 0u : 0xffffffffu << (d + 8);
-      for (int i = tid; i < old; i += kSelThreads) {
-        const uint32_t u = weight_key(w[i]);
-        if ((u & mask) == key) atomicAdd(&hist[(u >> d) & 255u], 1u);
+      each([&](int i, float v) {
+        const uint32_t u = weight_key(v);
+        const bool same = d == 0 || u >> (low + kWidth[d]) == key >> (low + kWidth[d]);
+        if (i < old && same) atomicAdd(&sh.hist[(u >> low) & digit], 1u);
+      });
+      __syncthreads();
+      // thread t counts bins 2 t' and 2 t' + 1 from above: t' = kSelThreads - 1 - t
+      const int bin = 2 * (kSelThreads - 1 - tid);
+      const uint32_t lo = sh.hist[bin], hi = sh.hist[bin + 1];
+      uint32_t sum = lo + hi;
+#pragma unroll
+      for (int o = 1; o < kWave; o *= 2) {
+        const uint32_t v = __shfl_up((int)sum, o, kWave);
+        if (lane >= o) sum += v;
+      }
+      if (lane == kWave - 1) sh.wave_count[wave] = sum;
+      __syncthreads();
+      uint32_t above = sum - lo - hi;                // keys in bins over this thread's
+#pragma unroll
+      for (int q = 0; q < kSelThreads / kWave; ++q)
+        if (q < wave) above += sh.wave_count[q];
+      if (above < need && need <= above + lo + hi) {
+        const bool top = need <= above + hi;
+        sh.pick[0] = (uint32_t)(top ? bin + 1 : bin);
+        sh.pick[1] = top ? above : above + hi;
       }
       __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0;
-        int v = 255;
-        while (v > 0 && above + hist[v] < need) above += hist[v--];
-        pick[0] = (uint32_t)v;
-        pick[1] = above;
-      }
-      __syncthreads();
-      key |= pick[0] << d;
-      need -= pick[1];
-    }
-    ties = need;
-  }
-  // rank the kept rows in their order
-  const int lane = tid & (kWave - 1), wave = tid / kWave;
-  int32_t* src = a.src + g * a.budget;
-  if (tid == 0) first = a.budget;
-  uint32_t over0 = 0, tie0 = 0;     // rows above the border, rows on it, before this tile
-  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const float x = i < n ? w[i] : 0.0f;
-    const uint32_t u = weight_key(x);
-    const bool over = i < n && (i >= old || (a.budget > a.recent && u > key));
-    const bool tie = i < old && a.budget > a.recent && u == key;
-    const uint64_t mo = __ballot(over), mt = __ballot(tie);
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    uint32_t ro = over0 + __popcll(mo & below), rt = tie0 + __popcll(mt & below);
-    __syncthreads();
-    if (lane == 0) {
-      wave_sum[0][wave] = __popcll(mo);
-      wave_sum[1][wave] = __popcll(mt);
-    }
-    __syncthreads();
-    for (int q = 0; q < kWaves; ++q) {
-      if (q < wave) {
-        ro += wave_sum[0][q];
-        rt += wave_sum[1][q];
-      }
-      over0 += wave_sum[0][q];
-      tie0 += wave_sum[1][q];
-    }
-    if (over || (tie && rt < ties)) {
-      const uint32_t rank = ro + min(rt, ties);
-      src[rank] = i;
-      out[rank] = x;
-    } else if (i < n) {
-      atomicMin(&first, i);
+      key |= sh.pick[0] << low;
+      need -= sh.pick[1];
     }
   }
+  // need: how many of the rows on the border stay
+  auto over = [&](int i, uint32_t u) { return i >= old || (choose && u > key); };
+  auto tie = [&](int i, uint32_t u) { return i < old && choose && u == key; };
+  uint32_t overs = 0, ties = 0;
+  each([&](int i, float v) {
+    const uint32_t u = weight_key(v);
+    overs += over(i, u);
+    ties += tie(i, u);
+  });
+  const uint64_t own = (uint64_t)overs << 32 | ties;
+  uint64_t sum = own;
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const uint64_t v = __shfl_up((unsigned long long)sum, o, kWave);
+    if (lane >= o) sum += v;
+  }
+  if (lane == kWave - 1) sh.wave_rank[wave] = sum;
+  if (tid == 0) sh.first = a.budget;
   __syncthreads();
-  if (tid == 0) a.first[g] = first;
-  for (int64_t i = a.budget + tid; i < a.W; i += kSelThreads) out[i] = 0.0f;
+  sum -= own;
+#pragma unroll
+  for (int q = 0; q < kSelThreads / kWave; ++q)
+    if (q < wave) sum += sh.wave_rank[q];
+  uint32_t ro = (uint32_t)(sum >> 32), rt = (uint32_t)sum;
+  int32_t* src = a.src + g * a.budget;
+  int first = a.budget;
+  each([&](int i, float v) {
+    const uint32_t u = weight_key(v);
+    const bool o = over(i, u), t = tie(i, u);
+    if (o || (t && rt < need)) {
+      const uint32_t rank = ro + min(rt, need);
+      src[rank] = i;
+      out[rank] = v;
+    } else {
+      first = min(first, i);
+    }
+    ro += o;
+    rt += t;
+  });
+  if (first < a.budget) atomicMin(&sh.first, first);
+  __syncthreads();
+  if (tid == 0) a.first[g] = sh.first;
 }
 
 // Moves the kept rows of one (sequence, kv head) to their ranks, one slice of
 // 16-byte columns of K or of V (or the row scales) per workgroup.  A row only
 // moves down and ranks rise with positions, so tiles of rows in order need no
 // second buffer: every row that a tile overwrites is one that this tile or an
-// earlier one has read, or one that goes.
-constexpr int kMoveUnroll = 8;
+// earlier one has read, or one that goes.  A tile's places are looked up while
+// the one before it is on its way.
+constexpr int kMoveUnroll = 4;
+
+template <typename T, typename Offset>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& c,
+                                          const int32_t* src, const int32_t* table, int h,
+                                          int begin, int r, int step, T* base, Offset offset) {
+  int64_t at[kMoveUnroll], to[kMoveUnroll];
+  auto find = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int row = r0 + u * step + r;
+      at[u] = to[u] = -1;
+      if (row >= a.budget) continue;
+      const int32_t from = src[row];
+      const int32_t pf = paged_page(c, table, from), pt = paged_page(c, table, row);
+      if (pf < 0 || pt < 0) continue;
+      at[u] = offset(pf, from);
+      to[u] = offset(pt, row);
+    }
+  };
+  find(begin);
+  for (int r0 = begin; r0 < a.budget; r0 += step * kMoveUnroll) {
+    T x[kMoveUnroll];
+    int64_t put[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      put[u] = to[u];
+      x[u] = T{};
+      if (at[u] >= 0) x[u] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at[u]);
+    }
+    find(r0 + step * kMoveUnroll);
+    // every load of the tile has to be back before any store of it
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) asm volatile("" : "+v"(x[u]));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u)
+      if (put[u] >= 0) *reinterpret_cast<T*>(reinterpret_cast<char*>(base) + put[u]) = x[u];
+  }
+}
 
 __global__ __launch_bounds__(kPThreads) void evict_move_kernel(EvictArgs a, PagedView c,
-                                                               int slices, int lanes,
-                                                               int row_bytes) {
+                                                               int slices, int lanes) {
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t g = (int64_t)b * c.heads + h;
   const int begin = a.first[g];
@@ -212,56 +301,17 @@ __global__ __launch_bounds__(kPThreads) void evict_move_kernel(EvictArgs a, Page
   const int32_t* table = c.table + b * c.table_stride;
   const int kind = blockIdx.x / slices;     // 0: K, 1: V, 2: the scales
   if (kind == 2) {
-    // four bytes a row: K's in the first half of the threads, V's in the second
+    // K's in the first half of the threads, V's in the second
     float* s = threadIdx.x < kPThreads / 2 ? c.ks : c.vs;
-    for (int r0 = begin; r0 < a.budget; r0 += kPThreads / 2) {
-      const int r = r0 + (threadIdx.x & (kPThreads / 2 - 1));
-      float x = 0.0f;
-      int64_t to = -1;
-      if (r < a.budget) {
-        const int32_t from = src[r];
-        const int32_t pf = paged_page(c, table, from), pt = paged_page(c, table, r);
-        if (pf >= 0 && pt >= 0) {
-          x = s[paged_scale(c, pf, h, from)];
-          to = paged_scale(c, pt, h, r);
-        }
-      }
-      asm volatile("s_waitcnt vmcnt(0)" : "+v"(x)::"memory");
-      __syncthreads();
-      if (to >= 0) s[to] = x;
-    }
+    move_rows(a, c, src, table, h, begin, threadIdx.x & (kPThreads / 2 - 1), kPThreads / 2, s,
+              [&](int32_t p, int64_t pos) { return paged_scale(c, p, h, pos) * 4; });
     return;
   }
-  char* base = kind == 0 ? c.k : c.v;
+  u32x4r* base = reinterpret_cast<u32x4r*>(kind == 0 ? c.k : c.v);
   const int eb = c.ks ? 1 : 2;
   const int col = ((blockIdx.x % slices) * lanes + threadIdx.x % lanes) * 16;
-  const int rows = kPThreads / lanes;
-  for (int r0 = begin; r0 < a.budget; r0 += rows * kMoveUnroll) {
-    u32x4r x[kMoveUnroll];
-    int64_t to[kMoveUnroll];
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) {
-      const int r = r0 + u * rows + threadIdx.x / lanes;
-      to[u] = -1;
-      x[u] = u32x4r{0u, 0u, 0u, 0u};
-      if (r < a.budget && col < row_bytes) {
-        const int32_t from = src[r];
-        const int32_t pf = paged_page(c, table, from), pt = paged_page(c, table, r);
-        if (pf >= 0 && pt >= 0) {
-          x[u] = *reinterpret_cast<const u32x4r*>(base + paged_row(c, pf, h, from) * eb + col);
-          to[u] = paged_row(c, pt, h, r) * eb + col;
-        }
-      }
-    }
-    // every load of the tile has to be back before any store of it
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u) asm volatile("" : "+v"(x[u]));
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; ++u)
-      if (to[u] >= 0) *reinterpret_cast<u32x4r*>(base + to[u]) = x[u];
-  }
+  move_rows(a, c, src, table, h, begin, threadIdx.x / lanes, kPThreads / lanes, base,
+            [&](int32_t p, int64_t pos) { return paged_row(c, p, h, pos) * eb + col; });
 }
 
 }  // namespace
@@ -364,13 +414,16 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
   const EvictArgs a{seq_lens, weights, wsb, wsh, (int32_t)budget, (int32_t)recent, new_lens,
                     new_weights, W, src, first};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)c.heads, (unsigned)B), dim3(kSelThreads),
-                     0, st, a, c);
+  const dim3 grid((unsigned)c.heads, (unsigned)B);
+  if (c.capacity() <= kSelThreads * kSelKeep)
+    hipLaunchKernelGGL(evict_select_kernel<true>, grid, dim3(kSelThreads), 0, st, a, c);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<false>, grid, dim3(kSelThreads), 0, st, a, c);
   const int row_bytes = (int)cache->head_dim * cache_elem_bytes(cache->dtype);
   const int lanes = row_bytes >= 64 ? 4 : row_bytes / 16;
   const int slices = row_bytes / (16 * lanes);
   hipLaunchKernelGGL(evict_move_kernel,
                      dim3((unsigned)(2 * slices + (c.ks ? 1 : 0)), (unsigned)c.heads, (unsigned)B),
-                     dim3(kPThreads), 0, st, a, c, slices, lanes, row_bytes);
+                     dim3(kPThreads), 0, st, a, c, slices, lanes);
   return paged_launched("paged_kv_evict");
 }
