@@ -53,8 +53,8 @@ __global__ __launch_bounds__(kPThreads) void append_kernel(AppendArgs a, PagedVi
   const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const int n = a.lengths ? min(a.lengths[b], a.S) : a.S;
-  const int i = (int)(r / c.heads), h = (int)(r % c.heads);
-  const bool live = i < n;
+  const int h = (int)(r / a.S), i = (int)(r % a.S);   // a head's rows are neighbours in a page
+  const bool live = h < c.heads && i < n;
   const int64_t pos = (int64_t)a.start[b] + i;
   const int32_t page = live ? paged_page(c, c.table + b * c.table_stride, pos) : -1;
   u32x4r x{0u, 0u, 0u, 0u}, y{0u, 0u, 0u, 0u};
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, 
 // second buffer: every row that a tile overwrites is one that this tile or an
 // earlier one has read, or one that goes.  A tile's places are looked up while
 // the one before it is on its way.
-constexpr int kMoveUnroll = 4;
+constexpr int kMoveThreads = 1024, kMoveUnroll = 4;
 
 template <typename T, typename Offset>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& c,
@@ -291,7 +291,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& c
   }
 }
 
-__global__ __launch_bounds__(kPThreads) void evict_move_kernel(EvictArgs a, PagedView c,
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, PagedView c,
                                                                int slices, int lanes) {
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t g = (int64_t)b * c.heads + h;
@@ -302,15 +302,15 @@ __global__ __launch_bounds__(kPThreads) void evict_move_kernel(EvictArgs a, Page
   const int kind = blockIdx.x / slices;     // 0: K, 1: V, 2: the scales
   if (kind == 2) {
     // K's in the first half of the threads, V's in the second
-    float* s = threadIdx.x < kPThreads / 2 ? c.ks : c.vs;
-    move_rows(a, c, src, table, h, begin, threadIdx.x & (kPThreads / 2 - 1), kPThreads / 2, s,
+    float* s = threadIdx.x < kMoveThreads / 2 ? c.ks : c.vs;
+    move_rows(a, c, src, table, h, begin, threadIdx.x & (kMoveThreads / 2 - 1), kMoveThreads / 2, s,
               [&](int32_t p, int64_t pos) { return paged_scale(c, p, h, pos) * 4; });
     return;
   }
   u32x4r* base = reinterpret_cast<u32x4r*>(kind == 0 ? c.k : c.v);
   const int eb = c.ks ? 1 : 2;
   const int col = ((blockIdx.x % slices) * lanes + threadIdx.x % lanes) * 16;
-  move_rows(a, c, src, table, h, begin, threadIdx.x / lanes, kPThreads / lanes, base,
+  move_rows(a, c, src, table, h, begin, threadIdx.x / lanes, kMoveThreads / lanes, base,
             [&](int32_t p, int64_t pos) { return paged_row(c, p, h, pos) * eb + col; });
 }
 
@@ -420,10 +420,14 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
   else
     hipLaunchKernelGGL(evict_select_kernel<false>, grid, dim3(kSelThreads), 0, st, a, c);
   const int row_bytes = (int)cache->head_dim * cache_elem_bytes(cache->dtype);
-  const int lanes = row_bytes >= 64 ? 4 : row_bytes / 16;
+  // slices of whole 128-byte lines where that leaves a workgroup for each CU
+  // (32 caches x 8 heads of e4m3fn: 84 us, 98 us in half lines), else of 64
+  // bytes (one cache of 8 heads: 16 us, 18 us in whole lines)
+  const bool lines = row_bytes >= 128 && B * c.heads * 2 * (row_bytes / 128) >= 256;
+  const int lanes = lines ? 8 : row_bytes >= 64 ? 4 : row_bytes / 16;
   const int slices = row_bytes / (16 * lanes);
   hipLaunchKernelGGL(evict_move_kernel,
                      dim3((unsigned)(2 * slices + (c.ks ? 1 : 0)), (unsigned)c.heads, (unsigned)B),
-                     dim3(kPThreads), 0, st, a, c, slices, lanes);
+                     dim3(kMoveThreads), 0, st, a, c, slices, lanes);
   return paged_launched("paged_kv_evict");
 }
