@@ -85,7 +85,6 @@ void launch_append(const AppendArgs& a, const PagedView& c, int64_t B, int64_t D
 // ------------------------------------------------------------------ eviction
 
 constexpr int kSelThreads = 1024;
-constexpr int kSelKeep = 8;
 constexpr int kBins = 2048;
 
 // fp32 -> an unsigned key in the same order; -0 as 0, NaN above everything.
@@ -106,6 +105,7 @@ struct EvictArgs {
   int64_t W;
   int32_t* src;        // (B, heads, budget): the position each kept row comes from
   int32_t* first;      // (B, heads): ranks below it are their own positions
+  bool aligned;        // every row of weights lies on a 16-byte border
 };
 
 struct SelectShared {
@@ -117,12 +117,12 @@ struct SelectShared {
 };
 
 // One workgroup per (sequence, kv head).  Each thread owns `per` consecutive
-// positions (REG: at most kSelKeep, held in registers; else read again in each
-// pass).  The border key is found eleven bits at a time: a histogram of the
+// positions, four at a time (KEEP > 0: at most KEEP, held in registers; 0: read
+// again in each pass).  The border key is found eleven bits at a time: a histogram of the
 // digit among the keys that share the digits found so far, and the bin in
 // which the count from above passes `need`.  A scan of each thread's rows above
 // and on the border then ranks the kept rows in one go.
-template <bool REG>
+template <int KEEP>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, PagedView c) {
   __shared__ SelectShared sh;
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -138,21 +138,32 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, 
     return;
   }
   for (int64_t i = a.budget + tid; i < a.W; i += kSelThreads) out[i] = 0.0f;
-  const int per = (n + kSelThreads - 1) / kSelThreads;
-  const int from = min((int64_t)n, (int64_t)tid * per), to = min(n, from + per);
-  float x[kSelKeep];
-  if constexpr (REG) {
+  const int per = (int)(((int64_t)n + 4 * kSelThreads - 1) / (4 * kSelThreads) * 4);
+  const int from = (int)min((int64_t)n, (int64_t)tid * per), to = min(n, from + per);
+  auto load4 = [&](int i) -> f32x4 {                // positions i .. i + 3, those before `to`
+    if (a.aligned && i + 4 <= to) return *reinterpret_cast<const f32x4*>(w + i);
+    f32x4 v;
 #pragma unroll
-    for (int i = 0; i < kSelKeep; ++i) x[i] = from + i < to ? w[from + i] : 0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = i + e < to ? w[i + e] : 0.0f;
+    return v;
+  };
+  f32x4 x[KEEP > 0 ? KEEP / 4 : 1];
+  if constexpr (KEEP > 0) {
+#pragma unroll
+    for (int q = 0; q < KEEP / 4; ++q) x[q] = load4(from + 4 * q);
   }
   // calls f(position, weight) for each of the thread's rows, in order
   auto each = [&](auto f) {
-    if constexpr (REG) {
+    auto four = [&](int i, f32x4 v) {
 #pragma unroll
-      for (int i = 0; i < kSelKeep; ++i)
-        if (from + i < to) f(from + i, x[i]);
+      for (int e = 0; e < 4; ++e)
+        if (i + e < to) f(i + e, v[e]);
+    };
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int q = 0; q < KEEP / 4; ++q) four(from + 4 * q, x[q]);
     } else {
-      for (int i = from; i < to; ++i) f(i, w[i]);
+      for (int i = from; i < to; i += 4) four(i, load4(i));
     }
   };
 
@@ -412,13 +423,16 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
   int32_t* first = static_cast<int32_t*>(workspace);
   int32_t* src = first + (B * c.heads * 4 + 255) / 256 * 64;
   const EvictArgs a{seq_lens, weights, wsb, wsh, (int32_t)budget, (int32_t)recent, new_lens,
-                    new_weights, W, src, first};
+                    new_weights, W, src, first,
+                    ((wsb | wsh) & 3) == 0 && (reinterpret_cast<uintptr_t>(weights) & 15) == 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)c.heads, (unsigned)B);
-  if (c.capacity() <= kSelThreads * kSelKeep)
-    hipLaunchKernelGGL(evict_select_kernel<true>, grid, dim3(kSelThreads), 0, st, a, c);
+  if (c.capacity() <= 8 * kSelThreads)
+    hipLaunchKernelGGL(evict_select_kernel<8>, grid, dim3(kSelThreads), 0, st, a, c);
+  else if (c.capacity() <= 32 * kSelThreads)
+    hipLaunchKernelGGL(evict_select_kernel<32>, grid, dim3(kSelThreads), 0, st, a, c);
   else
-    hipLaunchKernelGGL(evict_select_kernel<false>, grid, dim3(kSelThreads), 0, st, a, c);
+    hipLaunchKernelGGL(evict_select_kernel<0>, grid, dim3(kSelThreads), 0, st, a, c);
   const int row_bytes = (int)cache->head_dim * cache_elem_bytes(cache->dtype);
   // slices of whole 128-byte lines where that leaves a workgroup for each CU
   // (32 caches x 8 heads of e4m3fn: 84 us, 98 us in half lines), else of 64
