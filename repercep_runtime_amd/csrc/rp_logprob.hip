@@ -30,7 +30,7 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxThreads = 512;
 constexpr int kHits = 128;                     // vectors collected per workgroup
-constexpr int kMaxParts = 64;                  // of 2^21 logits
+constexpr int kMaxParts = 64, kMaxV = kMaxParts * kMaxThreads * 64;
 constexpr int kJoinRows = 4, kJoinThreads = kJoinRows * kWave;
 constexpr double kLn2 = 0.693147180559945309417;
 
@@ -70,9 +70,10 @@ __device__ __forceinline__ float logit_at(const char* row, int64_t i) {
   else return in_to_f32<DT == RP_OUT_F16 ? kInF16 : kInBf16>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
-// Whether M c is far from fp32's range: then t is one fma about B = fp32(M c),
-// an exact base like any other; a row of lowest values takes (x - M) c.
-__device__ __forceinline__ bool near(float m, float c) { return fabsf(m * c) < 0x1p100f; }
+// Whether fp32(M c) is within 2^-4 of M c: then t is one fma about it, an exact
+// base like any other.  A low temperature or a row of lowest values takes
+// (x - M) c.
+__device__ __forceinline__ bool near(float m, float c) { return fabsf(m * c) < 0x1p20f; }
 
 // What one (M, s, u) says of a row: its log probabilities and entropy.
 struct Row {
@@ -123,7 +124,7 @@ __device__ __forceinline__ float half_max(uint32_t w) {
   const uint32_t x = (uint32_t)(lo > hi ? lo : hi) & 0xffffu;
   return DT == RP_OUT_F16 ? f16_to_f32(x) : bf16_to_f32(x);
 }
-// 16-bit logits whose t may leave fp32's range: -2^100 and below, fp16's -inf
+// 16-bit logits whose t may leave fp32's range (c up to 2^20): -2^100 and below, fp16's -inf
 template <int DT>
 constexpr uint32_t kLow16 = DT == RP_OUT_F16 ? 0xfc00u : 0xf180u;
 
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   const bool fma = near(m0, a.c);
   if (!fma) {
     weigh([&](float x) { return nmax((x - m0) * a.c, -200.0f); });
-  } else if (!PACKED || __any(low16 >= kLow16<DT>)) {
+  } else if (!PACKED || a.c > 0x1p20f || __any(low16 >= kLow16<DT>)) {
     weigh([&](float x) { return nmax(__builtin_fmaf(x, a.c, -base), -200.0f); });
   } else {
     weigh([&](float x) { return __builtin_fmaf(x, a.c, -base); });
@@ -476,7 +477,10 @@ using namespace rp;
 
 extern "C" size_t rp_token_logprobs_workspace_bytes(int64_t N, int64_t V, int logits_dtype,
                                                     int top) {
-  if (N <= 0 || V <= 0 || top < 0) return 0;
+  // sizes that the call refuses need none
+  if (N <= 0 || N > 0x7fffffff / kMaxParts || V <= 0 || V > kMaxV || top < 0 ||
+      top > RP_LOGPROB_MAX_TOP)
+    return 0;
   const LogprobPlan p = logprob_plan(V, logits_dtype);
   return p.parts == 1 ? 0 : logprob_sums_bytes(N, p.parts) + (size_t)(N * p.parts * top * 8);
 }
@@ -512,7 +516,7 @@ extern "C" int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N
     rp_set_error("token_logprobs: temperature too small");
     return RP_ERR_INVALID_ARGUMENT;
   }
-  if (V > (1 << 21) || N > 0x7fffffff / kMaxParts) {
+  if (V > kMaxV || N > 0x7fffffff / kMaxParts) {
     rp_set_error("token_logprobs: too many rows or logits");
     return RP_ERR_UNSUPPORTED;
   }

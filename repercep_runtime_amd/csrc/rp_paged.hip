@@ -50,10 +50,10 @@ template <int DT, bool FP8, int TPR>
 __global__ __launch_bounds__(kPThreads) void append_kernel(AppendArgs a, PagedView c) {
   constexpr int RPB = kPThreads / TPR;
   const int b = blockIdx.y;
-  const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const uint32_t r = blockIdx.x * RPB + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const int n = a.lengths ? min(a.lengths[b], a.S) : a.S;
-  const int h = (int)(r / a.S), i = (int)(r % a.S);   // a head's rows are neighbours in a page
+  const int h = (int)(r / (uint32_t)a.S), i = (int)(r % (uint32_t)a.S);   // a head's rows are neighbours in a page
   const bool live = h < c.heads && i < n;
   const int64_t pos = (int64_t)a.start[b] + i;
   const int32_t page = live ? paged_page(c, c.table + b * c.table_stride, pos) : -1;
@@ -347,7 +347,8 @@ extern "C" int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int
     return RP_ERR_INVALID_ARGUMENT;
   }
   PagedView c;
-  const int rc = paged_view("paged_kv_append", cache, &c);
+  int rc = paged_view("paged_kv_append", cache, &c);
+  if (rc == RP_OK) rc = paged_writable("paged_kv_append", cache);
   if (rc != RP_OK) return rc;
   if (x_dtype != RP_DTYPE_BF16 && x_dtype != RP_DTYPE_F16) {
     rp_set_error("paged_kv_append: unknown input dtype %d", x_dtype);
@@ -383,7 +384,13 @@ extern "C" int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int
 
 extern "C" size_t rp_paged_evict_workspace_bytes(int64_t B, const rp_paged_cache* cache,
                                                  int64_t budget) {
-  if (!cache || B <= 0 || budget <= 0 || cache->heads <= 0) return 0;
+  // sizes that the call refuses need none; no more than the table's positions stay
+  if (!cache || B <= 0 || B > 65535 || budget <= 0 || cache->heads <= 0 || cache->heads > 65535 ||
+      cache->page_size <= 0 || cache->max_pages <= 0 ||
+      cache->max_pages > (1 << 30) / cache->page_size)
+    return 0;
+  const int64_t cap = cache->max_pages * cache->page_size;
+  budget = budget < cap ? budget : cap;
   return (size_t)((B * cache->heads * 4 + 255) / 256 * 256 + B * cache->heads * budget * 4);
 }
 
@@ -396,7 +403,8 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
     return RP_ERR_INVALID_ARGUMENT;
   }
   PagedView c;
-  const int rc = paged_view("paged_kv_evict", cache, &c);
+  int rc = paged_view("paged_kv_evict", cache, &c);
+  if (rc == RP_OK) rc = paged_writable("paged_kv_evict", cache);
   if (rc != RP_OK) return rc;
   if (B <= 0 || budget <= 0 || recent < 0 || recent > budget) {
     rp_set_error("paged_kv_evict: needs B > 0 and 0 <= recent <= budget, budget > 0 (B=%lld "

@@ -681,8 +681,11 @@ using namespace rp;
 
 extern "C" size_t rp_paged_attn_workspace_bytes(int64_t B, int64_t H, const rp_paged_cache* cache,
                                                 int64_t max_seq_len, int with_key_weights) {
-  if (!cache || B <= 0 || H <= 0 || cache->heads <= 0 || cache->max_pages <= 0 ||
-      cache->page_size <= 0 || cache->head_dim <= 0)
+  // sizes that the call refuses need none
+  if (!cache || B <= 0 || B > 65535 || H <= 0 || H > 65535 || cache->heads <= 0 ||
+      cache->heads > H || cache->page_size <= 0 || cache->max_pages <= 0 ||
+      cache->max_pages > (1 << 30) / cache->page_size || cache->head_dim <= 0 ||
+      cache->head_dim > 256 || max_seq_len < 0)
     return 0;
   return decode_layout(B, H, cache, max_seq_len, with_key_weights != 0).total;
 }
@@ -723,7 +726,7 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_decode: too many sequences or heads, or rows too far apart");
     return RP_ERR_UNSUPPORTED;
   }
-  if (fp8 && ((reinterpret_cast<uintptr_t>(c.ks) | reinterpret_cast<uintptr_t>(c.vs)) & 15) != 0) {
+  if (fp8 && c.shift >= 4 && ((reinterpret_cast<uintptr_t>(c.ks) | reinterpret_cast<uintptr_t>(c.vs)) & 15) != 0) {
     rp_set_error("paged_attn_decode: scales must be 16-byte aligned");
     return RP_ERR_UNSUPPORTED;
   }
@@ -732,8 +735,8 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_decode: q rows must be 16-byte and out rows 8-byte aligned");
     return RP_ERR_UNSUPPORTED;
   }
-  if (key_weights && (wsb < 0 || wsh < 0)) {
-    rp_set_error("paged_attn_decode: bad key_weights strides");
+  if ((B > 1 && osb < cache->head_dim) || (H > 1 && osh < cache->head_dim)) {
+    rp_set_error("paged_attn_decode: out rows overlap");
     return RP_ERR_INVALID_ARGUMENT;
   }
   const int64_t tiles = (H / cache->heads + 15) / 16;
@@ -747,6 +750,11 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
                       (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) {
     rp_set_error("paged_attn_decode: workspace of %zu bytes, 256-byte aligned, needed", l.total);
     return RP_ERR_WORKSPACE;
+  }
+  if (key_weights && ((B > 1 && wsb < c.capacity()) || (cache->heads > 1 && wsh < c.capacity()))) {
+    rp_set_error("paged_attn_decode: key_weights rows of %lld positions overlap",
+                 (long long)c.capacity());
+    return RP_ERR_INVALID_ARGUMENT;
   }
   char* ws = static_cast<char*>(workspace);
   DecodeArgs a{};

@@ -109,6 +109,16 @@ inline int paged_view(const char* what, const rp_paged_cache* c, PagedView* v) {
   return RP_OK;
 }
 
+// Refuses a cache whose rows share memory, for the calls that write it.
+inline int paged_writable(const char* what, const rp_paged_cache* c) {
+  if ((c->num_pages > 1 && c->stride_page < c->head_dim) ||
+      (c->heads > 1 && c->stride_head < c->head_dim)) {
+    rp_set_error("%s: cache rows overlap", what);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  return RP_OK;
+}
+
 inline int paged_launched(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

@@ -1097,6 +1097,15 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
         block_table.stride(0) if B > 1 else 0, table[1], dt)
 
 
+def _on_device(dev: int, fn: Callable[..., int], *args: object) -> int:
+    """``fn(*args)`` with GPU ``dev`` current: the raw handle of a device's
+    default stream is the same for every device."""
+    if torch.cuda.current_device() == dev:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
 def _unit_stride(name: str, t: torch.Tensor) -> None:
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
@@ -1147,8 +1156,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
         _on_device_of(k_cache, k=k, v=v, start=start, lengths=lengths)
     if B == 0 or S == 0:
         return
-    C.check(C.lib().rp_paged_kv_append(
-        k.data_ptr(), v.data_ptr(), dt, B, S, *_strides(k, 3), *_strides(v, 3), cache,
+    C.check(_on_device(
+        dev, C.lib().rp_paged_kv_append, k.data_ptr(), v.data_ptr(), dt, B, S, *_strides(k, 3), *_strides(v, 3), cache,
         start.data_ptr(), lengths.data_ptr() if lengths is not None else None, _stream(k)),
         "rp_paged_kv_append")
 
@@ -1217,8 +1226,8 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         hint = max_seq_len if max_seq_len is not None else 0
         n = C.lib().rp_paged_attn_workspace_bytes(B, H, cache, hint, w_ptr is not None)
         ws = q.new_empty(n, dtype=torch.uint8) if n else None
-        rc = C.lib().rp_paged_attn_decode(
-            q.data_ptr(), dt, B, H, *_strides(q, 2), cache, seq_lens.data_ptr(),
+        rc = _on_device(
+            dev, C.lib().rp_paged_attn_decode, q.data_ptr(), dt, B, H, *_strides(q, 2), cache, seq_lens.data_ptr(),
             1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(),
             *_strides(out, 2), lse.data_ptr() if return_lse else None, w_ptr, wsb, wsh, hint,
             ws.data_ptr() if n else None, n, _stream(q))
@@ -1268,8 +1277,8 @@ def paged_kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: to
     budget = min(budget, slots)
     n = C.lib().rp_paged_evict_workspace_bytes(B, cache, budget)
     ws = kept.new_empty(n, dtype=torch.uint8)
-    C.check(C.lib().rp_paged_kv_evict(
-        cache, seq_lens.data_ptr(), B, key_weights.data_ptr(), *_strides(key_weights, 2), budget,
+    C.check(_on_device(
+        dev, C.lib().rp_paged_kv_evict, cache, seq_lens.data_ptr(), B, key_weights.data_ptr(), *_strides(key_weights, 2), budget,
         min(recent, budget), new_lens.data_ptr(), kept.data_ptr(), kept.shape[2], ws.data_ptr(), n,
         _stream(k_cache)), "rp_paged_kv_evict")
     return new_lens, kept
@@ -1324,8 +1333,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     if N > 0:
         n = C.lib().rp_token_logprobs_workspace_bytes(N, V, dt, top)
         ws = logprobs.new_empty(n, dtype=torch.uint8) if n else None
-        rc = C.lib().rp_token_logprobs(
-            x.data_ptr(), dt, N, V, x.stride(0) if N > 1 else V, t.data_ptr(), temperature, top,
+        rc = _on_device(
+            dev, C.lib().rp_token_logprobs, x.data_ptr(), dt, N, V, x.stride(0) if N > 1 else V, t.data_ptr(), temperature, top,
             logprobs.data_ptr(), entropy.data_ptr(), top_lp.data_ptr() if top else None,
             ids.data_ptr() if top else None, ws.data_ptr() if n else None, n, _stream(x))
         C.check(rc, "rp_token_logprobs")

@@ -80,6 +80,26 @@ def test_temperature(gpu, T) -> None:
     check(gpu, logits(4, 5000, "bf16", 1), 8, T)
 
 
+@pytest.mark.parametrize("T", [1e-7, 1e-20, 1e20])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_extreme_temperatures(gpu, dt, T) -> None:
+    """All weight on the best tokens, or the same on every one.  The logits are
+    whole, so their differences are 0 or at least 1 / T."""
+    x = torch.randint(-9, 10, (3, 3000), generator=torch.Generator().manual_seed(3)).to(DTYPES[dt])
+    r = ops.token_logprobs(x.to(gpu), torch.zeros(3, dtype=torch.int64, device=gpu), top=4,
+                           temperature=T)
+    z = x.double() / T
+    lp = torch.log_softmax(z, -1)
+    p = lp.exp()
+    ent = -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(-1)
+    # log p of the best is -log of their number; of the others about -1 / T: both to 2^-20
+    assert ((r.entropy.cpu().double() - ent).abs() <= 2.0 ** -20 * (1 + ent)).all()
+    got, want = r.logprobs.cpu().double(), lp[:, 0]
+    assert ((got - want).abs() <= 2.0 ** -20 * (1 + want.abs())).all()
+    assert ((r.top_logprobs.cpu().double() - lp.gather(1, r.top_ids.cpu())).abs() <= 2.0 ** -20
+            * 10).all()
+
+
 @pytest.mark.parametrize("shift", [-3e4, 1e3, 3e4])
 def test_large_logits(gpu, shift) -> None:
     """Logits far from zero: only their differences count."""

@@ -161,6 +161,27 @@ def test_decode_over_long_caches(gpu, kind, qt, n, weights, H, Hkv) -> None:
     check_decode(gpu, c, [n], H, qt, weights=weights, hint=n)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [2, 4, 8, 1024])
+def test_decode_of_small_and_large_pages(gpu, kind, page) -> None:
+    lens = [1, 7, 500, 1100]
+    c = Cache(lens, 2, 128, page, kind, seed=page)
+    check_decode(gpu, c, lens, 6, "bf16", weights=True)
+
+
+def test_decode_reads_an_expanded_cache(gpu) -> None:
+    """One head's rows seen as several heads': equal to copies of them."""
+    lens = [90, 33]
+    c = Cache(lens, 1, 64, 16, "bf16", seed=7)
+    dev = c.to(gpu)
+    q = torch.randn(2, 6, 1, 64).to(torch.bfloat16).to(gpu)
+    kx, vx = (dev[n].expand(-1, 3, -1, -1) for n in ("k_cache", "v_cache"))
+    got = ops.paged_attention_decode(q, kx, vx, dev["block_table"], i32(lens, gpu))
+    want = ops.paged_attention_decode(q, kx.contiguous(), vx.contiguous(), dev["block_table"],
+                                      i32(lens, gpu))
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("hint", [None, 1, 64, 3000, 10 ** 9])
 @pytest.mark.parametrize("weights", [False, True])
 def test_decode_does_not_depend_on_the_expected_length(gpu, hint, weights) -> None:

@@ -94,6 +94,10 @@ def test_cache_refusals(kw: dict, status: int, msg: str) -> None:
     (decode, dict(qsh=132), 2, "aligned"),
     (decode, dict(out=FAKE + 2), 2, "aligned"),
     (decode, dict(w=FAKE, wsb=-1), 1, "key_weights"),
+    (decode, dict(w=FAKE, wsb=128, wsh=63), 1, "key_weights"),
+    (decode, dict(w=FAKE, wsb=0, wsh=64), 1, "key_weights"),
+    (decode, dict(osb=0), 1, "overlap"),
+    (decode, dict(osh=64), 1, "overlap"),
     (decode, dict(w=FAKE, ws=None, nbytes=0), 3, "workspace"),
     (evict, dict(lens=None), 1, "null"),
     (evict, dict(budget=0), 1, "budget"),
@@ -110,6 +114,35 @@ def test_call_refusals(call, kw: dict, status: int, msg: str) -> None:
     assert msg in _capi.lib().rp_last_error().decode()
 
 
+@pytest.mark.parametrize("call", [append, evict])
+@pytest.mark.parametrize("kw", [dict(stride_page=0), dict(stride_head=0), dict(stride_head=64)])
+def test_writers_refuse_rows_that_overlap(call, kw: dict) -> None:
+    """A cache expanded over its pages or heads can be read, not written."""
+    assert call(cache(**kw)) == 1
+    assert "overlap" in _capi.lib().rp_last_error().decode()
+
+
+BIG = (0, 1, -1, 1 << 16, 1 << 31, 1 << 32, 1 << 47, 1 << 62, -(1 << 62))
+
+
+def test_workspace_sizes_of_any_arguments() -> None:
+    """Sizes that the calls refuse need no workspace, and none divides by zero."""
+    L = _capi.lib()
+    for x in BIG:
+        for y in BIG:
+            L.rp_token_logprobs_workspace_bytes(x, y, 0, 5)
+            L.rp_paged_attn_workspace_bytes(x, y, cache(), 0, 1)
+            L.rp_paged_attn_workspace_bytes(2, 4, cache(heads=x, page_size=y), 0, 1)
+            L.rp_paged_attn_workspace_bytes(2, 4, cache(max_pages=x, head_dim=y), x, 1)
+            L.rp_paged_evict_workspace_bytes(x, cache(), y)
+            L.rp_paged_evict_workspace_bytes(2, cache(heads=x, max_pages=y), 5)
+    assert L.rp_token_logprobs_workspace_bytes(4, 1 << 62, 0, 5) == 0
+    assert L.rp_paged_attn_workspace_bytes(1 << 62, 4, cache(), 0, 1) == 0
+    assert L.rp_paged_attn_workspace_bytes(2, 1, cache(), 0, 1) == 0        # H below the heads
+    assert L.rp_paged_evict_workspace_bytes(2, cache(), 1 << 62) == \
+        L.rp_paged_evict_workspace_bytes(2, cache(), 64) == 256 + 2 * 2 * 64 * 4
+
+
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(logits=None), 1, "null"),
     (dict(tokens=None), 1, "null"),
@@ -124,6 +157,12 @@ def test_call_refusals(call, kw: dict, status: int, msg: str) -> None:
     (dict(temperature=float("nan")), 1, "temperature"),
     (dict(temperature=float("inf")), 1, "temperature"),
     (dict(V=1 << 31, ld=1 << 31), 2, "too many"),
+    (dict(V=(1 << 21) + 1, ld=1 << 22), 2, "too many"),
+    (dict(N=1 << 31), 2, "too many"),
+    (dict(temperature=1e-45), 1, "temperature"),
+    (dict(logits=FAKE + 1), 1, "aligned"),
+    (dict(V=40000, ld=40000, ws=None), 3, "workspace"),
+    (dict(V=40000, ld=40000, ws=FAKE + 16), 3, "workspace"),
 ])
 def test_logprob_refusals(kw: dict, status: int, msg: str) -> None:
     a = dict(logits=FAKE, dt=0, N=4, V=100, ld=100, tokens=FAKE, temperature=1.0, top=5, lp=FAKE,
