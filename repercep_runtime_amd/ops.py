@@ -59,6 +59,10 @@ _CACHE_DTYPES = {torch.bfloat16: C.RP_CACHE_BF16, torch.float16: C.RP_CACHE_F16,
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+# the current GPU's index, likewise
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _stream(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.get_device())
@@ -1100,7 +1104,7 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
 def _on_device(dev: int, fn: Callable[..., int], *args: object) -> int:
     """``fn(*args)`` with GPU ``dev`` current: the raw handle of a device's
     default stream is the same for every device."""
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         return fn(*args)
     with torch.cuda.device(dev):
         return fn(*args)

@@ -66,6 +66,44 @@ def test_append_writes_its_rows_and_no_others(gpu, kind, qt, D, page, Hkv, layou
             assert torch.equal(bits(gs), bits(scale)), name
 
 
+@pytest.mark.parametrize("kind", ["fp16", "e4m3"])
+@pytest.mark.parametrize("D,Hkv", [(256, 2), (128, 5)])
+def test_append_of_many_rows(gpu, kind, D, Hkv) -> None:
+    """Prompts of thousands of rows, ragged, one shorter than its padding by all but one."""
+    new, page = [7001, 1, 6900], 32
+    S = max(new)
+    P = sum(-(-n // page) for n in new)
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    table = torch.full((3, -(-S // page)), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(new):
+        table[b, :-(-n // page)] = order[at:at + -(-n // page)]
+        at += -(-n // page)
+    g = torch.Generator(device=gpu).manual_seed(3)
+    k, v = (torch.randn(3, Hkv, S, D, generator=g, device=gpu).to(torch.float16) for _ in range(2))
+    dt = CACHE_DTYPES[kind]
+    kc, vc = (torch.zeros((P, Hkv, page, D), dtype=torch.uint8 if kind == "e4m3" else dt,
+                          device=gpu).view(dt) for _ in range(2))
+    ks, vs = (torch.zeros((P, Hkv, page), device=gpu) if kind == "e4m3" else None
+              for _ in range(2))
+    ops.paged_kv_append(k, v, kc, vc, table.to(gpu), i32([0, 0, 0], gpu), i32(new, gpu),
+                        k_scale=ks, v_scale=vs)
+    for x, got, gs in ((k, kc, ks), (v, vc, vs)):
+        want, scale = x, None
+        if kind == "e4m3":
+            scale, want = ops.rowwise_quantize(x)
+        raw = got.view(torch.uint8) if kind == "e4m3" else got
+        for b, n in enumerate(new):
+            pages = table[b, :-(-n // page)].long().to(gpu)
+            rows = raw[pages].transpose(0, 1).reshape(Hkv, -1, D)
+            ref = want[b].view(torch.uint8) if kind == "e4m3" else want[b]
+            assert torch.equal(rows[:, :n], ref[:, :n])
+            assert (rows[:, n:] == 0).all()
+            if scale is not None:
+                s = gs[pages].transpose(0, 1).reshape(Hkv, -1)
+                assert torch.equal(s[:, :n], scale[b, :, :n]) and (s[:, n:] == 0).all()
+
+
 def test_append_leaves_out_what_has_no_place(gpu) -> None:
     """Rows past the table, before its start, and in pages that are none."""
     c = Cache([64, 64], 2, 64, 16, "bf16", seed=3)
