@@ -112,7 +112,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
 
 // One wave's state over its keys.  PG16: pages hold 16 rows or more, so each
 // half of a step lies in one page.
-template <int QT, int CT, int D, bool PG16>
+template <int QT, int CT, int D, bool PG16, bool STREAM>
 struct Wave {
   static constexpr bool FP8 = CT == RP_CACHE_E4M3;
   static constexpr bool QF16 = QT == kInF16;          // the first product's type
@@ -178,19 +178,25 @@ struct Wave {
     }
   }
 
+  template <typename T>
+  __device__ __forceinline__ static T v_load(const char* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+    else return *reinterpret_cast<const T*>(p);
+  }
+
   __device__ __forceinline__ void v_row(const char* p, int e) {
     if constexpr (VB == 2) {
-      vr[e][0] = *reinterpret_cast<const uint16_t*>(p);
+      vr[e][0] = v_load<uint16_t>(p);
     } else if constexpr (VB == 4) {
-      vr[e][0] = *reinterpret_cast<const uint32_t*>(p);
+      vr[e][0] = v_load<uint32_t>(p);
     } else if constexpr (VB == 8) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      const u32x2 x = v_load<u32x2>(p);
       vr[e][0] = x[0];
       vr[e][1] = x[1];
     } else {
 #pragma unroll
       for (int i = 0; i < VB / 16; ++i) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 256 * i);
+        const u32x4 x = v_load<u32x4>(p + 256 * i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) vr[e][4 * i + j] = x[j];
       }
@@ -370,9 +376,9 @@ struct Wave {
   }
 };
 
-template <int QT, int CT, int D, bool PG16>
+template <int QT, int CT, int D, bool PG16, bool STREAM>
 __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedView c) {
-  typedef Wave<QT, CT, D, PG16> W;
+  typedef Wave<QT, CT, D, PG16, STREAM> W;
   __shared__ f32x4 sacc[kDWaves / 2][W::DPL][kWave];
   __shared__ float sbase[kDWaves][16], ssum[kDWaves][16];
   const int split = blockIdx.x, b = blockIdx.z;
@@ -612,13 +618,31 @@ struct Plan {
 //   4100 keys: 22 us, 25.6 us at 512).
 // * Else a second launch is worth its 4 us where a workgroup's keys take
 //   longer than that: not up to 384 KB of them (640 keys of 128: 12.5 us a call
-//   unsplit, 16.9 in five parts), nor with two workgroups a CU already (16
-//   sequences x 32 heads: 17 us unsplit, 23 in two parts); 131071 keys in 8
-//   heads take 55 us on 512 workgroups, 58 on 1024, 64 on 2048.
+//   unsplit, 16.9 in five parts), nor with two workgroups a CU, what its
+//   registers hold, already (16 sequences x 32 heads: 17 us unsplit, 23 in two
+//   parts).  Fewer are split to no more than those 512: 131071 keys in 8 heads
+//   take 55 us on 512 workgroups, 58 on 1024, 64 on 2048.
+// * More than 512 are split where the last round of them would leave most CUs
+//   without work: a workgroup alone on its CU streams a third as fast as the
+//   whole card's share of 172 of them.
 inline Plan decode_plan(int64_t groups, int64_t keys, int64_t key_bytes, bool weights) {
-  constexpr int64_t kUnit = kDWaves * kStep;
-  const int64_t want = weights ? 1024 : keys * key_bytes <= 384 << 10 ? 1 : 512;
-  int64_t splits = (want + groups - 1) / groups;
+  constexpr int64_t kUnit = kDWaves * kStep, kRound = 512;
+  int64_t splits = 1;
+  if (weights) {
+    splits = (2 * kRound + groups - 1) / groups;
+  } else if (keys * key_bytes > 384 << 10) {
+    splits = kRound / groups;
+    if (splits == 0) {
+      splits = 1;
+      for (int64_t s = 1; s <= 4; ++s) {
+        const int64_t last = groups * s % kRound;
+        if (last == 0 || last >= kRound / 3) {
+          splits = s;
+          break;
+        }
+      }
+    }
+  }
   const int64_t most = (keys + kUnit - 1) / kUnit;
   if (splits > most) splits = most;
   if (splits > kMaxSplits) splits = kMaxSplits;
@@ -628,8 +652,17 @@ inline Plan decode_plan(int64_t groups, int64_t keys, int64_t key_bytes, bool we
   return Plan{(int32_t)splits, (int32_t)chunk};
 }
 
+// Caches larger than the 256 MB last-level cache, of which nothing would be
+// left by the next call, are read past it: V's rows, whose lines one
+// instruction takes whole, with the non-temporal hint.  One state of 8 heads
+// of 128, per call: 403 MB 71 us against 84, 806 MB 130 against 144, e4m3fn
+// 554 MB 87 against 102; 202 MB 40.5 us against 38.7 without the hint.  K's
+// rows, taken a half line at a time, are slower with it at every size.
+constexpr int64_t kStreamBytes = 256 << 20;
+
 struct Layout {
   Plan plan;
+  bool stream;
   int64_t score_ld;
   size_t ml, part, scores, total;      // byte offsets
 };
@@ -639,8 +672,10 @@ inline Layout decode_layout(int64_t B, int64_t H, const rp_paged_cache* c, int64
   const int64_t cap = c->max_pages * c->page_size, group = H / c->heads;
   const int64_t keys = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
   Layout l;
-  l.plan = decode_plan(B * c->heads * ((group + 15) / 16), keys,
-                       2 * c->head_dim * cache_elem_bytes(c->dtype), weights);
+  const int64_t key_bytes =
+      2 * (c->head_dim * cache_elem_bytes(c->dtype) + (c->dtype == RP_CACHE_E4M3 ? 4 : 0));
+  l.plan = decode_plan(B * c->heads * ((group + 15) / 16), keys, key_bytes, weights);
+  l.stream = B * c->heads * keys * key_bytes > kStreamBytes;
   auto up = [](int64_t x) { return (size_t)((x + 255) / 256 * 256); };
   const bool split = l.plan.splits > 1;
   // whole steps are written, the last one past the capacity
@@ -653,12 +688,15 @@ inline Layout decode_layout(int64_t B, int64_t H, const rp_paged_cache* c, int64
 }
 
 template <int QT, int CT, int D>
-void launch_decode_d(const DecodeArgs& a, const PagedView& c, int64_t B, hipStream_t st) {
+void launch_decode_d(const DecodeArgs& a, const PagedView& c, int64_t B, bool stream,
+                     hipStream_t st) {
   const dim3 grid((unsigned)a.splits, (unsigned)(c.heads * a.tiles), (unsigned)B);
-  if (c.shift >= 4)
-    hipLaunchKernelGGL((attend_kernel<QT, CT, D, true>), grid, dim3(kDThreads), 0, st, a, c);
-  else
-    hipLaunchKernelGGL((attend_kernel<QT, CT, D, false>), grid, dim3(kDThreads), 0, st, a, c);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kDThreads), 0, st, a, c);
+  };
+  if (c.shift < 4) go(attend_kernel<QT, CT, D, false, false>);
+  else if (stream) go(attend_kernel<QT, CT, D, true, true>);
+  else go(attend_kernel<QT, CT, D, true, false>);
   const int heads_x = a.splits > 1 ? a.H : 0;
   const int64_t blocks = a.weights ? (c.capacity() + 4 * kJThreads - 1) / (4 * kJThreads) : 0;
   if (heads_x + blocks > 0)
@@ -667,11 +705,12 @@ void launch_decode_d(const DecodeArgs& a, const PagedView& c, int64_t B, hipStre
 }
 
 template <int QT, int CT>
-void launch_decode(const DecodeArgs& a, const PagedView& c, int64_t B, int64_t D, hipStream_t st) {
-  if (D == 32) launch_decode_d<QT, CT, 32>(a, c, B, st);
-  else if (D == 64) launch_decode_d<QT, CT, 64>(a, c, B, st);
-  else if (D == 128) launch_decode_d<QT, CT, 128>(a, c, B, st);
-  else launch_decode_d<QT, CT, 256>(a, c, B, st);
+void launch_decode(const DecodeArgs& a, const PagedView& c, int64_t B, int64_t D, bool stream,
+                   hipStream_t st) {
+  if (D == 32) launch_decode_d<QT, CT, 32>(a, c, B, stream, st);
+  else if (D == 64) launch_decode_d<QT, CT, 64>(a, c, B, stream, st);
+  else if (D == 128) launch_decode_d<QT, CT, 128>(a, c, B, stream, st);
+  else launch_decode_d<QT, CT, 256>(a, c, B, stream, st);
 }
 
 }  // namespace
@@ -782,11 +821,11 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t D = cache->head_dim;
   if (q_dtype == RP_DTYPE_F16) {
-    if (fp8) launch_decode<kInF16, RP_CACHE_E4M3>(a, c, B, D, st);
-    else launch_decode<kInF16, RP_CACHE_F16>(a, c, B, D, st);
+    if (fp8) launch_decode<kInF16, RP_CACHE_E4M3>(a, c, B, D, l.stream, st);
+    else launch_decode<kInF16, RP_CACHE_F16>(a, c, B, D, l.stream, st);
   } else {
-    if (fp8) launch_decode<kInBf16, RP_CACHE_E4M3>(a, c, B, D, st);
-    else launch_decode<kInBf16, RP_CACHE_BF16>(a, c, B, D, st);
+    if (fp8) launch_decode<kInBf16, RP_CACHE_E4M3>(a, c, B, D, l.stream, st);
+    else launch_decode<kInBf16, RP_CACHE_BF16>(a, c, B, D, l.stream, st);
   }
   return paged_launched("paged_attn_decode");
 }
