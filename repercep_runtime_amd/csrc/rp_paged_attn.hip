@@ -615,7 +615,7 @@ struct Plan {
 
 // * Key weights need join_kernel anyway, so their calls split down to 1024
 //   workgroups, four a CU, which evens out ragged lengths (8 sequences of 1 to
-//   4100 keys: 22 us, 25.6 us at 512).
+//   4100 keys: a seventh less time than on 512).
 // * Else a second launch is worth its 4 us where a workgroup's keys take
 //   longer than that: not up to 384 KB of them (640 keys of 128: 12.5 us a call
 //   unsplit, 16.9 in five parts), nor with two workgroups a CU, what its
@@ -623,8 +623,12 @@ struct Plan {
 //   parts).  Fewer are split to no more than those 512: 131071 keys in 8 heads
 //   take 55 us on 512 workgroups, 58 on 1024, 64 on 2048.
 // * More than 512 are split where the last round of them would leave most CUs
-//   without work: a workgroup alone on its CU streams a third as fast as the
-//   whole card's share of 172 of them.
+//   without work (a third of the workgroups, two of three CUs, still take most
+//   of the card's rate), and so are 257 to 384, of which some CUs get two and
+//   the others one: 264 heads of 4096 keys 120 -> 95 us in three parts, 320
+//   129 -> 111 us; 416 heads 140 us unsplit, 151 in two parts; 520 heads
+//   203 -> 183 us in eight.  Parts of less than 256 KB lose more than they
+//   gain: 520 heads of 900 keys 46 us unsplit, 56 in eight parts.
 inline Plan decode_plan(int64_t groups, int64_t keys, int64_t key_bytes, bool weights) {
   constexpr int64_t kUnit = kDWaves * kStep, kRound = 512;
   int64_t splits = 1;
@@ -632,15 +636,16 @@ inline Plan decode_plan(int64_t groups, int64_t keys, int64_t key_bytes, bool we
     splits = (2 * kRound + groups - 1) / groups;
   } else if (keys * key_bytes > 384 << 10) {
     splits = kRound / groups;
-    if (splits == 0) {
-      splits = 1;
-      for (int64_t s = 1; s <= 4; ++s) {
+    if (splits == 0 || (groups > kRound / 2 && groups <= kRound * 3 / 4)) {
+      splits = 8;                                  // a short last round at least
+      for (int64_t s = groups < kRound ? 2 : 1; s <= 4; ++s) {
         const int64_t last = groups * s % kRound;
         if (last == 0 || last >= kRound / 3) {
           splits = s;
           break;
         }
       }
+      splits = max((int64_t)1, min(splits, keys * key_bytes / (256 << 10)));
     }
   }
   const int64_t most = (keys + kUnit - 1) / kUnit;

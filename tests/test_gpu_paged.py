@@ -135,7 +135,11 @@ def test_append_takes_all_rows_without_lengths_and_a_single_token(gpu) -> None:
 
 def check_decode(gpu, c: Cache, lens: list[int], H: int, qt: str, layout: str = "hnd",
                  weights: bool = False, scale: float | None = None, hint: int | None = None,
-                 seed: int = 0, q: torch.Tensor | None = None) -> None:
+                 seed: int = 0, q: torch.Tensor | None = None, columns: int = 0) -> None:
+    if columns:                            # a table wider than any sequence
+        wide = torch.full((len(lens), columns), -1, dtype=torch.int32)
+        wide[:, :c.table.shape[1]] = c.table
+        c.table = wide
     g = torch.Generator().manual_seed(100 + seed)
     if q is None:
         q = torch.randn(len(lens), H, c.D, generator=g).to(Q_DTYPES[qt])
@@ -197,6 +201,46 @@ def test_decode_over_long_caches(gpu, kind, qt, n, weights, H, Hkv) -> None:
     """Few rows and many keys: the keys are split and the parts joined."""
     c = Cache([n], Hkv, 128, 16, kind, seed=n)
     check_decode(gpu, c, [n], H, qt, weights=weights, hint=n)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "e4m3"])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode_with_room_for_long_sequences(gpu, kind, D, weights) -> None:
+    """Tables of a million positions, so the call is planned for a cache of
+    gigabytes: its V rows read past the last-level cache, a sequence's chunks
+    shared by few workgroups or ending in the first one."""
+    lens = [9000, 0, 130]
+    c = Cache(lens, 2, D, 16, kind, seed=D)
+    check_decode(gpu, c, lens, 4, "fp16" if kind == "fp16" else "bf16", weights=weights,
+                 columns=1 << 16)
+
+
+@pytest.mark.parametrize("B,Hkv", [(35, 8), (65, 8), (20, 32)])
+def test_decode_of_many_heads(gpu, B, Hkv) -> None:
+    """More workgroups than a round: 280, 520 and 640 heads, split and not."""
+    g = torch.Generator(device=gpu).manual_seed(B)
+    n, page, D = 1300, 64, 64
+    P = -(-n // page)
+    k, v = (torch.randn(P * 4, Hkv, page, D, generator=g, device=gpu).to(torch.bfloat16)
+            for _ in range(2))
+    table = torch.stack([torch.randperm(P * 4, generator=g, device=gpu)[:P] for _ in range(B)])
+    q = torch.randn(B, Hkv, 1, D, generator=g, device=gpu).to(torch.bfloat16)
+    lens = torch.randint(1, n + 1, (B,), generator=g, device=gpu)
+    out, lse = ops.paged_attention_decode(q, k, v, table.to(torch.int32), lens.to(torch.int32),
+                                          return_lse=True)
+    for b in range(0, B, 7):
+        rows = [x[table[b]].permute(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :lens[b]].double().cpu()
+                for x in (k, v)]
+        s = (rows[0] @ q[b, :, 0].double().cpu().unsqueeze(-1)).squeeze(-1) / 8.0
+        p = torch.softmax(s, -1).unsqueeze(1)
+        want, size = (p @ rows[1]).squeeze(1), (p @ rows[1].abs()).squeeze(1)
+        # the output's rounding; the fp32 sums and the weights' 16 bits within 2^-13 of sum p|v|
+        assert ((out[b, :, 0].double().cpu() - want).abs()
+                <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * size).all()
+        # scores below 16 off by (64 + 8) 2^-24 of sum |q k| / 8 < 16, and 1300 roundings of a sum
+        assert ((lse[b].double().cpu() - torch.logsumexp(s, -1)).abs()
+                <= (72 * 16 + 2600 + 200) * 2.0 ** -24).all()
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])

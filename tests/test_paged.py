@@ -143,6 +143,33 @@ def test_workspace_sizes_of_any_arguments() -> None:
         L.rp_paged_evict_workspace_bytes(2, cache(), 64) == 256 + 2 * 2 * 64 * 4
 
 
+@pytest.mark.parametrize("B,H,heads,keys,weights,parts", [
+    (1, 32, 32, 640, 0, 1),          # 320 KB of keys: one launch
+    (16, 32, 32, 640, 0, 1),         # a round of workgroups without a split
+    (1, 40, 8, 131072, 0, 64),       # 512 workgroups
+    (12, 32, 8, 4096, 0, 5),         # 480: no second round
+    (33, 32, 8, 4096, 0, 3),         # 264 would leave most CUs one, some two
+    (52, 32, 8, 4096, 0, 1),
+    (65, 32, 8, 4096, 0, 8),         # 520: 8 in a second round
+    (65, 32, 8, 900, 0, 1),          # parts of less than 256 KB
+    (75, 32, 8, 4096, 0, 2),
+    (1, 8, 1, 131072, 0, 512),
+    (8, 32, 8, 4096, 1, 16),         # with key weights: 1024 workgroups
+    (1, 1, 1, 100, 1, 1),            # no more than a workgroup's keys
+    (1, 1, 1, 1 << 30, 1, 1024),
+    (1, 32, 1, 131072, 0, 256),      # 32 query heads of a kv head: two tiles of 16
+])
+def test_attention_splits(B: int, H: int, heads: int, keys: int, weights: int,
+                          parts: int) -> None:
+    """The parts a call's keys are split into, read from the workspace they need."""
+    c = cache(heads=heads, page_size=16, max_pages=-(-keys // 16))
+    pad = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    want = pad(B * H * parts * 8) if parts > 1 or weights else 0
+    want += pad(B * H * parts * 128 * 4) if parts > 1 else 0
+    want += pad(B * H * (-(-keys // 32) * 32) * 4) if weights else 0
+    assert _capi.lib().rp_paged_attn_workspace_bytes(B, H, c, keys, weights) == want
+
+
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(logits=None), 1, "null"),
     (dict(tokens=None), 1, "null"),
