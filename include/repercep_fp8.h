@@ -571,7 +571,8 @@ int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64
  * contiguous with W >= max_pages * page_size, gets the kept rows' weights and
  * zeros behind them; new_lens[b] = min(seq_lens[b], budget).  Sequences within
  * the budget keep their rows and weights.  The sequences' pages are their own
- * (none is shared).  workspace: rp_paged_evict_workspace_bytes, 256-byte
+ * (none is shared), and new_lens and new_weights do not overlap the inputs.
+ * workspace: rp_paged_evict_workspace_bytes, 256-byte
  * aligned. */
 size_t rp_paged_evict_workspace_bytes(int64_t B, const rp_paged_cache* cache, int64_t budget);
 int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq_lens, int64_t B,

@@ -7,7 +7,8 @@ Importable spelling of the ``repercep-runtime_amd`` package.  Layers:
                  ``lib/librepercep_fp8.so`` by ``build.py``;
 * ``_capi``      ctypes binding of that library (no fallback: a missing
                  library raises);
-* ``ops``        kernel-layer torch entry points (quantize, attention, GEMM);
+* ``ops``        kernel-layer torch entry points (quantize, attention, GEMM, a
+                 decoder's step on a paged cache);
 * ``attention``  the reference's AttentionOp surface (protocol, registry,
                  FP8 op, diffusers-layout bridge);
 * ``backend``    the reference's Backend seam with MI355X added;

@@ -1066,6 +1066,10 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
         raise ValueError(f"k_cache and v_cache must share one (pages, Hkv, page_size, D) shape "
                          f"(got {tuple(k_cache.shape)}, {tuple(v_cache.shape)})")
     P, Hkv, page, D = shape
+    if D not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"head_dim {D} not in compiled tile shapes {sorted(SUPPORTED_HEAD_DIMS)}")
+    if page & (page - 1) or not 0 < page <= 65536:
+        raise ValueError(f"page_size {page} is not a power of two up to 65536")
     dtype = k_cache.dtype
     dt = _CACHE_DTYPES.get(dtype)
     if dt is None or v_cache.dtype != dtype:
@@ -1186,7 +1190,8 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     ``key_weights`` (B, Hkv, at least max_pages * page_size) fp32: each
     attended key's weight, summed over the query heads of its kv head, is
-    added to it in place, the totals that ``paged_kv_evict`` goes by.
+    added to it in place, the totals that ``paged_kv_evict`` goes by (a
+    workspace of 4 bytes a query head and position of the table).
     ``max_seq_len`` says where the lengths are expected to end (default: the
     table's end) and sets how the keys are split, not the result."""
     if q.dim() != 4 or q.shape[2] != 1:
@@ -1200,8 +1205,6 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         raise TypeError(f"q must be bfloat16 or float16 (got {q.dtype})")
     if k_cache.element_size() == 2 and k_cache.dtype != q.dtype:
         raise TypeError(f"a {k_cache.dtype} cache is not read with {q.dtype} queries")
-    if D not in SUPPORTED_HEAD_DIMS:
-        raise ValueError(f"head_dim {D} not in compiled tile shapes {sorted(SUPPORTED_HEAD_DIMS)}")
     _unit_stride("q", q)
     _int32_vector("seq_lens", seq_lens, B)
     if out is not None:
@@ -1261,9 +1264,8 @@ def paged_kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: to
     if not 0 <= recent <= budget or budget < 1:
         raise ValueError(f"needs 0 <= recent <= budget and budget >= 1 (got recent={recent}, "
                          f"budget={budget})")
-    if k_cache.dim() != 4 or k_cache.shape[3] not in SUPPORTED_HEAD_DIMS:
-        raise ValueError(f"cache {tuple(k_cache.shape)}: head_dim not in compiled tile shapes "
-                         f"{sorted(SUPPORTED_HEAD_DIMS)}")
+    if k_cache.dim() != 4:
+        raise ValueError(f"k_cache must be (pages, Hkv, page_size, D), got {tuple(k_cache.shape)}")
     slots = block_table.shape[-1] * k_cache.shape[2]
     if key_weights.dtype != torch.float32 or key_weights.dim() != 3 \
             or key_weights.shape[:2] != (B, k_cache.shape[1]) or key_weights.shape[2] < slots:

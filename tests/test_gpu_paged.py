@@ -455,11 +455,22 @@ def test_evict_ties_go_to_the_lower_position(gpu, values) -> None:
     check_evict(gpu, c, lens, torch.tensor(values)[pick], 700, 50)
 
 
-def test_evict_of_a_long_cache(gpu) -> None:
-    lens = [40000]
+@pytest.mark.parametrize("lens,odd", [([40000], 0), ([20000, 9000, 70], 0), ([20000, 8200], 3),
+                                      ([40001], 1)])
+def test_evict_of_a_long_cache(gpu, lens, odd) -> None:
+    """Weights that do not fit the short tables' registers, on and off 16-byte borders."""
     c = Cache(lens, 1, 32, 64, "bf16", seed=23)
-    w = torch.rand(1, 1, c.table.shape[1] * 64, generator=torch.Generator().manual_seed(5))
-    check_evict(gpu, c, lens, w, 20000, 1000)
+    w = torch.rand(len(lens), 1, c.table.shape[1] * 64 + odd,
+                   generator=torch.Generator().manual_seed(5))
+    check_evict(gpu, c, lens, w, max(lens) // 2, 1000)
+
+
+def test_evict_writes_every_head_of_many_caches(gpu) -> None:
+    """Caches enough for whole-line column slices: 24 x 6 heads of 256-byte rows."""
+    lens = [40 + 9 * b for b in range(24)]
+    c = Cache(lens, 6, 128, 16, "fp16", seed=25)
+    w = torch.rand(24, 6, c.table.shape[1] * 16, generator=torch.Generator().manual_seed(6))
+    check_evict(gpu, c, lens, w, 100, 10)
 
 
 def test_evict_weight_views_and_lengths_past_the_table(gpu) -> None:

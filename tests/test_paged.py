@@ -58,8 +58,8 @@ def decode(c: _capi.PagedCache, **kw) -> int:
 
 
 def evict(c: _capi.PagedCache, **kw) -> int:
-    a = dict(cache=c, lens=FAKE, B=2, w=FAKE, wsb=128, wsh=64, budget=32, recent=8, new=FAKE,
-             kept=FAKE, W=64, ws=FAKE, nbytes=1 << 20, stream=None)
+    a = dict(cache=c, lens=FAKE, B=2, w=FAKE, wsb=128, wsh=64, budget=32, recent=8, new=2 * FAKE,
+             kept=2 * FAKE, W=64, ws=FAKE, nbytes=1 << 20, stream=None)
     a.update(kw)
     return _capi.lib().rp_paged_kv_evict(*a.values())
 
@@ -100,6 +100,8 @@ def test_cache_refusals(kw: dict, status: int, msg: str) -> None:
     (decode, dict(osh=64), 1, "overlap"),
     (decode, dict(w=FAKE, ws=None, nbytes=0), 3, "workspace"),
     (evict, dict(lens=None), 1, "null"),
+    (evict, dict(new=FAKE), 1, "not the inputs"),
+    (evict, dict(kept=FAKE), 1, "not the inputs"),
     (evict, dict(budget=0), 1, "budget"),
     (evict, dict(recent=33), 1, "recent"),
     (evict, dict(recent=-1), 1, "recent"),
@@ -245,6 +247,7 @@ E4M3 = torch.float8_e4m3fn
 @pytest.mark.parametrize("kw,err,msg", [
     ({}, ValueError, "GPU tensor"),
     (dict(v_cache=_t(8, 2, 16, 64)), ValueError, "share one"),
+    (dict(k_cache=_t(8, 2, 24, 128), v_cache=_t(8, 2, 24, 128)), ValueError, "page_size"),
     (dict(v_cache=_t(8, 2, 16, 128, dtype=torch.float16)), TypeError, "both"),
     (dict(k_cache=_t(8, 2, 16, 256)[..., ::2], v_cache=_t(8, 2, 16, 256)[..., ::2]), ValueError,
      "unit stride"),
