@@ -4,7 +4,7 @@
 //   the row-wise e4m3fn quantizer (rp_rowwise_dev.h).  D / 8 lanes hold one
 //   row, a 16-byte vector each, so a row is read once, its maximum found by a
 //   butterfly and its codes written once.  Bound by HBM: 131 MB of rows into
-//   69 MB of codes and scales in 51 us (3.9 TB/s).
+//   69 MB of codes and scales in 48 us (4.2 TB/s).
 // * evict_select_kernel: which rows of one (sequence, kv head) stay: the
 //   budget-th largest weight by a radix select over order-preserving integer
 //   keys, then one ordered pass that ranks the kept rows and writes their
@@ -20,8 +20,9 @@ namespace {
 constexpr int kPThreads = 256;
 // Rows a group of lanes takes where there are workgroups enough (4096 of one
 // row a group, sixteen a CU): 16 ragged prompts of up to 4000 rows, 8 heads
-// of 128 into e4m3fn pages, take 51 us with two, 55 with one and 53 with four
-// (200 MB; 40 us at the rate of a large copy).
+// of 128 into e4m3fn pages, take 51 us with two, 55 with one and 53 with four;
+// such calls read and write past the caches: 48 us (200 MB; 40 us at the rate
+// of a large copy).
 constexpr int kAppendUnroll = 2;
 constexpr int64_t kManyRows = 4096;
 
@@ -34,8 +35,20 @@ struct AppendArgs {
   int32_t S;
 };
 
+template <bool STREAM, typename T>
+__device__ __forceinline__ void put(T x, char* to) {
+  if constexpr (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<T*>(to));
+  else *reinterpret_cast<T*>(to) = x;
+}
+
+template <bool STREAM>
+__device__ __forceinline__ u32x4r get(const uint16_t* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const u32x4r*>(p));
+  else return *reinterpret_cast<const u32x4r*>(p);
+}
+
 // One row of K or V from registers to its place.
-template <int DT, bool FP8, int TPR>
+template <int DT, bool FP8, int TPR, bool STREAM>
 __device__ __forceinline__ void append_row(const u32x4r& x, char* cache, float* scale, int64_t row,
                                            int64_t srow, int t) {
   if constexpr (FP8) {
@@ -45,11 +58,12 @@ __device__ __forceinline__ void append_row(const u32x4r& x, char* cache, float* 
     float qm, dq;
     rowwise_scales<DT>(m, &qm, &dq);
     if (row >= 0) {
-      *reinterpret_cast<uint2*>(cache + row + 8 * t) = quant8<DT>(x, qm);
+      const uint2 o = quant8<DT>(x, qm);
+      put<STREAM>(u32x2r{o.x, o.y}, cache + row + 8 * t);
       if (t == 0) scale[srow] = dq;
     }
   } else if (row >= 0) {
-    *reinterpret_cast<u32x4r*>(cache + 2 * row + 16 * t) = x;
+    put<STREAM>(x, cache + 2 * row + 16 * t);
   }
 }
 
@@ -73,16 +87,16 @@ __global__ __launch_bounds__(kPThreads) void append_kernel(AppendArgs a, PagedVi
     x[j] = y[j] = u32x4r{0u, 0u, 0u, 0u};
     row[j] = srow[j] = -1;
     if (page >= 0) {
-      x[j] = *reinterpret_cast<const u32x4r*>(a.k + b * a.ksb + h * a.ksh + i * a.kss + 8 * t);
-      y[j] = *reinterpret_cast<const u32x4r*>(a.v + b * a.vsb + h * a.vsh + i * a.vss + 8 * t);
+      x[j] = get<(U > 1)>(a.k + b * a.ksb + h * a.ksh + i * a.kss + 8 * t);
+      y[j] = get<(U > 1)>(a.v + b * a.vsb + h * a.vsh + i * a.vss + 8 * t);
       row[j] = paged_row(c, page, h, pos);
       if constexpr (FP8) srow[j] = paged_scale(c, page, h, pos);
     }
   }
 #pragma unroll
   for (int j = 0; j < U; ++j) {
-    append_row<DT, FP8, TPR>(x[j], c.k, c.ks, row[j], srow[j], t);
-    append_row<DT, FP8, TPR>(y[j], c.v, c.vs, row[j], srow[j], t);
+    append_row<DT, FP8, TPR, (U > 1)>(x[j], c.k, c.ks, row[j], srow[j], t);
+    append_row<DT, FP8, TPR, (U > 1)>(y[j], c.v, c.vs, row[j], srow[j], t);
   }
 }
 
@@ -298,7 +312,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, 
 // move 2 x 120 MB in 64 us (3.8 TB/s).
 constexpr int kMoveThreads = 1024, kMoveUnroll = 4;
 
-template <typename T, typename Offset>
+template <bool STREAM, typename T, typename Offset>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& c,
                                           const int32_t* src, const int32_t* table, int h,
                                           int begin, int r, int step, T* base, Offset offset) {
@@ -319,10 +333,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& c
   find(begin);
   for (int r0 = begin; r0 < a.budget; r0 += step * kMoveUnroll) {
     T x[kMoveUnroll];
-    int64_t put[kMoveUnroll];
+    int64_t dst[kMoveUnroll];
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
-      put[u] = to[u];
+      dst[u] = to[u];
       x[u] = T{};
       if (at[u] >= 0) x[u] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at[u]);
     }
@@ -334,12 +348,15 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& c
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u)
-      if (put[u] >= 0) *reinterpret_cast<T*>(reinterpret_cast<char*>(base) + put[u]) = x[u];
+      if (dst[u] >= 0) put<STREAM>(x[u], reinterpret_cast<char*>(base) + dst[u]);
   }
 }
 
+// LINES: slices of whole 128-byte lines, written past the caches (32 caches of
+// 8 heads cut to 2048 rows: 77 us a call against 82).
+template <bool LINES>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, PagedView c,
-                                                               int slices, int lanes) {
+                                                                  int slices, int lanes) {
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t g = (int64_t)b * c.heads + h;
   const int begin = a.first[g];
@@ -350,14 +367,15 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, P
   if (kind == 2) {
     // K's in the first half of the threads, V's in the second
     float* s = threadIdx.x < kMoveThreads / 2 ? c.ks : c.vs;
-    move_rows(a, c, src, table, h, begin, threadIdx.x & (kMoveThreads / 2 - 1), kMoveThreads / 2, s,
+    move_rows<false>(a, c, src, table, h, begin, threadIdx.x & (kMoveThreads / 2 - 1),
+                     kMoveThreads / 2, s,
               [&](int32_t p, int64_t pos) { return paged_scale(c, p, h, pos) * 4; });
     return;
   }
   u32x4r* base = reinterpret_cast<u32x4r*>(kind == 0 ? c.k : c.v);
   const int eb = c.ks ? 1 : 2;
   const int col = ((blockIdx.x % slices) * lanes + threadIdx.x % lanes) * 16;
-  move_rows(a, c, src, table, h, begin, threadIdx.x / lanes, kMoveThreads / lanes, base,
+  move_rows<LINES>(a, c, src, table, h, begin, threadIdx.x / lanes, kMoveThreads / lanes, base,
             [&](int32_t p, int64_t pos) { return paged_row(c, p, h, pos) * eb + col; });
 }
 
@@ -488,8 +506,12 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
   const bool lines = row_bytes >= 128 && B * c.heads * 2 * (row_bytes / 128) >= 256;
   const int lanes = lines ? 8 : row_bytes >= 64 ? 4 : row_bytes / 16;
   const int slices = row_bytes / (16 * lanes);
-  hipLaunchKernelGGL(evict_move_kernel,
-                     dim3((unsigned)(2 * slices + (c.ks ? 1 : 0)), (unsigned)c.heads, (unsigned)B),
-                     dim3(kMoveThreads), 0, st, a, c, slices, lanes);
+  auto move = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel,
+                       dim3((unsigned)(2 * slices + (c.ks ? 1 : 0)), (unsigned)c.heads, (unsigned)B),
+                       dim3(kMoveThreads), 0, st, a, c, slices, lanes);
+  };
+  if (lines) move(evict_move_kernel<true>);
+  else move(evict_move_kernel<false>);
   return paged_launched("paged_kv_evict");
 }

@@ -1050,7 +1050,8 @@ def fp8_scaled_mm_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *
 # A decoder's step: new keys and values into a cache of pages, one new token's
 # attention over it, its eviction by attention weight, and the scores of the
 # chosen tokens.  The reference decodes through HF generate on bf16 SDPA and
-# has no counterpart of these.
+# has no counterpart of these.  Inference only, as all of this module: no
+# gradient passes through.
 
 def _int32_vector(name: str, t: torch.Tensor, n: int) -> None:
     if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
@@ -1083,6 +1084,9 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
             or block_table.stride(1) != 1:
         raise ValueError(f"block_table must be int32 ({B}, max_pages) with contiguous rows "
                          f"(got {block_table.dtype} {tuple(block_table.shape)})")
+    if P < 1 or Hkv < 1 or table[1] < 1:
+        raise ValueError(f"a cache needs pages, heads and a table to name them (got "
+                         f"{tuple(k_cache.shape)}, block_table {tuple(block_table.shape)})")
     dev = k_cache.get_device()
     ks = vs = 0
     if dt == C.RP_CACHE_E4M3:

@@ -248,6 +248,8 @@ E4M3 = torch.float8_e4m3fn
     ({}, ValueError, "GPU tensor"),
     (dict(v_cache=_t(8, 2, 16, 64)), ValueError, "share one"),
     (dict(k_cache=_t(8, 2, 24, 128), v_cache=_t(8, 2, 24, 128)), ValueError, "page_size"),
+    (dict(k_cache=_t(0, 2, 16, 128), v_cache=_t(0, 2, 16, 128)), ValueError, "needs pages"),
+    (dict(block_table=_t(3, 0, dtype=torch.int32)), ValueError, "needs pages"),
     (dict(v_cache=_t(8, 2, 16, 128, dtype=torch.float16)), TypeError, "both"),
     (dict(k_cache=_t(8, 2, 16, 256)[..., ::2], v_cache=_t(8, 2, 16, 256)[..., ::2]), ValueError,
      "unit stride"),
