@@ -4,8 +4,8 @@
 // VALU about 15 lane operations each, so a row is read once, into registers,
 // and everything is computed from there:
 //   M = max x,  t = x c - M c  (c = log2(e) / temperature),
-//   s = sum 2^t,  u = sum 2^t t,
-//   log p(x) = ln 2 (t - log2 s),  entropy = ln 2 (log2 s - u / s).
+//   s = n + r = sum 2^t (n: largest logits left out of r),  u = sum 2^t t,
+//   log p(x) = ln 2 t - log(s),  entropy = log(s) - ln 2 u / s.
 // t is one fma, so logits far from zero lose nothing; t below -200 (2^t = 0)
 // is held there, so a masked logit adds 0 and not 0 * inf.
 //
@@ -48,7 +48,7 @@ struct LogprobArgs {
   float* entropy;
   float* top_logprobs;
   int64_t* top_ids;
-  f32x4* sums;              // (N, parts): M, s, u of each part
+  f32x4* sums;              // (N, parts): M, n, r, u of each part
   uint64_t* keys;           // (N, parts, top)
 };
 
@@ -74,25 +74,27 @@ __device__ __forceinline__ float logit_at(const char* row, int64_t i) {
   else return in_to_f32<DT == RP_OUT_F16 ? kInF16 : kInBf16>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
-// Whether fp32(M c) is within 2^-4 of M c: then t is one fma about it, an exact
-// base like any other.  A low temperature or a row of lowest values takes
-// (x - M) c.
+// Whether fp32(M c) is within 2^-4 of M c: then t is one fma about it, and the
+// sums are moved to M c afterwards.  A low temperature or a row of lowest
+// values takes (x - M) c.
 __device__ __forceinline__ bool near(float m, float c) { return fabsf(m * c) < 0x1p20f; }
 
-// What one (M, s, u) says of a row: its log probabilities and entropy.
+// What a row's sums say of it: its log probabilities and entropy.  s = n + r:
+// n largest logits weigh 1 each, the others r together, kept apart so that a
+// row that is all but certain keeps its small entropy and log probability.
 struct Row {
   double base;
-  float s, u, c;
-  __device__ __forceinline__ Row(float m, float s_, float u_, float c_) : s(s_), u(u_), c(c_) {
-    base = near(m, c) ? (double)(m * c) : (double)m * (double)c;
-  }
+  float n, r, u, c, lg;
+  __device__ __forceinline__ Row(float m, float n_, float r_, float u_, float c_)
+      : base((double)m * (double)c_), n(n_), r(r_), u(u_), c(c_), lg(log1pf(n_ - 1.0f + r_)) {}
+  __device__ __forceinline__ bool none() const { return n == 0.0f && r == 0.0f; }
   __device__ __forceinline__ float logprob(float x) const {
-    if (s == 0.0f) return -__builtin_inff();
+    if (none()) return -__builtin_inff();
     // in 64 bits: a lowest value's log probability is finite
-    return (float)(((double)x * (double)c - base - (double)__builtin_amdgcn_logf(s)) * kLn2);
+    return (float)(((double)x * (double)c - base) * kLn2 - (double)lg);
   }
   __device__ __forceinline__ float entropy() const {
-    return s == 0.0f ? 0.0f : (float)(((double)__builtin_amdgcn_logf(s) - (double)u / (double)s) * kLn2);
+    return none() ? 0.0f : lg - (float)kLn2 * u / (n + r);
   }
 };
 
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   constexpr int GROUP = T / kWave;                  // threads per group: 64 groups
   constexpr bool PACKED = EB == 2;
   __shared__ float group_max[kWave];
-  __shared__ float wave_sum[2][WAVES];
+  __shared__ float wave_sum[3][WAVES];
   __shared__ u32x4 hit[kHits];                      // vectors that reach the bound
   __shared__ int32_t hit_at[kHits];                 // their first logits
   __shared__ uint64_t found[kHits * EPV + 2 * EPV];
@@ -276,15 +278,16 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   phase();
 
   float s = 0.0f, u = 0.0f;
-  auto weigh = [&](auto power) {
+  // power(x) gives t, weight(x, p) a logit's weight (p, or 0 for one left out)
+  auto weigh = [&](auto power, auto weight) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       forget(v);                                      // or the branches' common unpacking moves up
       float s1 = 0.0f, u1 = 0.0f;                     // short sums, then theirs
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
-        const float t = power(value(v, e));
-        const float p = __builtin_amdgcn_exp2f(t);
+        const float x = value(v, e), t = power(x);
+        const float p = weight(x, __builtin_amdgcn_exp2f(t));
         s1 += p;
         u1 = __builtin_fmaf(p, t, u1);
       }
@@ -293,20 +296,37 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  auto all = [](float, float p) { return p; };
   const float base = m0 * a.c;
-  const bool fma = near(m0, a.c);
-  if (!fma) {
-    weigh([&](float x) { return nmax((x - m0) * a.c, -200.0f); });
-  } else if (!PACKED || a.c > 0x1p20f || __any(low16 >= kLow16<DT>)) {
-    weigh([&](float x) { return nmax(__builtin_fmaf(x, a.c, -base), -200.0f); });
-  } else {
-    weigh([&](float x) { return __builtin_fmaf(x, a.c, -base); });
+  const bool fma = near(m0, a.c), best = mine == m && m > -__builtin_inff();
+  const float shift = fma ? __builtin_fmaf(m0, a.c, -base) : 0.0f;     // exact
+  const uint64_t bests = __ballot(best);
+  bool left_out = !best;                              // a thread that holds M leaves one M out
+  if (has_edge) {
+    const float t = nmax((extra - m0) * a.c, -200.0f);
+    const bool skip = !left_out && extra == m;
+    left_out |= skip;
+    s = skip ? 0.0f : __builtin_amdgcn_exp2f(t);
+    u = s * t;
   }
-  if (wave == 0) {                                    // the edges are in its first 16 lanes
-    const float t = nmax(fma ? __builtin_fmaf(extra, a.c, -base) : (extra - m0) * a.c, -200.0f);
-    const float p = __builtin_amdgcn_exp2f(t);
-    s += p;
-    u = __builtin_fmaf(p, t, u);
+  if (bests || !fma) {
+    weigh([&](float x) { return nmax((x - m0) * a.c, -200.0f); },
+          [&](float x, float p) {
+            const bool skip = !left_out && x == m;
+            left_out |= skip;
+            return skip ? 0.0f : p;
+          });
+  } else {
+    const float s0 = s, u0 = u;
+    s = u = 0.0f;
+    if (!PACKED || a.c > 0x1p20f || __any(low16 >= kLow16<DT>))
+      weigh([&](float x) { return nmax(__builtin_fmaf(x, a.c, -base), -200.0f); }, all);
+    else
+      weigh([&](float x) { return __builtin_fmaf(x, a.c, -base); }, all);
+    // from powers about fp32(M c) to powers about M c
+    const float f = __builtin_amdgcn_exp2f(-shift);
+    u = __builtin_fmaf(f, __builtin_fmaf(-shift, s, u), u0);
+    s = __builtin_fmaf(f, s, s0);
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
@@ -316,19 +336,23 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   if (lane == 0) {
     wave_sum[0][wave] = s;
     wave_sum[1][wave] = u;
+    wave_sum[2][wave] = (float)__popcll(bests);
   }
   __syncthreads();
   s = u = 0.0f;
+  float n_best = 0.0f;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
     s += wave_sum[0][w];
     u += wave_sum[1][w];
+    n_best += wave_sum[2][w];
   }
-  const bool odd = s != s;                            // a NaN or +inf: no distribution
-  const Row r(m0, s, u, a.c);
+  const bool odd = s != s || !(m < __builtin_inff());   // a NaN or +inf: no distribution
+  if (odd) s = __builtin_nanf("");
+  const Row r(m0, n_best, s, u, a.c);
   if (tid == 0) {
     if (a.parts == 1) write_row(a, r, row, token, xt);
-    else a.sums[row * a.parts + part] = f32x4{m0, s, u, 0.0f};
+    else a.sums[row * a.parts + part] = f32x4{m0, n_best, s, u};
   }
   if (a.top == 0) return;
   uint64_t* keys = a.keys + (row * a.parts + part) * a.top;
@@ -399,24 +423,26 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
   // a part a lane; one of nothing but -inf has no maximum
   static_assert(kMaxParts <= kWave, "a row's parts fit a wave");
   const f32x4 p = lane < a.parts ? a.sums[row * a.parts + lane] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const bool some = p[1] != 0.0f;
+  const float whole = p[1] + p[2];
+  const bool some = whole != 0.0f;
   float m = some ? p[0] : -__builtin_inff();
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) m = nmax(m, __shfl_xor(m, o, kWave));
-  const double base = Row(m, 0.0f, 0.0f, a.c).base;
-  float s = 0.0f, u = 0.0f;
+  float nb = 0.0f, s = 0.0f, u = 0.0f;
   if (some) {
-    const float t = nmax((float)(Row(p[0], 0.0f, 0.0f, a.c).base - base), -200.0f);
+    const float t = nmax((float)((double)p[0] * (double)a.c - (double)m * (double)a.c), -200.0f);
     const float f = __builtin_amdgcn_exp2f(t);
-    s = p[1] * f;
-    u = f * __builtin_fmaf(p[1], t, p[2]);
+    nb = t == 0.0f ? p[1] : 0.0f;                    // the parts that hold the row's maximum
+    s = t == 0.0f ? p[2] : whole * f;
+    u = f * __builtin_fmaf(whole, t, p[3]);
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
+    nb += __shfl_xor(nb, o, kWave);
     s += __shfl_xor(s, o, kWave);
     u += __shfl_xor(u, o, kWave);
   }
-  const Row r(m, s, u, a.c);
+  const Row r(m, nb, s, u, a.c);
   for (int i = lane; i < n; i += kWave) {
     const uint64_t key = keys[i];
     if (key == 0) continue;

@@ -106,6 +106,34 @@ def test_large_logits(gpu, shift) -> None:
     check(gpu, (logits(3, 3001, "fp32", 2) + shift).float(), 8)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("V", [60, 5001, 33000, 100000])
+@pytest.mark.parametrize("gap", [12.0, 25.0, 60.0])
+def test_nearly_certain_rows(gpu, dt, V, gap) -> None:
+    """One logit far above the others: the small entropy and the small log
+    probability of its token keep their relative precision.  With r the others'
+    weight, log(1 + r) and sum p |z| are sums of positive terms, each off by
+    the rounding of its power's argument (at most 90: 90 u, a few u more), a
+    sum's V u at most (trees: far less) and a handful of operations."""
+    x = logits(3, V, dt, V, std=1.0)
+    best = torch.tensor([0, V // 2, V - 1])
+    x[torch.arange(3), best] = x.amax(-1) + torch.tensor(gap).to(x.dtype)
+    lp, ent, _, _ = reference(x, best, 1, 1.0)
+    z = x.double() - x.double().amax(-1, keepdim=True)
+    rest = torch.exp(z)
+    rest[torch.arange(3), best] = 0.0
+    # in 64 bits from the others alone: logsumexp's own 1 + r loses r below 2^-53
+    r = rest.sum(-1)
+    lp = -torch.log1p(r)
+    ent = torch.log1p(r) - (rest * z).sum(-1) / (1 + r)
+    got = ops.token_logprobs(x.to(gpu), best.to(gpu), top=1)
+    tol = (2 * 100 + min(V, 4096) + 32) * U
+    assert torch.equal(got.top_ids[:, 0].cpu(), best)
+    assert ((got.logprobs.cpu().double() - lp).abs() <= tol * lp.abs()).all()
+    assert ((got.top_logprobs[:, 0].cpu().double() - lp).abs() <= tol * lp.abs()).all()
+    assert ((got.entropy.cpu().double() - ent).abs() <= tol * ent).all()
+
+
 def test_wide_spread(gpu) -> None:
     """One token takes all; the others' probabilities leave the type's range."""
     check(gpu, logits(3, 5000, "fp32", 3, std=200.0), 32)
