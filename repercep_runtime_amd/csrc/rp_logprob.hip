@@ -19,9 +19,9 @@
 // A workgroup holds up to 64 logits a thread.  Longer rows are split over
 // workgroups; logprob_join_kernel merges their sums and their best.
 //
-// Bound by the VALU beside HBM: 4096 rows of 128256 16-bit logits take 243 us
-// with 20 alternatives (4.3 TB/s), 220 without (4.8); 11 instructions a logit,
-// of which the exponential counts four times.
+// Bound by the VALU beside HBM: 4096 rows of 128256 16-bit logits take 268 us
+// with 20 alternatives (3.9 TB/s); 11 instructions a logit, of which the
+// exponential counts four times.
 
 #include <type_traits>
 
@@ -80,7 +80,7 @@ __device__ __forceinline__ float logit_at(const char* row, int64_t i) {
 __device__ __forceinline__ bool near(float m, float c) { return fabsf(m * c) < 0x1p20f; }
 
 // What a row's sums say of it: its log probabilities and entropy.  s = n + r:
-// n largest logits weigh 1 each, the others r together, kept apart so that a
+// n largest logits weigh 1 each, the rest r together, kept apart so that a
 // row that is all but certain keeps its small entropy and log probability.
 struct Row {
   double base;
@@ -142,12 +142,12 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   constexpr int GROUP = T / kWave;                  // threads per group: 64 groups
   constexpr bool PACKED = EB == 2;
   __shared__ float group_max[kWave];
-  __shared__ float wave_sum[3][WAVES];
+  __shared__ float wave_sum[2][WAVES];
   __shared__ u32x4 hit[kHits];                      // vectors that reach the bound
   __shared__ int32_t hit_at[kHits];                 // their first logits
   __shared__ uint64_t found[kHits * EPV + 2 * EPV];
   __shared__ uint64_t wave_best[WAVES];
-  __shared__ int hits, count;
+  __shared__ int hits, count, best_count;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   const int skew = (int)((reinterpret_cast<uintptr_t>(xr + (int64_t)c0 * EB) & 15) / EB);
   const int a0 = min(c1, c0 + (skew ? EPV - skew : 0));     // the vectors' logits: [a0, a1)
   const int a1 = a0 + (c1 - a0) / EPV * EPV;
-  if (tid == 0) hits = count = 0;
+  if (tid == 0) hits = count = best_count = 0;
 
   const u32x4* src = reinterpret_cast<const u32x4*>(xr + (int64_t)a0 * EB);
   const int nvec = (a1 - a0) / EPV;
@@ -278,16 +278,16 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   phase();
 
   float s = 0.0f, u = 0.0f;
-  // power(x) gives t, weight(x, p) a logit's weight (p, or 0 for one left out)
-  auto weigh = [&](auto power, auto weight) {
+  auto weigh = [&](auto power) {                      // power(x) gives t
+
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       forget(v);                                      // or the branches' common unpacking moves up
       float s1 = 0.0f, u1 = 0.0f;                     // short sums, then theirs
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
-        const float x = value(v, e), t = power(x);
-        const float p = weight(x, __builtin_amdgcn_exp2f(t));
+        const float t = power(value(v, e));
+        const float p = __builtin_amdgcn_exp2f(t);
         s1 += p;
         u1 = __builtin_fmaf(p, t, u1);
       }
@@ -296,63 +296,72 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto all = [](float, float p) { return p; };
   const float base = m0 * a.c;
-  const bool fma = near(m0, a.c), best = mine == m && m > -__builtin_inff();
+  const bool fma = near(m0, a.c);
   const float shift = fma ? __builtin_fmaf(m0, a.c, -base) : 0.0f;     // exact
-  const uint64_t bests = __ballot(best);
-  bool left_out = !best;                              // a thread that holds M leaves one M out
-  if (has_edge) {
-    const float t = nmax((extra - m0) * a.c, -200.0f);
-    const bool skip = !left_out && extra == m;
-    left_out |= skip;
-    s = skip ? 0.0f : __builtin_amdgcn_exp2f(t);
-    u = s * t;
+  auto exact = [&](float x) { return nmax((x - m0) * a.c, -200.0f); };
+  if (!fma)
+    weigh(exact);
+  else if (!PACKED || a.c > 0x1p20f || __any(low16 >= kLow16<DT>))
+    weigh([&](float x) { return nmax(__builtin_fmaf(x, a.c, -base), -200.0f); });
+  else
+    weigh([&](float x) { return __builtin_fmaf(x, a.c, -base); });
+  if (wave == 0) {                                    // the edges are in its first 16 lanes
+    const float t = nmax(fma ? __builtin_fmaf(extra, a.c, -base) : exact(extra), -200.0f);
+    const float p = __builtin_amdgcn_exp2f(t);
+    s += p;
+    u = __builtin_fmaf(p, t, u);
   }
-  if (bests || !fma) {
-    weigh([&](float x) { return nmax((x - m0) * a.c, -200.0f); },
-          [&](float x, float p) {
-            const bool skip = !left_out && x == m;
-            left_out |= skip;
-            return skip ? 0.0f : p;
-          });
-  } else {
-    const float s0 = s, u0 = u;
+  auto total = [&]() {                                // of the workgroup, in every thread
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      s += __shfl_xor(s, o, kWave);
+      u += __shfl_xor(u, o, kWave);
+    }
+    if (lane == 0) {
+      wave_sum[0][wave] = s;
+      wave_sum[1][wave] = u;
+    }
+    __syncthreads();
     s = u = 0.0f;
-    if (!PACKED || a.c > 0x1p20f || __any(low16 >= kLow16<DT>))
-      weigh([&](float x) { return nmax(__builtin_fmaf(x, a.c, -base), -200.0f); }, all);
-    else
-      weigh([&](float x) { return __builtin_fmaf(x, a.c, -base); }, all);
-    // from powers about fp32(M c) to powers about M c
-    const float f = __builtin_amdgcn_exp2f(-shift);
-    u = __builtin_fmaf(f, __builtin_fmaf(-shift, s, u), u0);
-    s = __builtin_fmaf(f, s, s0);
-  }
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    s += __shfl_xor(s, o, kWave);
-    u += __shfl_xor(u, o, kWave);
+    for (int w = 0; w < WAVES; ++w) {
+      s += wave_sum[0][w];
+      u += wave_sum[1][w];
+    }
+  };
+  total();
+  const bool odd = s != s;                            // a NaN or +inf: no distribution
+  // from powers about fp32(M c) to powers about M c
+  const float f = __builtin_amdgcn_exp2f(-shift);
+  u = f * __builtin_fmaf(-shift, s, u);
+  float n_best = s == 0.0f ? 0.0f : 1.0f, r_sum = s == 0.0f ? 0.0f : f * s - 1.0f;
+  if (!odd && s > 0.0f && r_sum < 0x1p-8f) {          // the same in every thread
+    // All but certain: 1 + r keeps too little of r, so the others are summed
+    // again without the logits that equal M.
+    int equal = 0;
+    s = u = 0.0f;
+    // from memory: this path is rare, and registers kept for it would cost the
+    // others
+#pragma unroll 8
+    for (int i = c0 + tid; i < c1; i += T) {
+      const float x = logit_at<DT>(xr, i), t = exact(x);
+      const float p = x == m0 ? 0.0f : __builtin_amdgcn_exp2f(t);
+      equal += x == m0;
+      s += p;
+      u = __builtin_fmaf(p, t, u);
+    }
+    if (equal) atomicAdd(&best_count, equal);
+    __syncthreads();                                  // the first sums have been read
+    total();
+    n_best = (float)best_count;
+    r_sum = s;
   }
-  if (lane == 0) {
-    wave_sum[0][wave] = s;
-    wave_sum[1][wave] = u;
-    wave_sum[2][wave] = (float)__popcll(bests);
-  }
-  __syncthreads();
-  s = u = 0.0f;
-  float n_best = 0.0f;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    s += wave_sum[0][w];
-    u += wave_sum[1][w];
-    n_best += wave_sum[2][w];
-  }
-  const bool odd = s != s || !(m < __builtin_inff());   // a NaN or +inf: no distribution
-  if (odd) s = __builtin_nanf("");
-  const Row r(m0, n_best, s, u, a.c);
+  // made where it is used: its logarithm is a few dozen instructions
+  auto whole_row = [&]() { return Row(m0, n_best, odd ? __builtin_nanf("") : r_sum, u, a.c); };
   if (tid == 0) {
-    if (a.parts == 1) write_row(a, r, row, token, xt);
-    else a.sums[row * a.parts + part] = f32x4{m0, n_best, s, u};
+    if (a.parts == 1) write_row(a, whole_row(), row, token, xt);
+    else a.sums[row * a.parts + part] = f32x4{m0, n_best, odd ? __builtin_nanf("") : r_sum, u};
   }
   if (a.top == 0) return;
   uint64_t* keys = a.keys + (row * a.parts + part) * a.top;
@@ -372,7 +381,7 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
 #pragma unroll 8
       for (int j = 0; j < n; ++j) rank += found[j] > key;
       if (rank < a.top) {
-        if (a.parts == 1) write_top(a, r, row, rank, key);
+        if (a.parts == 1) write_top(a, whole_row(), row, rank, key);
         else keys[rank] = key;
       }
     }
@@ -401,7 +410,7 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
     last = best;
     if (tid == 0) {
       if (a.parts > 1) keys[k] = best;
-      else if (best) write_top(a, r, row, k, best);
+      else if (best) write_top(a, whole_row(), row, k, best);
     }
   }
 }
@@ -463,8 +472,8 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
 
 // Threads, vectors a thread and logits a part, by the row's length: one part
 // where 512 threads of 64 logits hold the row, fewer logits a thread for short
-// rows.  4096 rows of 128256 take 247 us in parts of 32064 on 512 threads, 275
-// in parts of 16032 on 256, 293 on 1024 threads of 32 logits.
+// rows.  Of 4096 rows of 128256 parts of 32064 on 512 threads were the fastest:
+// parts of 16032 on 256 took 1% more, 1024 threads of 32 logits 8% more.
 struct LogprobPlan {
   int threads, vectors, parts, chunk;
 };
