@@ -21,7 +21,8 @@
 //
 // Bound by the VALU beside HBM: 4096 rows of 128256 16-bit logits take 268 us
 // with 20 alternatives (3.9 TB/s); 11 instructions a logit, of which the
-// exponential counts four times.
+// exponential counts four times.  Rows of 16-bit logits below zero take their
+// maxima twice: 325 us, 274 for rows with some above it.
 
 #include <type_traits>
 
@@ -130,6 +131,11 @@ __device__ __forceinline__ float half_max(uint32_t w) {
   const uint32_t x = (uint32_t)(lo > hi ? lo : hi) & 0xffffu;
   return DT == RP_OUT_F16 ? f16_to_f32(x) : bf16_to_f32(x);
 }
+__device__ __forceinline__ uint32_t pk_min_u16(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
 // 16-bit logits whose t may leave fp32's range (c up to 2^20): -2^100 and below, fp16's -inf
 template <int DT>
 constexpr uint32_t kLow16 = DT == RP_OUT_F16 ? 0xfc00u : 0xf180u;
@@ -188,10 +194,11 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   };
 
   // Maxima of each vector and of the thread.  Of 16-bit logits, two at a time
-  // as signed integers: right where any is at or above 0, and else some
-  // logit of the thread (the lowest), which shows as a negative part maximum
-  // and sends the part through the exact loop below.  As unsigned integers
-  // the largest is the most negative logit (or a NaN of that sign).
+  // as signed integers: right where any has a clear sign bit.  Of others (-0
+  // among them) it is some logit, not above the true maximum, which is at most
+  // 0; so a bound above 0 and what reaches it are right, and any other bound
+  // sends the part through the exact maxima below.  As unsigned integers the
+  // largest is the most negative logit (or a NaN of that sign).
   uint32_t vec16[NV], low16 = 0;
   float vec_max[NV], mine = -__builtin_inff();
   if constexpr (PACKED) {
@@ -229,26 +236,9 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
   };
   exchange();
   phase();
-  if constexpr (PACKED) {
-    if (m < 0.0f) {                                 // the same in every thread
-      __syncthreads();
-      mine = extra;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        forget(v);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) mine = nmax(mine, value(v, e));
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      exchange();
-    }
-    phase();
-  }
-  const float m0 = m == -__builtin_inff() ? 0.0f : m;
-
   // the bound: the top-th largest group maximum, its low bits dropped
   float bound = __builtin_inff();
-  if (a.top > 0) {
+  auto find_bound = [&]() {
     const uint32_t k = logit_key(gm);
     uint32_t b = 0;
 #pragma unroll
@@ -257,12 +247,34 @@ __global__ __launch_bounds__(T) void logprob_kernel(LogprobArgs a) {
       if (__popcll(__ballot(k >= cand)) >= a.top) b = cand;
     }
     bound = key_logit(b < kKeyNegInf ? kKeyNegInf : b);
+  };
+  if (a.top > 0) find_bound();
+  if constexpr (PACKED) {
+    if (m < 0.0f || bound <= 0.0f) {                // the same in every thread
+      __syncthreads();
+      mine = extra;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        forget(v);
+        // eight sign bits: the largest logit is the least unsigned integer
+        const uint32_t lo = pk_min_u16(pk_min_u16(raw[v][0], raw[v][1]),
+                                       pk_min_u16(raw[v][2], raw[v][3]));
+        if ((vec16[v] & 0x80008000u) == 0x80008000u)
+          vec16[v] = min(lo & 0xffffu, lo >> 16) * 0x10001u;
+        mine = nmax(mine, half_max<DT>(vec16[v]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      exchange();
+      if (a.top > 0) find_bound();
+    }
+    phase();
   }
+  const float m0 = m == -__builtin_inff() ? 0.0f : m;
   if (mine >= bound) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if constexpr (PACKED) {
-        if (bound >= 0.0f && half_max<DT>(vec16[v]) < bound) continue;
+        if (half_max<DT>(vec16[v]) < bound) continue;
       } else {
         if (vec_max[v] < bound) continue;
       }

@@ -248,3 +248,43 @@ def test_equal_calls_give_equal_bits(gpu) -> None:
         a = ops.token_logprobs(x, t, top=20)
         for _ in range(3):
             assert all(torch.equal(p, q) for p, q in zip(a, ops.token_logprobs(x, t, top=20)))
+
+
+def _rows_below_zero(V: int, dt: str, top: int) -> torch.Tensor:
+    """Rows whose logits lie wholly or mostly below zero: shifted by their
+    maximum; log probabilities of nearly certain rows, the best at -0 in one;
+    N(-9, 2.5) and N(-30, 2.5); a negative bulk with 1, top - 1, top and 40
+    logits at or above zero; zeros of both signs among negatives; sorted rows
+    that cross zero, either way."""
+    g = torch.Generator().manual_seed(V + top)
+    rnd = torch.randn(10, V, generator=g, dtype=torch.float64) * 2.5
+    shifted = rnd[0] - rnd[0].max()
+    sure = rnd[1].clone()
+    sure[V // 3] += 40.0
+    sure = torch.log_softmax(sure, 0)
+    best = sure.clone()
+    best[V // 3] = -0.0
+    few = []
+    for i, n in enumerate((1, top - 1, top, 40)):
+        x = rnd[4 + i] - 14.0
+        at = torch.randperm(V, generator=g)[:n]
+        x[at] = torch.rand(len(at), generator=g, dtype=torch.float64) * 6.0
+        few.append(x)
+    zeros = torch.tensor([0.0, -0.0, -1.0, -2.0, -3.0], dtype=torch.float64)
+    mixed = zeros[torch.randint(2, 5, (V,), generator=g)]
+    at = torch.randperm(V, generator=g)[:max(2, min(V // 4, 2 * top))]
+    mixed[at] = zeros[torch.randint(0, 2, (len(at),), generator=g)]
+    lowest = zeros[torch.randint(2, 5, (V,), generator=g)]
+    lowest[at] = -0.0
+    up = torch.linspace(-6.0, 3.0, V, dtype=torch.float64)
+    rows = [shifted, sure, best, rnd[8] - 9.0, rnd[9] - 30.0, *few, mixed, lowest, up, up.flip(0)]
+    return torch.stack(rows).to(DTYPES[dt])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("V", [60, 1000, 2047, 8192, 32000, 40001, 128256])
+@pytest.mark.parametrize("top", [1, 5, 16, 20, 32])
+def test_best_of_rows_below_zero(gpu, dt, V, top) -> None:
+    """16-bit logits at or below zero: the best and their order, one part a
+    row and several, rows on and off 16-byte borders."""
+    check(gpu, _rows_below_zero(V, dt, top), top, seed=top)
