@@ -16,9 +16,13 @@
 // * V's operand needs eight keys of one column in a register quad.  A lane
 //   loads D / 16 columns of each of its eight rows and transposes them with
 //   byte permutes (v_perm_b32), one per pair of values.
-// * P enters the second product as the sum of two 16-bit numbers, the rounded
-//   weight and the rounded rest (16 bits of it or more), so the output keeps
-//   the accuracy of an fp32 weight; the products are idle otherwise.
+// * P enters the second product as the sum of two bf16 numbers, the rounded
+//   weight and the rounded rest: 16 bits of any weight, however small beside
+//   the largest (fp16 would cut weights below 2^-20 of it).  An fp16 V is the
+//   exact sum of two bf16 numbers, its first eight bits and the other three,
+//   so its second product is four instead of two (640 keys of 32 heads 12.1 us
+//   against 10.0 with fp16 weights, 32 long sequences 257 against 251); the
+//   products are idle otherwise.
 // * The running maximum is lazy: a lane's scores are weighed against its
 //   column's base, and only when one exceeds it by 2^8 (kSlack) does the wave
 //   agree on a new base and rescale.  Every lane of a column holds the same
@@ -97,22 +101,24 @@ __device__ __forceinline__ uint32_t codes_to_16(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 
-// Weights a, b as packed 16-bit numbers `hi` and the rest `lo`.
-template <bool F16>
+// Weights a, b as packed bf16 numbers `hi` and the rest `lo`.
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo) {
-  if constexpr (F16) {
-    // toward zero: the rest is exact in fp32 and keeps 10 more bits
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    *hi = __builtin_bit_cast(uint32_t, h);
-    *lo = __builtin_bit_cast(uint32_t,
-                             __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
-  } else {
-    typedef float f32x2_t __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-    *hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
-    const float ra = a - __uint_as_float(*hi << 16), rb = b - __uint_as_float(*hi & 0xffff0000u);
-    *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{ra, rb}, bf16x2_t));
-  }
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  *hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+  const float ra = a - __uint_as_float(*hi << 16), rb = b - __uint_as_float(*hi & 0xffff0000u);
+  *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{ra, rb}, bf16x2_t));
+}
+
+// Two fp16 values as packed bf16 numbers `hi` (toward zero) and the rest `lo`, both exact.
+__device__ __forceinline__ void split_f16(uint32_t w, uint32_t* hi, uint32_t* lo) {
+  const float a = f16_to_f32(w & 0xffffu), b = f16_to_f32(w >> 16);
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  // the rest is 2^8 at most; what an infinity or a NaN leaves counts for nothing beside `hi`
+  const float ra = fminf(a - __uint_as_float(ua & 0xffff0000u), 512.0f);
+  const float rb = fminf(b - __uint_as_float(ub & 0xffff0000u), 512.0f);
+  *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+  *lo = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
 }
 
 // One wave's state over its keys.  PG16: pages hold 16 rows or more, so each
@@ -120,16 +126,14 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint3
 template <int QT, int CT, int D, bool PG16, bool STREAM>
 struct Wave {
   static constexpr bool FP8 = CT == RP_CACHE_E4M3;
-  static constexpr bool QF16 = QT == kInF16;          // the first product's type
-  static constexpr bool PF16 = QF16 && !FP8;          // the second's: a scaled weight fits bf16 only
+  static constexpr bool QF16 = QT == kInF16;          // the first product's type; the second's is bf16
+  static constexpr bool VF16 = CT == RP_CACHE_F16;
   static constexpr int EB = FP8 ? 1 : 2;
   static constexpr int NT = D / 32;                   // first products per 16 keys
   static constexpr int DPL = D / 16;                  // V columns per lane
   static constexpr int KL = FP8 ? (D + 63) / 64 : NT; // 16-byte K loads per 16 keys (8 at D = 32, fp8)
   static constexpr int VB = DPL * EB;                 // V bytes per lane and row
   static constexpr int VW = VB < 4 ? 1 : VB / 4;
-  // fp16 weights: a lift of 2^14 keeps them off the subnormals (2^8 of slack fits)
-  static constexpr float kLift = PF16 ? 6.0f : 0.0f;
 
   const PagedView& c;
   const DecodeArgs& a;
@@ -143,8 +147,6 @@ struct Wave {
   u32x4 kr[2][KL];
   uint32_t vr[8][VW];
   f32x4 kscale[2], vscale[2];
-  int32_t vpage[8];              // !PG16: pages of the lane's eight rows of the loaded step's V
-  int32_t kvalid;                // !PG16: of the step whose K is loaded, the keys that exist
   f32x4 acc[DPL];
   float base, sum;
   float* score_row;
@@ -287,6 +289,21 @@ struct Wave {
     }
   }
 
+  // A pair of columns of eight rows, times the weights, into two sums.
+  __device__ __forceinline__ static void add_columns(const uint32_t* w, u32x4 hi, u32x4 lo,
+                                                     f32x4* to) {
+    u32x4 f0, f1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f0[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+      f1[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+    }
+    to[0] = mma<false>(f0, hi, to[0]);
+    to[1] = mma<false>(f1, hi, to[1]);
+    to[0] = mma<false>(f0, lo, to[0]);
+    to[1] = mma<false>(f1, lo, to[1]);
+  }
+
   // Keys [k, k + 32) of which those below `end` exist; `more`: another step follows.
   template <bool MORE>
   __device__ __forceinline__ void step(int k, int end) {
@@ -319,10 +336,10 @@ struct Wave {
     }
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
                       fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(top > base + (kSlack + kLift))) {
+    if (__any(top > base + kSlack)) {
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      const float next = fmaxf(base, top - kLift);
+      const float next = fmaxf(base, top);
       const float r = next == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(base - next);
       sum *= r;
 #pragma unroll
@@ -353,29 +370,22 @@ struct Wave {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t h, l;
-      split_pair<PF16>(p[2 * i], p[2 * i + 1], &h, &l);
+      split_pair(p[2 * i], p[2 * i + 1], &h, &l);
       hi[i] = h;
       lo[i] = l;
     }
 #pragma unroll
     for (int j = 0; j < DPL; j += 2) {
-      // the pair of columns j, j + 1 of each row as 16-bit values
-      uint32_t w[8];
+      // the pair of columns j, j + 1 of each row as bf16 values
+      uint32_t w[8], rest[VF16 ? 8 : 1];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if constexpr (!FP8) w[e] = vr[e][j / 2];
-        else w[e] = j % 4 ? codes_to_16<PF16, true>(vr[e][j / 4]) : codes_to_16<PF16, false>(vr[e][j / 4]);
+        if constexpr (VF16) split_f16(vr[e][j / 2], &w[e], &rest[e]);
+        else if constexpr (!FP8) w[e] = vr[e][j / 2];
+        else w[e] = j % 4 ? codes_to_16<false, true>(vr[e][j / 4]) : codes_to_16<false, false>(vr[e][j / 4]);
       }
-      u32x4 f0, f1;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f0[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
-        f1[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
-      }
-      acc[j] = mma<PF16>(f0, hi, acc[j]);
-      acc[j + 1] = mma<PF16>(f1, hi, acc[j + 1]);
-      acc[j] = mma<PF16>(f0, lo, acc[j]);
-      acc[j + 1] = mma<PF16>(f1, lo, acc[j + 1]);
+      add_columns(w, hi, lo, &acc[j]);
+      if constexpr (VF16) add_columns(rest, hi, lo, &acc[j]);
     }
     if constexpr (MORE) load_v(k + kStep);
   }

@@ -701,3 +701,33 @@ def test_batches_of_none(gpu) -> None:
                                    torch.empty((0, 2, 16), device=gpu), budget=4, recent=1)
     assert new.shape == (0,) and kept.shape == (0, 2, 16)
     assert torch.equal(bits(dev["k_cache"]), bits(c.k))
+
+
+# ------------------------------------------- weights and values of all sizes
+
+def _rows_of(c: Cache, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The pages and offsets of the first n rows of sequence 0."""
+    j = torch.arange(n)
+    return c.table[0, j // c.page].long(), j % c.page
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("n,page", [(700, 16), (700, 4), (20000, 16)])
+@pytest.mark.parametrize("gap", [14, 18, 22, 26, 30, 36])
+def test_decode_of_a_heavy_key_without_value(gpu, kind, n, page, gap) -> None:
+    """One key takes nearly all the weight and its value is 0; the others, 2^-gap
+    of it to half that each, are the output: they keep 16 bits as any weight
+    does."""
+    D = 64
+    c = Cache([n], 1, D, page, kind, seed=gap)
+    pg, at = _rows_of(c, n)
+    g = torch.Generator().manual_seed(n + gap)
+    c.k[pg, 0, at] = 0
+    c.k[pg, 0, at, 0] = -torch.rand(n, generator=g).to(c.k.dtype)
+    c.v[pg, 0, at] = (torch.rand(n, D, generator=g) * 4e4 + 2e4).to(c.v.dtype)
+    heavy = n // 3
+    c.k[pg[heavy], 0, at[heavy], 0] = gap
+    c.v[pg[heavy], 0, at[heavy]] = 0
+    q = torch.zeros(1, 2, D, dtype=Q_DTYPES[kind])
+    q[0, :, 0] = 1.0
+    check_decode(gpu, c, [n], 2, kind, q=q, scale=math.log(2.0), weights=True, hint=n)
