@@ -16,8 +16,8 @@
 // * V's operand needs eight keys of one column in a register quad.  A lane
 //   loads D / 16 columns of each of its eight rows and transposes them with
 //   byte permutes (v_perm_b32), one per pair of values.
-// * P enters the second product as the sum of two bf16 numbers, the rounded
-//   weight and the rounded rest: 16 bits of any weight, however small beside
+// * P enters the second product as the sum of two bf16 numbers, the cut or
+//   rounded weight and the rounded rest: 16 bits of any weight, however small beside
 //   the largest (fp16 would cut weights below 2^-20 of it).  An fp16 V is the
 //   exact sum of two bf16 numbers, its first eight bits and the other three,
 //   so its second product is four instead of two (640 keys of 32 heads 12.1 us
@@ -101,11 +101,21 @@ __device__ __forceinline__ uint32_t codes_to_16(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 
-// Weights a, b as packed bf16 numbers `hi` and the rest `lo`.
+// Weights a, b as packed bf16 numbers `hi` and the rest `lo`, off by 2^-16 at
+// most.  For an infinity in V (POSITIVE; e4m3fn has none) both parts of a
+// positive weight are positive, or 0 * inf and inf - inf would make NaN of it:
+// cut toward zero, the weight's last bit set so that there is a rest.
+template <bool POSITIVE>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo) {
   typedef float f32x2_t __attribute__((ext_vector_type(2)));
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  *hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+  if constexpr (POSITIVE) {
+    a = __uint_as_float(__float_as_uint(a) | 1u);
+    b = __uint_as_float(__float_as_uint(b) | 1u);
+    *hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  } else {
+    *hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+  }
   const float ra = a - __uint_as_float(*hi << 16), rb = b - __uint_as_float(*hi & 0xffff0000u);
   *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{ra, rb}, bf16x2_t));
 }
@@ -370,7 +380,7 @@ struct Wave {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t h, l;
-      split_pair(p[2 * i], p[2 * i + 1], &h, &l);
+      split_pair<!FP8>(p[2 * i], p[2 * i + 1], &h, &l);
       hi[i] = h;
       lo[i] = l;
     }

@@ -1188,8 +1188,9 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     fills it, of q's dtype or float8_e4m3fn with its scales; ``seq_lens`` (B,)
     int32, the rows of each sequence that are attended to.  Returns out (B, H,
     1, D) in q's dtype, or (out, lse) with ``return_lse``, lse (B, H) fp32 the
-    log of the sum of exponentials.  A sequence without rows gives zeros and
-    -inf.  Pages may be shared between sequences, as the candidates of one
+    log of the sum of exponentials.  A sequence without rows, or with scores of
+    -inf only, gives zeros and -inf; infinities and NaNs in attended rows of
+    ``v_cache`` reach out as in the sum.  Pages may be shared between sequences, as the candidates of one
     prompt share its pages.
 
     ``key_weights`` (B, Hkv, at least max_pages * page_size) fp32: each

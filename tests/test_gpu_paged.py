@@ -731,3 +731,32 @@ def test_decode_of_a_heavy_key_without_value(gpu, kind, n, page, gap) -> None:
     q = torch.zeros(1, 2, D, dtype=Q_DTYPES[kind])
     q[0, :, 0] = 1.0
     check_decode(gpu, c, [n], 2, kind, q=q, scale=math.log(2.0), weights=True, hint=n)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,page", [(1, 16), (2, 4), (40, 16), (700, 16), (300, 4), (6000, 16)])
+def test_decode_of_infinite_values(gpu, kind, n, page) -> None:
+    """Infinities in attended rows of V come out as the sum's: of one sign
+    infinite, of both or with a NaN NaN, in their columns only."""
+    D, H = 64, 3
+    c = Cache([n], 1, D, page, kind, seed=n)
+    pg, at = _rows_of(c, n)
+    inf = float("inf")
+    for column, values in ((3, [inf]), (5, [-inf]), (7, [inf, -inf]), (9, [float("nan")]),
+                           (11, [inf, inf, inf]), (D - 1, [-inf, -inf])):
+        for i, x in enumerate(values):
+            j = (n // 2 + 17 * i) % n if n > 2 else i % n
+            c.v[pg[j], 0, at[j], column] = x
+    q = torch.randn(1, H, D, generator=torch.Generator().manual_seed(n)).to(Q_DTYPES[kind])
+    want, lse, _, eo, el = decode(q, c, [n], 0.125)
+    dev = c.to(gpu)
+    got, got_lse = ops.paged_attention_decode(q.unsqueeze(2).to(gpu), dev["k_cache"],
+                                              dev["v_cache"], dev["block_table"], i32([n], gpu),
+                                              return_lse=True, max_seq_len=n)
+    got = got.squeeze(2).double().cpu()
+    fin = torch.isfinite(want)
+    assert int((~fin).sum()) == 6 * H
+    assert torch.equal(got[~fin].nan_to_num(nan=7.0), want[~fin].nan_to_num(nan=7.0))
+    half = torch.finfo(q.dtype).eps / 2
+    assert ((got - want).abs()[fin] <= (eo + half * (want.abs() + eo))[fin]).all()
+    assert ((got_lse.cpu().double() - lse).abs() <= el).all()
