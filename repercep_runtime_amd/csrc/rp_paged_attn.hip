@@ -26,7 +26,11 @@
 // * The running maximum is lazy: a lane's scores are weighed against its
 //   column's base, and only when one exceeds it by 2^8 (kSlack) does the wave
 //   agree on a new base and rescale.  Every lane of a column holds the same
-//   base, and the final sums are exact about any base.
+//   base, and the final sums are exact about any base.  Sums about a base of
+//   values near fp32's largest may overflow where their mean does not: a wave
+//   whose sums are not finite takes its keys again about a base so high that
+//   the weights' sum stays below 1.  Waves, chunks and parts are joined as
+//   means, which fit.
 // * K rows of step i + 1 are requested as soon as step i's first product has
 //   read its registers, V rows after the second one, so a wave always has a
 //   step's K or V on its way.
@@ -66,6 +70,7 @@ struct DecodeArgs {
   int64_t qsb, qsh;
   const int32_t* lens;
   float c;                       // sm_scale * log2(e)
+  float lift;                    // how far the high base lies above the scores, in powers of two
   uint16_t* out;
   int64_t osb, osh;
   float* lse;
@@ -73,7 +78,7 @@ struct DecodeArgs {
   int64_t wsb, wsh;
   int32_t H, group, tiles;       // query heads, per kv head, 16-head tiles per kv head
   int32_t splits, chunk;
-  float* part;                   // (B, H, splits, D): sums about the part's base
+  float* part;                   // (B, H, splits, D): the part's weighted means
   float2* ml;                    // (B, H, splits): base (in powers of two), sum of weights
   float* scores;                 // (B, H, score_ld): scores in powers of two, for the key weights
   int64_t score_ld;
@@ -158,7 +163,7 @@ struct Wave {
   uint32_t vr[8][VW];
   f32x4 kscale[2], vscale[2];
   f32x4 acc[DPL];
-  float base, sum;
+  float base, sum, lift;
   float* score_row;
 
   __device__ __forceinline__ Wave(const DecodeArgs& a_, const PagedView& c_) : c(c_), a(a_) {}
@@ -169,6 +174,23 @@ struct Wave {
       const int d = FP8 && D >= 64 ? 64 * (t / 2) + 16 * g + 8 * (t % 2) : 32 * t + 8 * g;
       q[t] = live ? *reinterpret_cast<const u32x4*>(src + d) : u32x4{0u, 0u, 0u, 0u};
     }
+  }
+
+  __device__ __forceinline__ void reset(float lift_) {
+    base = neg_inf();
+    sum = 0.0f;
+    lift = lift_;
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // Whether any sum of a live column is infinite or NaN.
+  __device__ __forceinline__ bool overflown(bool live) const {
+    f32x4 z = acc[0] * 0.0f;
+#pragma unroll
+    for (int j = 1; j < DPL; ++j) z += acc[j] * 0.0f;
+    const float y = (z[0] + z[1]) + (z[2] + z[3]);
+    return __any(live && y != y);
   }
 
   __device__ __forceinline__ void begin(int from) {
@@ -346,10 +368,10 @@ struct Wave {
     }
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
                       fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(top > base + kSlack)) {
+    if (__any(top > base + (kSlack - lift))) {
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      const float next = fmaxf(base, top);
+      const float next = fmaxf(base, top + lift);
       const float r = next == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(base - next);
       sum *= r;
 #pragma unroll
@@ -426,23 +448,24 @@ __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedVi
   w.koff = (uint32_t)(w.m * c.sr * W::EB);
 #pragma unroll
   for (int r = 0; r < 4; ++r) w.voff[r] = (uint32_t)((4 * w.g + r) * c.sr * W::EB) + w.v_col();
-  w.base = neg_inf();
-  w.sum = 0.0f;
-#pragma unroll
-  for (int j = 0; j < W::DPL; ++j) w.acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   w.score_row = a.scores && live ? a.scores + ((int64_t)b * a.H + h) * a.score_ld : nullptr;
 
-  for (int64_t c0 = (int64_t)split * a.chunk; c0 < n; c0 += (int64_t)a.splits * a.chunk) {
-    const int rem = (int)min((int64_t)a.chunk, n - c0);
-    const int per = ((rem + kDWaves - 1) / kDWaves + kStep - 1) / kStep * kStep;
-    const int from = (int)c0 + wave * per, end = min(from + per, (int)c0 + rem);
-    if (from >= end) continue;
-    w.begin(from);
-    w.load_k(from);
-    w.load_v(from);
-    int k = from;
-    for (; k + kStep < end; k += kStep) w.template step<true>(k, end);
-    w.template step<false>(k, end);
+  for (float lift = 0.0f;; lift = a.lift) {
+    w.reset(lift);
+    for (int64_t c0 = (int64_t)split * a.chunk; c0 < n; c0 += (int64_t)a.splits * a.chunk) {
+      const int rem = (int)min((int64_t)a.chunk, n - c0);
+      const int per = ((rem + kDWaves - 1) / kDWaves + kStep - 1) / kStep * kStep;
+      const int from = (int)c0 + wave * per, end = min(from + per, (int)c0 + rem);
+      if (from >= end) continue;
+      w.begin(from);
+      w.load_k(from);
+      w.load_v(from);
+      int k = from;
+      for (; k + kStep < end; k += kStep) w.template step<true>(k, end);
+      w.template step<false>(k, end);
+    }
+    // fp16 values cannot take the sums out of range
+    if (W::VF16 || lift != 0.0f || !w.overflown(live)) break;
   }
 
   // the waves' parts about one base
@@ -460,7 +483,7 @@ __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedVi
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < kDWaves; ++i) sum += ssum[i][w.m] * __builtin_amdgcn_exp2f(sbase[i][w.m] - b0);
-  const float r = __builtin_amdgcn_exp2f(w.base - b0);
+  const float r = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(w.base - b0) / sum;
 #pragma unroll
   for (int j = 0; j < W::DPL; ++j) w.acc[j] *= r;
 #pragma unroll
@@ -487,13 +510,12 @@ __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedVi
     if (w.g == 0) a.ml[bh * a.splits + split] = float2{base, sum};
     return;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   uint16_t* out = a.out + b * a.osb + h * a.osh;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < W::DPL; ++j) {
-      const float x = sum == 0.0f ? 0.0f : w.acc[j][i] * inv;
+      const float x = sum == 0.0f ? 0.0f : w.acc[j][i];
       out[W::column(4 * w.g + i, j)] = QT == kInF16
           ? __builtin_bit_cast(uint16_t, (_Float16)x) : (uint16_t)f32_to_bf16_bits(x);
     }
@@ -514,8 +536,8 @@ struct JoinShared {
   float red[2][kJThreads / kWave];
 };
 
-// The parts' joint base and sum, and in sh.factor what each part's sums are
-// multiplied by.  Called by the whole block.
+// The parts' joint base and sum, and in sh.factor each part's sum about that
+// base.  Called by the whole block.
 __device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinShared& sh) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   constexpr int PER = kMaxSplits / kJThreads;
@@ -538,9 +560,9 @@ __device__ __forceinline__ float2 join_parts(const float2* ml, int parts, JoinSh
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = threadIdx.x + i * kJThreads;
-    const float f = __builtin_amdgcn_exp2f(p[i].x - b0);
+    const float f = p[i].y * __builtin_amdgcn_exp2f(p[i].x - b0);
     if (at < parts) sh.factor[at] = f;
-    sum += p[i].y * f;
+    sum += f;
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, kWave);
@@ -579,9 +601,10 @@ __global__ __launch_bounds__(kJThreads) void join_kernel(DecodeArgs a, PagedView
     const float2 t = join_parts(a.ml + bh * a.splits, parts, sh);
     const int d = threadIdx.x % COLS, gr = threadIdx.x / COLS;
     const f32x4* part = reinterpret_cast<const f32x4*>(a.part + bh * a.splits * D) + d;
+    const float inv = t.y == 0.0f ? 0.0f : 1.0f / t.y;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int i = gr; i < parts; i += GR) x += part[(int64_t)i * COLS] * sh.factor[i];
+    for (int i = gr; i < parts; i += GR) x += part[(int64_t)i * COLS] * (sh.factor[i] * inv);
     group_sum[gr][d] = x;
     __syncthreads();
     if (gr != 0) return;
@@ -590,7 +613,7 @@ __global__ __launch_bounds__(kJThreads) void join_kernel(DecodeArgs a, PagedView
     uint16_t* out = a.out + b * a.osb + h * a.osh + 4 * d;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float y = t.y == 0.0f ? 0.0f : x[e] / t.y;
+      const float y = t.y == 0.0f ? 0.0f : x[e];
       out[e] = QT == kInF16 ? __builtin_bit_cast(uint16_t, (_Float16)y) : (uint16_t)f32_to_bf16_bits(y);
     }
     if (threadIdx.x == 0 && a.lse)
@@ -831,6 +854,8 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
   a.qsb = qsb;
   a.qsh = qsh;
   a.lens = seq_lens;
+  // weights of 2^(kSlack - lift) at most, of no more keys than the table has places
+  a.lift = kSlack + (float)(64 - __builtin_clzll((unsigned long long)c.capacity()));
   a.c = sm_scale * kLog2e;
   a.out = static_cast<uint16_t*>(out);
   a.osb = osb;

@@ -760,3 +760,34 @@ def test_decode_of_infinite_values(gpu, kind, n, page) -> None:
     half = torch.finfo(q.dtype).eps / 2
     assert ((got - want).abs()[fin] <= (eo + half * (want.abs() + eo))[fin]).all()
     assert ((got_lse.cpu().double() - lse).abs() <= el).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "e4m3"])
+@pytest.mark.parametrize("n,page", [(1, 16), (33, 16), (700, 16), (700, 4), (9000, 16)])
+def test_decode_of_very_large_and_small_values(gpu, kind, n, page) -> None:
+    """Values up to the type's largest: sums of weights about a base may leave
+    fp32's range where the weighted mean does not.  And values near its
+    smallest, which a scale against that would lose."""
+    D = 64
+    c = Cache([n], 1, D, page, kind, seed=n)
+    pg, at = _rows_of(c, n)
+    if kind == "e4m3":
+        c.vs[pg[::2], 0, at[::2]] = 7e35
+        raw = c.v.view(torch.uint8)
+        raw[pg, 0, at, 3] = 0x7E                              # 448
+        raw[pg, 0, at, 5] = 0x7E + (torch.arange(n) % 2 * 128).to(torch.uint8)
+    else:
+        top = torch.finfo(c.v.dtype).max
+        c.v[pg, 0, at, 3] = top
+        c.v[pg, 0, at, 5] = (top * (-1.0) ** torch.arange(n)).to(c.v.dtype)
+        c.v[pg, 0, at, 7] = top / 2 ** 14
+        c.v[pg, 0, at, 9] = -top
+        c.v[pg, 0, at, 11] *= 1e-30 if kind == "bf16" else 1e-6
+    g = torch.Generator().manual_seed(n)
+    qt = "fp16" if kind == "fp16" else "bf16"
+    q = torch.randn(1, 2, D, generator=g).to(Q_DTYPES[qt])
+    check_decode(gpu, c, [n], 2, qt, q=q, weights=True, hint=n)
+    if kind != "e4m3":                                        # small values alone
+        small = 1e-33 if kind == "bf16" else 1e-6
+        c.v[pg, 0, at] = (torch.randn(n, D, generator=g) * small).to(c.v.dtype)
+        check_decode(gpu, c, [n], 2, qt, q=q, hint=n)
