@@ -507,6 +507,10 @@ int rp_fp8_transpose(const uint8_t* src, uint8_t* dst, int64_t R, int64_t C,
  *   block_table   int32, `table_stride` elements between sequences, max_pages
  *             entries each
  * page_size is a power of two up to 65536; head_dim is 32, 64, 128 or 256.
+ * A call that writes takes no two rows that share memory, K's and V's among
+ * them: in rising order the strides, and the distance of k and v, each pass
+ * what the smaller ones span.  Reading also takes pages and heads that share
+ * memory.
  *
  * What the device reads from the caller's memory is checked there: a
  * position past max_pages * page_size, or in a page whose id is outside
@@ -548,11 +552,12 @@ int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int64_t B, int
  * rounded once.  Values up to the type's largest do not overflow on the way.
  * Infinities and NaNs in V reach out as they do in that sum (an infinite scale
  * of an RP_CACHE_E4M3 row as NaN); a weight below 2^-64 of the largest may
- * count as 0 there (0 * inf is NaN).  A sequence that sees no row, or whose scores are all -inf, gets zeros and lse
- * -inf.
+ * count as 0 there (0 * inf is NaN).  A sequence that sees no row, or whose
+ * scores are all -inf, gets zeros and lse -inf.
  * key_weights, if not NULL: float (B, heads, >= max_pages * page_size), strides
  * wsb, wsh and 1; each seen key's softmax weights, summed over its kv head's
  * query heads, are added to it (in a fixed order: equal calls give equal bits).
+ * No two rows of key_weights, or of out, share memory.
  * max_seq_len (0: unknown) is where the lengths are expected to end: it sets
  * how the work is split, not what is computed.
  * workspace: rp_paged_attn_workspace_bytes of the same arguments, 256-byte

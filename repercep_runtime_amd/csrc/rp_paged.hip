@@ -402,7 +402,6 @@ extern "C" int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int
   }
   PagedView c;
   int rc = paged_view("paged_kv_append", cache, &c);
-  if (rc == RP_OK) rc = paged_writable("paged_kv_append", cache);
   if (rc != RP_OK) return rc;
   if (x_dtype != RP_DTYPE_BF16 && x_dtype != RP_DTYPE_F16) {
     rp_set_error("paged_kv_append: unknown input dtype %d", x_dtype);
@@ -426,6 +425,8 @@ extern "C" int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int
     rp_set_error("paged_kv_append: new rows must be 16-byte aligned");
     return RP_ERR_UNSUPPORTED;
   }
+  rc = paged_writable("paged_kv_append", cache);
+  if (rc != RP_OK) return rc;
   const AppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                      ksb, ksh, kss, vsb, vsh, vss, start, lengths, (int32_t)S};
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -462,7 +463,6 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
   }
   PagedView c;
   int rc = paged_view("paged_kv_evict", cache, &c);
-  if (rc == RP_OK) rc = paged_writable("paged_kv_evict", cache);
   if (rc != RP_OK) return rc;
   if (B <= 0 || budget <= 0 || recent < 0 || recent > budget) {
     rp_set_error("paged_kv_evict: needs B > 0 and 0 <= recent <= budget, budget > 0 (B=%lld "
@@ -486,6 +486,8 @@ extern "C" int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq
     rp_set_error("paged_kv_evict: workspace of %zu bytes, 256-byte aligned, needed", want);
     return RP_ERR_WORKSPACE;
   }
+  rc = paged_writable("paged_kv_evict", cache);
+  if (rc != RP_OK) return rc;
   int32_t* first = static_cast<int32_t*>(workspace);
   int32_t* src = first + (B * c.heads * 4 + 255) / 256 * 64;
   const EvictArgs a{seq_lens, weights, wsb, wsh, (int32_t)budget, (int32_t)recent, new_lens,

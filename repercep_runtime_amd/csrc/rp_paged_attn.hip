@@ -827,7 +827,7 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_decode: q rows must be 16-byte and out rows 8-byte aligned");
     return RP_ERR_UNSUPPORTED;
   }
-  if ((B > 1 && osb < cache->head_dim) || (H > 1 && osh < cache->head_dim)) {
+  if (!rows_apart(cache->head_dim, {{B, osb}, {H, osh}})) {
     rp_set_error("paged_attn_decode: out rows overlap");
     return RP_ERR_INVALID_ARGUMENT;
   }
@@ -843,7 +843,7 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_decode: workspace of %zu bytes, 256-byte aligned, needed", l.total);
     return RP_ERR_WORKSPACE;
   }
-  if (key_weights && ((B > 1 && wsb < c.capacity()) || (cache->heads > 1 && wsh < c.capacity()))) {
+  if (key_weights && !rows_apart(c.capacity(), {{B, wsb}, {cache->heads, wsh}})) {
     rp_set_error("paged_attn_decode: key_weights rows of %lld positions overlap",
                  (long long)c.capacity());
     return RP_ERR_INVALID_ARGUMENT;

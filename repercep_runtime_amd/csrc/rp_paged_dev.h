@@ -109,10 +109,39 @@ inline int paged_view(const char* what, const rp_paged_cache* c, PagedView* v) {
   return RP_OK;
 }
 
-// Refuses a cache whose rows share memory, for the calls that write it.
+struct Dim {
+  int64_t size, stride;
+};
+
+// Whether no two rows of `unit` elements share memory: in rising order of
+// stride, each dimension steps past all that the smaller ones span.  (Layouts
+// that interleave without sharing, but do not nest, count as sharing.)
+template <int N>
+inline bool rows_apart(int64_t unit, const Dim (&dims)[N]) {
+  Dim d[N];
+  for (int i = 0; i < N; ++i) {
+    int j = i;
+    for (; j > 0 && d[j - 1].stride > dims[i].stride; --j) d[j] = d[j - 1];
+    d[j] = dims[i];
+  }
+  __int128 span = unit;
+  for (int i = 0; i < N; ++i) {
+    if (d[i].size <= 1) continue;
+    if (d[i].stride < span) return false;
+    span += (__int128)(d[i].size - 1) * d[i].stride;
+  }
+  return true;
+}
+
+// Refuses a cache of which two rows share memory, K's and V's among them, for
+// the calls that write it.
 inline int paged_writable(const char* what, const rp_paged_cache* c) {
-  if ((c->num_pages > 1 && c->stride_page < c->head_dim) ||
-      (c->heads > 1 && c->stride_head < c->head_dim)) {
+  const int64_t eb = cache_elem_bytes(c->dtype);
+  const uintptr_t k = reinterpret_cast<uintptr_t>(c->k), v = reinterpret_cast<uintptr_t>(c->v);
+  if (!rows_apart(c->head_dim * eb, {{c->num_pages, c->stride_page * eb},
+                                     {c->heads, c->stride_head * eb},
+                                     {c->page_size, c->stride_row * eb},
+                                     {2, (int64_t)(k < v ? v - k : k - v)}})) {
     rp_set_error("%s: cache rows overlap", what);
     return RP_ERR_INVALID_ARGUMENT;
   }

@@ -1144,7 +1144,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     scales in ``k_scale``, ``v_scale`` (pages, Hkv, page_size) fp32.
 
     Positions past the table, and pages whose id is not in [0, pages), are
-    left out.  A page that is written belongs to one sequence."""
+    left out.  A page that is written belongs to one sequence, and no two rows
+    of the caches share memory (an expanded cache can be read only)."""
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"k and v must share one (B, Hkv, S, D) shape (got {tuple(k.shape)}, "
                          f"{tuple(v.shape)})")

@@ -791,3 +791,71 @@ def test_decode_of_very_large_and_small_values(gpu, kind, n, page) -> None:
         small = 1e-33 if kind == "bf16" else 1e-6
         c.v[pg, 0, at] = (torch.randn(n, D, generator=g) * small).to(c.v.dtype)
         check_decode(gpu, c, [n], 2, qt, q=q, hint=n)
+
+
+def _halves(layout: str, P: int, Hkv: int, page: int, D: int, dev: torch.device
+            ) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V as two halves of one buffer, none of their rows shared."""
+    def buf(*s: int) -> torch.Tensor:
+        return torch.zeros(s, dtype=torch.bfloat16, device=dev)
+
+    if layout == "columns":
+        x = buf(P, Hkv, page, 2 * D)
+        return x[..., :D], x[..., D:]
+    if layout == "heads":
+        x = buf(P, 2 * Hkv, page, D)
+        return x[:, Hkv:], x[:, :Hkv]
+    if layout == "every other head":
+        x = buf(P, page, 2 * Hkv, D).permute(0, 2, 1, 3)
+        return x[:, ::2], x[:, 1::2]
+    if layout == "every other page":
+        x = buf(2 * P, page, Hkv, D).permute(0, 2, 1, 3)
+        return x[::2], x[1::2]
+    x = buf(2 * P, Hkv, page, D)
+    return x[P:], x[:P]
+
+
+@pytest.mark.parametrize("layout", ["columns", "heads", "every other head", "every other page",
+                                    "pages"])
+def test_caches_that_are_halves_of_one_buffer(gpu, layout) -> None:
+    """Written, read and cut as two separate caches are."""
+    P, Hkv, page, D, lens = 12, 3, 16, 64, [70, 33, 40]
+    g = torch.Generator(device=gpu).manual_seed(1)
+    table = torch.randperm(P, generator=g, device=gpu)[:12].view(3, 4).to(torch.int32)
+    table = torch.cat([table, torch.full_like(table[:, :1], -1)], 1)
+    x, y = (torch.randn(3, Hkv, 70, D, generator=g, device=gpu).to(torch.bfloat16)
+            for _ in range(2))
+    q = torch.randn(3, 6, 1, D, generator=g, device=gpu).to(torch.bfloat16)
+    n, got = i32(lens, gpu), []
+    separate = [torch.zeros(P, Hkv, page, D, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    for k, v in (_halves(layout, P, Hkv, page, D, gpu), separate):
+        ops.paged_kv_append(x, y, k, v, table, i32([0, 0, 0], gpu), n)
+        # totals and output with the heads outermost
+        w = torch.zeros(Hkv, 3, 5 * page, device=gpu).transpose(0, 1)
+        out = torch.empty(6, 1, 3, D, dtype=torch.bfloat16, device=gpu).permute(2, 0, 1, 3)
+        ops.paged_attention_decode(q, k, v, table, n, key_weights=w, out=out)
+        got.append([w, out, *ops.paged_kv_evict(k, v, table, n, w, budget=36, recent=4), k, v])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_shared_memory_is_refused(gpu) -> None:
+    """One tensor as K and V, totals that two heads share, an expanded output."""
+    c = Cache([20, 20], 2, 64, 16, "bf16")
+    d = c.to(gpu)
+    n = i32([20, 20], gpu)
+    x = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16, device=gpu)
+    k, table = d["k_cache"], d["block_table"]
+    w = torch.zeros(2, 2, table.shape[1] * 16, device=gpu)
+    with pytest.raises(ops.C.HipLibraryError, match="overlap"):
+        ops.paged_kv_append(x, x, k, k, table, n)
+    with pytest.raises(ops.C.HipLibraryError, match="overlap"):
+        ops.paged_kv_evict(k, k, table, n, w, budget=4, recent=1)
+    both = torch.zeros(3, table.shape[1] * 16, device=gpu)
+    both = both.as_strided((2, 2, both.shape[1]), (both.shape[1], both.shape[1], 1))
+    with pytest.raises(ops.C.HipLibraryError, match="overlap"):
+        ops.paged_attention_decode(x, k, k, table, n, key_weights=both)
+    with pytest.raises(ops.C.HipLibraryError, match="overlap"):
+        ops.paged_attention_decode(x, k, k, table, n, out=x[:1].expand(2, -1, -1, -1))
+    want = ops.paged_attention_decode(x, k, k.clone(), table, n)
+    assert torch.equal(ops.paged_attention_decode(x, k, k, table, n), want)     # reading may

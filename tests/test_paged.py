@@ -345,3 +345,40 @@ def test_torch_evict_refusals(kw: dict, msg: str) -> None:
 def test_torch_logprob_refusals(args: tuple, kw: dict, err: type, msg: str) -> None:
     with pytest.raises(err, match=msg):
         ops.token_logprobs(*args, **kw)
+
+
+# rows of 64 x 2 and 3 elements apart: each stride is as long as a row, and some rows are the same
+@pytest.mark.parametrize("call", [append, evict])
+@pytest.mark.parametrize("kw", [
+    dict(stride_page=16 * 128, stride_head=16 * 128),
+    dict(stride_page=128, stride_head=128),
+    dict(stride_page=4 * 128, stride_head=16 * 128),
+    dict(stride_page=16 * 128, stride_head=8 * 16 * 128 - 128),
+    dict(v=FAKE),                                   # K's memory
+    dict(v=FAKE + 2 * 128),                         # K's second row
+    dict(v=FAKE + 2 * 16 * 128),                    # K's second head
+    dict(v=FAKE + 2 * 7 * 2 * 16 * 128),            # K's last page
+    dict(v=FAKE - 2 * 2 * 16 * 128),                # a page early: K begins inside V
+    dict(stride_row=192, v=FAKE + 2 * 96),          # not past K's columns
+])
+def test_writers_refuse_rows_that_share_memory(call, kw: dict) -> None:
+    """Strides and places under which two rows of K, of V or of both overlap."""
+    a = dict(v=3 * FAKE)
+    if "v" in kw and "stride_row" in kw:
+        a |= dict(stride_head=16 * 192, stride_page=2 * 16 * 192)
+    a.update(kw)
+    assert call(cache(**a)) == 1
+    assert "overlap" in _capi.lib().rp_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(w=FAKE, wsb=64, wsh=64),                   # both strides a row: sequence 1 is head 1
+    dict(w=FAKE, wsb=64, wsh=127),
+    dict(w=FAKE, wsb=100, wsh=64),
+    dict(osb=128, osh=128),
+    dict(osb=384, osh=128),                         # four heads of 128
+    dict(osb=128, osh=252),
+])
+def test_attention_refuses_outputs_that_share_memory(kw: dict) -> None:
+    assert decode(cache(), **kw) == 1
+    assert "overlap" in _capi.lib().rp_last_error().decode()
