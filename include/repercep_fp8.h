@@ -590,8 +590,9 @@ int rp_paged_kv_evict(const rp_paged_cache* cache, const int32_t* seq_lens, int6
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------- token log probabilities
- * For each of N rows of V logits (row stride ld elements; RP_OUT_BF16,
- * RP_OUT_F16 or RP_OUT_F32 by logits_dtype), z = x / temperature:
+ * For each of N rows of V logits (row stride ld elements, V or more, or 0: one
+ * row for all tokens; RP_OUT_BF16, RP_OUT_F16 or RP_OUT_F32 by logits_dtype),
+ * z = x / temperature:
  *   logprobs[i]  log softmax(z)[tokens[i]]; 0 for a negative token (padding),
  *                NaN for one >= V
  *   entropy[i]   -sum p log p                            (NULL: not written)

@@ -551,7 +551,7 @@ extern "C" int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N
     rp_set_error("token_logprobs: unknown logits dtype %d", logits_dtype);
     return RP_ERR_INVALID_ARGUMENT;
   }
-  if (N <= 0 || V <= 0 || ld < V) {
+  if (N <= 0 || V <= 0 || (ld < V && ld != 0)) {
     rp_set_error("token_logprobs: bad sizes N=%lld V=%lld ld=%lld", (long long)N, (long long)V,
                  (long long)ld);
     return RP_ERR_INVALID_ARGUMENT;

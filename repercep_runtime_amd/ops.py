@@ -1309,8 +1309,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
     """Log probabilities of given tokens, with entropy and best alternatives.
 
-    ``logits`` (..., V) bf16, fp16 or fp32 with a unit stride on V and rows
-    that flatten to one row stride; ``tokens`` (...) int64.  Under softmax(logits
+    ``logits`` (..., V) bf16, fp16 or fp32 with a unit stride on V, one row
+    expanded to many among them (leading dimensions that do not flatten to one
+    row stride are copied first); ``tokens`` (...) int64.  Under softmax(logits
     / temperature), in fp32: ``logprobs`` (...) of the tokens (0 for a negative
     token, the padding of a ragged batch; NaN for one >= V), ``entropy`` (...)
     in nats, and with ``top`` <= 32 the largest log probabilities

@@ -288,3 +288,30 @@ def test_best_of_rows_below_zero(gpu, dt, V, top) -> None:
     """16-bit logits at or below zero: the best and their order, one part a
     row and several, rows on and off 16-byte borders."""
     check(gpu, _rows_below_zero(V, dt, top), top, seed=top)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [50, 40000])
+def test_one_row_of_logits_for_many_tokens(gpu, dt, V) -> None:
+    """An expanded row is read as it lies: what copies of it give."""
+    x = logits(1, V, dt, V).to(gpu)
+    t = torch.tensor([0, V - 1, -1, V // 2, 3, V], device=gpu)
+    got = ops.token_logprobs(x.expand(6, V), t, top=7)
+    want = ops.token_logprobs(x, t[:1], top=7)
+    assert got.logprobs[2] == 0 and got.logprobs[5].isnan()
+    for i in range(6):
+        assert torch.equal(got.entropy[i], want.entropy[0])
+        assert torch.equal(got.top_ids[i], want.top_ids[0])
+        assert torch.equal(got.top_logprobs[i], want.top_logprobs[0])
+    for i in (0, 1, 3, 4):
+        one = ops.token_logprobs(x, t[i:i + 1])
+        assert torch.equal(got.logprobs[i], one.logprobs[0])
+
+
+def test_logits_that_do_not_flatten(gpu) -> None:
+    """Leading dimensions of no one row stride: copied first, the same answers."""
+    x = logits(12, 300, "fp32", 3).to(gpu).view(3, 4, 300)
+    t = torch.arange(12, device=gpu).view(4, 3)
+    got = ops.token_logprobs(x.transpose(0, 1), t, top=3)
+    want = ops.token_logprobs(x.transpose(0, 1).contiguous(), t, top=3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
