@@ -545,6 +545,7 @@ int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int64_t B, int
 /* Attention of one new token per sequence over its first seq_lens[b] rows:
  *   s_j = sm_scale * q . k_j,  out = sum_j softmax(s)_j v_j,
  *   lse = log(sum_j exp(s_j))                        (lse NULL: not written)
+ * (sm_scale finite and below 2.3e38).
  * q (B, H, head_dim) bf16 or fp16 with strides qsb, qsh; out of the same type
  * with strides osb, osh; lse float (B, H).  A 16-bit cache has q's type.
  * Query head h reads kv head h / (H / heads).  Products are exact in fp32

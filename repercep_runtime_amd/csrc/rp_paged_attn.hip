@@ -810,8 +810,9 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
                  (long long)H);
     return RP_ERR_INVALID_ARGUMENT;
   }
-  if (!(sm_scale - sm_scale == 0.0f)) {
-    rp_set_error("paged_attn_decode: sm_scale must be finite");
+  const float c2 = sm_scale * kLog2e;              // scores in powers of two
+  if (!(c2 - c2 == 0.0f)) {
+    rp_set_error("paged_attn_decode: sm_scale and sm_scale * log2(e) must be finite");
     return RP_ERR_INVALID_ARGUMENT;
   }
   if (B > 65535 || H > 65535 || cache->stride_row > (1 << 25)) {
@@ -856,7 +857,7 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
   a.lens = seq_lens;
   // weights of 2^(kSlack - lift) at most, of no more keys than the table has places
   a.lift = kSlack + (float)(64 - __builtin_clzll((unsigned long long)c.capacity()));
-  a.c = sm_scale * kLog2e;
+  a.c = c2;
   a.out = static_cast<uint16_t*>(out);
   a.osb = osb;
   a.osh = osh;

@@ -382,3 +382,10 @@ def test_writers_refuse_rows_that_share_memory(call, kw: dict) -> None:
 def test_attention_refuses_outputs_that_share_memory(kw: dict) -> None:
     assert decode(cache(), **kw) == 1
     assert "overlap" in _capi.lib().rp_last_error().decode()
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, 2.4e38])
+def test_a_scale_that_leaves_the_range_is_refused(scale: float) -> None:
+    """Scores are taken in powers of two: scale * log2(e) has to be finite too."""
+    assert decode(cache(), scale=scale) == 1
+    assert "sm_scale" in _capi.lib().rp_last_error().decode()
