@@ -1077,7 +1077,8 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
         raise TypeError(f"k_cache and v_cache must both be bfloat16, float16 or float8_e4m3fn "
                         f"(got {k_cache.dtype}, {v_cache.dtype})")
     strides = k_cache.stride()
-    if v_cache.stride() != strides or strides[3] != 1:
+    if strides[3] != 1 or v_cache.stride(3) != 1 or (
+            v_cache.stride() != strides and _strides(v_cache, 3) != _strides(k_cache, 3)):
         raise ValueError("k_cache and v_cache must share their strides, with a unit stride on D")
     table = block_table.shape
     if len(table) != 2 or table[0] != B or block_table.dtype != torch.int32 \

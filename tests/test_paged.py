@@ -389,3 +389,18 @@ def test_a_scale_that_leaves_the_range_is_refused(scale: float) -> None:
     """Scores are taken in powers of two: scale * log2(e) has to be finite too."""
     assert decode(cache(), scale=scale) == 1
     assert "sm_scale" in _capi.lib().rp_last_error().decode()
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_strides_of_single_dimensions_do_not_count(dim: int) -> None:
+    """K and V of one page, head or row a page: that dimension's stride means
+    nothing, and may differ between them."""
+    shape = [8, 2, 16, 128]
+    shape[dim] = 1
+    k, v = _t(*shape), _t(*shape)
+    strides = list(v.stride())
+    strides[dim] += 8
+    step = _step(k_cache=k, v_cache=v.as_strided(shape, strides))
+    lens = _t(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU tensor"):          # the last check
+        ops.paged_attention_decode(_t(3, 2 * shape[1], 1, 128), seq_lens=lens, **step)
