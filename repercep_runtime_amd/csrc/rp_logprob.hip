@@ -131,11 +131,6 @@ __device__ __forceinline__ float half_max(uint32_t w) {
   const uint32_t x = (uint32_t)(lo > hi ? lo : hi) & 0xffffu;
   return DT == RP_OUT_F16 ? f16_to_f32(x) : bf16_to_f32(x);
 }
-__device__ __forceinline__ uint32_t pk_min_u16(uint32_t a, uint32_t b) {
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a),
-                                                                __builtin_bit_cast(u16x2, b)));
-}
 // 16-bit logits whose t may leave fp32's range (c up to 2^20): -2^100 and below, fp16's -inf
 template <int DT>
 constexpr uint32_t kLow16 = DT == RP_OUT_F16 ? 0xfc00u : 0xf180u;

@@ -16,20 +16,19 @@
 // * V's operand needs eight keys of one column in a register quad.  A lane
 //   loads D / 16 columns of each of its eight rows and transposes them with
 //   byte permutes (v_perm_b32), one per pair of values.
-// * P enters the second product as the sum of two bf16 numbers, the cut or
-//   rounded weight and the rounded rest: 16 bits of any weight, however small beside
-//   the largest (fp16 would cut weights below 2^-20 of it).  An fp16 V is the
-//   exact sum of two bf16 numbers, its first eight bits and the other three,
-//   so its second product is four instead of two (640 keys of 32 heads 12.1 us
-//   against 10.0 with fp16 weights, 32 long sequences 257 against 251); the
-//   products are idle otherwise.
+// * P enters the second product as the sum of three bf16 numbers, which is the
+//   fp32 weight exactly, however small it is beside the largest; fp16 would end
+//   at 2^-24.  An fp16 V is the exact sum of two bf16 numbers, its first eight
+//   bits and the other three.  So a value takes three instructions, an fp16 one
+//   six; the products are idle otherwise.
 // * The running maximum is lazy: a lane's scores are weighed against its
 //   column's base, and only when one exceeds it by 2^8 (kSlack) does the wave
 //   agree on a new base and rescale.  Every lane of a column holds the same
 //   base, and the final sums are exact about any base.  Sums about a base of
-//   values near fp32's largest may overflow where their mean does not: a wave
-//   whose sums are not finite takes its keys again about a base so high that
-//   the weights' sum stays below 1.  Waves, chunks and parts are joined as
+//   values near fp32's largest may overflow where their mean does not, and a
+//   zero part of a weight makes NaN of an infinite value: a wave whose sums are
+//   not finite takes its keys again, about a base so high that the weights' sum
+//   stays below 1 and with no part zero.  Waves, chunks and parts are joined as
 //   means, which fit.
 // * K rows of step i + 1 are requested as soon as step i's first product has
 //   read its registers, V rows after the second one, so a wave always has a
@@ -106,34 +105,28 @@ __device__ __forceinline__ uint32_t codes_to_16(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 
-// Weights a, b as packed bf16 numbers `hi` and the rest `lo`, off by 2^-16 at
-// most.  For an infinity in V (POSITIVE; e4m3fn has none) both parts of a
-// positive weight are positive, or 0 * inf and inf - inf would make NaN of it:
-// cut toward zero, the weight's last bit set so that there is a rest.
-template <bool POSITIVE>
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t* hi, uint32_t* lo) {
-  typedef float f32x2_t __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  if constexpr (POSITIVE) {
-    a = __uint_as_float(__float_as_uint(a) | 1u);
-    b = __uint_as_float(__float_as_uint(b) | 1u);
-    *hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-  } else {
-    *hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
-  }
-  const float ra = a - __uint_as_float(*hi << 16), rb = b - __uint_as_float(*hi & 0xffff0000u);
-  *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{ra, rb}, bf16x2_t));
+__device__ __forceinline__ float bf16_cut(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_cut(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+// Weights a, b as three packed bf16 numbers each, eight bits at a time: exact.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t* to) {
+  to[0] = pack_cut(a, b);
+  a -= bf16_cut(a);
+  b -= bf16_cut(b);
+  to[1] = pack_cut(a, b);
+  to[2] = pack_cut(a - bf16_cut(a), b - bf16_cut(b));
 }
 
 // Two fp16 values as packed bf16 numbers `hi` (toward zero) and the rest `lo`, both exact.
 __device__ __forceinline__ void split_f16(uint32_t w, uint32_t* hi, uint32_t* lo) {
   const float a = f16_to_f32(w & 0xffffu), b = f16_to_f32(w >> 16);
-  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  *hi = pack_cut(a, b);
   // the rest is 2^8 at most; what an infinity or a NaN leaves counts for nothing beside `hi`
-  const float ra = fminf(a - __uint_as_float(ua & 0xffff0000u), 512.0f);
-  const float rb = fminf(b - __uint_as_float(ub & 0xffff0000u), 512.0f);
-  *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-  *lo = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
+  *lo = pack_cut(fminf(a - bf16_cut(a), 512.0f), fminf(b - bf16_cut(b), 512.0f));
 }
 
 // One wave's state over its keys.  PG16: pages hold 16 rows or more, so each
@@ -164,6 +157,7 @@ struct Wave {
   f32x4 kscale[2], vscale[2];
   f32x4 acc[DPL];
   float base, sum, lift;
+  uint32_t least;                // the least a positive weight's second and third part may be
   float* score_row;
 
   __device__ __forceinline__ Wave(const DecodeArgs& a_, const PagedView& c_) : c(c_), a(a_) {}
@@ -180,6 +174,9 @@ struct Wave {
     base = neg_inf();
     sum = 0.0f;
     lift = lift_;
+    // For an infinity in V each part of a positive weight has to be positive, or
+    // 0 * inf makes NaN of it (e4m3fn has none): 2^-126 where it is 0.
+    least = lift_ == 0.0f ? 0u : 0x00800080u;
 #pragma unroll
     for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -322,7 +319,7 @@ struct Wave {
   }
 
   // A pair of columns of eight rows, times the weights, into two sums.
-  __device__ __forceinline__ static void add_columns(const uint32_t* w, u32x4 hi, u32x4 lo,
+  __device__ __forceinline__ static void add_columns(const uint32_t* w, const u32x4* w3,
                                                      f32x4* to) {
     u32x4 f0, f1;
 #pragma unroll
@@ -330,10 +327,11 @@ struct Wave {
       f0[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
       f1[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
     }
-    to[0] = mma<false>(f0, hi, to[0]);
-    to[1] = mma<false>(f1, hi, to[1]);
-    to[0] = mma<false>(f0, lo, to[0]);
-    to[1] = mma<false>(f1, lo, to[1]);
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      to[0] = mma<false>(f0, w3[e], to[0]);
+      to[1] = mma<false>(f1, w3[e], to[1]);
+    }
   }
 
   // Keys [k, k + 32) of which those below `end` exist; `more`: another step follows.
@@ -398,13 +396,18 @@ struct Wave {
         for (int i = 0; i < VW; ++i) vr[e][i] = in ? vr[e][i] : 0u;
       }
     }
-    u32x4 hi, lo;
+    u32x4 w3[3];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t h, l;
-      split_pair<!FP8>(p[2 * i], p[2 * i + 1], &h, &l);
-      hi[i] = h;
-      lo[i] = l;
+      uint32_t t[3];
+      split_pair(p[2 * i], p[2 * i + 1], t);
+      if constexpr (!FP8) {
+        const uint32_t f = pk_min_u16(t[0], least);
+        t[1] = pk_max_u16(t[1], f);
+        t[2] = pk_max_u16(t[2], f);
+      }
+#pragma unroll
+      for (int e = 0; e < 3; ++e) w3[e][i] = t[e];
     }
 #pragma unroll
     for (int j = 0; j < DPL; j += 2) {
@@ -416,8 +419,8 @@ struct Wave {
         else if constexpr (!FP8) w[e] = vr[e][j / 2];
         else w[e] = j % 4 ? codes_to_16<false, true>(vr[e][j / 4]) : codes_to_16<false, false>(vr[e][j / 4]);
       }
-      add_columns(w, hi, lo, &acc[j]);
-      if constexpr (VF16) add_columns(rest, hi, lo, &acc[j]);
+      add_columns(w, w3, &acc[j]);
+      if constexpr (VF16) add_columns(rest, w3, &acc[j]);
     }
     if constexpr (MORE) load_v(k + kStep);
   }
@@ -464,8 +467,7 @@ __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedVi
       for (; k + kStep < end; k += kStep) w.template step<true>(k, end);
       w.template step<false>(k, end);
     }
-    // fp16 values cannot take the sums out of range
-    if (W::VF16 || lift != 0.0f || !w.overflown(live)) break;
+    if (lift != 0.0f || !w.overflown(live)) break;
   }
 
   // the waves' parts about one base

@@ -859,3 +859,46 @@ def test_shared_memory_is_refused(gpu) -> None:
         ops.paged_attention_decode(x, k, k, table, n, out=x[:1].expand(2, -1, -1, -1))
     want = ops.paged_attention_decode(x, k, k.clone(), table, n)
     assert torch.equal(ops.paged_attention_decode(x, k, k, table, n), want)     # reading may
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "e4m3"])
+@pytest.mark.parametrize("page", [16, 4])
+def test_decode_weights_have_32_bits(gpu, kind, page) -> None:
+    """Two keys whose weighted values nearly cancel leave what the weights lost.
+
+    Scores are single products below 1 in size: rounded three times on the way
+    to the exponential's argument (8 u with its own 2 u in a weight), the sum
+    and its reciprocal as often again, at both keys, and the mean's up to twelve
+    partial sums one u each: 40 u sum p|v| beside the output's rounding.  A
+    weight of 16 bits would be off by up to 2^-16 = 256 u."""
+    B, H, D, u = 64, 4, 64, 2.0 ** -24
+    lens = [2] * B
+    c = Cache(lens, 1, D, page, kind, seed=page)
+    g = torch.Generator().manual_seed(5)
+    qt = "fp16" if kind == "fp16" else "bf16"
+    q = torch.zeros(B, H, D, dtype=Q_DTYPES[qt])
+    q[:, :, 0] = (torch.rand(B, H, generator=g) * 2 - 1).to(q.dtype)
+    pg = c.table[:, 0].long()
+    for j in (0, 1):
+        c.k[pg, 0, j] = torch.zeros(B, D).to(c.k.dtype)
+        c.k[pg, 0, j, 0] = (torch.rand(B, generator=g) * 2 - 1).to(c.k.dtype)
+    if kind == "e4m3":
+        c.ks[pg] = 0.875
+    p = torch.stack([w[0] for w in decode(q, c, lens, 1.0)[2]])         # head 0's weights
+    ratio = p[:, :1] / p[:, 1:]
+    if kind == "e4m3":
+        ratio = ratio * (c.vs[pg, 0, 0] / c.vs[pg, 0, 1]).double().unsqueeze(1)
+    c.v[pg, 0, 1] = (c.v[pg, 0, 0].double() * -ratio).clamp(-448.0, 448.0).to(c.v.dtype)
+    out = decode(q, c, lens, 1.0)[0]
+    assert torch.isfinite(out).all()
+    size = torch.stack([(w.unsqueeze(-1) * c.rows(c.v, c.vs, b, 2).abs()).sum(1)
+                        for b, w in enumerate(decode(q, c, lens, 1.0)[2])])
+    dev = c.to(gpu)
+    got = ops.paged_attention_decode(q.unsqueeze(2).to(gpu), dev["k_cache"], dev["v_cache"],
+                                     dev["block_table"], i32(lens, gpu), scale=1.0,
+                                     k_scale=dev["k_scale"], v_scale=dev["v_scale"])
+    half = torch.finfo(q.dtype).eps / 2
+    tiny = torch.finfo(q.dtype).smallest_normal * half
+    err = (got.squeeze(2).double().cpu() - out).abs()
+    assert (err <= 40 * u * size * (1 + half) + half * out.abs() + tiny).all(), \
+        float(((err - half * out.abs()) / (u * size)).max())
