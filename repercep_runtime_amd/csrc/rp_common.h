@@ -128,6 +128,9 @@ __device__ __forceinline__ float add_row_ror(float v) {
 
 __device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
+// Threads along one dimension of a grid that the runtime launches.
+constexpr int64_t kMaxGridThreads = 0xffffffffll;
+
 // Two independent 16-bit unsigned maxima in one dword (v_pk_max_u16).
 __device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));

@@ -574,6 +574,10 @@ extern "C" int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N
     return RP_ERR_INVALID_ARGUMENT;
   }
   const LogprobPlan p = logprob_plan(V, logits_dtype);
+  if (N * p.parts * p.threads > kMaxGridThreads) {
+    rp_set_error("token_logprobs: too many rows");
+    return RP_ERR_UNSUPPORTED;
+  }
   const size_t sums = logprob_sums_bytes(N, p.parts);
   const size_t want = p.parts == 1 ? 0 : sums + (size_t)(N * p.parts * top * 8);
   if (want > 0 && (!workspace || workspace_bytes < want ||

@@ -416,7 +416,9 @@ extern "C" int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int
     rp_set_error("paged_kv_append: non-positive size B=%lld S=%lld", (long long)B, (long long)S);
     return RP_ERR_INVALID_ARGUMENT;
   }
-  if (B > 65535 || S > 0x7fffffff / cache->heads) {
+  // head_dim / 8 threads take kAppendUnroll rows of so many
+  if (B > 65535 || S > 0x7fffffff / cache->heads ||
+      (S * cache->heads / kAppendUnroll + kPThreads) * (cache->head_dim / 8) > kMaxGridThreads) {
     rp_set_error("paged_kv_append: too many sequences or rows");
     return RP_ERR_UNSUPPORTED;
   }

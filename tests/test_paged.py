@@ -404,3 +404,22 @@ def test_strides_of_single_dimensions_do_not_count(dim: int) -> None:
     lens = _t(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="GPU tensor"):          # the last check
         ops.paged_attention_decode(_t(3, 2 * shape[1], 1, 128), seq_lens=lens, **step)
+
+
+def test_calls_past_the_launch_limit_are_refused() -> None:
+    """2^32 threads along the grid, which the runtime does not launch: refused
+    before any kernel has run."""
+    L = _capi.lib()
+    wide = (FAKE, 0, 1 << 24, 100, 0, FAKE, 1.0, 0, FAKE, None, None, None, None, 0, None)
+    assert L.rp_token_logprobs(*wide) == 2
+    assert "too many" in L.rp_last_error().decode()
+    # sixteen rows of 256 a workgroup, 2^28 of them
+    big = cache(v=3 * FAKE, head_dim=256, stride_row=256, stride_head=16 * 256,
+                stride_page=2 * 16 * 256)
+    assert append(big, S=1 << 27, ksb=0, ksh=0, kss=0, vsb=0, vsh=0, vss=0, B=1) == 2
+    assert "too many" in L.rp_last_error().decode()
+    # key weights of 2^30 positions and 16 heads: 2^24 workgroups of the second launch
+    long = cache(heads=16, max_pages=1 << 26, stride_page=16 * 16 * 128)
+    assert decode(long, H=16, w=FAKE, wsb=1 << 34, wsh=1 << 30, nbytes=1 << 62, qsb=2048,
+                  osb=2048) == 2
+    assert "too many" in L.rp_last_error().decode()
