@@ -549,11 +549,12 @@ int rp_paged_kv_append(const void* k, const void* v, int x_dtype, int64_t B, int
  * q (B, H, head_dim) bf16 or fp16 with strides qsb, qsh; out of the same type
  * with strides osb, osh; lse float (B, H).  A 16-bit cache has q's type.
  * Query head h reads kv head h / (H / heads).  Products are exact in fp32
- * sums, those of the fp32 weights with V too, and out is rounded once.  Values up to the type's largest do not overflow on the way.
- * Infinities and NaNs in V reach out as they do in that sum (an infinite scale
- * of an RP_CACHE_E4M3 row as NaN); a weight below 2^-64 of the largest may
- * count as 0 there (0 * inf is NaN).  A sequence that sees no row, or whose
- * scores are all -inf, gets zeros and lse -inf.
+ * sums, those of the fp32 weights with V too, and out is rounded once.  Values
+ * up to the type's largest do not overflow on the way.  Infinities and NaNs in
+ * V reach out as they do in that sum (an infinite scale of an RP_CACHE_E4M3 row
+ * as NaN); a weight below 2^-64 of the largest may count as 0 there (0 * inf
+ * is NaN).  A sequence that sees no row, or whose scores are all -inf, gets
+ * zeros and lse -inf.
  * key_weights, if not NULL: float (B, heads, >= max_pages * page_size), strides
  * wsb, wsh and 1; each seen key's softmax weights, summed over its kv head's
  * query heads, are added to it (in a fixed order: equal calls give equal bits).

@@ -151,8 +151,8 @@ struct SelectShared {
   int first;
 };
 
-// Bound by its chain of passes, a few dependent latencies each: 11.8 us at
-// 1100 rows, 16.9 at 256 caches' heads of up to 8192 (256 threads instead of
+// Bound by its chain of passes, a few dependent latencies each: 11.6 us at
+// 1100 rows, 16.2 at 256 caches' heads of up to 8192 (256 threads instead of
 // 1024 take 12.7 us at 1100).
 //
 // One workgroup per (sequence, kv head).  Each thread owns `per` consecutive

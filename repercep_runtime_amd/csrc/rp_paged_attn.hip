@@ -20,7 +20,8 @@
 //   fp32 weight exactly, however small it is beside the largest; fp16 would end
 //   at 2^-24.  An fp16 V is the exact sum of two bf16 numbers, its first eight
 //   bits and the other three.  So a value takes three instructions, an fp16 one
-//   six; the products are idle otherwise.
+//   six (with two fp16 parts of a weight, 32 long fp16 sequences took 251 us and
+//   640 keys 10.1, now 259 and 12.3); the products are idle otherwise.
 // * The running maximum is lazy: a lane's scores are weighed against its
 //   column's base, and only when one exceeds it by 2^8 (kSlack) does the wave
 //   agree on a new base and rescale.  Every lane of a column holds the same
@@ -35,9 +36,9 @@
 //   step's K or V on its way.
 //
 // Bound by HBM where the cache is large: 64 sequences of 2048 to 16384 keys, 32
-// heads on 8 of 128, bf16, 2.4 GB in 431 us (5.6 TB/s), one of 131071 e4m3fn keys
+// heads on 8 of 128, bf16, 2.4 GB in 445 us (5.4 TB/s), one of 131071 e4m3fn keys
 // in 46 us and 5 of the join; by the latencies of a wave's steps where it is
-// small: 640 keys of 32 heads in 11.8 us.
+// small: 640 keys of 32 heads in 11.7 us.
 //
 // The keys of a (sequence, kv head) are split into chunks of equal size over
 // workgroups, a chunk over a workgroup's waves; waves join through LDS,
@@ -668,7 +669,8 @@ struct Plan {
 //   4100 keys: a seventh less time than on 512).
 // * Else a second launch is worth its 4 us where a workgroup's keys take
 //   longer than that: not up to 384 KB of them (640 keys of 128: 12.5 us a call
-//   unsplit, 16.9 in five parts), nor with two workgroups a CU, what its
+//   unsplit, 16.9 in five parts; captured, where launches cost less, 11.3 and
+//   9.8), nor with two workgroups a CU, what its
 //   registers hold, already (16 sequences x 32 heads: 17 us unsplit, 23 in two
 //   parts).  Fewer are split to no more than those 512: 131071 keys in 8 heads
 //   take 55 us on 512 workgroups, 58 on 1024, 64 on 2048.
@@ -707,8 +709,10 @@ inline Plan decode_plan(int64_t groups, int64_t keys, int64_t key_bytes, bool we
   return Plan{(int32_t)splits, (int32_t)chunk};
 }
 
-// Caches larger than the 256 MB last-level cache, of which nothing would be
-// left by the next call, are read past it: V's rows, whose lines one
+// Calls that read more than the 256 MB last-level cache, of which nothing would
+// be left by the next call, read past it (a page that sequences share counts
+// once for each, which is too much for long prompts with many candidates): V's
+// rows, whose lines one
 // instruction takes whole, with the non-temporal hint.  One state of 8 heads
 // of 128, per call: 403 MB 71 us against 84, 806 MB 130 against 144, e4m3fn
 // 554 MB 87 against 102; 202 MB 40.5 us against 38.7 without the hint.  K's
