@@ -839,8 +839,8 @@ extern "C" int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64
     return RP_ERR_INVALID_ARGUMENT;
   }
   const int64_t tiles = (H / cache->heads + 15) / 16;
-  if (cache->heads * tiles > 65535 ||
-      (H + (c.capacity() / (4 * kJThreads) + 1) * cache->heads) * kJThreads > kMaxGridThreads) {
+  const int64_t blocks = key_weights ? c.capacity() / (4 * kJThreads) + 1 : 0;
+  if (cache->heads * tiles > 65535 || (H + blocks * cache->heads) * kJThreads > kMaxGridThreads) {
     rp_set_error("paged_attn_decode: too many heads or positions");
     return RP_ERR_UNSUPPORTED;
   }

@@ -423,3 +423,10 @@ def test_calls_past_the_launch_limit_are_refused() -> None:
     assert decode(long, H=16, w=FAKE, wsb=1 << 34, wsh=1 << 30, nbytes=1 << 62, qsb=2048,
                   osb=2048) == 2
     assert "too many" in L.rp_last_error().decode()
+
+
+def test_wide_tables_without_key_weights_are_taken() -> None:
+    """The key weights' launch limits only the calls that have them: this one
+    gets as far as its workspace."""
+    long = cache(heads=16, max_pages=1 << 26, stride_page=16 * 16 * 128)
+    assert decode(long, H=16, qsb=2048, osb=2048, ws=None, nbytes=0) == 3
