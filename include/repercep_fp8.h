@@ -610,6 +610,59 @@ int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N, int64_t V
                       float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------- drafted tokens
+ * The verdict on a sequence's drafted tokens d_0 .. d_{n-1} (n = lens[b], at
+ * least 0 and at most N; lens NULL: N), by random numbers that the caller
+ * draws: draft i is accepted while
+ *   u_i * q_i(d_i) < p_i(d_i),
+ * and behind the first m accepted ones one token is drawn: the lowest t with
+ *   w(0) + .. + w(t) > u_N * (w(0) + .. + w(V - 1)),
+ * w = max(p_m - q_m, 0) where draft m was rejected, w = p_m where all n were
+ * accepted or p_m - q_m leaves nothing; the last t with w(t) > 0 where no sum
+ * passes (u_N >= 1).  All in 64 bits.
+ *   tokens   (B, N); a draft outside [0, V) is rejected
+ *   target   p (B, N + 1, V), draft q (B, N, V) of one type (RP_OUT_* by
+ *            dtype), unit stride along V, strides tsb, tsn, dsb, dsn (>= 0) in
+ *            elements; they need not add up to 1, and a NaN weighs nothing.
+ *            draft NULL: the drafts were certain, q_i(d_i) = 1 and 0 elsewhere
+ *   u        (B, N + 1) in [0, 1)
+ *   out      (B, N + 1): the accepted drafts, the drawn token (-1 where every
+ *            w is 0), then -1; accepted (B): m
+ * N may be 0 (a draw from p_0).  V up to 2^22.  Equal calls give equal tokens.
+ * workspace: rp_verify_drafts_workspace_bytes, 256-byte aligned.
+ * No counterpart in the reference. */
+size_t rp_verify_drafts_workspace_bytes(int64_t B, int64_t V);
+int rp_verify_drafts(const int64_t* tokens, const int32_t* lens, int64_t B, int64_t N,
+                     const void* target, int64_t tsb, int64_t tsn, const void* draft, int64_t dsb,
+                     int64_t dsn, int dtype, int64_t V, const float* u, int64_t* out,
+                     int32_t* accepted, void* workspace, size_t workspace_bytes, void* stream);
+
+/* --------------------------------------- QK norm and rotation in 16 bits
+ * For each row x of q (B, H, S, D) and k (B, Hkv, S, D), bf16 or fp16:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (norm 0: y = x; a NULL weight: 1)
+ * and the pairs of its first `rot` dims turned by the token's position:
+ * pair j < rot / 2 is (y_j, y_{j + rot/2}) (RP_ROPE_HALF) or (y_{2j},
+ * y_{2j+1}) (RP_ROPE_INTERLEAVED), its angle positions[axis][b][s] * freq[j]
+ * radians; the first sections[0] pairs turn by axis 0, the next sections[1]
+ * by axis 1, ... (sections: host memory, `axes` of them, rot / 2 in all).
+ * Angles are formed in 64 bits, all else in fp32, the result rounded once.
+ *   q, k, q_out, k_out   strides sb, sh, ss in elements, unit stride along D,
+ *            rows 16-byte aligned; an output may be its input (same strides),
+ *            rows of an output do not overlap.  Hkv 0: no k
+ *   weights  (D) of q's type, 16-byte aligned
+ *   positions   int32, strides psa, psb, pss
+ *   freq     (rot / 2) float, or double where freq_is_double
+ * D 32, 64, 128 or 256; rot a multiple of 16.  The 16-bit counterpart of
+ * rp_fp8_rmsnorm_scale_quantize, whose rotation takes tables. */
+#define RP_ROPE_MAX_AXES 4
+int rp_qk_norm_rope(const void* q, const void* k, int dtype, int64_t B, int64_t S, int64_t H,
+                    int64_t Hkv, int64_t D, int64_t qsb, int64_t qsh, int64_t qss, int64_t ksb,
+                    int64_t ksh, int64_t kss, const void* q_weight, const void* k_weight, int norm,
+                    float eps, const int32_t* positions, int64_t psa, int64_t psb, int64_t pss,
+                    const void* freq, int freq_is_double, int64_t rot, const int64_t* sections,
+                    int axes, int rope_mode, void* q_out, int64_t qob, int64_t qoh, int64_t qos,
+                    void* k_out, int64_t kob, int64_t koh, int64_t kos, void* stream);
+
 /* ---------------------------------------------------------- self-test
  * Device routines exposed so the tests can pin them exhaustively against
  * the CPU oracle.  They run the same device functions the kernels above use.

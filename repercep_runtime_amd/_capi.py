@@ -12,6 +12,7 @@ import ctypes
 import os
 import struct
 from pathlib import Path
+from typing import Sequence
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "librepercep_fp8.so"
 
@@ -39,6 +40,7 @@ RP_CACHE_BF16 = 0
 RP_CACHE_F16 = 1
 RP_CACHE_E4M3 = 2
 RP_LOGPROB_MAX_TOP = 32
+RP_ROPE_MAX_AXES = 4
 
 #: Every function include/repercep_fp8.h declares.
 EXPORTS = (
@@ -63,6 +65,7 @@ EXPORTS = (
     "rp_paged_kv_append", "rp_paged_attn_workspace_bytes", "rp_paged_attn_decode",
     "rp_paged_evict_workspace_bytes", "rp_paged_kv_evict",
     "rp_token_logprobs_workspace_bytes", "rp_token_logprobs",
+    "rp_qk_norm_rope", "rp_verify_drafts_workspace_bytes", "rp_verify_drafts",
     "rp_selftest_e4m3", "rp_selftest_scale", "rp_selftest_quant_one_launch",
     "rp_selftest_rope_block", "rp_selftest_paged_row",
 )
@@ -99,6 +102,11 @@ class PagedCache(ctypes.Structure):
 #: 0): quicker than building the structure.
 pack_paged_cache = struct.Struct("5P10q").pack
 assert struct.calcsize("5P10q") == ctypes.sizeof(PagedCache)
+
+
+def pack_sections(counts: Sequence[int]) -> bytes:
+    """A host array of int64."""
+    return struct.pack(f"{len(counts)}q", *counts)
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -209,6 +217,15 @@ def _declare(L: ctypes.CDLL) -> None:
     L.rp_token_logprobs.restype = _int
     L.rp_token_logprobs.argtypes = ([_vp, _int, _i64, _i64, _i64, _vp, _f32, _int]
                                     + [_vp] * 5 + [_sz, _vp])
+    L.rp_qk_norm_rope.restype = _int
+    L.rp_qk_norm_rope.argtypes = ([_vp, _vp, _int] + [_i64] * 11 + [_vp, _vp, _int, _f32, _vp]
+                                  + [_i64] * 3 + [_vp, _int, _i64, _vp, _int, _int, _vp]
+                                  + [_i64] * 3 + [_vp] + [_i64] * 3 + [_vp])
+    L.rp_verify_drafts_workspace_bytes.restype = _sz
+    L.rp_verify_drafts_workspace_bytes.argtypes = [_i64, _i64]
+    L.rp_verify_drafts.restype = _int
+    L.rp_verify_drafts.argtypes = ([_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int,
+                                    _i64] + [_vp] * 4 + [_sz, _vp])
     L.rp_selftest_paged_row.restype = _i64
     L.rp_selftest_paged_row.argtypes = [cache, _i64, _i64]
     L.rp_fp8_transpose.restype = _int

@@ -202,6 +202,31 @@ __device__ __forceinline__ float dequant_from_amax(uint32_t amax_bits) {
   else return dequant_from_amax_bits(amax_bits);
 }
 
+// ------------------------------------------------------- host checks
+struct Dim {
+  int64_t size, stride;
+};
+
+// Whether no two rows of `unit` elements share memory: in rising order of
+// stride, each dimension steps past all that the smaller ones span.  (Layouts
+// that interleave without sharing, but do not nest, count as sharing.)
+template <int N>
+inline bool rows_apart(int64_t unit, const Dim (&dims)[N]) {
+  Dim d[N];
+  for (int i = 0; i < N; ++i) {
+    int j = i;
+    for (; j > 0 && d[j - 1].stride > dims[i].stride; --j) d[j] = d[j - 1];
+    d[j] = dims[i];
+  }
+  __int128 span = unit;
+  for (int i = 0; i < N; ++i) {
+    if (d[i].size <= 1) continue;
+    if (d[i].stride < span) return false;
+    span += (__int128)(d[i].size - 1) * d[i].stride;
+  }
+  return true;
+}
+
 }  // namespace rp
 
 // Thread-local last-error message shared by all entry points.

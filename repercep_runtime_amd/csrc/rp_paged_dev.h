@@ -109,30 +109,6 @@ inline int paged_view(const char* what, const rp_paged_cache* c, PagedView* v) {
   return RP_OK;
 }
 
-struct Dim {
-  int64_t size, stride;
-};
-
-// Whether no two rows of `unit` elements share memory: in rising order of
-// stride, each dimension steps past all that the smaller ones span.  (Layouts
-// that interleave without sharing, but do not nest, count as sharing.)
-template <int N>
-inline bool rows_apart(int64_t unit, const Dim (&dims)[N]) {
-  Dim d[N];
-  for (int i = 0; i < N; ++i) {
-    int j = i;
-    for (; j > 0 && d[j - 1].stride > dims[i].stride; --j) d[j] = d[j - 1];
-    d[j] = dims[i];
-  }
-  __int128 span = unit;
-  for (int i = 0; i < N; ++i) {
-    if (d[i].size <= 1) continue;
-    if (d[i].stride < span) return false;
-    span += (__int128)(d[i].size - 1) * d[i].stride;
-  }
-  return true;
-}
-
 // Refuses a cache of which two rows share memory, K's and V's among them, for
 // the calls that write it.
 inline int paged_writable(const char* what, const rp_paged_cache* c) {

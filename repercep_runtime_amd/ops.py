@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import functools
 import math
-from typing import Callable, Literal, NamedTuple
+from typing import Callable, Literal, NamedTuple, Sequence
 
 import torch
 
@@ -1353,6 +1353,173 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
             ids.data_ptr() if top else None, ws.data_ptr() if n else None, n, _stream(x))
         C.check(rc, "rp_token_logprobs")
     return TokenLogprobs(logprobs, entropy, top_lp, ids)
+
+
+class DraftVerdict(NamedTuple):
+    """``verify_drafts``' answer."""
+
+    tokens: torch.Tensor
+    accepted: torch.Tensor
+
+
+def verify_drafts(draft_tokens: torch.Tensor, target_probs: torch.Tensor, uniforms: torch.Tensor,
+                  *, draft_probs: torch.Tensor | None = None,
+                  draft_lens: torch.Tensor | None = None) -> DraftVerdict:
+    """The verdict on drafted tokens, by given random numbers.
+
+    ``draft_tokens`` (B, N) int64, of which sequence b has ``draft_lens[b]``
+    (int32; None: all N); ``target_probs`` p (B, N + 1, V) and ``draft_probs``
+    q (B, N, V), the probabilities that the target and the draft model gave
+    position i, both fp32, bf16 or fp16 with a unit stride on V (None: the
+    drafts were certain); ``uniforms`` (B, N + 1) fp32 in [0, 1).  Draft i is
+    accepted while ``uniforms[:, i] * q_i < p_i`` at its token.  Behind the
+    first m accepted ones a token is drawn with ``uniforms[:, N]``, by the
+    running sums of max(p_m - q_m, 0) in token order if draft m was rejected
+    (of p_m where that leaves nothing), of p_m if none was; so tokens come out
+    as if drawn from p.  Probabilities need not add up to 1.
+
+    Returns ``tokens`` (B, N + 1) int64, the accepted drafts, the drawn token
+    and -1 behind it (-1 in its place too where p_m has no positive value),
+    and ``accepted`` (B,) int32, the numbers m."""
+    if draft_tokens.dim() != 2 or target_probs.dim() != 3:
+        raise ValueError(f"draft_tokens must be (B, N) and target_probs (B, N + 1, V), got "
+                         f"{tuple(draft_tokens.shape)}, {tuple(target_probs.shape)}")
+    B, N = draft_tokens.shape
+    V = target_probs.shape[2]
+    if target_probs.shape[:2] != (B, N + 1) or V < 1:
+        raise ValueError(f"target_probs {tuple(target_probs.shape)} must be ({B}, {N + 1}, V)")
+    if draft_probs is not None and draft_probs.shape != (B, N, V):
+        raise ValueError(f"draft_probs {tuple(draft_probs.shape)} must be ({B}, {N}, {V})")
+    if draft_tokens.dtype != torch.int64:
+        raise TypeError(f"draft_tokens must be int64 (got {draft_tokens.dtype})")
+    dt = _OUT_DTYPES.get(target_probs.dtype)
+    if dt is None or (draft_probs is not None and draft_probs.dtype != target_probs.dtype):
+        raise TypeError(f"target_probs and draft_probs must share one of bfloat16, float16 and "
+                        f"float32 (got {target_probs.dtype}"
+                        + (f", {draft_probs.dtype})" if draft_probs is not None else ")"))
+    if uniforms.dtype != torch.float32 or uniforms.shape != (B, N + 1):
+        raise ValueError(f"uniforms must be float32 ({B}, {N + 1}), got {uniforms.dtype} "
+                         f"{tuple(uniforms.shape)}")
+    _unit_stride("target_probs", target_probs)
+    if draft_probs is not None:
+        _unit_stride("draft_probs", draft_probs)
+    if draft_lens is not None:
+        _int32_vector("draft_lens", draft_lens, B)
+    _on_device_of(target_probs, target_probs=target_probs, draft_tokens=draft_tokens,
+                  uniforms=uniforms, draft_probs=draft_probs, draft_lens=draft_lens)
+    t, u = draft_tokens.contiguous(), uniforms.contiguous()
+    tokens = t.new_empty((B, N + 1))
+    accepted = t.new_empty((B,), dtype=torch.int32)
+    if B > 0:
+        n = C.lib().rp_verify_drafts_workspace_bytes(B, V)
+        ws = t.new_empty(n, dtype=torch.uint8)
+        q = draft_probs if N > 0 else None
+        C.check(_on_device(
+            target_probs.get_device(), C.lib().rp_verify_drafts, t.data_ptr() if N else None,
+            draft_lens.data_ptr() if draft_lens is not None else None, B, N,
+            target_probs.data_ptr(), *_strides(target_probs, 2),
+            q.data_ptr() if q is not None else None, *(_strides(q, 2) if q is not None else (0, 0)),
+            dt, V, u.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), n,
+            _stream(t)), "rp_verify_drafts")
+    return DraftVerdict(tokens, accepted)
+
+
+def _rope_rows(name: str, x: torch.Tensor, like: torch.Tensor, weight: torch.Tensor | None,
+               out: torch.Tensor | None) -> torch.Tensor:
+    """The output for the rows ``x``, both and the weight checked."""
+    if x.dim() != 4 or (x.shape[0], *x.shape[2:]) != (like.shape[0], *like.shape[2:]):
+        raise ValueError(f"{name} {tuple(x.shape)} must be (B, heads, S, D) with q's B, S and D")
+    if x.dtype != like.dtype:
+        raise TypeError(f"{name} is {x.dtype}, q {like.dtype}")
+    _unit_stride(name, x)
+    if weight is not None and (weight.shape != (x.shape[3],) or weight.dtype != x.dtype
+                               or not weight.is_contiguous()):
+        raise ValueError(f"norm_{name}_weight must be a contiguous ({x.shape[3]},) {x.dtype} vector")
+    if out is None:
+        B, H, S, D = x.shape
+        return x.new_empty((B, H, S, D))
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError(f"out_{name} must be {tuple(x.shape)} {x.dtype}")
+    _unit_stride(f"out_{name}", out)
+    return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
+                 inv_freq: torch.Tensor, *, sections: Sequence[int] | None = None,
+                 norm_q_weight: torch.Tensor | None = None,
+                 norm_k_weight: torch.Tensor | None = None, eps: float | None = 1e-6,
+                 rope_layout: Literal["half", "interleaved"] = "half",
+                 out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """RMSNorm of each head of q and k and their rotation by position, in one
+    pass and in 16 bits: what ``rmsnorm_scale_quantize`` does on the way to
+    FP8 codes, for rows that go into a paged cache or a 16-bit attention.
+
+    ``q`` (B, H, S, D) and ``k`` (B, Hkv, S, D) or None, bf16 or fp16 with a
+    unit stride on D and 16-byte aligned rows (slices of a fused projection).
+    Each row is divided by sqrt(mean(x^2) + eps) and multiplied by its weight
+    (D,) (``eps`` None: no norm); then, of its first ``2 * len(inv_freq)``
+    dims, pair j ("half": j and j + len(inv_freq), "interleaved": 2 j and
+    2 j + 1) is turned by ``position * inv_freq[j]``.  ``positions`` int32: (B,
+    S), or with ``sections`` (axes, B, S), where the first ``sections[0]``
+    pairs turn by the positions along axis 0 (a video's frames), the next by
+    axis 1 (rows), axis 2 (columns); any strides, so one grid can be expanded
+    over the batch.  ``inv_freq`` fp32 or fp64, a multiple of 8 long.  Angles
+    are formed in 64 bits, so far positions lose nothing; all else is fp32,
+    rounded once.  Returns (q, k) of q's dtype; ``out_q`` may be q itself, and
+    ``out_k`` k."""
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, H, S, D), got {tuple(q.shape)}")
+    B, H, S, D = q.shape
+    dt = _IN_DTYPES.get(q.dtype)
+    if dt is None:
+        raise TypeError(f"q must be bfloat16 or float16 (got {q.dtype})")
+    if D not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"head_dim {D} not in compiled tile shapes {sorted(SUPPORTED_HEAD_DIMS)}")
+    mode = _ROPE.get(rope_layout)
+    if not mode:
+        raise ValueError(f"rope_layout must be 'half' or 'interleaved' (got {rope_layout!r})")
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) \
+            or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be a contiguous float32 or float64 vector (got "
+                         f"{inv_freq.dtype} {tuple(inv_freq.shape)})")
+    pairs = inv_freq.shape[0]
+    if pairs % 8 != 0 or not 0 < 2 * pairs <= D:
+        raise ValueError(f"inv_freq must have a multiple of 8 values up to {D // 2} (got {pairs})")
+    lead = (B, S) if sections is None else (len(sections), B, S)
+    if positions.dtype != torch.int32 or positions.shape != lead:
+        raise ValueError(f"positions must be int32 {lead} (got {positions.dtype} "
+                         f"{tuple(positions.shape)})")
+    if sections is not None and (not 0 < len(sections) <= C.RP_ROPE_MAX_AXES or sum(sections) != pairs
+                                 or min(sections) < 0):
+        raise ValueError(f"sections {tuple(sections)} must be up to {C.RP_ROPE_MAX_AXES} counts of "
+                         f"pairs that add up to {pairs}")
+    if eps is None and (norm_q_weight is not None or norm_k_weight is not None):
+        raise ValueError("weights without a norm (eps is None)")
+    if eps is not None and not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative (got {eps})")
+    if k is None and (norm_k_weight is not None or out_k is not None):
+        raise ValueError("norm_k_weight and out_k come with k")
+    yq = _rope_rows("q", q, q, norm_q_weight, out_q)
+    yk = _rope_rows("k", k, q, norm_k_weight, out_k) if k is not None else None
+    _on_device_of(q, q=q, k=k, positions=positions, inv_freq=inv_freq, norm_q_weight=norm_q_weight,
+                  norm_k_weight=norm_k_weight, out_q=out_q, out_k=out_k)
+    Hkv = k.shape[1] if k is not None else 0
+    if B == 0 or S == 0 or H + Hkv == 0:
+        return yq, yk
+    counts = sections if sections is not None else (pairs,)
+    pst = [0, *_strides(positions, 2)] if sections is None else _strides(positions, 3)
+    none = (0, 0, 0)
+    C.check(_on_device(
+        q.get_device(), C.lib().rp_qk_norm_rope, q.data_ptr(), k.data_ptr() if Hkv else None, dt,
+        B, S, H, Hkv, D, *_strides(q, 3), *(_strides(k, 3) if Hkv else none),
+        norm_q_weight.data_ptr() if norm_q_weight is not None else None,
+        norm_k_weight.data_ptr() if norm_k_weight is not None else None, eps is not None,
+        eps if eps is not None else 0.0, positions.data_ptr(), *pst, inv_freq.data_ptr(),
+        inv_freq.dtype == torch.float64, 2 * pairs, C.pack_sections(counts), len(counts), mode,
+        yq.data_ptr(), *_strides(yq, 3), yk.data_ptr() if Hkv else None,
+        *(_strides(yk, 3) if Hkv else none), _stream(q)), "rp_qk_norm_rope")
+    return yq, yk
 
 
 def selftest_e4m3(x: torch.Tensor) -> torch.Tensor:
