@@ -571,6 +571,35 @@ int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64
                          float* key_weights, int64_t wsb, int64_t wsh, int64_t max_seq_len,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention of each sequence's last tokens over its rows, causal, within a
+ * window.  Sequence b has seq_lens[b] rows, the last q_lens[b] of them (at
+ * least 0 and at most S; NULL: S) the rows of its new tokens; token i stands
+ * at position p = seq_lens[b] - q_lens[b] + i and sees the rows j with
+ *   j <= p,  and  p - j < window (0: any)  or  j < sinks:
+ *   s_j = sm_scale * q_i . k_j,  out_i = sum_j softmax(s)_j v_j,
+ *   lse_i = log(sum_j exp(s_j))                      (lse NULL: not written)
+ * q (B, H, S, head_dim) with strides qsb, qsh, qss, out of q's type with
+ * strides osb, osh, oss (no two rows of out share memory); lse float (B, H, S).
+ * Types, heads, scale and cache as in rp_paged_attn_decode.  A token that sees
+ * no row, or scores of -inf only, and a token i >= q_lens[b] get zeros and lse
+ * -inf.  Sums are held in fp32; a weight enters the product with V rounded once
+ * to 16 bits or more (the type of out at least), and out is rounded once.
+ * Values up to the type's largest do not overflow on the way.  Infinities and
+ * NaNs in rows of V reach the tokens that see them and no others (a weight
+ * below 2^-31 of the largest may count as 0 beside an infinity: NaN).
+ * max_seq_len (0: unknown) as in rp_paged_attn_decode.
+ * workspace: rp_paged_window_workspace_bytes of the same arguments, 256-byte
+ * aligned (may be NULL where that is 0). */
+size_t rp_paged_window_workspace_bytes(int64_t B, int64_t H, int64_t S,
+                                       const rp_paged_cache* cache, int64_t window, int64_t sinks,
+                                       int64_t max_seq_len);
+int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64_t H, int64_t S, int64_t qsb,
+                         int64_t qsh, int64_t qss, const rp_paged_cache* cache,
+                         const int32_t* seq_lens, const int32_t* q_lens, int64_t window,
+                         int64_t sinks, float sm_scale, void* out, int64_t osb, int64_t osh,
+                         int64_t oss, float* lse, int64_t max_seq_len, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 /* Cuts each sequence longer than `budget` rows to `budget`, per kv head: the
  * last `recent` (<= budget) rows stay, and of the others those with the
  * largest weights, the lower position where weights are equal (-0 equals 0; a

@@ -65,7 +65,8 @@ EXPORTS = (
     "rp_paged_kv_append", "rp_paged_attn_workspace_bytes", "rp_paged_attn_decode",
     "rp_paged_evict_workspace_bytes", "rp_paged_kv_evict",
     "rp_token_logprobs_workspace_bytes", "rp_token_logprobs",
-    "rp_qk_norm_rope", "rp_verify_drafts_workspace_bytes", "rp_verify_drafts",
+    "rp_paged_window_workspace_bytes", "rp_paged_attn_window", "rp_qk_norm_rope",
+    "rp_verify_drafts_workspace_bytes", "rp_verify_drafts",
     "rp_selftest_e4m3", "rp_selftest_scale", "rp_selftest_quant_one_launch",
     "rp_selftest_rope_block", "rp_selftest_paged_row",
 )
@@ -217,6 +218,11 @@ def _declare(L: ctypes.CDLL) -> None:
     L.rp_token_logprobs.restype = _int
     L.rp_token_logprobs.argtypes = ([_vp, _int, _i64, _i64, _i64, _vp, _f32, _int]
                                     + [_vp] * 5 + [_sz, _vp])
+    L.rp_paged_window_workspace_bytes.restype = _sz
+    L.rp_paged_window_workspace_bytes.argtypes = [_i64] * 3 + [cache] + [_i64] * 3
+    L.rp_paged_attn_window.restype = _int
+    L.rp_paged_attn_window.argtypes = ([_vp, _int] + [_i64] * 6 + [cache, _vp, _vp, _i64, _i64, _f32,
+                                       _vp] + [_i64] * 3 + [_vp, _i64, _vp, _sz, _vp])
     L.rp_qk_norm_rope.restype = _int
     L.rp_qk_norm_rope.argtypes = ([_vp, _vp, _int] + [_i64] * 11 + [_vp, _vp, _int, _f32, _vp]
                                   + [_i64] * 3 + [_vp, _int, _i64, _vp, _int, _int, _vp]

@@ -1,0 +1,601 @@
+// Attention of many new tokens per sequence (a prompt, a chunk of one) over a
+// paged key-value cache, causal, within a window, with sinks.
+//
+// Both products run on the matrix cores (32x32x16).  A wave owns 32 rows; a
+// workgroup's waves share tiles of 64 keys, K and V staged in LDS as 16-bit
+// rows, two tiles deep.
+//
+// * S^T = K Q^T: a lane ends up with 32 scores of one row, so the softmax's
+//   maximum and sum stay in the lane but for its partner in the wave's other
+//   half.  The keys it holds are those that O^T = V^T P^T asks of it, if V's
+//   operand is read in that order (ds_read_b64_tr_b16: four keys of a column):
+//   P never leaves the lane.
+// * The running maximum is lazy: rows are weighed about their base, which is
+//   only moved, and the sums rescaled, when a score exceeds it by 2^kSlack.
+//   A bf16 P is weighed about a base so high that a row's weights add up to
+//   less than 1, so sums of values near fp32's largest cannot overflow; an fp16
+//   P about one below the largest score, so that weights down to 2^-21 of the
+//   largest keep their 11 bits, and smaller ones 2^-31 of it.
+// * P enters the second product rounded once to 16 bits, as precise as the
+//   output.  For an e4m3fn cache, whose row scales can be of any size, it is
+//   bf16; an fp16 output then takes it as the sum of two bf16 numbers.
+// * A row of V that only some of a wave's rows see may hold infinities or NaNs,
+//   which 0 P does not silence.  Sums that come out infinite or NaN are taken
+//   again token by token, V masked for each.
+
+#include "rp_paged_window.h"
+
+namespace rp {
+namespace {
+
+constexpr int kTile = 64;                       // keys a tile: one page entry a lane
+constexpr float kSlack = 8.0f;                  // powers of two
+
+template <bool F16>
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (F16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  }
+}
+
+// Four keys of a column: the 16 lanes of a row of lanes bring four rows of 16
+// columns, four lanes a row, and each takes a column.
+__device__ __forceinline__ u32x2 column4(const uint16_t* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (lds_s16x4)(uintptr_t)(uint32_t)(uintptr_t)p));
+}
+
+template <int QT, int CT, int D, int NW>
+struct Prompt {
+  static constexpr bool FP8 = CT == RP_CACHE_E4M3;
+  static constexpr bool QF16 = QT == kInF16;            // the first product's type
+  static constexpr bool VF16 = CT == RP_CACHE_F16;      // the second's
+  static constexpr int PARTS = FP8 && QF16 ? 2 : 1;     // of a weight
+  static constexpr int EB = FP8 ? 1 : 2, NT = NW * kWave;
+  static constexpr int QSTEPS = D / 16, DB = D / 32;
+  static constexpr int LD = D + 8;                      // a row of LDS: 16 bytes more
+  static constexpr int CPR = D * EB / 16;               // 16-byte chunks a row
+  static constexpr int NCH = (kTile * CPR + NT - 1) / NT;
+  static constexpr int ROWS = NW * 32;
+
+  struct Shared {
+    uint16_t k[2][kTile][LD];
+    uint16_t v[2][kTile][LD];
+    float ks[2][kTile], vs[2][kTile];                   // e4m3fn only
+    int redo;
+  };
+};
+
+template <int QT, int CT, int D, int NW>
+__global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedView c) {
+  typedef Prompt<QT, CT, D, NW> P;
+  __shared__ typename P::Shared sh;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int m = lane & 31, h = lane >> 5;
+
+  // The workgroups of eight (sequence, kv head) pairs at a time, one pair an
+  // XCD, so that a pair's keys stay in one L2; the tiles with most keys first.
+  int64_t at = blockIdx.x;
+  const int split = (int)(at % a.splits);
+  at /= a.splits;
+  const int64_t lanes8 = min((int64_t)8, a.groups);
+  const int64_t eight = at / (lanes8 * a.tiles);
+  const int64_t width = min(lanes8, a.groups - eight * lanes8);
+  at -= eight * lanes8 * a.tiles;
+  const int64_t pair = eight * lanes8 + at % width;
+  const int tile = a.tiles - 1 - (int)(at / width);
+  const int b = (int)(pair / c.heads), kv = (int)(pair % c.heads);
+
+  const Place pl(a, b);
+  const int rows = pl.m * a.group, all = a.S * a.group;
+  const int r0 = tile * P::ROWS;                         // the workgroup's first row
+  const int row = r0 + 32 * wave + m;
+  const int token = row / a.group, head = kv * a.group + row % a.group;
+  const bool live = row < rows;
+  const int64_t orow = ((int64_t)b * a.H + head) * a.S + token;
+  const int32_t pos = live ? pl.first + token : -1;
+  // the wave's rows' first and last positions
+  const int w0 = r0 + 32 * wave, w1 = min(w0 + 32, rows) - 1;
+  const int32_t pmin = pl.first + w0 / a.group, pmax = w1 >= w0 ? pl.first + w1 / a.group : -1;
+  const int last = min(r0 + P::ROWS, rows) - 1;
+  const KeyTiles<kTile> keys(a, c, pl.first + r0 / a.group,
+                             last >= r0 ? pl.first + last / a.group : -1);
+  const int t0 = (int)((int64_t)keys.count * split / a.splits);
+  const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
+  const int32_t* table = c.table + b * c.table_stride;
+
+  u32x4 q[P::QSTEPS];
+  {
+    const uint16_t* src = a.q + b * a.qsb + (int64_t)head * a.qsh + (int64_t)token * a.qss + 8 * h;
+#pragma unroll
+    for (int t = 0; t < P::QSTEPS; ++t) {
+      q[t] = live ? *reinterpret_cast<const u32x4*>(src + 16 * t) : u32x4{0u, 0u, 0u, 0u};
+      q[t] ^= a.flip;
+    }
+  }
+
+  f32x16 acc[P::DB];
+  float base, sum;
+
+  // ---- staging
+  u32x4 kreg[P::NCH], vreg[P::NCH];
+  float sreg = 0.0f;
+  uint64_t present;                                      // of the tile in the registers
+  auto page_of = [&](int t) -> int32_t {                 // lane l: the page of key l of tile t
+    const int32_t j = keys.key(t) + lane;
+    return t < t1 && keys.any(j) ? paged_page(c, table, j) : -1;
+  };
+  auto load = [&](int t, int32_t pages) {
+    const int32_t kb = keys.key(t);
+    present = __ballot(pages >= 0);
+#pragma unroll
+    for (int i = 0; i < P::NCH; ++i) {
+      const int ch = min(tid + i * P::NT, kTile * P::CPR - 1);
+      const int r = ch / P::CPR, col = ch % P::CPR * 16;
+      // what is no row is read as a row of page 0 and put into LDS as zeros
+      const int32_t page = max(0, __shfl(pages, r, kWave));
+      const int64_t off = paged_row(c, page, kv, kb + r) * P::EB + col;
+      kreg[i] = *reinterpret_cast<const u32x4*>(c.k + off);
+      vreg[i] = *reinterpret_cast<const u32x4*>(c.v + off);
+    }
+    if constexpr (P::FP8) {
+      if (wave < 2)
+        sreg = (wave == 0 ? c.ks : c.vs)[paged_scale(c, max(0, pages), kv, kb + lane)];
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < P::NCH; ++i) {
+      const int ch = tid + i * P::NT;
+      if (kTile * P::CPR % P::NT != 0 && ch >= kTile * P::CPR) break;
+      const int r = ch / P::CPR;
+      const uint32_t keep = (present >> r & 1) ? 0xffffffffu : 0u;
+      u32x4 kk = kreg[i] & keep, vv = vreg[i] & keep;
+      if constexpr (!P::FP8) {
+        const int col = ch % P::CPR * 8;
+        *reinterpret_cast<u32x4*>(&sh.k[buf][r][col]) = kk;
+        *reinterpret_cast<u32x4*>(&sh.v[buf][r][col]) = vv;
+      } else {
+        const int col = ch % P::CPR * 16;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          u32x4 x, y;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[2 * e] = codes_to_16<P::QF16, false>(kk[2 * half + e]);
+            x[2 * e + 1] = codes_to_16<P::QF16, true>(kk[2 * half + e]);
+            y[2 * e] = codes_to_16<false, false>(vv[2 * half + e]);
+            y[2 * e + 1] = codes_to_16<false, true>(vv[2 * half + e]);
+          }
+          *reinterpret_cast<u32x4*>(&sh.k[buf][r][col + 8 * half]) = x;
+          *reinterpret_cast<u32x4*>(&sh.v[buf][r][col + 8 * half]) = y;
+        }
+      }
+    }
+    if constexpr (P::FP8) {
+      if (wave < 2) {
+        const float s = present >> lane & 1 ? sreg : 0.0f;
+        if (wave == 0) sh.ks[buf][lane] = s * a.c;
+        else sh.vs[buf][lane] = s;
+      }
+    }
+  };
+
+  // ---- one tile of keys for the wave's rows
+  auto attend = [&](int buf, int32_t kb, uint64_t here, bool careful) {
+    // no row of the wave sees a key of the tile
+    if (kb > pmax || (kb + kTile - 1 <= max(0, pmin) - a.window && kb >= a.sinks)) return;
+    const bool whole = here == ~0ull && kb + kTile - 1 <= pmin &&
+                       (kb > pmax - a.window || kb + kTile <= a.sinks);
+    f32x16 s[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < P::QSTEPS; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const u32x4 f = *reinterpret_cast<const u32x4*>(&sh.k[buf][32 * k + m][16 * t + 8 * h]);
+        s[k] = mma32<P::QF16>(f, q[t], s[k]);
+      }
+    float x[2][16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 f = {a.c, a.c, a.c, a.c};
+        if constexpr (P::FP8) f = *reinterpret_cast<const f32x4*>(&sh.ks[buf][32 * k + 8 * i + 4 * h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][4 * i + e] = s[k][4 * i + e] * f[e];
+      }
+    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};       // bit 8 i + e: key 8 i + 4 h + e
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t pk = (uint32_t)(here >> 32 * k) >> 4 * h;
+        seen[k] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int32_t j = kb + 32 * k + 8 * i + 4 * h + e;
+            const bool in = (pk >> (8 * i + e) & 1) && sees(a, pos, j);
+            seen[k] |= in ? 1u << (8 * i + e) : 0u;
+            x[k][4 * i + e] = in ? x[k][4 * i + e] : neg_inf();
+          }
+      }
+    }
+    float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(x[0][i], x[1][i]));
+    if (__any(top > base + (kSlack - a.lift))) {
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float next = fmaxf(base, top + a.lift);
+      const float r = next == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(base - next);
+      sum *= r;
+#pragma unroll
+      for (int d = 0; d < P::DB; ++d) acc[d] *= r;
+      base = next;
+    }
+    const float b0 = base == neg_inf() ? 0.0f : base;    // no score yet: exp2(-inf) is 0
+    uint32_t p[P::PARTS][2][8];
+    float part_sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float w[4];
+        f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+        if constexpr (P::FP8) f = *reinterpret_cast<const f32x4*>(&sh.vs[buf][32 * k + 8 * i + 4 * h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(x[k][4 * i + e] - b0);
+          part_sum[k] += w[e];
+          if constexpr (P::FP8) {
+            w[e] *= f[e];
+            if (!whole) w[e] = seen[k] >> (8 * i + e) & 1 ? w[e] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float u = w[2 * e], v = w[2 * e + 1];
+          if constexpr (P::PARTS == 1) {
+            p[0][k][2 * i + e] = round_pair<P::VF16>(u, v);
+          } else {
+            p[0][k][2 * i + e] = pack_cut(u, v);
+            p[P::PARTS - 1][k][2 * i + e] = round_pair<false>(u - bf16_cut(u), v - bf16_cut(v));
+          }
+        }
+      }
+    sum += part_sum[0] + part_sum[1];
+
+    // columns 32 d .. + 31 of keys 32 k + 16 u + 4 h + {0..3, 8..11}
+    const int l16 = lane & 15, cb = (lane >> 4 & 1) * 16 + (l16 & 3) * 4;
+    auto v_frag = [&](int d, int k, int u) -> u32x4 {
+      const uint16_t* at = &sh.v[buf][32 * k + 16 * u + 4 * h + (l16 >> 2)][32 * d + cb];
+      const u32x2 lo = column4(at), hi = column4(at + 8 * P::LD);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    if (!careful) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int d = 0; d < P::DB; ++d) {
+            const u32x4 f = v_frag(d, k, u);
+#pragma unroll
+            for (int e = 0; e < P::PARTS; ++e)
+              acc[d] = mma32<P::VF16>(f, u32x4{p[e][k][4 * u], p[e][k][4 * u + 1],
+                                               p[e][k][4 * u + 2], p[e][k][4 * u + 3]}, acc[d]);
+          }
+      return;
+    }
+    // one token of the wave at a time, V as that token sees it
+    for (int32_t at = pmin; at <= pmax; ++at) {
+      const bool mine = pos == at;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t mask[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int32_t j = kb + 32 * k + 16 * u + 4 * h + (e < 2 ? 2 * e : 4 + 2 * e);
+            mask[e] = (sees(a, at, j) ? 0xffffu : 0u) | (sees(a, at, j + 1) ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int d = 0; d < P::DB; ++d) {
+            u32x4 f = v_frag(d, k, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] &= mask[e];
+            f32x16 y = mma32<P::VF16>(f, u32x4{p[0][k][4 * u], p[0][k][4 * u + 1],
+                                               p[0][k][4 * u + 2], p[0][k][4 * u + 3]}, acc[d]);
+            if constexpr (P::PARTS == 2) {
+              // a second part of 0 would make NaN of an infinity
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] = finite_pair<P::VF16>(f[e]);
+              y = mma32<P::VF16>(f, u32x4{p[1][k][4 * u], p[1][k][4 * u + 1],
+                                          p[1][k][4 * u + 2], p[1][k][4 * u + 3]}, y);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = mine ? y[i] : acc[d][i];
+          }
+        }
+    }
+  };
+
+  for (int careful = 0; careful < 2; ++careful) {
+    base = neg_inf();
+    sum = 0.0f;
+#pragma unroll
+    for (int d = 0; d < P::DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+    if (t0 < t1) {
+      load(t0, page_of(t0));
+      int32_t pages = page_of(t0 + 1);
+      store(0);
+      uint64_t here = present;
+      __syncthreads();
+      for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        const bool more = t + 1 < t1;
+        if (more) {
+          load(t + 1, pages);
+          pages = page_of(t + 2);
+        }
+        attend(buf, keys.key(t), here, careful != 0);
+        if (more) {
+          store(buf ^ 1);
+          here = present;
+        }
+        __syncthreads();
+      }
+    }
+    if (careful) break;
+    f32x16 z = acc[0] * 0.0f;
+#pragma unroll
+    for (int d = 1; d < P::DB; ++d) z += acc[d] * 0.0f;
+    float y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y += z[i];
+    if (tid == 0) sh.redo = 0;
+    __syncthreads();
+    if (live && y != y) sh.redo = 1;
+    __syncthreads();
+    if (!sh.redo) break;
+    __syncthreads();
+  }
+
+  if (row >= all) return;
+  sum += __shfl_xor(sum, 32, kWave);
+  if (!live) sum = 0.0f;                                 // a row past the new tokens
+  const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (a.splits > 1) {
+    if (h == 0) a.ml[orow * a.splits + split] = float2{base, sum};
+    if (sum == 0.0f) return;
+    float* part = a.part + (orow * a.splits + split) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < P::DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(part + 32 * d + 8 * i) =
+            f32x4{acc[d][4 * i] * r, acc[d][4 * i + 1] * r, acc[d][4 * i + 2] * r, acc[d][4 * i + 3] * r};
+    return;
+  }
+  uint16_t* out = a.out + b * a.osb + (int64_t)head * a.osh + (int64_t)token * a.oss + 4 * h;
+#pragma unroll
+  for (int d = 0; d < P::DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 y = {acc[d][4 * i] * r, acc[d][4 * i + 1] * r, acc[d][4 * i + 2] * r, acc[d][4 * i + 3] * r};
+      if (sum == 0.0f) y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      *reinterpret_cast<u32x2*>(out + 32 * d + 8 * i) =
+          u32x2{pack_out<QT>(y[0], y[1]), pack_out<QT>(y[2], y[3])};
+    }
+  if (a.lse && h == 0)
+    a.lse[orow] = sum == 0.0f ? neg_inf() : (base + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <int QT, int CT, int D>
+void launch_prompt_d(const WindowArgs& a, const PagedView& c, int waves, hipStream_t st) {
+  const dim3 grid((unsigned)(a.groups * a.tiles * a.splits));
+  if (waves == 8)
+    hipLaunchKernelGGL((prompt_kernel<QT, CT, D, 8>), grid, dim3(8 * kWave), 0, st, a, c);
+  else
+    hipLaunchKernelGGL((prompt_kernel<QT, CT, D, 4>), grid, dim3(4 * kWave), 0, st, a, c);
+}
+
+template <int QT, int CT>
+void launch_prompt(const WindowArgs& a, const PagedView& c, int64_t D, int waves, hipStream_t st) {
+  if (D == 32) launch_prompt_d<QT, CT, 32>(a, c, waves, st);
+  else if (D == 64) launch_prompt_d<QT, CT, 64>(a, c, waves, st);
+  else if (D == 128) launch_prompt_d<QT, CT, 128>(a, c, waves, st);
+  else launch_prompt_d<QT, CT, 256>(a, c, waves, st);
+}
+
+template <int QT>
+void launch_join(const WindowArgs& a, int64_t D, int64_t rows, hipStream_t st) {
+  auto go = [&](auto one, auto four) {
+    if (a.splits <= 16)
+      hipLaunchKernelGGL(one, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows);
+    else
+      hipLaunchKernelGGL(four, dim3((unsigned)rows), dim3(256), 0, st, a, rows);
+  };
+  if (D == 32) go(window_join_kernel<QT, 32, 1>, window_join_kernel<QT, 32, 4>);
+  else if (D == 64) go(window_join_kernel<QT, 64, 1>, window_join_kernel<QT, 64, 4>);
+  else if (D == 128) go(window_join_kernel<QT, 128, 1>, window_join_kernel<QT, 128, 4>);
+  else go(window_join_kernel<QT, 256, 1>, window_join_kernel<QT, 256, 4>);
+}
+
+constexpr int64_t kMaxSplits = 256;
+
+struct Layout {
+  int waves;
+  int64_t tiles, splits;
+  size_t ml, total;                                     // byte offsets: parts first
+};
+
+inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cache* c,
+                            int64_t window, int64_t sinks, int64_t max_seq_len) {
+  const int64_t cap = c->max_pages * c->page_size, group = H / c->heads;
+  const int64_t longest = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
+  const int64_t groups = B * c->heads;
+  Layout l;
+  l.waves = S * group > 128 && groups * ((S * group + 255) / 256) >= 256 ? 8 : 4;
+  const int64_t rows = 32 * l.waves;
+  l.tiles = (S * group + rows - 1) / rows;
+  // a tile's keys: its tokens', the window's before them, the sinks
+  const int64_t tokens = min(S, rows / group + 2);
+  int64_t keys = longest;
+  if (window > 0 && window + sinks + tokens < keys) keys = window + sinks + tokens;
+  const int64_t blocks = groups * l.tiles;
+  l.splits = blocks >= 256 ? 1 : min((512 + blocks - 1) / blocks, (keys + 511) / 512);
+  l.splits = max((int64_t)1, min(l.splits, kMaxSplits));
+  const int64_t parts = l.splits > 1 ? B * H * S * l.splits : 0;
+  l.ml = (size_t)(parts * c->head_dim * 4);
+  l.total = l.ml + (size_t)(parts * 8);
+  return l;
+}
+
+}  // namespace
+}  // namespace rp
+
+using namespace rp;
+
+extern "C" size_t rp_paged_window_workspace_bytes(int64_t B, int64_t H, int64_t S,
+                                                  const rp_paged_cache* cache, int64_t window,
+                                                  int64_t sinks, int64_t max_seq_len) {
+  // sizes that the call refuses need none
+  if (!cache || B <= 0 || B > 65535 || H <= 0 || H > 65535 || S <= 0 || cache->heads <= 0 ||
+      cache->heads > H || cache->page_size <= 0 || cache->max_pages <= 0 ||
+      cache->max_pages > (1 << 30) / cache->page_size || cache->head_dim <= 0 ||
+      cache->head_dim > 256 || max_seq_len < 0 || window < 0 || sinks < 0 ||
+      S > 0x7fffffff / (H / cache->heads) || B * cache->heads > 0x7fffffff / S)
+    return 0;
+  return window_layout(B, H, S, cache, window, sinks, max_seq_len).total;
+}
+
+extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64_t H, int64_t S,
+                                    int64_t qsb, int64_t qsh, int64_t qss,
+                                    const rp_paged_cache* cache, const int32_t* seq_lens,
+                                    const int32_t* q_lens, int64_t window, int64_t sinks,
+                                    float sm_scale, void* out, int64_t osb, int64_t osh,
+                                    int64_t oss, float* lse, int64_t max_seq_len, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (!q || !out || !seq_lens) {
+    rp_set_error("paged_attn_window: null pointer");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  PagedView c;
+  const int rc = paged_view("paged_attn_window", cache, &c);
+  if (rc != RP_OK) return rc;
+  if (q_dtype != RP_DTYPE_BF16 && q_dtype != RP_DTYPE_F16) {
+    rp_set_error("paged_attn_window: unknown q dtype %d", q_dtype);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  const bool fp8 = cache->dtype == RP_CACHE_E4M3;
+  if (!fp8 && (cache->dtype == RP_CACHE_F16) != (q_dtype == RP_DTYPE_F16)) {
+    rp_set_error("paged_attn_window: a 16-bit cache has q's dtype");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  if (B <= 0 || S <= 0 || H <= 0 || H % cache->heads != 0 || max_seq_len < 0 || window < 0 ||
+      sinks < 0) {
+    rp_set_error("paged_attn_window: needs B, S > 0, H a multiple of the cache's %lld heads and "
+                 "window, sinks, max_seq_len >= 0 (B=%lld S=%lld H=%lld)", (long long)cache->heads,
+                 (long long)B, (long long)S, (long long)H);
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  const float c2 = sm_scale * kLog2e;              // scores in powers of two
+  if (!(c2 - c2 == 0.0f)) {
+    rp_set_error("paged_attn_window: sm_scale and sm_scale * log2(e) must be finite");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  const int64_t group = H / cache->heads;
+  if (B > 65535 || H > 65535 || S > 0x7fffffff / group - 512 ||
+      B * cache->heads > 0x7fffffff / S) {
+    rp_set_error("paged_attn_window: too many sequences, heads or tokens");
+    return RP_ERR_UNSUPPORTED;
+  }
+  if (((qsb | qsh | qss) & 7) != 0 || ((osb | osh | oss) & 3) != 0 ||
+      (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 7) != 0) {
+    rp_set_error("paged_attn_window: q rows must be 16-byte and out rows 8-byte aligned");
+    return RP_ERR_UNSUPPORTED;
+  }
+  if (!rows_apart(cache->head_dim, {{B, osb}, {H, osh}, {S, oss}})) {
+    rp_set_error("paged_attn_window: out rows overlap");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
+  const Layout l = window_layout(B, H, S, cache, window, sinks, max_seq_len);
+  const int64_t groups = B * cache->heads;
+  if (groups * l.tiles * l.splits * l.waves * kWave > kMaxGridThreads ||
+      (l.splits > 1 && B * H * S * 256 > kMaxGridThreads)) {
+    rp_set_error("paged_attn_window: too many sequences, heads or tokens");
+    return RP_ERR_UNSUPPORTED;
+  }
+  if (l.total > 0 && (!workspace || workspace_bytes < l.total ||
+                      (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) {
+    rp_set_error("paged_attn_window: workspace of %zu bytes, 256-byte aligned, needed", l.total);
+    return RP_ERR_WORKSPACE;
+  }
+  char* ws = static_cast<char*>(workspace);
+  WindowArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.qsb = qsb;
+  a.qsh = qsh;
+  a.qss = qss;
+  a.lens = seq_lens;
+  a.qlens = q_lens;
+  a.c = c2 < 0.0f ? -c2 : c2;
+  a.flip = c2 < 0.0f ? 0x80008000u : 0u;
+  // bf16 weights: of at most as many keys as the table has places, 1 in all;
+  // fp16 ones: up to 2^15
+  a.lift = cache->dtype == RP_CACHE_F16
+      ? kSlack - 15.0f
+      : kSlack + (float)(64 - __builtin_clzll((unsigned long long)c.capacity()));
+  a.window = window == 0 || window > 0x7fffffff ? 0x7fffffff : (int32_t)window;
+  a.sinks = (int32_t)min(sinks, (int64_t)0x7fffffff);
+  a.out = static_cast<uint16_t*>(out);
+  a.osb = osb;
+  a.osh = osh;
+  a.oss = oss;
+  a.lse = lse;
+  a.H = (int32_t)H;
+  a.group = (int32_t)group;
+  a.S = (int32_t)S;
+  a.tiles = (int32_t)l.tiles;
+  a.splits = (int32_t)l.splits;
+  a.groups = groups;
+  a.part = reinterpret_cast<float*>(ws);
+  a.ml = reinterpret_cast<float2*>(ws + l.ml);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t D = cache->head_dim;
+  if (q_dtype == RP_DTYPE_F16) {
+    if (fp8) launch_prompt<kInF16, RP_CACHE_E4M3>(a, c, D, l.waves, st);
+    else launch_prompt<kInF16, RP_CACHE_F16>(a, c, D, l.waves, st);
+    if (l.splits > 1) launch_join<kInF16>(a, D, B * H * S, st);
+  } else {
+    if (fp8) launch_prompt<kInBf16, RP_CACHE_E4M3>(a, c, D, l.waves, st);
+    else launch_prompt<kInBf16, RP_CACHE_BF16>(a, c, D, l.waves, st);
+    if (l.splits > 1) launch_join<kInBf16>(a, D, B * H * S, st);
+  }
+  return paged_launched("paged_attn_window");
+}

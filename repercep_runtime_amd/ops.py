@@ -1249,6 +1249,74 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     return (out, lse) if return_lse else out
 
 
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    q_lens: torch.Tensor | None = None, *, window: int | None = None,
+                    sinks: int = 0, scale: float | None = None,
+                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                    max_seq_len: int | None = None, return_lse: bool = False,
+                    out: torch.Tensor | None = None
+                    ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of each sequence's last tokens over a paged cache, causal.
+
+    ``q``: (B, H, S, D) bf16 or fp16, the queries of a prompt, of a chunk of
+    one, of drafted tokens, or of one token; their own rows are in the cache
+    already (``paged_kv_append``).  ``seq_lens`` (B,) int32 counts a sequence's
+    rows, the new ones among them, ``q_lens`` (B,) int32 its new tokens (None:
+    S each): token i stands at position p = seq_lens - q_lens + i.  It sees the
+    rows at positions j <= p, with ``window`` only those with p - j < window
+    and the first ``sinks`` ones.  Pages that no token sees any more may be
+    given away and their table entries set to -1.
+
+    Caches, heads, ``scale``, ``max_seq_len``, ``out`` as in
+    ``paged_attention_decode``.  Returns out (B, H, S, D) in q's dtype, or (out,
+    lse) with ``return_lse``, lse (B, H, S) fp32.  A token that sees no row and
+    the rows past q_lens give zeros and -inf."""
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, H, S, D), got {tuple(q.shape)}")
+    B, H, S, D = q.shape
+    if k_cache.dim() != 4 or k_cache.shape[3] != D or k_cache.shape[1] == 0 \
+            or H % k_cache.shape[1] != 0:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {tuple(k_cache.shape)}")
+    dt = _IN_DTYPES.get(q.dtype)
+    if dt is None:
+        raise TypeError(f"q must be bfloat16 or float16 (got {q.dtype})")
+    if k_cache.element_size() == 2 and k_cache.dtype != q.dtype:
+        raise TypeError(f"a {k_cache.dtype} cache is not read with {q.dtype} queries")
+    if (window is not None and window < 1) or sinks < 0:
+        raise ValueError(f"window must be positive or None and sinks not negative (got {window}, "
+                         f"{sinks})")
+    _unit_stride("q", q)
+    _int32_vector("seq_lens", seq_lens, B)
+    if q_lens is not None:
+        _int32_vector("q_lens", q_lens, B)
+    if out is not None:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
+        _unit_stride("out", out)
+    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    dev = k_cache.get_device()
+    if q.get_device() != dev or seq_lens.get_device() != dev or \
+            (q_lens is not None and q_lens.get_device() != dev) or \
+            (out is not None and out.get_device() != dev):
+        _on_device_of(k_cache, q=q, seq_lens=seq_lens, q_lens=q_lens, out=out)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, H, S), dtype=torch.float32) if return_lse else None
+    if B > 0 and S > 0 and H > 0:
+        hint = max_seq_len if max_seq_len is not None else 0
+        n = C.lib().rp_paged_window_workspace_bytes(B, H, S, cache, window or 0, sinks, hint)
+        ws = q.new_empty(n, dtype=torch.uint8) if n else None
+        rc = _on_device(
+            dev, C.lib().rp_paged_attn_window, q.data_ptr(), dt, B, H, S, *_strides(q, 3), cache,
+            seq_lens.data_ptr(), q_lens.data_ptr() if q_lens is not None else None, window or 0,
+            sinks, 1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(),
+            *_strides(out, 3), lse.data_ptr() if return_lse else None, hint,
+            ws.data_ptr() if n else None, n, _stream(q))
+        C.check(rc, "rp_paged_attn_window")
+    return (out, lse) if return_lse else out
+
+
 def paged_kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, key_weights: torch.Tensor, *, budget: int,
                    recent: int, k_scale: torch.Tensor | None = None,
