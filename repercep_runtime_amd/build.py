@@ -41,7 +41,8 @@ COMMON = [
 ]
 SOURCES = ["rp_api.hip", "rp_quant.hip", "rp_prologue.hip", "rp_attn.hip", "rp_gemm.hip",
            "rp_rowwise.hip", "rp_paged.hip", "rp_paged_attn.hip", "rp_logprob.hip", "rp_rope.hip",
-           "rp_verify.hip", "rp_paged_prompt.hip"]
+           "rp_verify.hip", "rp_paged_window.hip",
+           *(f"rp_paged_window_{t}.hip" for t in ("bf16", "f16", "bf16_e4m3", "f16_e4m3"))]
 # Per-source flags.  The attention kernel schedules better under the
 # memory-clause strategy: C3 self 54.60-54.77 ms against 55.31-55.49 ms, C2
 # 24.23-24.25 against 24.50-24.54 ms, alternating on one box.  The same flag

@@ -52,7 +52,6 @@ namespace {
 
 constexpr int kDWaves = 4;
 constexpr int kDThreads = kDWaves * kWave;
-constexpr int kStep = 32;                       // keys per step of a wave
 constexpr int kMaxChunk = kDWaves * 1024;       // a wave holds 64 tiles' pages in one register
 constexpr int kJThreads = 256;
 constexpr int kMaxSplits = 1024;
@@ -97,35 +96,25 @@ __device__ __forceinline__ void split_f16(uint32_t w, uint32_t* hi, uint32_t* lo
 // One wave's state over its keys.  PG16: pages hold 16 rows or more, so each
 // half of a step lies in one page.
 template <int QT, int CT, int D, bool PG16, bool STREAM>
-struct Wave {
-  static constexpr bool FP8 = CT == RP_CACHE_E4M3;
+struct Wave : StepRows<QT == kInF16, CT, D, STREAM> {
+  typedef StepRows<QT == kInF16, CT, D, STREAM> Rows;
+  using Rows::FP8, Rows::EB, Rows::NT, Rows::DPL, Rows::VW;
+  using Rows::c, Rows::lane, Rows::m, Rows::g, Rows::head, Rows::kr, Rows::vr, Rows::kscale,
+      Rows::vscale, Rows::v_col, Rows::k_frag;
   static constexpr bool QF16 = QT == kInF16;          // the first product's type; the second's is bf16
   static constexpr bool VF16 = CT == RP_CACHE_F16;
-  static constexpr int EB = FP8 ? 1 : 2;
-  static constexpr int NT = D / 32;                   // first products per 16 keys
-  static constexpr int DPL = D / 16;                  // V columns per lane
-  static constexpr int KL = FP8 ? (D + 63) / 64 : NT; // 16-byte K loads per 16 keys (8 at D = 32, fp8)
-  static constexpr int VB = DPL * EB;                 // V bytes per lane and row
-  static constexpr int VW = VB < 4 ? 1 : VB / 4;
 
-  const PagedView& c;
   const DecodeArgs& a;
-  int lane, m, g, n;
-  int64_t head;                  // kv head
   const int32_t* table;
   int32_t pages;                 // lane i: page of 16-key tile i of this wave's range (PG16)
   int k0;
-  uint32_t koff, voff[4];        // byte offsets of a lane's rows within a tile (PG16)
   u32x4 q[NT];
-  u32x4 kr[2][KL];
-  uint32_t vr[8][VW];
-  f32x4 kscale[2], vscale[2];
   f32x4 acc[DPL];
   float base, sum, lift;
   uint32_t least;                // the least a positive weight's second and third part may be
   float* score_row;
 
-  __device__ __forceinline__ Wave(const DecodeArgs& a_, const PagedView& c_) : c(c_), a(a_) {}
+  __device__ __forceinline__ Wave(const DecodeArgs& a_, const PagedView& c_) : Rows(c_), a(a_) {}
 
   __device__ __forceinline__ void load_q(const uint16_t* src, bool live) {
 #pragma unroll
@@ -160,103 +149,26 @@ struct Wave {
     if constexpr (PG16) pages = paged_page(c, table, (int64_t)from + 16 * lane);
   }
 
-  __device__ __forceinline__ int key(int k, int e) const {
-    return k + 4 * g + (e < 4 ? e : 12 + e);
-  }
-
   __device__ __forceinline__ int32_t tile_page(int k, int half) const {
     return __builtin_amdgcn_readlane(pages, ((k - k0) >> 4) + half);
   }
 
-  __device__ __forceinline__ void k_row(const char* p, int half) {
-    if constexpr (FP8 && D == 32) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p + 8 * g);
-      kr[half][0] = u32x4{x[0], x[1], 0u, 0u};
-    } else {
-#pragma unroll
-      for (int t = 0; t < KL; ++t)
-        kr[half][t] = *reinterpret_cast<const u32x4*>(p + 64 * t + 16 * g);
-    }
-  }
-
-  template <typename T>
-  __device__ __forceinline__ static T v_load(const char* p) {
-    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
-    else return *reinterpret_cast<const T*>(p);
-  }
-
-  __device__ __forceinline__ void v_row(const char* p, int e) {
-    if constexpr (VB == 2) {
-      vr[e][0] = v_load<uint16_t>(p);
-    } else if constexpr (VB == 4) {
-      vr[e][0] = v_load<uint32_t>(p);
-    } else if constexpr (VB == 8) {
-      const u32x2 x = v_load<u32x2>(p);
-      vr[e][0] = x[0];
-      vr[e][1] = x[1];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VB / 16; ++i) {
-        const u32x4 x = v_load<u32x4>(p + 256 * i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vr[e][4 * i + j] = x[j];
-      }
-    }
-  }
-
-  // Bytes of a lane's first column, and the column of its value j.
-  __device__ __forceinline__ int v_col() const { return m * (VB > 16 ? 16 : VB); }
-  __device__ __forceinline__ static int column(int mm, int j) {
-    if constexpr (VB > 16) return (j < 8 ? 0 : 128) + 8 * mm + j % 8;
-    else return mm * DPL + j;
-  }
-
   __device__ __forceinline__ void load_k(int k) {
     if constexpr (PG16) {
+      // a page that is none is read as page 0 and masked
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        // a page that is none is read as page 0 and masked
-        const int32_t p = max(tile_page(k, half), 0);
-        const char* tile = c.k + paged_row(c, p, head, k + 16 * half) * EB;
-        k_row(tile + koff, half);
-        if constexpr (FP8)
-          kscale[half] = *reinterpret_cast<const f32x4*>(c.ks + paged_scale(c, p, head, k + 16 * half) + 4 * g);
-      }
+      for (int half = 0; half < 2; ++half) this->load_k16(half, max(tile_page(k, half), 0), k + 16 * half);
     } else {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int j = k + 16 * half + m;
-        const int32_t p = max(paged_page(c, table, j), 0);
-        k_row(c.k + paged_row(c, p, head, j) * EB, half);
-      }
-      if constexpr (FP8) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int32_t p = max(paged_page(c, table, key(k, e)), 0);
-          kscale[e / 4][e % 4] = c.ks[paged_scale(c, p, head, key(k, e))];
-        }
-      }
+      this->load_k_any([&](int j) { return max(paged_page(c, table, j), 0); }, k);
     }
   }
 
   __device__ __forceinline__ void load_v(int k) {
     if constexpr (PG16) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int32_t p = max(tile_page(k, half), 0);
-        const char* tile = c.v + paged_row(c, p, head, k + 16 * half) * EB;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v_row(tile + voff[r], 4 * half + r);
-        if constexpr (FP8)
-          vscale[half] = *reinterpret_cast<const f32x4*>(c.vs + paged_scale(c, p, head, k + 16 * half) + 4 * g);
-      }
+      for (int half = 0; half < 2; ++half) this->load_v16(half, max(tile_page(k, half), 0), k + 16 * half);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int32_t p = max(paged_page(c, table, key(k, e)), 0);
-        v_row(c.v + paged_row(c, p, head, key(k, e)) * EB + v_col(), e);
-        if constexpr (FP8) vscale[e / 4][e % 4] = c.vs[paged_scale(c, p, head, key(k, e))];
-      }
+      this->load_v_any([&](int j) { return max(paged_page(c, table, j), 0); }, k);
     }
   }
 
@@ -265,22 +177,10 @@ struct Wave {
     uint32_t mask = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool in = PG16 ? tile_page(k, e / 4) >= 0 : paged_page(c, table, key(k, e)) >= 0;
-      if (in && key(k, e) < end) mask |= 1u << e;
+      const bool in = PG16 ? tile_page(k, e / 4) >= 0 : paged_page(c, table, this->key(k, e)) >= 0;
+      if (in && this->key(k, e) < end) mask |= 1u << e;
     }
     return mask;
-  }
-
-  // Operand words of K's fragment t of a half step.
-  __device__ __forceinline__ u32x4 k_frag(int half, int t) const {
-    if constexpr (!FP8) {
-      return kr[half][t];
-    } else {
-      const u32x4& x = kr[half][t / 2];
-      const uint32_t w0 = t % 2 ? x[2] : x[0], w1 = t % 2 ? x[3] : x[1];
-      return u32x4{codes_to_16<QF16, false>(w0), codes_to_16<QF16, true>(w0),
-                   codes_to_16<QF16, false>(w1), codes_to_16<QF16, true>(w1)};
-    }
   }
 
   // A pair of columns of eight rows, times the weights, into two sums.
@@ -404,18 +304,12 @@ __global__ __launch_bounds__(kDThreads) void attend_kernel(DecodeArgs a, PagedVi
   // not ask it; the first part always answers
   if (split > 0 && (int64_t)split * a.chunk >= n) return;
   W w(a, c);
-  w.lane = threadIdx.x & (kWave - 1);
-  w.m = w.lane & 15;
-  w.g = w.lane >> 4;
-  w.head = kv;
+  w.place(threadIdx.x & (kWave - 1), kv);
   w.table = c.table + b * c.table_stride;
   const int first = tile * 16;                         // of the group's query heads
   const bool live = first + w.m < a.group;
   const int h = kv * a.group + first + w.m;
   w.load_q(a.q + b * a.qsb + (int64_t)h * a.qsh, live);
-  w.koff = (uint32_t)(w.m * c.sr * W::EB);
-#pragma unroll
-  for (int r = 0; r < 4; ++r) w.voff[r] = (uint32_t)((4 * w.g + r) * c.sr * W::EB) + w.v_col();
   w.score_row = a.scores && live ? a.scores + ((int64_t)b * a.H + h) * a.score_ld : nullptr;
 
   for (float lift = 0.0f;; lift = a.lift) {

@@ -1,12 +1,11 @@
 // The paged key-value cache as the kernels see it, its row lookup and the
-// host checks that its entry points share.  Everything here has internal
-// linkage.
+// host checks that its entry points share.  But for PagedView itself,
+// everything here has internal linkage.
 #pragma once
 
 #include "rp_common.h"
 
 namespace rp {
-namespace {
 
 struct PagedView {
   char* k;
@@ -20,6 +19,8 @@ struct PagedView {
 
   __host__ __device__ int64_t capacity() const { return (int64_t)max_pages << shift; }
 };
+
+namespace {
 
 // The page that holds position `pos` of the sequence whose table entries
 // begin at `row`; -1 where there is none: the position is past the table, or

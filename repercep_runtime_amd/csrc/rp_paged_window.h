@@ -1,6 +1,5 @@
 // Attention of each sequence's last tokens over a paged cache, as its kernels
-// share it: the arguments, which keys a run of tokens sees, and the join of
-// parts.  Everything here has internal linkage.
+// share it: the arguments, and which keys a run of tokens sees.
 //
 // The rows of a kv head are its query heads' tokens, token by token: row r is
 // token r / group, head r % group, so one tile of rows reads a key once for all
@@ -12,7 +11,6 @@
 #include "rp_paged_mma.h"
 
 namespace rp {
-namespace {
 
 struct WindowArgs {
   const uint16_t* q;
@@ -32,6 +30,23 @@ struct WindowArgs {
   float* part;                   // (B, H, S, splits, D): the parts' weighted means
   float2* ml;                    // (B, H, S, splits): base (in powers of two), sum of weights
 };
+
+// How a call is launched.
+struct WindowLaunch {
+  int columns;                   // of 16 rows, few_kernel; 0: prompt_kernel
+  int waves;                     // of prompt_kernel
+  bool stream;                   // few_kernel: V past the caches
+};
+
+// The kernels for one type of q and of the cache, each in a source file of its
+// own (they compile side by side).
+template <int QT, int CT>
+void launch_window(const WindowArgs& a, const PagedView& c, int64_t D, const WindowLaunch& l,
+                   hipStream_t st);
+
+namespace {
+
+constexpr float kSlack = 8.0f;                  // powers of two, see rp_paged_prompt.h
 
 // A sequence's place: its length, its new tokens, the first one's position.
 struct Place {
@@ -83,57 +98,22 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
   return w;
 }
 
+template <bool F16>
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (F16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  }
+}
+
 template <int QT>
 __device__ __forceinline__ uint32_t pack_out(float a, float b) {
   if constexpr (QT == kInF16) return pack_f16x2(a, b);
   else return f32_to_bf16_bits(a) | f32_to_bf16_bits(b) << 16;
-}
-
-// Joins the parts of 256 / (64 W) rows, W waves a row: each part's mean counts
-// by its sum about the largest base.  Half a wave or more takes a part's columns.
-template <int QT, int D, int W>
-__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, int64_t rows) {
-  constexpr int COLS = D / 4, GR = W * kWave / COLS;     // lanes a part, parts at a time
-  __shared__ f32x4 sums[256];
-  const int64_t row = (int64_t)blockIdx.x * (4 / W) + threadIdx.x / (W * kWave);
-  const int tid = threadIdx.x % (W * kWave), lane = threadIdx.x & (kWave - 1);
-  const int col = tid % COLS, gr = tid / COLS;
-  const bool in = row < rows;
-  const int64_t bh = in ? row / a.S : 0;
-  const int i = in ? (int)(row % a.S) : 0;
-  const float2* ml = a.ml + (in ? row : 0) * a.splits;
-  float base = neg_inf(), sum = 0.0f;
-  for (int s = lane; s < a.splits; s += kWave)
-    if (ml[s].y != 0.0f) base = fmaxf(base, ml[s].x);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) base = fmaxf(base, __shfl_xor(base, o, kWave));
-  const float b0 = base == neg_inf() ? 0.0f : base;
-  for (int s = lane; s < a.splits; s += kWave)
-    if (ml[s].y != 0.0f) sum += ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - b0);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const f32x4* part = reinterpret_cast<const f32x4*>(a.part + (in ? row : 0) * a.splits * D) + col;
-  f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int s = gr; s < a.splits; s += GR) {
-    const float2 p = ml[s];
-    const f32x4 y = part[(int64_t)s * COLS];
-    const float f = p.y * __builtin_amdgcn_exp2f(p.x - b0) * inv;
-    // a part without keys wrote nothing
-    if (p.y != 0.0f) x += y * f;
-  }
-  sums[threadIdx.x] = x;
-  __syncthreads();
-  if (gr != 0 || !in) return;
-#pragma unroll
-  for (int g = 1; g < GR; ++g) x += sums[threadIdx.x + g * COLS];
-  const int64_t b = bh / a.H, h = bh % a.H;
-  uint16_t* out = a.out + b * a.osb + h * a.osh + (int64_t)i * a.oss + 4 * col;
-  if (sum == 0.0f) x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  *reinterpret_cast<u32x2*>(out) = u32x2{pack_out<QT>(x[0], x[1]), pack_out<QT>(x[2], x[3])};
-  if (col == 0 && a.lse)
-    a.lse[row] = sum == 0.0f ? neg_inf() : (b0 + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 }  // namespace
