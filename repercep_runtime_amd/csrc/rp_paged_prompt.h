@@ -25,6 +25,8 @@
 
 #pragma once
 
+#include <type_traits>
+
 #include "rp_paged_window.h"
 
 namespace rp {
@@ -40,6 +42,11 @@ __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Bits 0 .. n of a word: none below 0, all from 31.
+__device__ __forceinline__ uint32_t bits_up_to(int32_t n) {
+  return n < 0 ? 0u : 0xffffffffu >> (31 - min(n, 31));
 }
 
 // Four keys of a column: the 16 lanes of a row of lanes bring four rows of 16
@@ -64,7 +71,7 @@ struct Prompt {
   static constexpr int NCH = (kTile * CPR + NT - 1) / NT;
   static constexpr int ROWS = NW * 32;
 
-  struct Shared {
+  struct alignas(16) Shared {
     uint16_t k[2][kTile][LD];
     uint16_t v[2][kTile][LD];
     float ks[2][kTile], vs[2][kTile];                   // e4m3fn only
@@ -189,7 +196,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
 
   // ---- one tile of keys for the wave's rows
-  auto attend = [&](int buf, int32_t kb, uint64_t here, bool careful) {
+  auto attend = [&](auto careful, int buf, int32_t kb, uint64_t here) {
     // no row of the wave sees a key of the tile
     if (kb > pmax || (kb + kTile - 1 <= max(0, pmin) - a.window && kb >= a.sinks)) return;
     const bool whole = here == ~0ull && kb + kTile - 1 <= pmin &&
@@ -204,36 +211,33 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
         const u32x4 f = *reinterpret_cast<const u32x4*>(&sh.k[buf][32 * k + m][16 * t + 8 * h]);
         s[k] = mma32<P::QF16>(f, q[t], s[k]);
       }
-    float x[2][16];
+    if constexpr (P::FP8) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 f = {a.c, a.c, a.c, a.c};
-        if constexpr (P::FP8) f = *reinterpret_cast<const f32x4*>(&sh.ks[buf][32 * k + 8 * i + 4 * h]);
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 f = *reinterpret_cast<const f32x4*>(&sh.ks[buf][32 * k + 8 * i + 4 * h]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[k][4 * i + e] = s[k][4 * i + e] * f[e];
-      }
+          for (int e = 0; e < 4; ++e) s[k][4 * i + e] *= f[e];
+        }
+    }
+    const float c1 = P::FP8 ? 1.0f : a.c;                // what makes them powers of two
     uint32_t seen[2] = {0xffffffffu, 0xffffffffu};       // bit 8 i + e: key 8 i + 4 h + e
     if (!whole) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const uint32_t pk = (uint32_t)(here >> 32 * k) >> 4 * h;
-        seen[k] = 0;
+        const int32_t j = kb + 32 * k + 4 * h;
+        seen[k] = (uint32_t)(here >> 32 * k) >> 4 * h & bits_up_to(pos - j) &
+                  (~bits_up_to(pos - a.window - j) | bits_up_to(a.sinks - 1 - j));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int32_t j = kb + 32 * k + 8 * i + 4 * h + e;
-            const bool in = (pk >> (8 * i + e) & 1) && sees(a, pos, j);
-            seen[k] |= in ? 1u << (8 * i + e) : 0u;
-            x[k][4 * i + e] = in ? x[k][4 * i + e] : neg_inf();
-          }
+        for (int i = 0; i < 16; ++i)
+          s[k][i] = seen[k] & 1u << (8 * (i / 4) + i % 4) ? s[k][i] : neg_inf();
       }
     }
-    float top = fmaxf(x[0][0], x[1][0]);
+    float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(x[0][i], x[1][i]));
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+    top *= c1;
     if (__any(top > base + (kSlack - a.lift))) {
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
       const float next = fmaxf(base, top + a.lift);
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
         if constexpr (P::FP8) f = *reinterpret_cast<const f32x4*>(&sh.vs[buf][32 * k + 8 * i + 4 * h]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(x[k][4 * i + e] - b0);
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][4 * i + e], c1, -b0));
           part_sum[k] += w[e];
           if constexpr (P::FP8) {
             w[e] *= f[e];
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       const u32x2 lo = column4(at), hi = column4(at + 8 * P::LD);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
-    if (!careful) {
+    if constexpr (!decltype(careful)::value) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -331,47 +335,47 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     }
   };
 
-  for (int careful = 0; careful < 2; ++careful) {
+  auto run = [&](auto careful) {
     base = neg_inf();
     sum = 0.0f;
 #pragma unroll
     for (int d = 0; d < P::DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
-    if (t0 < t1) {
-      load(t0, page_of(t0));
-      int32_t pages = page_of(t0 + 1);
-      store(0);
-      uint64_t here = present;
-      __syncthreads();
-      for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        const bool more = t + 1 < t1;
-        if (more) {
-          load(t + 1, pages);
-          pages = page_of(t + 2);
-        }
-        attend(buf, keys.key(t), here, careful != 0);
-        if (more) {
-          store(buf ^ 1);
-          here = present;
-        }
-        __syncthreads();
+    if (t0 >= t1) return;
+    load(t0, page_of(t0));
+    int32_t pages = page_of(t0 + 1);
+    store(0);
+    uint64_t here = present;
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      const bool more = t + 1 < t1;
+      if (more) {
+        load(t + 1, pages);
+        pages = page_of(t + 2);
       }
+      attend(careful, buf, keys.key(t), here);
+      if (more) {
+        store(buf ^ 1);
+        here = present;
+      }
+      __syncthreads();
     }
-    if (careful) break;
+  };
+  if (tid == 0) sh.redo = 0;
+  run(std::false_type{});
+  {
     f32x16 z = acc[0] * 0.0f;
 #pragma unroll
     for (int d = 1; d < P::DB; ++d) z += acc[d] * 0.0f;
     float y = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) y += z[i];
-    if (tid == 0) sh.redo = 0;
     __syncthreads();
     if (live && y != y) sh.redo = 1;
     __syncthreads();
-    if (!sh.redo) break;
-    __syncthreads();
+    if (sh.redo) run(std::true_type{});
   }
 
   if (row >= all) return;

@@ -202,7 +202,9 @@ extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64
   a.qss = qss;
   a.lens = seq_lens;
   a.qlens = q_lens;
-  a.c = c2 < 0.0f ? -c2 : c2;
+  // not 0, beside which a masked score of -inf would be NaN: 2^-149 of a score
+  // is less than 2^-21
+  a.c = c2 == 0.0f ? 0x1p-149f : c2 < 0.0f ? -c2 : c2;
   a.flip = c2 < 0.0f ? 0x80008000u : 0u;
   // bf16 weights: of at most as many keys as the table has places, 1 in all;
   // fp16 ones: up to 2^15
