@@ -66,14 +66,16 @@ struct Prompt {
   static constexpr int PARTS = FP8 && QF16 ? 2 : 1;     // of a weight
   static constexpr int EB = FP8 ? 1 : 2, NT = NW * kWave;
   static constexpr int QSTEPS = D / 16, DB = D / 32;
-  static constexpr int LD = D + 8;                      // a row of LDS: 16 bytes more
+  // Rows of LDS, without bank conflicts: eight rows of K at one column are read
+  // at a time, four rows of V's 64 bytes.
+  static constexpr int LDK = D + 8, LDV = D == 32 ? 32 : D + 32;
   static constexpr int CPR = D * EB / 16;               // 16-byte chunks a row
   static constexpr int NCH = (kTile * CPR + NT - 1) / NT;
   static constexpr int ROWS = NW * 32;
 
   struct alignas(16) Shared {
-    uint16_t k[2][kTile][LD];
-    uint16_t v[2][kTile][LD];
+    uint16_t k[2][kTile][LDK];
+    uint16_t v[2][kTile][LDV];
     float ks[2][kTile], vs[2][kTile];                   // e4m3fn only
     int redo;
   };
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     const int l16 = lane & 15, cb = (lane >> 4 & 1) * 16 + (l16 & 3) * 4;
     auto v_frag = [&](int d, int k, int u) -> u32x4 {
       const uint16_t* at = &sh.v[buf][32 * k + 16 * u + 4 * h + (l16 >> 2)][32 * d + cb];
-      const u32x2 lo = column4(at), hi = column4(at + 8 * P::LD);
+      const u32x2 lo = column4(at), hi = column4(at + 8 * P::LDV);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
     if constexpr (!decltype(careful)::value) {
