@@ -18,6 +18,7 @@ struct PagedView {
   int32_t num_pages, heads, max_pages, shift;   // page_size = 1 << shift
 
   __host__ __device__ int64_t capacity() const { return (int64_t)max_pages << shift; }
+  __host__ __device__ int32_t page_mask() const { return (1 << shift) - 1; }
 };
 
 namespace {

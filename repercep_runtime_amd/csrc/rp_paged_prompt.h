@@ -29,6 +29,8 @@
 
 #include "rp_paged_window.h"
 
+#define RP_INLINE __attribute__((always_inline))
+
 namespace rp {
 namespace {
 
@@ -71,12 +73,17 @@ struct Prompt {
   static constexpr int LDK = D + 8, LDV = D == 32 ? 32 : D + 32;
   static constexpr int CPR = D * EB / 16;               // 16-byte chunks a row
   static constexpr int NCH = (kTile * CPR + NT - 1) / NT;
+  static constexpr int WROWS = kWave / CPR;             // rows of a wave's chunks
   static constexpr int ROWS = NW * 32;
+
+  // 256 registers a lane, two waves a SIMD, do not hold a wave's rows of Q too.
+  static constexpr bool QLDS = D == 128 && NW == 8;
 
   struct alignas(16) Shared {
     uint16_t k[2][kTile][LDK];
     uint16_t v[2][kTile][LDV];
     float ks[2][kTile], vs[2][kTile];                   // e4m3fn only
+    uint16_t q[QLDS ? ROWS : 1][LDK];
     int redo;
   };
 };
@@ -120,99 +127,136 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
   const int32_t* table = c.table + b * c.table_stride;
 
-  u32x4 q[P::QSTEPS];
+  u32x4 q[P::QLDS ? 1 : P::QSTEPS];
   {
     const uint16_t* src = a.q + b * a.qsb + (int64_t)head * a.qsh + (int64_t)token * a.qss + 8 * h;
 #pragma unroll
     for (int t = 0; t < P::QSTEPS; ++t) {
-      q[t] = live ? *reinterpret_cast<const u32x4*>(src + 16 * t) : u32x4{0u, 0u, 0u, 0u};
-      q[t] ^= a.flip;
+      u32x4 x = live ? *reinterpret_cast<const u32x4*>(src + 16 * t) : u32x4{0u, 0u, 0u, 0u};
+      x ^= a.flip;
+      if constexpr (P::QLDS) *reinterpret_cast<u32x4*>(&sh.q[32 * wave + m][16 * t + 8 * h]) = x;
+      else q[t] = x;
     }
   }
+  auto q_frag = [&](int t) RP_INLINE -> u32x4 {
+    if constexpr (P::QLDS) return *reinterpret_cast<const u32x4*>(&sh.q[32 * wave + m][16 * t + 8 * h]);
+    else return q[t];
+  };
 
   f32x16 acc[P::DB];
   float base, sum;
 
-  // ---- staging
+  // ---- staging: lane l's page entry says where key l of a tile lies; a thread
+  // brings chunks of 16 bytes, a row's by threads next to each other
   u32x4 kreg[P::NCH], vreg[P::NCH];
-  float sreg = 0.0f;
-  uint64_t present;                                      // of the tile in the registers
-  auto page_of = [&](int t) -> int32_t {                 // lane l: the page of key l of tile t
-    const int32_t j = keys.key(t) + lane;
-    return t < t1 && keys.any(j) ? paged_page(c, table, j) : -1;
+  float ksreg = 0.0f, vsreg = 0.0f;
+  // (the entry as it stands in the table: checking it here would wait for it)
+  auto entry = [&](int t) RP_INLINE -> int32_t {
+    return table[min((keys.key(t) + lane) >> c.shift, c.max_pages - 1)];
   };
-  auto load = [&](int t, int32_t pages) {
-    const int32_t kb = keys.key(t);
-    present = __ballot(pages >= 0);
+  // the page, or -1 where there is none
+  auto page_of = [&](int t, int32_t e) RP_INLINE -> int32_t {
+    return t < t1 && keys.key(t) + lane < keys.hi && e >= 0 && e < c.num_pages ? e : -1;
+  };
+  // which keys of tile t any of the workgroup's rows sees
+  auto present = [&](int t, int32_t pages) RP_INLINE -> uint64_t {
+    return __ballot(pages >= 0 && keys.any(keys.key(t) + lane));
+  };
+  // a wave's rows of a chunk lie in one page, unless pages are smaller
+  const bool one_page = c.page_mask() >= P::WROWS - 1;
+  const uint32_t lane_off = (uint32_t)((lane / P::CPR) * c.sr * P::EB + lane % P::CPR * 16);
+  // What is no row is read as a row of page 0; what no row sees is put into LDS
+  // as zeros.
+  auto load = [&](auto one, u32x4* to, const char* from, int32_t kb, int32_t pages) RP_INLINE {
 #pragma unroll
     for (int i = 0; i < P::NCH; ++i) {
-      const int ch = min(tid + i * P::NT, kTile * P::CPR - 1);
-      const int r = ch / P::CPR, col = ch % P::CPR * 16;
-      // what is no row is read as a row of page 0 and put into LDS as zeros
-      const int32_t page = max(0, __shfl(pages, r, kWave));
-      const int64_t off = paged_row(c, page, kv, kb + r) * P::EB + col;
-      kreg[i] = *reinterpret_cast<const u32x4*>(c.k + off);
-      vreg[i] = *reinterpret_cast<const u32x4*>(c.v + off);
-    }
-    if constexpr (P::FP8) {
-      if (wave < 2)
-        sreg = (wave == 0 ? c.ks : c.vs)[paged_scale(c, max(0, pages), kv, kb + lane)];
+      const int rw = min(wave * P::WROWS + i * (P::NT / P::CPR), kTile - P::WROWS);
+      if constexpr (decltype(one)::value) {
+        const int32_t page = __builtin_amdgcn_readlane(pages, rw);
+        to[i] = *reinterpret_cast<const u32x4*>(from + paged_row(c, page, kv, kb + rw) * P::EB + lane_off);
+      } else {
+        const int r = rw + lane / P::CPR;
+        const int32_t page = __shfl(pages, r, kWave);
+        to[i] = *reinterpret_cast<const u32x4*>(from + paged_row(c, page, kv, kb + r) * P::EB + lane % P::CPR * 16);
+      }
     }
   };
-  auto store = [&](int buf) {
+  // K's rows of tile tk and V's of tile tv
+  auto load_rows = [&](int tk, int32_t kpages, int tv, int32_t vpages) RP_INLINE {
+    const int32_t kb = keys.key(tk), vb = keys.key(tv);
+    kpages = max(0, kpages);
+    vpages = max(0, vpages);
+    if (one_page) {
+      load(std::true_type{}, kreg, c.k, kb, kpages);
+      load(std::true_type{}, vreg, c.v, vb, vpages);
+    } else {
+      load(std::false_type{}, kreg, c.k, kb, kpages);
+      load(std::false_type{}, vreg, c.v, vb, vpages);
+    }
+    if constexpr (P::FP8) {
+      if (wave == 0) ksreg = c.ks[paged_scale(c, kpages, kv, kb + lane)];
+      if (wave == 1) vsreg = c.vs[paged_scale(c, vpages, kv, vb + lane)];
+    }
+    __builtin_amdgcn_sched_barrier(0);                   // on their way before the products
+  };
+  auto store = [&](uint16_t* to, int ld, u32x4* from, uint64_t here, auto f16) RP_INLINE {
 #pragma unroll
     for (int i = 0; i < P::NCH; ++i) {
       const int ch = tid + i * P::NT;
       if (kTile * P::CPR % P::NT != 0 && ch >= kTile * P::CPR) break;
       const int r = ch / P::CPR;
-      const uint32_t keep = (present >> r & 1) ? 0xffffffffu : 0u;
-      u32x4 kk = kreg[i] & keep, vv = vreg[i] & keep;
+      u32x4 x = from[i];
+      if (here != ~0ull) x &= here >> r & 1 ? 0xffffffffu : 0u;
       if constexpr (!P::FP8) {
-        const int col = ch % P::CPR * 8;
-        *reinterpret_cast<u32x4*>(&sh.k[buf][r][col]) = kk;
-        *reinterpret_cast<u32x4*>(&sh.v[buf][r][col]) = vv;
+        *reinterpret_cast<u32x4*>(to + r * ld + ch % P::CPR * 8) = x;
       } else {
-        const int col = ch % P::CPR * 16;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          u32x4 x, y;
+          u32x4 y;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            x[2 * e] = codes_to_16<P::QF16, false>(kk[2 * half + e]);
-            x[2 * e + 1] = codes_to_16<P::QF16, true>(kk[2 * half + e]);
-            y[2 * e] = codes_to_16<false, false>(vv[2 * half + e]);
-            y[2 * e + 1] = codes_to_16<false, true>(vv[2 * half + e]);
+            y[2 * e] = codes_to_16<decltype(f16)::value, false>(x[2 * half + e]);
+            y[2 * e + 1] = codes_to_16<decltype(f16)::value, true>(x[2 * half + e]);
           }
-          *reinterpret_cast<u32x4*>(&sh.k[buf][r][col + 8 * half]) = x;
-          *reinterpret_cast<u32x4*>(&sh.v[buf][r][col + 8 * half]) = y;
+          *reinterpret_cast<u32x4*>(to + r * ld + ch % P::CPR * 16 + 8 * half) = y;
         }
       }
     }
+  };
+  auto store_k = [&](int buf, uint64_t here) RP_INLINE {
+    store(&sh.k[buf][0][0], P::LDK, kreg, here, std::bool_constant<P::QF16>{});
     if constexpr (P::FP8) {
-      if (wave < 2) {
-        const float s = present >> lane & 1 ? sreg : 0.0f;
-        if (wave == 0) sh.ks[buf][lane] = s * a.c;
-        else sh.vs[buf][lane] = s;
-      }
+      if (wave == 0) sh.ks[buf][lane] = here >> lane & 1 ? ksreg * a.c : 0.0f;
+    }
+  };
+  auto store_v = [&](int buf, uint64_t here) RP_INLINE {
+    store(&sh.v[buf][0][0], P::LDV, vreg, here, std::false_type{});
+    if constexpr (P::FP8) {
+      if (wave == 1) sh.vs[buf][lane] = here >> lane & 1 ? vsreg : 0.0f;
     }
   };
 
-  // ---- one tile of keys for the wave's rows
-  auto attend = [&](auto careful, int buf, int32_t kb, uint64_t here) {
-    // no row of the wave sees a key of the tile
-    if (kb > pmax || (kb + kTile - 1 <= max(0, pmin) - a.window && kb >= a.sinks)) return;
-    const bool whole = here == ~0ull && kb + kTile - 1 <= pmin &&
-                       (kb > pmax - a.window || kb + kTile <= a.sinks);
-    f32x16 s[2];
+  // ---- a tile's scores, in powers of two but for the factor c1
+  f32x16 s[2];
+  const float c1 = P::FP8 ? 1.0f : a.c;
+  auto product = [&](int buf, f32x16* to) RP_INLINE {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) to[0][i] = to[1][i] = 0.0f;
 #pragma unroll
-    for (int t = 0; t < P::QSTEPS; ++t)
+    for (int t = 0; t < P::QSTEPS; ++t) {
+      const u32x4 y = q_frag(t);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const u32x4 f = *reinterpret_cast<const u32x4*>(&sh.k[buf][32 * k + m][16 * t + 8 * h]);
-        s[k] = mma32<P::QF16>(f, q[t], s[k]);
+        to[k] = mma32<P::QF16>(f, y, to[k]);
       }
+    }
+  };
+  uint32_t seen[2];                                      // bit 8 i + e: key 8 i + 4 h + e
+  bool whole;
+  float top;
+  // Masks the scores s of the tile at kb and finds their largest.
+  auto weigh = [&](int buf, int32_t kb, uint64_t here) RP_INLINE {
     if constexpr (P::FP8) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -223,8 +267,8 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           for (int e = 0; e < 4; ++e) s[k][4 * i + e] *= f[e];
         }
     }
-    const float c1 = P::FP8 ? 1.0f : a.c;                // what makes them powers of two
-    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};       // bit 8 i + e: key 8 i + 4 h + e
+    whole = here == ~0ull && kb + kTile - 1 <= pmin &&
+            (kb > pmax - a.window || kb + kTile <= a.sinks);
     if (!whole) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -236,10 +280,14 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           s[k][i] = seen[k] & 1u << (8 * (i / 4) + i % 4) ? s[k][i] : neg_inf();
       }
     }
-    float top = fmaxf(s[0][0], s[1][0]);
+    // of a row with a NaN a NaN, which moves no base: the row is NaN
+    top = __builtin_elementwise_maximum(s[0][0], s[1][0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+    for (int i = 1; i < 16; ++i)
+      top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][i]), s[1][i]);
     top *= c1;
+  };
+  auto rebase = [&]() RP_INLINE {
     if (__any(top > base + (kSlack - a.lift))) {
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
       const float next = fmaxf(base, top + a.lift);
@@ -249,8 +297,12 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       for (int d = 0; d < P::DB; ++d) acc[d] *= r;
       base = next;
     }
+  };
+
+  // ---- P from s, and its product with V
+  uint32_t p[P::PARTS][2][8];
+  auto weights = [&](int buf) RP_INLINE {
     const float b0 = base == neg_inf() ? 0.0f : base;    // no score yet: exp2(-inf) is 0
-    uint32_t p[P::PARTS][2][8];
     float part_sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -265,6 +317,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           part_sum[k] += w[e];
           if constexpr (P::FP8) {
             w[e] *= f[e];
+            // what is not seen weighs 0 whatever its scale
             if (!whole) w[e] = seen[k] >> (8 * i + e) & 1 ? w[e] : 0.0f;
           }
         }
@@ -280,30 +333,31 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
         }
       }
     sum += part_sum[0] + part_sum[1];
-
-    // columns 32 d .. + 31 of keys 32 k + 16 u + 4 h + {0..3, 8..11}
-    const int l16 = lane & 15, cb = (lane >> 4 & 1) * 16 + (l16 & 3) * 4;
-    auto v_frag = [&](int d, int k, int u) -> u32x4 {
-      const uint16_t* at = &sh.v[buf][32 * k + 16 * u + 4 * h + (l16 >> 2)][32 * d + cb];
-      const u32x2 lo = column4(at), hi = column4(at + 8 * P::LDV);
-      return u32x4{lo[0], lo[1], hi[0], hi[1]};
-    };
-    if constexpr (!decltype(careful)::value) {
+  };
+  // columns 32 d .. + 31 of keys 32 k + 16 u + 4 h + {0..3, 8..11}
+  const int l16 = lane & 15, cb = (lane >> 4 & 1) * 16 + (l16 & 3) * 4;
+  auto v_frag = [&](int buf, int d, int k, int u) RP_INLINE -> u32x4 {
+    const uint16_t* at = &sh.v[buf][32 * k + 16 * u + 4 * h + (l16 >> 2)][32 * d + cb];
+    const u32x2 lo = column4(at), hi = column4(at + 8 * P::LDV);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto p_frag = [&](int e, int k, int u) RP_INLINE -> u32x4 {
+    return u32x4{p[e][k][4 * u], p[e][k][4 * u + 1], p[e][k][4 * u + 2], p[e][k][4 * u + 3]};
+  };
+  auto values = [&](int buf) RP_INLINE {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int d = 0; d < P::DB; ++d) {
-            const u32x4 f = v_frag(d, k, u);
+        for (int d = 0; d < P::DB; ++d) {
+          const u32x4 f = v_frag(buf, d, k, u);
 #pragma unroll
-            for (int e = 0; e < P::PARTS; ++e)
-              acc[d] = mma32<P::VF16>(f, u32x4{p[e][k][4 * u], p[e][k][4 * u + 1],
-                                               p[e][k][4 * u + 2], p[e][k][4 * u + 3]}, acc[d]);
-          }
-      return;
-    }
-    // one token of the wave at a time, V as that token sees it
+          for (int e = 0; e < P::PARTS; ++e) acc[d] = mma32<P::VF16>(f, p_frag(e, k, u), acc[d]);
+        }
+  };
+  // The same one token of the wave at a time, V as that token sees it.
+  auto values_apart = [&](int buf, int32_t kb) RP_INLINE {
     for (int32_t at = pmin; at <= pmax; ++at) {
       const bool mine = pos == at;
 #pragma unroll
@@ -318,17 +372,15 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           }
 #pragma unroll
           for (int d = 0; d < P::DB; ++d) {
-            u32x4 f = v_frag(d, k, u);
+            u32x4 f = v_frag(buf, d, k, u);
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] &= mask[e];
-            f32x16 y = mma32<P::VF16>(f, u32x4{p[0][k][4 * u], p[0][k][4 * u + 1],
-                                               p[0][k][4 * u + 2], p[0][k][4 * u + 3]}, acc[d]);
+            f32x16 y = mma32<P::VF16>(f, p_frag(0, k, u), acc[d]);
             if constexpr (P::PARTS == 2) {
               // a second part of 0 would make NaN of an infinity
 #pragma unroll
               for (int e = 0; e < 4; ++e) f[e] = finite_pair<P::VF16>(f[e]);
-              y = mma32<P::VF16>(f, u32x4{p[1][k][4 * u], p[1][k][4 * u + 1],
-                                          p[1][k][4 * u + 2], p[1][k][4 * u + 3]}, y);
+              y = mma32<P::VF16>(f, p_frag(1, k, u), y);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[d][i] = mine ? y[i] : acc[d][i];
@@ -337,7 +389,9 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     }
   };
 
-  auto run = [&](auto careful) {
+  // Tile t's weights and product with V, beside tile t + 1's scores: K is a
+  // tile ahead of V.
+  auto run = [&](auto apart) RP_INLINE {
     base = neg_inf();
     sum = 0.0f;
 #pragma unroll
@@ -345,25 +399,54 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
     if (t0 >= t1) return;
-    load(t0, page_of(t0));
-    int32_t pages = page_of(t0 + 1);
-    store(0);
-    uint64_t here = present;
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
+    int32_t pages1 = page_of(t0 + 1, entry(t0 + 1));     // of tile t + 1
+    int32_t entry2 = entry(t0 + 2);                      // of tile t + 2
+    uint64_t here1;                                      // in tile t + 1
+    {
+      const int32_t pages = page_of(t0, entry(t0));
+      const uint64_t here = present(t0, pages);
+      const int next = min(t0 + 1, t1 - 1);
+      load_rows(t0, pages, t0, pages);
+      store_k(0, here);
+      store_v(0, here);
+      here1 = present(t0 + 1, pages1);
+      load_rows(next, pages1, next, pages1);
+      store_k(1, here1);
+      __syncthreads();
+      product(0, s);
+      weigh(0, keys.key(t0), here);
+      rebase();
+      __syncthreads();                                   // K's first tile is overwritten next
+    }
+    auto step = [&](int t, auto more) RP_INLINE {
       const int buf = (t - t0) & 1;
-      const bool more = t + 1 < t1;
-      if (more) {
-        load(t + 1, pages);
-        pages = page_of(t + 2);
+      uint64_t here2 = 0;
+      if constexpr (decltype(more)::value) {
+        const int32_t pages2 = page_of(t + 2, entry2);
+        here2 = present(t + 2, pages2);
+        entry2 = entry(t + 3);
+        load_rows(min(t + 2, t1 - 1), pages2, t + 1, pages1);
+        pages1 = pages2;
       }
-      attend(careful, buf, keys.key(t), here);
-      if (more) {
-        store(buf ^ 1);
-        here = present;
+      f32x16 next[2];
+      if constexpr (decltype(more)::value) product(buf ^ 1, next);
+      weights(buf);
+      if constexpr (decltype(apart)::value) values_apart(buf, keys.key(t));
+      else values(buf);
+      if constexpr (decltype(more)::value) {
+        __builtin_amdgcn_sched_barrier(0);               // they are waited for after the products
+        s[0] = next[0];
+        s[1] = next[1];
+        store_k(buf, here2);
+        store_v(buf ^ 1, here1);
+        weigh(buf ^ 1, keys.key(t + 1), here1);
+        here1 = here2;
+        rebase();
       }
       __syncthreads();
-    }
+    };
+    for (int t = t0; t + 1 < t1; ++t) step(t, std::true_type{});
+    step(t1 - 1, std::false_type{});
   };
   if (tid == 0) sh.redo = 0;
   run(std::false_type{});
