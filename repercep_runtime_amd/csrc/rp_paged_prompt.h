@@ -35,6 +35,7 @@ namespace rp {
 namespace {
 
 constexpr int kTile = 64;                       // keys a tile: one page entry a lane
+constexpr int kAhead = 4;                       // matrix instructions that LDS reads are ahead
 
 template <bool F16>
 __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -51,13 +52,22 @@ __device__ __forceinline__ uint32_t bits_up_to(int32_t n) {
   return n < 0 ? 0u : 0xffffffffu >> (31 - min(n, 31));
 }
 
+// LDS by address, which the compiler takes as it is: one register and a constant
+// offset a read.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+  asm("" : "+v"(at));
+  return at;
+}
+__device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
+}
 // Four keys of a column: the 16 lanes of a row of lanes bring four rows of 16
 // columns, four lanes a row, and each takes a column.
-__device__ __forceinline__ u32x2 column4(const uint16_t* p) {
+__device__ __forceinline__ u32x2 column4(uint32_t at) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (lds_s16x4)(uintptr_t)(uint32_t)(uintptr_t)p));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(uintptr_t)at));
 }
 
 template <int QT, int CT, int D, int NW>
@@ -138,9 +148,15 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       else q[t] = x;
     }
   }
+  const uint32_t qlds = lds_address(&sh.q[P::QLDS ? 32 * wave + m : 0][8 * h]);
   auto q_frag = [&](int t) RP_INLINE -> u32x4 {
-    if constexpr (P::QLDS) return *reinterpret_cast<const u32x4*>(&sh.q[32 * wave + m][16 * t + 8 * h]);
+    if constexpr (P::QLDS) return lds_read16(qlds + 32 * t);
     else return q[t];
+  };
+  // the lane's part of a K operand: the key m of 32, dims 16 t + 8 h .. + 7
+  const uint32_t klds = lds_address(&sh.k[0][m][8 * h]);
+  auto k_frag = [&](int buf, int n) RP_INLINE -> u32x4 {     // of keys 32 (n % 2) .., t = n / 2
+    return lds_read16(klds + 2 * ((buf * kTile + 32 * (n % 2)) * P::LDK + 16 * (n / 2)));
   };
 
   f32x16 acc[P::DB];
@@ -237,26 +253,20 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
 
   // ---- a tile's scores, in powers of two but for the factor c1
-  f32x16 s[2];
   const float c1 = P::FP8 ? 1.0f : a.c;
   auto product = [&](int buf, f32x16* to) RP_INLINE {
 #pragma unroll
     for (int i = 0; i < 16; ++i) to[0][i] = to[1][i] = 0.0f;
 #pragma unroll
-    for (int t = 0; t < P::QSTEPS; ++t) {
-      const u32x4 y = q_frag(t);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const u32x4 f = *reinterpret_cast<const u32x4*>(&sh.k[buf][32 * k + m][16 * t + 8 * h]);
-        to[k] = mma32<P::QF16>(f, y, to[k]);
-      }
-    }
+    for (int n = 0; n < 2 * P::QSTEPS; ++n)
+      to[n % 2] = mma32<P::QF16>(k_frag(buf, n), q_frag(n / 2), to[n % 2]);
   };
   uint32_t seen[2];                                      // bit 8 i + e: key 8 i + 4 h + e
   bool whole;
   float top;
-  // Masks the scores s of the tile at kb and finds their largest.
-  auto weigh = [&](int buf, int32_t kb, uint64_t here) RP_INLINE {
+  // Masks the scores s of the tile at kb and finds their largest (`found`: it
+  // is, unless some are masked).
+  auto weigh = [&](f32x16* s, int buf, int32_t kb, uint64_t here, bool found) RP_INLINE {
     if constexpr (P::FP8) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -280,14 +290,14 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           s[k][i] = seen[k] & 1u << (8 * (i / 4) + i % 4) ? s[k][i] : neg_inf();
       }
     }
-    // of a row with a NaN a NaN, which moves no base: the row is NaN
-    top = __builtin_elementwise_maximum(s[0][0], s[1][0]);
+    if (!whole || !found) {
+      // of a row with a NaN a NaN, which moves no base: the row is NaN
+      top = __builtin_elementwise_maximum(s[0][0], s[1][0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i)
-      top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][i]), s[1][i]);
+      for (int i = 1; i < 16; ++i)
+        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][i]), s[1][i]);
+    }
     top *= c1;
-  };
-  auto rebase = [&]() RP_INLINE {
     if (__any(top > base + (kSlack - a.lift))) {
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
       const float next = fmaxf(base, top + a.lift);
@@ -301,107 +311,157 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
 
   // ---- P from s, and its product with V
   uint32_t p[P::PARTS][2][8];
-  auto weights = [&](int buf) RP_INLINE {
-    const float b0 = base == neg_inf() ? 0.0f : base;    // no score yet: exp2(-inf) is 0
-    float part_sum[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float w[4];
-        f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (P::FP8) f = *reinterpret_cast<const f32x4*>(&sh.vs[buf][32 * k + 8 * i + 4 * h]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][4 * i + e], c1, -b0));
-          part_sum[k] += w[e];
-          if constexpr (P::FP8) {
-            w[e] *= f[e];
-            // what is not seen weighs 0 whatever its scale
-            if (!whole) w[e] = seen[k] >> (8 * i + e) & 1 ? w[e] : 0.0f;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float u = w[2 * e], v = w[2 * e + 1];
-          if constexpr (P::PARTS == 1) {
-            p[0][k][2 * i + e] = round_pair<P::VF16>(u, v);
-          } else {
-            p[0][k][2 * i + e] = pack_cut(u, v);
-            p[P::PARTS - 1][k][2 * i + e] = round_pair<false>(u - bf16_cut(u), v - bf16_cut(v));
-          }
-        }
+  // Weights 2 j, 2 j + 1 of block k (of 16), about the base b0, f their scales.
+  auto weight_pair = [&](const f32x16* s, int k, int j, float b0, float f0, float f1) RP_INLINE {
+    float u = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][2 * j], c1, -b0));
+    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][2 * j + 1], c1, -b0));
+    sum += u + v;
+    if constexpr (P::FP8) {
+      u *= f0;
+      v *= f1;
+      if (!whole) {                                      // what is not seen weighs 0 whatever its scale
+        const uint32_t bit = 8 * (j / 2) + 2 * (j % 2);
+        u = seen[k] >> bit & 1 ? u : 0.0f;
+        v = seen[k] >> bit & 2 ? v : 0.0f;
       }
-    sum += part_sum[0] + part_sum[1];
+    }
+    if constexpr (P::PARTS == 1) {
+      p[0][k][j] = round_pair<P::VF16>(u, v);
+    } else {
+      p[0][k][j] = pack_cut(u, v);
+      p[P::PARTS - 1][k][j] = round_pair<false>(u - bf16_cut(u), v - bf16_cut(v));
+    }
   };
-  // columns 32 d .. + 31 of keys 32 k + 16 u + 4 h + {0..3, 8..11}
-  const int l16 = lane & 15, cb = (lane >> 4 & 1) * 16 + (l16 & 3) * 4;
-  auto v_frag = [&](int buf, int d, int k, int u) RP_INLINE -> u32x4 {
-    const uint16_t* at = &sh.v[buf][32 * k + 16 * u + 4 * h + (l16 >> 2)][32 * d + cb];
-    const u32x2 lo = column4(at), hi = column4(at + 8 * P::LDV);
+  auto scales = [&](int buf, int g) RP_INLINE -> f32x4 {      // of weights 4 g .. 4 g + 3 of 32
+    return *reinterpret_cast<const f32x4*>(&sh.vs[buf][32 * (g / 4) + 8 * (g % 4) + 4 * h]);
+  };
+  auto weight_base = [&]() RP_INLINE -> float {
+    return base == neg_inf() ? 0.0f : base;              // no score yet: exp2(-inf) is 0
+  };
+  auto weights = [&](const f32x16* s, int buf) RP_INLINE {
+    const float b0 = weight_base();
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+      if constexpr (P::FP8) f = scales(buf, g);
+      weight_pair(s, g / 4, 2 * (g % 4), b0, f[0], f[1]);
+      weight_pair(s, g / 4, 2 * (g % 4) + 1, b0, f[2], f[3]);
+    }
+  };
+  // V's operand n of a tile: columns 32 d .. + 31 (d = n % DB) of keys 16 (n / DB)
+  // + 4 h + {0..3, 8..11}
+  const int l16 = lane & 15;
+  const uint32_t vlds =
+      lds_address(&sh.v[0][4 * h + (l16 >> 2)][(lane >> 4 & 1) * 16 + (l16 & 3) * 4]);
+  auto v_frag = [&](int buf, int n) RP_INLINE -> u32x4 {
+    const uint32_t at =
+        vlds + 2 * ((buf * kTile + 16 * (n / P::DB)) * P::LDV + 32 * (n % P::DB));
+    const u32x2 lo = column4(at), hi = column4(at + 2 * 8 * P::LDV);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
-  auto p_frag = [&](int e, int k, int u) RP_INLINE -> u32x4 {
+  auto p_frag = [&](int e, int n) RP_INLINE -> u32x4 {
+    const int k = n / P::DB / 2, u = n / P::DB % 2;
     return u32x4{p[e][k][4 * u], p[e][k][4 * u + 1], p[e][k][4 * u + 2], p[e][k][4 * u + 3]};
   };
   auto values = [&](int buf) RP_INLINE {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int n = 0; n < 4 * P::DB; ++n) {
+      const u32x4 f = v_frag(buf, n);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int d = 0; d < P::DB; ++d) {
-          const u32x4 f = v_frag(buf, d, k, u);
-#pragma unroll
-          for (int e = 0; e < P::PARTS; ++e) acc[d] = mma32<P::VF16>(f, p_frag(e, k, u), acc[d]);
-        }
+      for (int e = 0; e < P::PARTS; ++e)
+        acc[n % P::DB] = mma32<P::VF16>(f, p_frag(e, n), acc[n % P::DB]);
+    }
   };
   // The same one token of the wave at a time, V as that token sees it.
   auto values_apart = [&](int buf, int32_t kb) RP_INLINE {
     for (int32_t at = pmin; at <= pmax; ++at) {
       const bool mine = pos == at;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int n = 0; n < 4 * P::DB; ++n) {
+        u32x4 f = v_frag(buf, n);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t mask[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int32_t j = kb + 32 * k + 16 * u + 4 * h + (e < 2 ? 2 * e : 4 + 2 * e);
-            mask[e] = (sees(a, at, j) ? 0xffffu : 0u) | (sees(a, at, j + 1) ? 0xffff0000u : 0u);
-          }
-#pragma unroll
-          for (int d = 0; d < P::DB; ++d) {
-            u32x4 f = v_frag(buf, d, k, u);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] &= mask[e];
-            f32x16 y = mma32<P::VF16>(f, p_frag(0, k, u), acc[d]);
-            if constexpr (P::PARTS == 2) {
-              // a second part of 0 would make NaN of an infinity
-#pragma unroll
-              for (int e = 0; e < 4; ++e) f[e] = finite_pair<P::VF16>(f[e]);
-              y = mma32<P::VF16>(f, p_frag(1, k, u), y);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[d][i] = mine ? y[i] : acc[d][i];
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int32_t j = kb + 16 * (n / P::DB) + 4 * h + (e < 2 ? 2 * e : 4 + 2 * e);
+          f[e] &= (sees(a, at, j) ? 0xffffu : 0u) | (sees(a, at, j + 1) ? 0xffff0000u : 0u);
         }
+        f32x16 y = mma32<P::VF16>(f, p_frag(0, n), acc[n % P::DB]);
+        if constexpr (P::PARTS == 2) {
+          // a second part of 0 would make NaN of an infinity
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = finite_pair<P::VF16>(f[e]);
+          y = mma32<P::VF16>(f, p_frag(1, n), y);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n % P::DB][i] = mine ? y[i] : acc[n % P::DB][i];
+      }
     }
   };
 
-  // Tile t's weights and product with V, beside tile t + 1's scores: K is a
-  // tile ahead of V.
-  auto run = [&](auto apart) RP_INLINE {
+  // Tile t's weights and product with V, from its scores s, beside tile t + 1's
+  // scores: matrix instructions one by one, each with the LDS reads of the one
+  // kAhead later and a share of the vector work, in the order written.
+  auto fused = [&](const f32x16* s, f32x16* next, int buf) RP_INLINE {
+    constexpr int NK = 2 * P::QSTEPS, NV = 4 * P::DB;
+    u32x4 kf[kAhead], vf[kAhead], qf[2];
+    f32x4 sf[2];
+    const float b0 = weight_base();
+    if constexpr (P::FP8) sf[0] = scales(buf, 0);
+    qf[0] = q_frag(0);
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) kf[n] = k_frag(buf ^ 1, n);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) next[0][i] = next[1][i] = 0.0f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      if (n % 2 == 0 && n / 2 + 1 < P::QSTEPS) qf[(n / 2 + 1) % 2] = q_frag(n / 2 + 1);
+      next[n % 2] = mma32<P::QF16>(kf[n % kAhead], qf[n / 2 % 2], next[n % 2]);
+      if (n + kAhead < NK) kf[n % kAhead] = k_frag(buf ^ 1, n + kAhead);
+      else vf[(n + kAhead - NK) % kAhead] = v_frag(buf, n + kAhead - NK);
+#pragma unroll
+      for (int j = 16 * n / NK; j < 16 * (n + 1) / NK; ++j) {
+        const int g = j / 2;
+        if constexpr (P::FP8) {
+          if (j % 2 == 0 && g + 1 < 8) sf[(g + 1) % 2] = scales(buf, g + 1);
+        }
+        const f32x4 f = P::FP8 ? sf[g % 2] : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+        weight_pair(s, j / 8, j % 8, b0, f[2 * (j % 2)], f[2 * (j % 2) + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+#pragma unroll
+      for (int e = 0; e < P::PARTS; ++e)
+        acc[n % P::DB] = mma32<P::VF16>(vf[n % kAhead], p_frag(e, n), acc[n % P::DB]);
+      if (n + kAhead < NV) vf[n % kAhead] = v_frag(buf, n + kAhead);
+      if constexpr (!P::FP8) {
+#pragma unroll
+        for (int i = 16 * n / NV; i < 16 * (n + 1) / NV; ++i)
+          top = i == 0 ? __builtin_elementwise_maximum(next[0][0], next[1][0])
+                       : __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[0][i]), next[1][i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!P::FP8) asm volatile("" : "+v"(top));   // found here, not where it is used
+  };
+
+  auto reset = [&]() RP_INLINE {
     base = neg_inf();
     sum = 0.0f;
 #pragma unroll
     for (int d = 0; d < P::DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+  };
+  // All tiles; K is a tile ahead of V.
+  auto run = [&]() RP_INLINE {
+    reset();
     if (t0 >= t1) return;
     int32_t pages1 = page_of(t0 + 1, entry(t0 + 1));     // of tile t + 1
     int32_t entry2 = entry(t0 + 2);                      // of tile t + 2
     uint64_t here1;                                      // in tile t + 1
+    f32x16 even[2], odd[2];                              // the tiles' scores in turn
     {
       const int32_t pages = page_of(t0, entry(t0));
       const uint64_t here = present(t0, pages);
@@ -413,43 +473,57 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       load_rows(next, pages1, next, pages1);
       store_k(1, here1);
       __syncthreads();
-      product(0, s);
-      weigh(0, keys.key(t0), here);
-      rebase();
+      product(0, even);
+      weigh(even, 0, keys.key(t0), here, false);
       __syncthreads();                                   // K's first tile is overwritten next
     }
-    auto step = [&](int t, auto more) RP_INLINE {
-      const int buf = (t - t0) & 1;
-      uint64_t here2 = 0;
-      if constexpr (decltype(more)::value) {
-        const int32_t pages2 = page_of(t + 2, entry2);
-        here2 = present(t + 2, pages2);
-        entry2 = entry(t + 3);
-        load_rows(min(t + 2, t1 - 1), pages2, t + 1, pages1);
-        pages1 = pages2;
-      }
-      f32x16 next[2];
-      if constexpr (decltype(more)::value) product(buf ^ 1, next);
-      weights(buf);
-      if constexpr (decltype(apart)::value) values_apart(buf, keys.key(t));
-      else values(buf);
-      if constexpr (decltype(more)::value) {
-        __builtin_amdgcn_sched_barrier(0);               // they are waited for after the products
-        s[0] = next[0];
-        s[1] = next[1];
-        store_k(buf, here2);
-        store_v(buf ^ 1, here1);
-        weigh(buf ^ 1, keys.key(t + 1), here1);
-        here1 = here2;
-        rebase();
-      }
+    auto step = [&](int t, int buf, const f32x16* s, f32x16* next) RP_INLINE {
+      const int32_t pages2 = page_of(t + 2, entry2);
+      const uint64_t here2 = present(t + 2, pages2);
+      entry2 = entry(t + 3);
+      load_rows(min(t + 2, t1 - 1), pages2, t + 1, pages1);
+      pages1 = pages2;
+      fused(s, next, buf);
+      store_k(buf, here2);
+      store_v(buf ^ 1, here1);
+      weigh(next, buf ^ 1, keys.key(t + 1), here1, !P::FP8);
+      here1 = here2;
       __syncthreads();
     };
-    for (int t = t0; t + 1 < t1; ++t) step(t, std::true_type{});
-    step(t1 - 1, std::false_type{});
+    int t = t0;
+    for (; t + 2 < t1; t += 2) {
+      step(t, 0, even, odd);
+      step(t + 1, 1, odd, even);
+    }
+    if (t + 1 < t1) {
+      step(t, 0, even, odd);
+      weights(odd, 1);
+      values(1);
+    } else {
+      weights(even, 0);
+      values(0);
+    }
+  };
+  // The same a tile after the other, each token's part of V by itself.
+  auto run_apart = [&]() RP_INLINE {
+    reset();
+    for (int t = t0; t < t1; ++t) {
+      const int32_t pages = page_of(t, entry(t));
+      const uint64_t here = present(t, pages);
+      load_rows(t, pages, t, pages);
+      __syncthreads();
+      store_k(0, here);
+      store_v(0, here);
+      __syncthreads();
+      f32x16 s[2];
+      product(0, s);
+      weigh(s, 0, keys.key(t), here, false);
+      weights(s, 0);
+      values_apart(0, keys.key(t));
+    }
   };
   if (tid == 0) sh.redo = 0;
-  run(std::false_type{});
+  run();
   {
     f32x16 z = acc[0] * 0.0f;
 #pragma unroll
@@ -460,7 +534,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     __syncthreads();
     if (live && y != y) sh.redo = 1;
     __syncthreads();
-    if (sh.redo) run(std::true_type{});
+    if (sh.redo) run_apart();
   }
 
   if (row >= all) return;
@@ -496,10 +570,13 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
 template <int QT, int CT, int D>
 void launch_prompt_d(const WindowArgs& a, const PagedView& c, int waves, hipStream_t st) {
   const dim3 grid((unsigned)(a.groups * a.tiles * a.splits));
-  if (waves == 8)
-    hipLaunchKernelGGL((prompt_kernel<QT, CT, D, 8>), grid, dim3(8 * kWave), 0, st, a, c);
-  else
-    hipLaunchKernelGGL((prompt_kernel<QT, CT, D, 4>), grid, dim3(4 * kWave), 0, st, a, c);
+  if constexpr (D < 256) {
+    if (waves == 8) {
+      hipLaunchKernelGGL((prompt_kernel<QT, CT, D, 8>), grid, dim3(8 * kWave), 0, st, a, c);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((prompt_kernel<QT, CT, D, 4>), grid, dim3(4 * kWave), 0, st, a, c);
 }
 
 template <int QT, int CT>

@@ -86,7 +86,7 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
       2 * (c->head_dim * cache_elem_bytes(c->dtype) + (c->dtype == RP_CACHE_E4M3 ? 4 : 0));
   Layout l;
   l.columns = all <= 16 ? 1 : all <= 32 ? 2 : all <= 64 && c->head_dim < 256 ? 4 : 0;
-  l.waves = groups * ((all + 255) / 256) >= 256 ? 8 : 4;
+  l.waves = c->head_dim < 256 && groups * ((all + 255) / 256) >= 256 ? 8 : 4;
   const int64_t rows = l.columns ? 16 * l.columns : 32 * l.waves;
   l.tiles = (all + rows - 1) / rows;
   // a tile's keys: its tokens', the window's before them, the sinks
