@@ -178,42 +178,43 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   auto present = [&](int t, int32_t pages) RP_INLINE -> uint64_t {
     return __ballot(pages >= 0 && keys.any(keys.key(t) + lane));
   };
+  // Where key l of a tile lies, in bytes from the head's first row.  What is no
+  // row is read as one of page 0; what no row sees is put into LDS as zeros.
+  auto offset_of = [&](int t, int32_t page) RP_INLINE -> int64_t {
+    return max(0, page) * (c.sp * P::EB) + ((keys.key(t) + lane) & c.page_mask()) * (c.sr * P::EB);
+  };
+  const char* const khead = c.k + kv * c.sh * P::EB;
+  const char* const vhead = c.v + kv * c.sh * P::EB;
   // a wave's rows of a chunk lie in one page, unless pages are smaller
   const bool one_page = c.page_mask() >= P::WROWS - 1;
   const uint32_t lane_off = (uint32_t)((lane / P::CPR) * c.sr * P::EB + lane % P::CPR * 16);
-  // What is no row is read as a row of page 0; what no row sees is put into LDS
-  // as zeros.
-  auto load = [&](auto one, u32x4* to, const char* from, int32_t kb, int32_t pages) RP_INLINE {
+  auto load = [&](auto one, u32x4* to, const char* from, int64_t off) RP_INLINE {
+    const int lo = (int)off, hi = (int)(off >> 32);
 #pragma unroll
     for (int i = 0; i < P::NCH; ++i) {
       const int rw = min(wave * P::WROWS + i * (P::NT / P::CPR), kTile - P::WROWS);
       if constexpr (decltype(one)::value) {
-        const int32_t page = __builtin_amdgcn_readlane(pages, rw);
-        to[i] = *reinterpret_cast<const u32x4*>(from + paged_row(c, page, kv, kb + rw) * P::EB + lane_off);
+        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, rw) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane(lo, rw);
+        to[i] = *reinterpret_cast<const u32x4*>(from + at + lane_off);
       } else {
         const int r = rw + lane / P::CPR;
-        const int32_t page = __shfl(pages, r, kWave);
-        to[i] = *reinterpret_cast<const u32x4*>(from + paged_row(c, page, kv, kb + r) * P::EB + lane % P::CPR * 16);
+        const uint64_t at = (uint64_t)(uint32_t)__shfl(hi, r, kWave) << 32 | (uint32_t)__shfl(lo, r, kWave);
+        to[i] = *reinterpret_cast<const u32x4*>(from + at + lane % P::CPR * 16);
       }
     }
   };
-  // K's rows of tile tk and V's of tile tv
-  auto load_rows = [&](int tk, int32_t kpages, int tv, int32_t vpages) RP_INLINE {
-    const int32_t kb = keys.key(tk), vb = keys.key(tv);
-    kpages = max(0, kpages);
-    vpages = max(0, vpages);
+  auto load_rows = [&](int64_t koff, int64_t voff) RP_INLINE {
     if (one_page) {
-      load(std::true_type{}, kreg, c.k, kb, kpages);
-      load(std::true_type{}, vreg, c.v, vb, vpages);
+      load(std::true_type{}, vreg, vhead, voff);
+      load(std::true_type{}, kreg, khead, koff);
     } else {
-      load(std::false_type{}, kreg, c.k, kb, kpages);
-      load(std::false_type{}, vreg, c.v, vb, vpages);
+      load(std::false_type{}, vreg, vhead, voff);
+      load(std::false_type{}, kreg, khead, koff);
     }
-    if constexpr (P::FP8) {
-      if (wave == 0) ksreg = c.ks[paged_scale(c, kpages, kv, kb + lane)];
-      if (wave == 1) vsreg = c.vs[paged_scale(c, vpages, kv, vb + lane)];
-    }
-    __builtin_amdgcn_sched_barrier(0);                   // on their way before the products
+  };
+  auto load_scale = [&](int t, int32_t page, const float* from) RP_INLINE -> float {
+    return from[paged_scale(c, max(0, page), kv, keys.key(t) + lane)];
   };
   auto store = [&](uint16_t* to, int ld, u32x4* from, uint64_t here, auto f16) RP_INLINE {
 #pragma unroll
@@ -405,21 +406,20 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     u32x4 kf[kAhead], vf[kAhead], qf[2];
     f32x4 sf[2];
     const float b0 = weight_base();
+    __builtin_amdgcn_s_setprio(1);                       // before the half that stages
     if constexpr (P::FP8) sf[0] = scales(buf, 0);
     qf[0] = q_frag(0);
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) kf[n] = k_frag(buf ^ 1, n);
 #pragma unroll
     for (int i = 0; i < 16; ++i) next[0][i] = next[1][i] = 0.0f;
-    __builtin_amdgcn_sched_barrier(0);
+    // The pairs of weights evenly over the steps before the product that asks for
+    // the last of them, each in time for its own.
+    auto some_weights = [&](int step) RP_INLINE {
+      constexpr int T = NK + 3 * NV / 4;
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      if (n % 2 == 0 && n / 2 + 1 < P::QSTEPS) qf[(n / 2 + 1) % 2] = q_frag(n / 2 + 1);
-      next[n % 2] = mma32<P::QF16>(kf[n % kAhead], qf[n / 2 % 2], next[n % 2]);
-      if (n + kAhead < NK) kf[n % kAhead] = k_frag(buf ^ 1, n + kAhead);
-      else vf[(n + kAhead - NK) % kAhead] = v_frag(buf, n + kAhead - NK);
-#pragma unroll
-      for (int j = 16 * n / NK; j < 16 * (n + 1) / NK; ++j) {
+      for (int j = 0; j < 16; ++j) {
+        if (2 * j * T / 33 != step) continue;
         const int g = j / 2;
         if constexpr (P::FP8) {
           if (j % 2 == 0 && g + 1 < 8) sf[(g + 1) % 2] = scales(buf, g + 1);
@@ -428,6 +428,15 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
         weight_pair(s, j / 8, j % 8, b0, f[2 * (j % 2)], f[2 * (j % 2) + 1]);
       }
       __builtin_amdgcn_sched_barrier(0);
+    };
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      if (n % 2 == 0 && n / 2 + 1 < P::QSTEPS) qf[(n / 2 + 1) % 2] = q_frag(n / 2 + 1);
+      next[n % 2] = mma32<P::QF16>(kf[n % kAhead], qf[n / 2 % 2], next[n % 2]);
+      if (n + kAhead < NK) kf[n % kAhead] = k_frag(buf ^ 1, n + kAhead);
+      else vf[(n + kAhead - NK) % kAhead] = v_frag(buf, n + kAhead - NK);
+      some_weights(n);
     }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
@@ -441,9 +450,12 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           top = i == 0 ? __builtin_elementwise_maximum(next[0][0], next[1][0])
                        : __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[0][i]), next[1][i]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      some_weights(NK + n);
     }
-    if constexpr (!P::FP8) asm volatile("" : "+v"(top));   // found here, not where it is used
+    __builtin_amdgcn_s_setprio(0);
+    // found here, not where they are used
+    asm volatile("" : "+v"(sum));
+    if constexpr (!P::FP8) asm volatile("" : "+v"(top));
   };
 
   auto reset = [&]() RP_INLINE {
@@ -454,40 +466,73 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
   };
-  // All tiles; K is a tile ahead of V.
+  // All tiles.  Of eight waves two share a SIMD, one of each half of the
+  // workgroup, and the halves take turns: while one runs its products (fused),
+  // the other masks and stages, between two barriers a tile.  K is staged a tile
+  // ahead of V; the second half, half a tile behind, stages one further ahead, so
+  // that a tile is whole before the first half asks for it:
+  //   first half   fused(t) | mask t + 1, store K t + 2 and V t + 1 | fused(t + 1)
+  //   second half  store K t + 2 and V t + 1 | fused(t) | mask t + 1, store t + 3 and t + 2
   auto run = [&]() RP_INLINE {
     reset();
     if (t0 >= t1) return;
-    int32_t pages1 = page_of(t0 + 1, entry(t0 + 1));     // of tile t + 1
-    int32_t entry2 = entry(t0 + 2);                      // of tile t + 2
-    uint64_t here1;                                      // in tile t + 1
+    const bool second = NW == 8 && wave >= 4;
+    uint64_t q0, q1 = 0, q2 = 0;                         // the tiles' keys that are there, t + 1 on
+    int32_t page, ahead;                                 // of tile tk; tile tk + 1's entry
+    int64_t off;                                         // of tile tk
+    int tk = t0;                                         // the tile whose K is in the registers
+    // K of tile tk + 1, V of tile tk; which of K's keys are there
+    auto next_rows = [&]() RP_INLINE -> uint64_t {
+      if constexpr (P::FP8) {
+        if (wave == 1) vsreg = load_scale(tk, page, c.vs);
+      }
+      page = page_of(++tk, ahead);
+      ahead = entry(tk + 1);
+      const int64_t before = off;
+      off = offset_of(tk, page);
+      load_rows(off, before);
+      if constexpr (P::FP8) {
+        if (wave == 0) ksreg = load_scale(tk, page, c.ks);
+      }
+      return present(tk, page);
+    };
+    auto put_rows = [&](uint64_t here, uint64_t before) RP_INLINE {
+      store_k((tk - t0) & 1, here);
+      store_v((tk - t0 + 1) & 1, before);
+    };
     f32x16 even[2], odd[2];                              // the tiles' scores in turn
     {
-      const int32_t pages = page_of(t0, entry(t0));
-      const uint64_t here = present(t0, pages);
-      const int next = min(t0 + 1, t1 - 1);
-      load_rows(t0, pages, t0, pages);
+      page = page_of(t0, entry(t0));
+      off = offset_of(t0, page);
+      ahead = entry(t0 + 1);
+      const uint64_t here = present(t0, page);
+      load_rows(off, off);
+      if constexpr (P::FP8) {
+        if (wave == 0) ksreg = load_scale(t0, page, c.ks);
+      }
       store_k(0, here);
-      store_v(0, here);
-      here1 = present(t0 + 1, pages1);
-      load_rows(next, pages1, next, pages1);
-      store_k(1, here1);
+      q0 = next_rows();
+      put_rows(q0, here);
       __syncthreads();
       product(0, even);
       weigh(even, 0, keys.key(t0), here, false);
+      q1 = next_rows();
       __syncthreads();                                   // K's first tile is overwritten next
+      if (second) {
+        put_rows(q1, q0);
+        q2 = next_rows();
+        __syncthreads();
+      }
     }
     auto step = [&](int t, int buf, const f32x16* s, f32x16* next) RP_INLINE {
-      const int32_t pages2 = page_of(t + 2, entry2);
-      const uint64_t here2 = present(t + 2, pages2);
-      entry2 = entry(t + 3);
-      load_rows(min(t + 2, t1 - 1), pages2, t + 1, pages1);
-      pages1 = pages2;
       fused(s, next, buf);
-      store_k(buf, here2);
-      store_v(buf ^ 1, here1);
-      weigh(next, buf ^ 1, keys.key(t + 1), here1, !P::FP8);
-      here1 = here2;
+      if constexpr (NW == 8) __syncthreads();
+      weigh(next, buf ^ 1, keys.key(t + 1), q0, !P::FP8);
+      put_rows(second ? q2 : q1, second ? q1 : q0);
+      const uint64_t here = next_rows();
+      q0 = q1;
+      q1 = second ? q2 : here;
+      q2 = here;
       __syncthreads();
     };
     int t = t0;
@@ -503,14 +548,20 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       weights(even, 0);
       values(0);
     }
+    if (NW == 8 && !second) __syncthreads();
   };
   // The same a tile after the other, each token's part of V by itself.
   auto run_apart = [&]() RP_INLINE {
     reset();
     for (int t = t0; t < t1; ++t) {
-      const int32_t pages = page_of(t, entry(t));
-      const uint64_t here = present(t, pages);
-      load_rows(t, pages, t, pages);
+      const int32_t page = page_of(t, entry(t));
+      const int64_t off = offset_of(t, page);
+      const uint64_t here = present(t, page);
+      load_rows(off, off);
+      if constexpr (P::FP8) {
+        if (wave == 0) ksreg = load_scale(t, page, c.ks);
+        if (wave == 1) vsreg = load_scale(t, page, c.vs);
+      }
       __syncthreads();
       store_k(0, here);
       store_v(0, here);
