@@ -6,7 +6,9 @@
 // products and the order of their operands are rp_paged_attn.hip's: S^T = K Q^T
 // leaves a lane with eight scores of its column's row, O^T = V^T P^T takes them
 // from the same lane.  The steps that the rows see between them, those of the
-// sinks first, are shared out evenly over the parts and a part's four waves.
+// sinks first, are shared out evenly over the parts and a part's four waves; a
+// sequence's parts are as many as its steps deserve, so that the batch's longest
+// one does not hold up the others.
 //
 // Weights enter the product with V as the sum of two 16-bit numbers, 16 bits
 // of them or more, which the matrix cores do while the next rows arrive.  Bases
@@ -273,25 +275,74 @@ struct Few : StepRows<QT == kInF16, CT, D, STREAM> {
   }
 };
 
+// Which part of which sequence a workgroup takes: of a kv head's `room` parts each
+// sequence has one, and of those left a share by its steps.
+struct Share {
+  int b, split, own;             // sequence (-1: none), its part, of how many
+};
+
+__device__ __forceinline__ Share part_of(const WindowArgs& a, const PagedView& c, int at, int r0,
+                                         int n) {
+  const int lane = threadIdx.x & (kWave - 1), B = (int)(a.groups / c.heads);
+  if (B == 1) return at < a.splits ? Share{0, at, a.splits} : Share{-1, 0, 1};
+  auto steps = [&](int b) { return b < B ? tile_keys<kStep>(a, c, Place(a, b), r0, n).count : 0; };
+  auto sum = [&](double x) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, kWave);
+    return x;
+  };
+  int mine = steps(lane);
+  double all = mine;                                     // whole numbers: exact
+  for (int b = kWave + lane; b < B + lane; b += kWave) all += steps(b);
+  all = fmax(sum(all), 1.0);
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += kWave) {
+    if (b0 > 0) mine = steps(b0 + lane);
+    const int own = b0 + lane < B ? min(a.splits, 1 + (int)((double)(a.room - B) * mine / all)) : 0;
+    int upto = own;
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) {
+      const int y = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += y;
+    }
+    const uint64_t past = __ballot(before + upto > at);
+    if (past) {
+      const int l = __builtin_ctzll(past), own_l = __shfl(own, l, kWave);
+      return Share{b0 + l, at - before - (__shfl(upto, l, kWave) - own_l), own_l};
+    }
+    before += __shfl(upto, kWave - 1, kWave);
+  }
+  return Share{-1, 0, 1};
+}
+
 template <int QT, int CT, int D, bool PG16, bool STREAM, int NQ>
-__global__ __launch_bounds__(kFewThreads) void few_kernel(WindowArgs a, PagedView c) {
+__global__ __launch_bounds__(kFewThreads, D <= 128 ? 2 : 1) void few_kernel(WindowArgs a, PagedView c) {
   typedef Few<QT, CT, D, PG16, STREAM, NQ> W;
   __shared__ f32x4 sacc[kFewWaves / 2][NQ][W::DPL][kWave];
   __shared__ float sbase[kFewWaves][NQ][16], ssum[kFewWaves][NQ][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  int64_t at = blockIdx.x;
-  const int split = (int)(at % a.splits);
-  at /= a.splits;
-  const int tile = (int)(at % a.tiles);
-  at /= a.tiles;
-  const int kv = (int)(at % c.heads), b = (int)(at / c.heads);
+  // The row tiles of a part's keys on one XCD, one after the other: what one
+  // brings the next ones find in its L2.
+  const int64_t parts = (a.splits > 1 ? (int64_t)a.room : a.groups / c.heads) * c.heads;
+  const int64_t lanes8 = parts % 8 == 0 ? 8 : 1;
+  const int64_t eight = blockIdx.x / (lanes8 * a.tiles), in = blockIdx.x % (lanes8 * a.tiles);
+  const int64_t at = eight * lanes8 + in % lanes8;
+  const int tile = (int)(in / lanes8), kv = (int)(at % c.heads), r0 = tile * 16 * NQ;
+  int b = (int)(at / c.heads), split = 0, own = 1;
+  if (a.splits > 1) {
+    const Share s = part_of(a, c, b, r0, 16 * NQ);
+    b = s.b;
+    split = s.split;
+    own = s.own;
+    if (b < 0) return;
+  }
 
   const Place pl(a, b);
   const int rows = pl.m * a.group, all = a.S * a.group;
-  const int r0 = tile * 16 * NQ, last = min(r0 + 16 * NQ, rows) - 1;
+  const int last = min(r0 + 16 * NQ, rows) - 1;
   const int32_t pmin = pl.first + r0 / a.group;
   const int32_t pmax = last >= r0 ? pl.first + last / a.group : -1;
-  const KeyTiles<kStep> keys(a, c, pmin, pmax);
+  const KeyTiles<kStep> keys = tile_keys<kStep>(a, c, pl, r0, 16 * NQ);
   W w(a, c, keys);
   w.place(threadIdx.x & (kWave - 1), kv);
   w.table = c.table + b * c.table_stride;
@@ -312,9 +363,18 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(WindowArgs a, PagedVie
       w.q[n][t] ^= a.flip;
     }
   }
+  if (split == 0) {                                      // the parts that the sequence has not
+    const int none = a.splits - own;
+    for (int i = threadIdx.x; i < 16 * NQ * none; i += kFewThreads) {
+      const int row = r0 + i / none;
+      if (row >= all) break;
+      const int64_t orow = ((int64_t)b * a.H + kv * a.group + row % a.group) * a.S + row / a.group;
+      a.ml[orow * a.splits + own + i % none] = float2{neg_inf(), 0.0f};
+    }
+  }
   // the part's steps, and the wave's of them
-  const int t0 = (int)((int64_t)keys.count * split / a.splits);
-  const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
+  const int t0 = (int)((int64_t)keys.count * split / own);
+  const int t1 = (int)((int64_t)keys.count * (split + 1) / own);
   const int from = t0 + (t1 - t0) * wave / kFewWaves, end = t0 + (t1 - t0) * (wave + 1) / kFewWaves;
   w.template run<false>(from, end);
   if (w.spoiled(live)) w.template run<true>(from, end);
@@ -392,7 +452,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(WindowArgs a, PagedVie
 
 template <int QT, int CT, int D, int NQ>
 void launch_few_n(const WindowArgs& a, const PagedView& c, bool stream, hipStream_t st) {
-  const dim3 grid((unsigned)(a.groups * a.tiles * a.splits));
+  const dim3 grid((unsigned)((a.splits > 1 ? (int64_t)a.room * c.heads : a.groups) * a.tiles));
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kFewThreads), 0, st, a, c); };
   if (c.shift < 4) go(few_kernel<QT, CT, D, false, false, NQ>);
   else if (stream) go(few_kernel<QT, CT, D, true, true, NQ>);
@@ -402,9 +462,10 @@ void launch_few_n(const WindowArgs& a, const PagedView& c, bool stream, hipStrea
 template <int QT, int CT, int D>
 void launch_few_d(const WindowArgs& a, const PagedView& c, int columns, bool stream,
                   hipStream_t st) {
-  if (columns == 1) launch_few_n<QT, CT, D, 1>(a, c, stream, st);
-  else if (columns == 2) launch_few_n<QT, CT, D, 2>(a, c, stream, st);
-  else if constexpr (D < 256) launch_few_n<QT, CT, D, 4>(a, c, stream, st);
+  if constexpr (D < 256) {
+    if (columns == 2) return launch_few_n<QT, CT, D, 2>(a, c, stream, st);
+  }
+  launch_few_n<QT, CT, D, 1>(a, c, stream, st);
 }
 
 template <int QT, int CT>

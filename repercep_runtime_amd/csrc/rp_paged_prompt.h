@@ -130,9 +130,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   // the wave's rows' first and last positions
   const int w0 = r0 + 32 * wave, w1 = min(w0 + 32, rows) - 1;
   const int32_t pmin = pl.first + w0 / a.group, pmax = w1 >= w0 ? pl.first + w1 / a.group : -1;
-  const int last = min(r0 + P::ROWS, rows) - 1;
-  const KeyTiles<kTile> keys(a, c, pl.first + r0 / a.group,
-                             last >= r0 ? pl.first + last / a.group : -1);
+  const KeyTiles<kTile> keys = tile_keys<kTile>(a, c, pl, r0, P::ROWS);
   const int t0 = (int)((int64_t)keys.count * split / a.splits);
   const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
   const int32_t* table = c.table + b * c.table_stride;

@@ -26,6 +26,7 @@ struct WindowArgs {
   float* lse;                    // (B, H, S), or null
   int32_t H, group, S;
   int32_t tiles, splits;         // row tiles of a kv head, parts of a tile's keys
+  int32_t room;                  // few_kernel: the whole batch's parts of a kv head and row tile
   int64_t groups;                // B * kv heads
   float* part;                   // (B, H, S, splits, D): the parts' weighted means
   float2* ml;                    // (B, H, S, splits): base (in powers of two), sum of weights
@@ -88,6 +89,14 @@ struct KeyTiles {
   // Whether any of the tokens sees key j.
   __device__ __forceinline__ bool any(int32_t j) const { return j < hi && (j >= lo || j < sinks); }
 };
+
+// The keys that rows r0 .. r0 + n - 1 of a sequence see between them.
+template <int T>
+__device__ __forceinline__ KeyTiles<T> tile_keys(const WindowArgs& a, const PagedView& c,
+                                                 const Place& pl, int r0, int n) {
+  const int last = min(r0 + n, pl.m * a.group) - 1;
+  return KeyTiles<T>(a, c, pl.first + r0 / a.group, last >= r0 ? pl.first + last / a.group : -1);
+}
 
 // 16-bit floats with infinities and NaNs as 0, a pair.
 template <bool F16>

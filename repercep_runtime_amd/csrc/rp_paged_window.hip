@@ -36,10 +36,8 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, int64_t 
 #pragma unroll 4
   for (int s = gr; s < a.splits; s += GR) {
     const float2 p = ml[s];
-    const f32x4 y = part[(int64_t)s * COLS];
-    const float f = p.y * __builtin_amdgcn_exp2f(p.x - b0) * inv;
-    // a part without keys wrote nothing
-    if (p.y != 0.0f) x += y * f;
+    if (p.y == 0.0f) continue;                           // a part without keys wrote nothing
+    x += part[(int64_t)s * COLS] * (p.y * __builtin_amdgcn_exp2f(p.x - b0) * inv);
   }
   sums[threadIdx.x] = x;
   __syncthreads();
@@ -71,9 +69,23 @@ void launch_join(const WindowArgs& a, int64_t D, int64_t rows, hipStream_t st) {
 constexpr int64_t kMaxSplits = 256;
 // see kStreamBytes of rp_paged_attn.hip
 constexpr int64_t kStreamBytes = 256 << 20;
+// few_kernel: rows of a kv head up to which a call is bound by its keys' bytes.
+// 16 sequences of 8000 keys, 8 kv heads of 128: 64 rows 142 us (prompt_kernel
+// takes 128 rows in 154), 128 rows 268 us; e4m3fn 64 rows 100 us.
+constexpr int64_t kFewRows = 64;
+// and its workgroups: two a CU, what its registers hold.  Of 16-bit keys one a CU
+// takes nearly the card's rate (93 us against 90 with half as many), but ragged
+// batches need the parts: 16 sequences of 640 to 8000 e4m3fn keys 72 us on 256
+// workgroups, 48 on 512, 58 on 1024.
+constexpr int64_t kFewGroups = 512;
+constexpr int64_t kFewPartBytes = 128 << 10;
+
+// prompt_kernel: workgroups that fill the card (its LDS and registers hold one a
+// CU), and the keys that are worth a part of their own.
+constexpr int64_t kPromptGroups = 256, kPromptPartKeys = 1024;
 
 struct Layout : WindowLaunch {
-  int64_t tiles, splits;
+  int64_t tiles, splits, room;
   size_t ml, total;                                     // byte offsets: parts first
 };
 
@@ -85,8 +97,13 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
   const int64_t key_bytes =
       2 * (c->head_dim * cache_elem_bytes(c->dtype) + (c->dtype == RP_CACHE_E4M3 ? 4 : 0));
   Layout l;
-  l.columns = all <= 16 ? 1 : all <= 32 ? 2 : all <= 64 && c->head_dim < 256 ? 4 : 0;
-  l.waves = c->head_dim < 256 && groups * ((all + 255) / 256) >= 256 ? 8 : 4;
+  l.columns = all > kFewRows ? 0 : all <= 16 || c->head_dim == 256 ? 1 : 2;
+  // Tiles of 256 rows where they are many or their keys can be split, of 128
+  // otherwise: prompts of 1024 tokens, 8 kv heads, 40 us in 128 workgroups, 36 in
+  // 256 of half the rows; 512 tokens after 15488 keys 162 us in 64 x 4 workgroups,
+  // 232 with half the rows.  (A head dim of 256 leaves no registers for eight waves.)
+  const bool many = groups * ((all + 255) / 256) >= kPromptGroups;
+  l.waves = c->head_dim < 256 && all > 128 && (many || longest >= 2048) ? 8 : 4;
   const int64_t rows = l.columns ? 16 * l.columns : 32 * l.waves;
   l.tiles = (all + rows - 1) / rows;
   // a tile's keys: its tokens', the window's before them, the sinks
@@ -94,13 +111,24 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
   int64_t keys = longest;
   if (window > 0 && window + sinks + tokens < keys) keys = window + sinks + tokens;
   const int64_t blocks = groups * l.tiles;
+  l.room = 0;
+  l.stream = false;
   if (l.columns) {
-    const int64_t round = l.columns == 4 ? 256 : 512;
-    l.splits = blocks >= round ? 1 : min((round + blocks - 1) / blocks, keys * key_bytes / (128 << 10));
-    l.stream = groups * keys * key_bytes > kStreamBytes;
+    // No more parts of a sequence than four times an even share.  Sequences within
+    // a window are alike, so one workgroup a CU is enough: 256 groups of 1056 keys
+    // 27 us unsplit, 32 in two parts.
+    l.room = kFewGroups / (c->heads * l.tiles);
+    l.splits = min(min(1 + l.room - B, 4 * ((l.room + B - 1) / B)), keys * key_bytes / kFewPartBytes);
+    if (keys < longest && blocks >= kFewGroups / 2) l.splits = 1;
+    // a second row tile finds V in the caches
+    l.stream = l.tiles == 1 && groups * keys * key_bytes > kStreamBytes;
+  } else if (blocks >= kPromptGroups) {
+    l.splits = 1;
   } else {
-    l.splits = blocks >= 256 ? 1 : min((512 + blocks - 1) / blocks, (keys + 511) / 512);
-    l.stream = false;
+    // One workgroup a CU; two where tiles of a prompt see few keys and many: 4096
+    // tokens on one kv head 113 us unsplit, 81 in four parts.
+    l.splits = keys >= 4 * S ? kPromptGroups / blocks : (2 * kPromptGroups + blocks - 1) / blocks;
+    l.splits = min(l.splits, keys / kPromptPartKeys);
   }
   l.splits = max((int64_t)1, min(l.splits, kMaxSplits));
   const int64_t parts = l.splits > 1 ? B * H * S * l.splits : 0;
@@ -223,6 +251,7 @@ extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64
   a.S = (int32_t)S;
   a.tiles = (int32_t)l.tiles;
   a.splits = (int32_t)l.splits;
+  a.room = (int32_t)l.room;
   a.groups = groups;
   a.part = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float2*>(ws + l.ml);
