@@ -658,8 +658,8 @@ int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N, int64_t V
  *   out      (B, N + 1): the accepted drafts, the drawn token (-1 where every
  *            w is 0), then -1; accepted (B): m
  * N may be 0 (a draw from p_0).  V up to 2^22.  Equal calls give equal tokens.
- * workspace: rp_verify_drafts_workspace_bytes, 256-byte aligned.
- * No counterpart in the reference. */
+ * workspace: rp_verify_drafts_workspace_bytes, 256-byte aligned (may be NULL
+ * where that is 0).  No counterpart in the reference. */
 size_t rp_verify_drafts_workspace_bytes(int64_t B, int64_t V);
 int rp_verify_drafts(const int64_t* tokens, const int32_t* lens, int64_t B, int64_t N,
                      const void* target, int64_t tsb, int64_t tsn, const void* draft, int64_t dsb,

@@ -11,19 +11,26 @@
 // token for about one draw in a hundred.
 //
 // Only row n of p and q is read whole (a test takes one value of each of the
-// other rows), so the floor is those rows' bytes.  A row is cut into parts of
-// kPart tokens: verify_sum_kernel finds n anew in each workgroup (three
-// dependent loads, less than a launch) and adds up its part, verify_draw_kernel
-// finds the part that the draw falls into and reads that part once more.
+// other rows), so the floor is those rows' bytes; small calls are a chain of
+// dependent loads.  A block reads tokens in chunks of four a thread and adds up
+// each wave's of each chunk (a segment); every wave then finds the segment that
+// the draw falls into from the segments' sums, and the one that holds it looks
+// among its lanes.
+//
+// Rows of up to kOne tokens take one launch: verify_one_kernel, a block a
+// sequence.  Longer ones are cut into parts of kPart tokens: verify_sum_kernel
+// finds n anew in each block (less than a launch) and adds up its part,
+// verify_draw_kernel finds the draw's part and reads it once more.
 
 #include "rp_common.h"
 
 namespace rp {
 namespace {
 
-constexpr int kSumThreads = 256, kPerSum = 16, kPart = kSumThreads * kPerSum;
-constexpr int kDrawThreads = 1024, kPerDraw = kPart / kDrawThreads;
-constexpr int64_t kMaxV = (int64_t)kPart * kDrawThreads;
+constexpr int kOneWaves = 16, kOneChunks = 8, kOne = kOneWaves * kWave * 4 * kOneChunks;
+constexpr int kSumThreads = 256, kPart = 4096, kDrawWaves = kSumThreads / kWave;
+constexpr int kDrawChunks = kPart / (kSumThreads * 4);
+constexpr int64_t kMaxV = 1024 * (int64_t)kPart;
 
 struct VerifyArgs {
   const char* target;            // (B, N + 1, V)
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a) {
   const Weights<DT> row(a, b, n, n < has);
   double sw = 0.0, sp = 0.0;
 #pragma unroll
-  for (int k = 0; k < kPerSum / 4; ++k) {
+  for (int k = 0; k < kDrawChunks; ++k) {
     double w[4], p[4];
     row.four(part * kPart + 4 * (k * kSumThreads + (int)threadIdx.x), w, p);
     sw += (w[0] + w[1]) + (w[2] + w[3]);
@@ -160,106 +167,179 @@ __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a) {
   a.sums[(int64_t)b * a.parts + part] = double2{sw, sp};
 }
 
-// The place of a draw among the block's values, one a thread.
-struct Draw {
-  double wave_sum[kDrawThreads / kWave];
-  int first, last;
-};
-
-// Sums of the threads' values before each thread's own, and of all.
-__device__ __forceinline__ double before(double x, double* total, Draw& sh) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  double inc = x;
+// Sums of the lanes' values up to and with each lane's own.
+__device__ __forceinline__ double upto(double x, int lane) {
 #pragma unroll
   for (int o = 1; o < kWave; o *= 2) {
-    const double y = __shfl_up(inc, o, kWave);
-    if (lane >= o) inc += y;
+    const double y = __shfl_up(x, o, kWave);
+    if (lane >= o) x += y;
   }
-  __syncthreads();
-  if (lane == kWave - 1) sh.wave_sum[wave] = inc;
-  __syncthreads();
-  double base = 0.0, all = 0.0;
-#pragma unroll
-  for (int w = 0; w < kDrawThreads / kWave; ++w) {
-    if (w == wave) base = all;
-    all += sh.wave_sum[w];
-  }
-  *total = all;
-  const double exc = __shfl_up(inc, 1, kWave);
-  return base + (lane == 0 ? 0.0 : exc);
+  return x;
 }
 
-// The lowest `at` that a thread offers (>= 0), else the highest `alt`, else -1.
-__device__ __forceinline__ int choose(int at, int alt, Draw& sh) {
-  if (threadIdx.x == 0) {
-    sh.first = 0x7fffffff;
-    sh.last = -1;
+// Where a draw falls among up to 128 sums, two a lane: the first entry with
+// lo + sums up to it > goal, else (rounding, or a goal of all there is and more)
+// the last positive one, else -1; and the sums before it.
+struct Place {
+  int at;
+  double before;
+};
+__device__ __forceinline__ Place place(double x0, double x1, double up, double lo, double goal,
+                                       int lane) {
+  const double b0 = lo + (up - (x0 + x1)), b1 = b0 + x0;
+  const uint64_t in0 = __ballot(b1 > goal && x0 > 0.0), in1 = __ballot(b1 + x1 > goal && x1 > 0.0);
+  const uint64_t any0 = __ballot(x0 > 0.0), any1 = __ballot(x1 > 0.0);
+  int at = -1;
+  if (in0 | in1) {
+    const int l = __builtin_ctzll(in0 | in1);
+    at = 2 * l + (in0 >> l & 1 ? 0 : 1);
+  } else if (any0 | any1) {
+    const int l = 63 - __builtin_clzll(any0 | any1);
+    at = 2 * l + (any1 >> l & 1 ? 1 : 0);
+  }
+  const int l = at < 0 ? 0 : at / 2;
+  return Place{at, at & 1 ? __shfl(b1, l, kWave) : __shfl(b0, l, kWave)};
+}
+
+// Draws a token among the K chunks of a block of W waves that begin at `first`,
+// weighed by `row`: with goal(sum of the block's weights) the sum that has to be
+// passed.  The wave that holds the token calls found(token); where there is
+// nothing to draw every wave calls none().
+template <int DT, int W, int K, typename G, typename F, typename N>
+__device__ __forceinline__ void draw(const Weights<DT>& row, bool rejected, int first, double lo,
+                                     double* sums, G goal, F found, N none) {
+  static_assert(W * K <= 2 * kWave, "two segments a lane");
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  double mine[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    double w[4], p[4];
+    row.four(first + 4 * (k * W * kWave + tid), w, p);
+    const double* x = rejected ? w : p;
+    mine[k] = (x[0] + x[1]) + (x[2] + x[3]);
+    double s = mine[k];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, kWave);
+    if (lane == 0) sums[k * W + wave] = s;
   }
   __syncthreads();
-  if (at >= 0) atomicMin(&sh.first, at);
-  if (alt >= 0) atomicMax(&sh.last, alt);
-  __syncthreads();
-  return sh.first != 0x7fffffff ? sh.first : sh.last;
+  const double x0 = 2 * lane < W * K ? sums[2 * lane] : 0.0;
+  const double x1 = 2 * lane + 1 < W * K ? sums[2 * lane + 1] : 0.0;
+  const double up = upto(x0 + x1, lane), all = __shfl(up, kWave - 1, kWave);
+  const double want = goal(all);
+  const Place seg = place(x0, x1, up, lo, want, lane);
+  if (seg.at < 0) return none();
+  if (seg.at % W != wave) return;
+  // the segment's lanes, four tokens each, once more
+  const int k = seg.at / W, i = first + 4 * (k * W * kWave + tid);
+  double w[4], p[4];
+  row.four(i, w, p);
+  double sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < K; ++c) sum = c == k ? mine[c] : sum;
+  double at = seg.before + (upto(sum, lane) - sum);
+  int in = -1, last = -1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const double x = rejected ? w[e] : p[e];
+    at += x;
+    if (x > 0.0) {
+      last = i + e;
+      if (in < 0 && at > want) in = i + e;
+    }
+  }
+  const uint64_t past = __ballot(in >= 0), some = __ballot(last >= 0);
+  const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  const int token = past ? __shfl(in, l, kWave) : __shfl(last, l, kWave);
+  if (lane == 0) found(token);
+}
+
+// The accepted drafts and the padding behind the drawn token.
+__device__ __forceinline__ void write_others(const VerifyArgs& a, int b, int n) {
+  for (int i = threadIdx.x; i <= a.N; i += blockDim.x)
+    if (i != n) a.out[(int64_t)b * (a.N + 1) + i] = i < n ? a.tokens[(int64_t)b * a.N + i] : -1;
 }
 
 template <int DT>
-__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ Draw sh;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const int n = a.accepted[b];
-  bool rejected = n < drafted(a, b);
-  const double2 mine = tid < a.parts ? a.sums[(int64_t)b * a.parts + tid] : double2{0.0, 0.0};
-  double part_sum = rejected ? mine.x : mine.y, total;
-  double lo = before(part_sum, &total, sh);
-  if (rejected && total == 0.0) {
-    // nothing is left of p beside q: the draw is from p
-    rejected = false;
-    part_sum = mine.y;
-    lo = before(part_sum, &total, sh);
-  }
-  const double goal = (double)a.u[(int64_t)b * (a.N + 1) + a.N] * total;
-  const int part = choose(lo + part_sum > goal ? tid : -1, part_sum > 0.0 ? tid : -1, sh);
-  int token = -1;
-  if (part >= 0) {
-    __syncthreads();
-    if (tid == part) sh.wave_sum[0] = lo;
-    __syncthreads();
-    const double base = sh.wave_sum[0];
-    const Weights<DT> row(a, b, n, rejected);
-    const int i = part * kPart + kPerDraw * tid;
-    double w[4], p[4], all;
-    row.four(i, w, p);
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      w[e] = rejected ? w[e] : p[e];
-      sum += w[e];
-    }
-    double at = base + before(sum, &all, sh);
-    int first = -1, last = -1;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      at += w[e];
-      if (w[e] > 0.0) {
-        last = i + e;
-        if (first < 0 && at > goal) first = i + e;
-      }
-    }
-    token = choose(first, last, sh);
-  }
-  for (int i = tid; i <= a.N; i += kDrawThreads)
-    a.out[(int64_t)b * (a.N + 1) + i] =
-        i < n ? a.tokens[(int64_t)b * a.N + i] : i == n ? (int64_t)token : -1;
+__global__ __launch_bounds__(kOneWaves* kWave) void verify_one_kernel(VerifyArgs a) {
+  __shared__ double sums[2][kOneWaves * kOneChunks];
+  const int b = blockIdx.x, lane = threadIdx.x & (kWave - 1);
+  const int has = drafted(a, b);
+  const int n = __builtin_amdgcn_readfirstlane(count_accepted<DT>(a, b, has, lane));
+  if (threadIdx.x == 0) a.accepted[b] = n;
+  write_others(a, b, n);
+  const double u = a.u[(int64_t)b * (a.N + 1) + a.N];
+  int64_t* to = a.out + (int64_t)b * (a.N + 1) + n;
+  bool again = false;
+  auto goal = [&](double all) { return u * all; };
+  auto found = [&](int token) { *to = token; };
+  const bool rejected = n < has;
+  const Weights<DT> row(a, b, n, rejected);
+  draw<DT, kOneWaves, kOneChunks>(row, rejected, 0, 0.0, sums[0], goal, found, [&] { again = true; });
+  if (!again) return;                                    // the same in every wave
+  // nothing is left of p beside q: the draw is from p
+  draw<DT, kOneWaves, kOneChunks>(row, false, 0, 0.0, sums[1], goal, found, [&] {
+    if (threadIdx.x == 0) *to = -1;
+  });
 }
-static_assert(kPerDraw == 4, "a thread draws among four tokens");
 
-inline int64_t verify_parts(int64_t V) { return (V + kPart - 1) / kPart; }
+template <int DT>
+__global__ __launch_bounds__(kSumThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ double sums[kDrawWaves * kDrawChunks];
+  const int b = blockIdx.x, lane = threadIdx.x & (kWave - 1);
+  const int n = a.accepted[b];
+  const double u = a.u[(int64_t)b * (a.N + 1) + a.N];
+  const double2* parts = a.sums + (int64_t)b * a.parts;
+  bool rejected = n < drafted(a, b);
+  write_others(a, b, n);
+  // every wave adds up the parts, 128 at a time, and looks for the draw's
+  double all = 0.0;
+  for (;;) {
+    for (int i = 0; i < a.parts; i += kWave)
+      all += i + lane < a.parts ? (rejected ? parts[i + lane].x : parts[i + lane].y) : 0.0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, kWave);
+    if (all != 0.0 || !rejected) break;
+    rejected = false;                                    // nothing is left of p beside q
+  }
+  const double goal = u * all;
+  Place part{-1, 0.0};
+  double lo = 0.0;
+  for (int i = 0; i < a.parts; i += 2 * kWave) {
+    const int j = i + 2 * lane;
+    const double2 none = {0.0, 0.0};
+    const double2 y0 = j < a.parts ? parts[j] : none, y1 = j + 1 < a.parts ? parts[j + 1] : none;
+    const double x0 = rejected ? y0.x : y0.y, x1 = rejected ? y1.x : y1.y;
+    const double up = upto(x0 + x1, lane), sum = __shfl(up, kWave - 1, kWave);
+    const Place p = place(x0, x1, up, lo, goal, lane);
+    if (p.at >= 0) part = Place{i + p.at, p.before};
+    lo += sum;
+    if (lo > goal) break;
+  }
+  int64_t* to = a.out + (int64_t)b * (a.N + 1) + n;
+  const Weights<DT> row(a, b, n, rejected);
+  auto found = [&](int token) { *to = token; };
+  auto none = [&] {
+    if (threadIdx.x == 0) *to = -1;
+  };
+  if (part.at < 0) return none();
+  draw<DT, kDrawWaves, kDrawChunks>(row, rejected, part.at * kPart, part.before, sums,
+                                    [&](double) { return goal; }, found, none);
+}
+
+// 0: one launch.
+inline int64_t verify_parts(int64_t V) { return V <= kOne ? 0 : (V + kPart - 1) / kPart; }
 
 template <int DT>
 void launch_verify(const VerifyArgs& a, int64_t B, hipStream_t st) {
+  if (a.parts == 0) {
+    hipLaunchKernelGGL(verify_one_kernel<DT>, dim3((unsigned)B), dim3(kOneWaves * kWave), 0, st, a);
+    return;
+  }
   hipLaunchKernelGGL(verify_sum_kernel<DT>, dim3((unsigned)a.parts, (unsigned)B),
                      dim3(kSumThreads), 0, st, a);
-  hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3((unsigned)B), dim3(kDrawThreads), 0, st, a);
+  hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3((unsigned)B), dim3(kSumThreads), 0, st, a);
 }
 
 }  // namespace
@@ -301,8 +381,8 @@ extern "C" int rp_verify_drafts(const int64_t* tokens, const int32_t* lens, int6
     return RP_ERR_INVALID_ARGUMENT;
   }
   const int64_t parts = verify_parts(V);
-  if (!workspace || workspace_bytes < (size_t)(B * parts * 16) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) {
+  if (parts > 0 && (!workspace || workspace_bytes < (size_t)(B * parts * 16) ||
+                    (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) {
     rp_set_error("verify_drafts: workspace of %zu bytes, 256-byte aligned, needed",
                  (size_t)(B * parts * 16));
     return RP_ERR_WORKSPACE;

@@ -1473,22 +1473,27 @@ def verify_drafts(draft_tokens: torch.Tensor, target_probs: torch.Tensor, unifor
         _unit_stride("draft_probs", draft_probs)
     if draft_lens is not None:
         _int32_vector("draft_lens", draft_lens, B)
-    _on_device_of(target_probs, target_probs=target_probs, draft_tokens=draft_tokens,
-                  uniforms=uniforms, draft_probs=draft_probs, draft_lens=draft_lens)
+    dev = target_probs.get_device()
+    if dev < 0 or draft_tokens.get_device() != dev or uniforms.get_device() != dev or \
+            (draft_probs is not None and draft_probs.get_device() != dev) or \
+            (draft_lens is not None and draft_lens.get_device() != dev):
+        _on_device_of(target_probs, target_probs=target_probs, draft_tokens=draft_tokens,
+                      uniforms=uniforms, draft_probs=draft_probs, draft_lens=draft_lens)
     t, u = draft_tokens.contiguous(), uniforms.contiguous()
     tokens = t.new_empty((B, N + 1))
     accepted = t.new_empty((B,), dtype=torch.int32)
     if B > 0:
         n = C.lib().rp_verify_drafts_workspace_bytes(B, V)
-        ws = t.new_empty(n, dtype=torch.uint8)
+        ws = t.new_empty(n, dtype=torch.uint8) if n else None
         q = draft_probs if N > 0 else None
-        C.check(_on_device(
-            target_probs.get_device(), C.lib().rp_verify_drafts, t.data_ptr() if N else None,
+        qsb, qsn = _strides(q, 2) if q is not None else (0, 0)
+        rc = _on_device(
+            dev, C.lib().rp_verify_drafts, t.data_ptr() if N else None,
             draft_lens.data_ptr() if draft_lens is not None else None, B, N,
             target_probs.data_ptr(), *_strides(target_probs, 2),
-            q.data_ptr() if q is not None else None, *(_strides(q, 2) if q is not None else (0, 0)),
-            dt, V, u.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), n,
-            _stream(t)), "rp_verify_drafts")
+            q.data_ptr() if q is not None else None, qsb, qsn, dt, V, u.data_ptr(),
+            tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr() if n else None, n, _stream(t))
+        C.check(rc, "rp_verify_drafts")
     return DraftVerdict(tokens, accepted)
 
 
@@ -1570,8 +1575,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise ValueError("norm_k_weight and out_k come with k")
     yq = _rope_rows("q", q, q, norm_q_weight, out_q)
     yk = _rope_rows("k", k, q, norm_k_weight, out_k) if k is not None else None
-    _on_device_of(q, q=q, k=k, positions=positions, inv_freq=inv_freq, norm_q_weight=norm_q_weight,
-                  norm_k_weight=norm_k_weight, out_q=out_q, out_k=out_k)
+    dev = q.get_device()
+    for t in (q, k, positions, inv_freq, norm_q_weight, norm_k_weight, out_q, out_k):
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            _on_device_of(q, q=q, k=k, positions=positions, inv_freq=inv_freq,
+                          norm_q_weight=norm_q_weight, norm_k_weight=norm_k_weight, out_q=out_q,
+                          out_k=out_k)
     Hkv = k.shape[1] if k is not None else 0
     if B == 0 or S == 0 or H + Hkv == 0:
         return yq, yk
@@ -1579,7 +1588,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     pst = [0, *_strides(positions, 2)] if sections is None else _strides(positions, 3)
     none = (0, 0, 0)
     C.check(_on_device(
-        q.get_device(), C.lib().rp_qk_norm_rope, q.data_ptr(), k.data_ptr() if Hkv else None, dt,
+        dev, C.lib().rp_qk_norm_rope, q.data_ptr(), k.data_ptr() if Hkv else None, dt,
         B, S, H, Hkv, D, *_strides(q, 3), *(_strides(k, 3) if Hkv else none),
         norm_q_weight.data_ptr() if norm_q_weight is not None else None,
         norm_k_weight.data_ptr() if norm_k_weight is not None else None, eps is not None,
