@@ -284,16 +284,16 @@ extern "C" int rp_qk_norm_rope(const void* q, const void* k, int dtype, int64_t 
     rp_set_error("qk_norm_rope: freq must be aligned to its type");
     return RP_ERR_INVALID_ARGUMENT;
   }
+  if (B > 0x7fffffff || S > 0x7fffffff / B || H > 65535 || Hkv > 65535) {
+    rp_set_error("qk_norm_rope: too many tokens or heads");
+    return RP_ERR_UNSUPPORTED;
+  }
   if (!rows_apart(D, {{B, qob}, {H, qoh}, {S, qos}}) ||
       (Hkv > 0 && !rows_apart(D, {{B, kob}, {Hkv, koh}, {S, kos}}))) {
     rp_set_error("qk_norm_rope: output rows overlap");
     return RP_ERR_INVALID_ARGUMENT;
   }
   const int64_t tokens_a_wave = kWave / (D / 16);
-  if (B > 0x7fffffff || S > 0x7fffffff / B || H > 65535 || Hkv > 65535) {
-    rp_set_error("qk_norm_rope: too many tokens or heads");
-    return RP_ERR_UNSUPPORTED;
-  }
   a.rows[0] = RopeRows{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(q_out),
                        static_cast<const uint16_t*>(q_weight), qsb, qsh, qss, qob, qoh, qos};
   a.rows[1] = RopeRows{static_cast<const uint16_t*>(k), static_cast<uint16_t*>(k_out),
