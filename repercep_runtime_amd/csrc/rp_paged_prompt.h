@@ -2,8 +2,9 @@
 // paged key-value cache, causal, within a window, with sinks.
 //
 // Both products run on the matrix cores (32x32x16).  A wave owns 32 rows; a
-// workgroup's waves share tiles of 64 keys, K and V staged in LDS as 16-bit
-// rows, two tiles deep.
+// workgroup's waves share tiles of 64 keys, K and V staged through registers into
+// LDS as 16-bit rows, two tiles deep: any page size, e4m3fn codes converted
+// once for all waves, what no row sees as zeros.
 //
 // * S^T = K Q^T: a lane ends up with 32 scores of one row, so the softmax's
 //   maximum and sum stay in the lane but for its partner in the wave's other
@@ -22,6 +23,18 @@
 // * A row of V that only some of a wave's rows see may hold infinities or NaNs,
 //   which 0 P does not silence.  Sums that come out infinite or NaN are taken
 //   again token by token, V masked for each.
+// * A tile takes a wave 32 matrix instructions (1024 cycles) and about 160 vector
+//   ones; one after the other they took 3000 cycles.  So a tile's weights and
+//   product with V run beside the next tile's scores (fused), in an order that is
+//   written out, since the compiler's own put the LDS reads right before their
+//   uses; and the two waves of a SIMD take turns at that and at staging.  What
+//   each brought, a prompt of 16384 tokens, 32 heads on 8 of 128, bf16:
+//   one phase after the other 2.59 ms, side by side 2.41, in written order 2.22,
+//   in turns and weights spread evenly 2.11-2.20.
+//
+// That is 1.0 to 1.04 PFLOP/s; a library product of 16384^2 reaches 1.39 on this
+// card.  Matrix cores 41% busy, the VALU 42%: what is left are the barriers, at
+// which the halves wait for each other, and a fused phase of 1800 cycles.
 
 #pragma once
 

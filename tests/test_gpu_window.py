@@ -252,6 +252,25 @@ def test_hint_changes_the_split_only(S: int, gpu: torch.device) -> None:
     check(c, q, lens, m, gpu, window=3000, sinks=70)
 
 
+def test_many_ragged_sequences(gpu: torch.device) -> None:
+    """More sequences than lanes, some long enough for several parts."""
+    lens = [1 + 7 * i % 50 for i in range(70)]
+    lens[0], lens[37], lens[69] = 2100, 1500, 1100
+    c = _paged.Cache(lens, 1, 64, 64, "bf16", seed=15)
+    check(c, queries(70, 2, 2, 64, "bf16"), lens, [i % 3 for i in range(70)], gpu)
+    check(c, queries(70, 20, 2, 64, "bf16"), lens, None, gpu, window=1050, sinks=2)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "e4m3"])
+@pytest.mark.parametrize("D,S,G", [(64, 10, 4), (128, 100, 2), (256, 9, 4), (256, 70, 2)])
+def test_row_tiles_of_long_sequences(D: int, S: int, G: int, kind: str, gpu: torch.device) -> None:
+    """Several row tiles and several parts of the keys, the last tile not full."""
+    n = 4200
+    c = _paged.Cache([n], 1, D, 32, kind, seed=16, std=0.7)
+    q = queries(1, G, S, D, "fp16" if kind == "fp16" else "bf16")
+    check(c, q, [n], [S - 1], gpu)
+
+
 def test_one_token_as_decode(gpu: torch.device) -> None:
     """Without a window one token's attention is ``paged_attention_decode``'s, to rounding."""
     for kind in ("bf16", "fp16", "e4m3"):
