@@ -30,11 +30,14 @@
 //   uses; and the two waves of a SIMD take turns at that and at staging.  What
 //   each brought, a prompt of 16384 tokens, 32 heads on 8 of 128, bf16:
 //   one phase after the other 2.59 ms, side by side 2.41, in written order 2.22,
-//   in turns and weights spread evenly 2.11-2.20.
+//   in turns and weights spread evenly 2.11-2.20, the rows of the tile after the
+//   next stored and asked for before the next tile's scores are weighed 2.06-2.12.
 //
-// That is 1.0 to 1.04 PFLOP/s; a library product of 16384^2 reaches 1.39 on this
-// card.  Matrix cores 41% busy, the VALU 42%: what is left are the barriers, at
-// which the halves wait for each other, and a fused phase of 1800 cycles.
+// That is 1.04 to 1.07 PFLOP/s; a library product of 16384^2 reaches 1.39 on this
+// card.  Matrix cores 48% busy, the VALU 51%, no LDS conflicts: what is left are the
+// barriers, at which the halves wait for each other, and a fused phase of 1800
+// cycles.  256 dims run four waves a workgroup, whose 512 registers spill part of Q:
+// 9.2-10.9 ms (0.40-0.48 PFLOP/s).
 
 #pragma once
 
@@ -99,7 +102,10 @@ struct Prompt {
   static constexpr int WROWS = kWave / CPR;             // rows of a wave's chunks
   static constexpr int ROWS = NW * 32;
 
-  // 256 registers a lane, two waves a SIMD, do not hold a wave's rows of Q too.
+  // 256 registers a lane, two waves a SIMD, hold a wave's rows of Q barely or not: read
+  // back from scratch they wait for the staged loads, which the same counter counts.
+  // 16384 tokens of 16-bit rows 2.24 ms with Q in LDS or in registers, of e4m3fn rows
+  // 2.59 and 3.02 (one box; the least of boxes is 2.06 for 16-bit rows).
   static constexpr bool QLDS = D == 128 && NW == 8;
 
   struct alignas(16) Shared {
@@ -438,7 +444,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
         const f32x4 f = P::FP8 ? sf[g % 2] : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
         weight_pair(s, j / 8, j % 8, b0, f[2 * (j % 2)], f[2 * (j % 2) + 1]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (step % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     };
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -538,9 +544,9 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     auto step = [&](int t, int buf, const f32x16* s, f32x16* next) RP_INLINE {
       fused(s, next, buf);
       if constexpr (NW == 8) __syncthreads();
-      weigh(next, buf ^ 1, keys.key(t + 1), q0, !P::FP8);
       put_rows(second ? q2 : q1, second ? q1 : q0);
       const uint64_t here = next_rows();
+      weigh(next, buf ^ 1, keys.key(t + 1), q0, !P::FP8);
       q0 = q1;
       q1 = second ? q2 : here;
       q2 = here;
