@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kFewThreads, D <= 128 ? 2 : 1) void few_kernel(Wind
   const int rows = pl.m * a.group, all = a.S * a.group;
   const int last = min(r0 + 16 * NQ, rows) - 1;
   const int32_t pmin = pl.first + r0 / a.group;
-  const int32_t pmax = last >= r0 ? pl.first + last / a.group : -1;
+  const int32_t pmax = last >= r0 ? max(-1, pl.first + last / a.group) : -1;
   const KeyTiles<kStep> keys = tile_keys<kStep>(a, c, pl, r0, 16 * NQ);
   W w(a, c, keys);
   w.place(threadIdx.x & (kWave - 1), kv);

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   const int32_t pos = live ? pl.first + token : -1;
   // the wave's rows' first and last positions
   const int w0 = r0 + 32 * wave, w1 = min(w0 + 32, rows) - 1;
-  const int32_t pmin = pl.first + w0 / a.group, pmax = w1 >= w0 ? pl.first + w1 / a.group : -1;
+  const int32_t pmin = pl.first + w0 / a.group, pmax = w1 >= w0 ? max(-1, pl.first + w1 / a.group) : -1;
   const KeyTiles<kTile> keys = tile_keys<kTile>(a, c, pl, r0, P::ROWS);
   const int t0 = (int)((int64_t)keys.count * split / a.splits);
   const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
@@ -300,9 +300,9 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     if (!whole) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int32_t j = kb + 32 * k + 4 * h;
-        seen[k] = (uint32_t)(here >> 32 * k) >> 4 * h & bits_up_to(pos - j) &
-                  (~bits_up_to(pos - a.window - j) | bits_up_to(a.sinks - 1 - j));
+        const int32_t j = kb + 32 * k + 4 * h, d = max(-1, pos - j);
+        seen[k] = (uint32_t)(here >> 32 * k) >> 4 * h & bits_up_to(d) &
+                  (~bits_up_to(d - a.window) | bits_up_to(a.sinks - 1 - j));
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           s[k][i] = seen[k] & 1u << (8 * (i / 4) + i % 4) ? s[k][i] : neg_inf();

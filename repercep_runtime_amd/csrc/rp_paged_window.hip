@@ -2,6 +2,8 @@
 // kernel takes a call, how its keys are split, the join of the parts, and the
 // entry point.
 
+#include <algorithm>
+
 #include "rp_paged_window.h"
 
 namespace rp {
@@ -89,6 +91,7 @@ struct Layout : WindowLaunch {
   size_t ml, total;                                     // byte offsets: parts first
 };
 
+// (std::min on the host: HIP's own takes int there.)
 inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cache* c,
                             int64_t window, int64_t sinks, int64_t max_seq_len) {
   const int64_t cap = c->max_pages * c->page_size, group = H / c->heads;
@@ -107,9 +110,10 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
   const int64_t rows = l.columns ? 16 * l.columns : 32 * l.waves;
   l.tiles = (all + rows - 1) / rows;
   // a tile's keys: its tokens', the window's before them, the sinks
-  const int64_t tokens = min(S, rows / group + 2);
+  const int64_t tokens = std::min(S, rows / group + 2);
   int64_t keys = longest;
-  if (window > 0 && window + sinks + tokens < keys) keys = window + sinks + tokens;
+  const int64_t past = std::min(window, longest) + std::min(sinks, longest);
+  if (window > 0 && past + tokens < keys) keys = past + tokens;
   const int64_t blocks = groups * l.tiles;
   l.room = 0;
   l.stream = false;
@@ -118,7 +122,7 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
     // a window are alike, so one workgroup a CU is enough: 256 groups of 1056 keys
     // 27 us unsplit, 32 in two parts.
     l.room = kFewGroups / (c->heads * l.tiles);
-    l.splits = min(min(1 + l.room - B, 4 * ((l.room + B - 1) / B)), keys * key_bytes / kFewPartBytes);
+    l.splits = std::min({1 + l.room - B, 4 * ((l.room + B - 1) / B), keys * key_bytes / kFewPartBytes});
     if (keys < longest && blocks >= kFewGroups / 2) l.splits = 1;
     // a second row tile finds V in the caches
     l.stream = l.tiles == 1 && groups * keys * key_bytes > kStreamBytes;
@@ -128,9 +132,9 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
     // One workgroup a CU; two where tiles of a prompt see few keys and many: 4096
     // tokens on one kv head 113 us unsplit, 81 in four parts.
     l.splits = keys >= 4 * S ? kPromptGroups / blocks : (2 * kPromptGroups + blocks - 1) / blocks;
-    l.splits = min(l.splits, keys / kPromptPartKeys);
+    l.splits = std::min(l.splits, keys / kPromptPartKeys);
   }
-  l.splits = max((int64_t)1, min(l.splits, kMaxSplits));
+  l.splits = std::max((int64_t)1, std::min(l.splits, kMaxSplits));
   const int64_t parts = l.splits > 1 ? B * H * S * l.splits : 0;
   l.ml = (size_t)(parts * c->head_dim * 4);
   l.total = l.ml + (size_t)(parts * 8);
@@ -240,7 +244,7 @@ extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64
       ? kSlack - 15.0f
       : kSlack + (float)(64 - __builtin_clzll((unsigned long long)c.capacity()));
   a.window = window == 0 || window > 0x7fffffff ? 0x7fffffff : (int32_t)window;
-  a.sinks = (int32_t)min(sinks, (int64_t)0x7fffffff);
+  a.sinks = (int32_t)std::min(sinks, (int64_t)0x7fffffff);
   a.out = static_cast<uint16_t*>(out);
   a.osb = osb;
   a.osh = osh;

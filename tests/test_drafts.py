@@ -131,6 +131,16 @@ def test_split_calls_ask_for_a_workspace() -> None:
     assert L.rp_verify_drafts_workspace_bytes(4, (1 << 22) + 1) == 0
 
 
+def test_windows_and_sinks_past_every_length() -> None:
+    """Sizes that 32 or 64 bits do not add up: the window takes all keys."""
+    L = _capi.lib()
+    c = test_paged.cache(max_pages=4096, num_pages=4096, table_stride=4096)
+    for S in (1, 200):
+        n = L.rp_paged_window_workspace_bytes(1, 4, S, c, 0, 0, 0)
+        for window, sinks in ((2 ** 63 - 1, 2 ** 63 - 1), (2 ** 32, 0), (16, 2 ** 32)):
+            assert L.rp_paged_window_workspace_bytes(1, 4, S, c, window, sinks, 0) == n
+
+
 def _step() -> dict:
     return {"q": torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16),
             "k_cache": torch.zeros(8, 2, 16, 64, dtype=torch.bfloat16),

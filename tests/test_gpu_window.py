@@ -106,6 +106,23 @@ def test_lengths_at_the_edges(S: int, gpu: torch.device) -> None:
     check(c, queries(5, 4, S, 64, "bf16"), [0, 1, 5, 70, 64], None, gpu, window=12, sinks=3)
 
 
+@pytest.mark.parametrize("S", [3, 90])
+def test_windows_and_sinks_past_every_length(S: int, gpu: torch.device) -> None:
+    """Also where tokens stand before the first row."""
+    c = _paged.Cache([600, 64, 64], 2, 64, 16, "bf16", seed=4)
+    q = queries(3, 4, S, 64, "bf16")
+    for window, sinks in ((2 ** 31 - 1, 2 ** 31 - 1), (2 ** 62, 0), (7, 2 ** 32)):
+        check(c, q, [600, 2, 64], None, gpu, window, sinks)
+
+
+@pytest.mark.parametrize("S", [3, 90])
+def test_largest_lengths(S: int, gpu: torch.device) -> None:
+    """Tokens far behind the table's last position see all of its rows."""
+    c = _paged.Cache([64, 64], 2, 64, 16, "bf16", seed=5)
+    check(c, queries(2, 4, S, 64, "bf16"), [2 ** 31 - 1, 2 ** 31 - 1], [S, 1], gpu)
+    check(c, queries(2, 4, S, 64, "bf16"), [2 ** 31 - 1, 64], None, gpu, window=9, sinks=3)
+
+
 @pytest.mark.parametrize("S", [3, 66])
 def test_given_away_pages(S: int, gpu: torch.device) -> None:
     """Pages between the sinks and the window that no token sees: their entries
