@@ -1497,24 +1497,34 @@ def verify_drafts(draft_tokens: torch.Tensor, target_probs: torch.Tensor, unifor
     return DraftVerdict(tokens, accepted)
 
 
-def _rope_rows(name: str, x: torch.Tensor, like: torch.Tensor, weight: torch.Tensor | None,
-               out: torch.Tensor | None) -> torch.Tensor:
-    """The output for the rows ``x``, both and the weight checked."""
-    if x.dim() != 4 or (x.shape[0], *x.shape[2:]) != (like.shape[0], *like.shape[2:]):
-        raise ValueError(f"{name} {tuple(x.shape)} must be (B, heads, S, D) with q's B, S and D")
-    if x.dtype != like.dtype:
-        raise TypeError(f"{name} is {x.dtype}, q {like.dtype}")
-    _unit_stride(name, x)
-    if weight is not None and (weight.shape != (x.shape[3],) or weight.dtype != x.dtype
+def _outer(shape: tuple[int, ...], strides: tuple[int, ...]) -> tuple[int, int, int]:
+    """``_strides`` of a 4-dimensional tensor's first three."""
+    return (strides[0] if shape[0] > 1 else 0, strides[1] if shape[1] > 1 else 0,
+            strides[2] if shape[2] > 1 else 0)
+
+
+def _rope_rows(name: str, x: torch.Tensor, lead: tuple[int, int, int], dtype: torch.dtype,
+               weight: torch.Tensor | None, out: torch.Tensor | None
+               ) -> tuple[torch.Tensor, tuple[int, int, int], tuple[int, int, int]]:
+    """The output for the rows ``x`` and both's strides, all and the weight checked."""
+    shape = x.shape
+    if len(shape) != 4 or (shape[0], shape[2], shape[3]) != lead:
+        raise ValueError(f"{name} {tuple(shape)} must be (B, heads, S, D) with q's B, S and D")
+    if x.dtype != dtype:
+        raise TypeError(f"{name} is {x.dtype}, q {dtype}")
+    st = x.stride()
+    if st[3] != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    B, H, S, D = shape
+    if weight is not None and (weight.shape != (D,) or weight.dtype != dtype
                                or not weight.is_contiguous()):
-        raise ValueError(f"norm_{name}_weight must be a contiguous ({x.shape[3]},) {x.dtype} vector")
+        raise ValueError(f"norm_{name}_weight must be a contiguous ({D},) {dtype} vector")
     if out is None:
-        B, H, S, D = x.shape
-        return x.new_empty((B, H, S, D))
-    if out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError(f"out_{name} must be {tuple(x.shape)} {x.dtype}")
+        return x.new_empty(B, H, S, D), _outer(shape, st), (H * S * D, S * D, D)
+    if out.shape != shape or out.dtype != dtype:
+        raise ValueError(f"out_{name} must be {tuple(shape)} {dtype}")
     _unit_stride(f"out_{name}", out)
-    return out
+    return out, _outer(shape, st), _outer(shape, out.stride())
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
@@ -1573,8 +1583,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise ValueError(f"eps must be finite and not negative (got {eps})")
     if k is None and (norm_k_weight is not None or out_k is not None):
         raise ValueError("norm_k_weight and out_k come with k")
-    yq = _rope_rows("q", q, q, norm_q_weight, out_q)
-    yk = _rope_rows("k", k, q, norm_k_weight, out_k) if k is not None else None
+    yq, q_st, yq_st = _rope_rows("q", q, (B, S, D), q.dtype, norm_q_weight, out_q)
+    yk = None
+    if k is not None:
+        yk, k_st, yk_st = _rope_rows("k", k, (B, S, D), q.dtype, norm_k_weight, out_k)
     dev = q.get_device()
     for t in (q, k, positions, inv_freq, norm_q_weight, norm_k_weight, out_q, out_k):
         if t is not None and (dev < 0 or t.get_device() != dev):
@@ -1584,18 +1596,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     Hkv = k.shape[1] if k is not None else 0
     if B == 0 or S == 0 or H + Hkv == 0:
         return yq, yk
+    if Hkv == 0:
+        k_st = yk_st = (0, 0, 0)
     counts = sections if sections is not None else (pairs,)
     pst = [0, *_strides(positions, 2)] if sections is None else _strides(positions, 3)
-    none = (0, 0, 0)
     C.check(_on_device(
         dev, C.lib().rp_qk_norm_rope, q.data_ptr(), k.data_ptr() if Hkv else None, dt,
-        B, S, H, Hkv, D, *_strides(q, 3), *(_strides(k, 3) if Hkv else none),
+        B, S, H, Hkv, D, *q_st, *k_st,
         norm_q_weight.data_ptr() if norm_q_weight is not None else None,
         norm_k_weight.data_ptr() if norm_k_weight is not None else None, eps is not None,
         eps if eps is not None else 0.0, positions.data_ptr(), *pst, inv_freq.data_ptr(),
         inv_freq.dtype == torch.float64, 2 * pairs, C.pack_sections(counts), len(counts), mode,
-        yq.data_ptr(), *_strides(yq, 3), yk.data_ptr() if Hkv else None,
-        *(_strides(yk, 3) if Hkv else none), _stream(q)), "rp_qk_norm_rope")
+        yq.data_ptr(), *yq_st, yk.data_ptr() if Hkv else None, *yk_st, _stream(q)),
+        "rp_qk_norm_rope")
     return yq, yk
 
 
