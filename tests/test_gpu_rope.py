@@ -139,6 +139,20 @@ def test_empty(gpu: torch.device) -> None:
         assert y.shape == (B, 2, S, 64) and z.shape == (B, 1, S, 64)
 
 
+def test_no_key_heads_and_one_row_for_all_tokens(gpu: torch.device) -> None:
+    """A k of no heads, whose strides mean nothing; q rows that share memory."""
+    c = make(2, 3, 1, 6, 64, 32, "bf16")
+    c["q"] = c["q"][:, :, :1].expand(2, 3, 6, 64)
+    q = c["q"][:, :, :1].to(gpu).expand(2, 3, 6, 64)
+    k = torch.empty((2, 0, 6, 67), dtype=torch.bfloat16, device=gpu)[..., 1:65]
+    y, z = call(c, gpu, "half", 1e-6, q=q, k=k)
+    assert z.shape == (2, 0, 6, 64)
+    c["k"] = c["wk"] = None
+    check(c, (y, None), "half", 1e-6)
+    with pytest.raises(RuntimeError, match="overlap"):
+        call(c, gpu, "half", 1e-6, q=q, out_q=q)
+
+
 def test_many_tokens(gpu: torch.device) -> None:
     """More row groups than one round of workgroups; checked at the ends."""
     c = make(1, 2, 1, 40001, 128, 64, "bf16")
