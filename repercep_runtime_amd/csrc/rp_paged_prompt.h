@@ -2,7 +2,7 @@
 // paged key-value cache, causal, within a window, with sinks.
 //
 // Both products run on the matrix cores (32x32x16).  A wave owns 32 rows; a
-// workgroup's waves share tiles of 64 keys, K and V staged through registers into
+// workgroup's waves share tiles of 64 keys (32 at 256 dims), K and V staged through registers into
 // LDS as 16-bit rows, two tiles deep: any page size, e4m3fn codes converted
 // once for all waves, what no row sees as zeros.
 //
@@ -36,8 +36,8 @@
 // That is 1.04 to 1.07 PFLOP/s; a library product of 16384^2 reaches 1.39 on this
 // card.  Matrix cores 48% busy, the VALU 51%, no LDS conflicts: what is left are the
 // barriers, at which the halves wait for each other, and a fused phase of 1800
-// cycles.  256 dims run four waves a workgroup, whose 512 registers spill part of Q:
-// 9.2-10.9 ms (0.40-0.48 PFLOP/s).
+// cycles.  256 dims, four waves a workgroup and so one a SIMD, take 6.4 ms (0.68
+// PFLOP/s).
 
 #pragma once
 
@@ -50,7 +50,6 @@
 namespace rp {
 namespace {
 
-constexpr int kTile = 64;                       // keys a tile: one page entry a lane
 constexpr int kAhead = 4;                       // matrix instructions that LDS reads are ahead
 
 template <bool F16>
@@ -94,24 +93,29 @@ struct Prompt {
   static constexpr int PARTS = FP8 && QF16 ? 2 : 1;     // of a weight
   static constexpr int EB = FP8 ? 1 : 2, NT = NW * kWave;
   static constexpr int QSTEPS = D / 16, DB = D / 32;
+  // Keys a tile, up to one page entry a lane, in blocks of 32.  At 256 dims a wave's
+  // sums and Q leave no registers, and LDS no room, for 64: Q spilled, and 16384
+  // tokens took 9.5 ms, with 32 6.4.
+  static constexpr int TILE = D == 256 ? 32 : 64, KB = TILE / 32;
+  static constexpr uint64_t ALL = ~0ull >> (64 - TILE);
   // Rows of LDS, without bank conflicts: eight rows of K at one column are read
   // at a time, four rows of V's 64 bytes.
   static constexpr int LDK = D + 8, LDV = D == 32 ? 32 : D + 32;
   static constexpr int CPR = D * EB / 16;               // 16-byte chunks a row
-  static constexpr int NCH = (kTile * CPR + NT - 1) / NT;
+  static constexpr int NCH = (TILE * CPR + NT - 1) / NT;
   static constexpr int WROWS = kWave / CPR;             // rows of a wave's chunks
   static constexpr int ROWS = NW * 32;
 
-  // 256 registers a lane, two waves a SIMD, hold a wave's rows of Q barely or not: read
+  // Q in LDS: 256 registers a lane, two waves a SIMD, hold it barely or not, read
   // back from scratch they wait for the staged loads, which the same counter counts.
   // 16384 tokens of 16-bit rows 2.24 ms with Q in LDS or in registers, of e4m3fn rows
-  // 2.59 and 3.02 (one box; the least of boxes is 2.06 for 16-bit rows).
-  static constexpr bool QLDS = D == 128 && NW == 8;
+  // 2.59 and 3.02.
+  static constexpr bool QLDS = D == 256 || (D == 128 && NW == 8);
 
   struct alignas(16) Shared {
-    uint16_t k[2][kTile][LDK];
-    uint16_t v[2][kTile][LDV];
-    float ks[2][kTile], vs[2][kTile];                   // e4m3fn only
+    uint16_t k[2][TILE][LDK];
+    uint16_t v[2][TILE][LDV];
+    float ks[2][TILE], vs[2][TILE];                   // e4m3fn only
     uint16_t q[QLDS ? ROWS : 1][LDK];
     int redo;
   };
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   // the wave's rows' first and last positions
   const int w0 = r0 + 32 * wave, w1 = min(w0 + 32, rows) - 1;
   const int32_t pmin = pl.first + w0 / a.group, pmax = w1 >= w0 ? max(-1, pl.first + w1 / a.group) : -1;
-  const KeyTiles<kTile> keys = tile_keys<kTile>(a, c, pl, r0, P::ROWS);
+  const KeyTiles<P::TILE> keys = tile_keys<P::TILE>(a, c, pl, r0, P::ROWS);
   const int t0 = (int)((int64_t)keys.count * split / a.splits);
   const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
   const int32_t* table = c.table + b * c.table_stride;
@@ -172,8 +176,8 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
   // the lane's part of a K operand: the key m of 32, dims 16 t + 8 h .. + 7
   const uint32_t klds = lds_address(&sh.k[0][m][8 * h]);
-  auto k_frag = [&](int buf, int n) RP_INLINE -> u32x4 {     // of keys 32 (n % 2) .., t = n / 2
-    return lds_read16(klds + 2 * ((buf * kTile + 32 * (n % 2)) * P::LDK + 16 * (n / 2)));
+  auto k_frag = [&](int buf, int n) RP_INLINE -> u32x4 {     // of keys 32 (n % KB) .., t = n / KB
+    return lds_read16(klds + 2 * ((buf * P::TILE + 32 * (n % P::KB)) * P::LDK + 16 * (n / P::KB)));
   };
 
   f32x16 acc[P::DB];
@@ -189,7 +193,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
   // the page, or -1 where there is none
   auto page_of = [&](int t, int32_t e) RP_INLINE -> int32_t {
-    return t < t1 && keys.key(t) + lane < keys.hi && e >= 0 && e < c.num_pages ? e : -1;
+    return t < t1 && lane < P::TILE && keys.key(t) + lane < keys.hi && e >= 0 && e < c.num_pages ? e : -1;
   };
   // which keys of tile t any of the workgroup's rows sees
   auto present = [&](int t, int32_t pages) RP_INLINE -> uint64_t {
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     const int lo = (int)off, hi = (int)(off >> 32);
 #pragma unroll
     for (int i = 0; i < P::NCH; ++i) {
-      const int rw = min(wave * P::WROWS + i * (P::NT / P::CPR), kTile - P::WROWS);
+      const int rw = min(wave * P::WROWS + i * (P::NT / P::CPR), P::TILE - P::WROWS);
       if constexpr (decltype(one)::value) {
         const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, rw) << 32 |
                             (uint32_t)__builtin_amdgcn_readlane(lo, rw);
@@ -237,10 +241,10 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
 #pragma unroll
     for (int i = 0; i < P::NCH; ++i) {
       const int ch = tid + i * P::NT;
-      if (kTile * P::CPR % P::NT != 0 && ch >= kTile * P::CPR) break;
+      if (P::TILE * P::CPR % P::NT != 0 && ch >= P::TILE * P::CPR) break;
       const int r = ch / P::CPR;
       u32x4 x = from[i];
-      if (here != ~0ull) x &= here >> r & 1 ? 0xffffffffu : 0u;
+      if (here != P::ALL) x &= here >> r & 1 ? 0xffffffffu : 0u;
       if constexpr (!P::FP8) {
         *reinterpret_cast<u32x4*>(to + r * ld + ch % P::CPR * 8) = x;
       } else {
@@ -260,13 +264,13 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   auto store_k = [&](int buf, uint64_t here) RP_INLINE {
     store(&sh.k[buf][0][0], P::LDK, kreg, here, std::bool_constant<P::QF16>{});
     if constexpr (P::FP8) {
-      if (wave == 0) sh.ks[buf][lane] = here >> lane & 1 ? ksreg * a.c : 0.0f;
+      if (wave == 0 && lane < P::TILE) sh.ks[buf][lane] = here >> lane & 1 ? ksreg * a.c : 0.0f;
     }
   };
   auto store_v = [&](int buf, uint64_t here) RP_INLINE {
     store(&sh.v[buf][0][0], P::LDV, vreg, here, std::false_type{});
     if constexpr (P::FP8) {
-      if (wave == 1) sh.vs[buf][lane] = here >> lane & 1 ? vsreg : 0.0f;
+      if (wave == 1 && lane < P::TILE) sh.vs[buf][lane] = here >> lane & 1 ? vsreg : 0.0f;
     }
   };
 
@@ -274,20 +278,25 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   const float c1 = P::FP8 ? 1.0f : a.c;
   auto product = [&](int buf, f32x16* to) RP_INLINE {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) to[0][i] = to[1][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) to[0][i] = to[P::KB - 1][i] = 0.0f;
 #pragma unroll
-    for (int n = 0; n < 2 * P::QSTEPS; ++n)
-      to[n % 2] = mma32<P::QF16>(k_frag(buf, n), q_frag(n / 2), to[n % 2]);
+    for (int n = 0; n < P::KB * P::QSTEPS; ++n)
+      to[n % P::KB] = mma32<P::QF16>(k_frag(buf, n), q_frag(n / P::KB), to[n % P::KB]);
   };
-  uint32_t seen[2];                                      // bit 8 i + e: key 8 i + 4 h + e
+  uint32_t seen[P::KB];                                      // bit 8 i + e: key 8 i + 4 h + e
   bool whole;
   float top;
+  auto larger = [&](const f32x16* s, int i) RP_INLINE {   // top, of scores i of each block too
+    if (i == 0) top = s[0][0];
+    else top = __builtin_elementwise_maximum(top, s[0][i]);
+    if constexpr (P::KB == 2) top = __builtin_elementwise_maximum(top, s[1][i]);
+  };
   // Masks the scores s of the tile at kb and finds their largest (`found`: it
   // is, unless some are masked).
   auto weigh = [&](f32x16* s, int buf, int32_t kb, uint64_t here, bool found) RP_INLINE {
     if constexpr (P::FP8) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < P::KB; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const f32x4 f = *reinterpret_cast<const f32x4*>(&sh.ks[buf][32 * k + 8 * i + 4 * h]);
@@ -295,11 +304,11 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
           for (int e = 0; e < 4; ++e) s[k][4 * i + e] *= f[e];
         }
     }
-    whole = here == ~0ull && kb + kTile - 1 <= pmin &&
-            (kb > pmax - a.window || kb + kTile <= a.sinks);
+    whole = here == P::ALL && kb + P::TILE - 1 <= pmin &&
+            (kb > pmax - a.window || kb + P::TILE <= a.sinks);
     if (!whole) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < P::KB; ++k) {
         const int32_t j = kb + 32 * k + 4 * h, d = max(-1, pos - j);
         seen[k] = (uint32_t)(here >> 32 * k) >> 4 * h & bits_up_to(d) &
                   (~bits_up_to(d - a.window) | bits_up_to(a.sinks - 1 - j));
@@ -310,10 +319,8 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     }
     if (!whole || !found) {
       // of a row with a NaN a NaN, which moves no base: the row is NaN
-      top = __builtin_elementwise_maximum(s[0][0], s[1][0]);
 #pragma unroll
-      for (int i = 1; i < 16; ++i)
-        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][i]), s[1][i]);
+      for (int i = 0; i < 16; ++i) larger(s, i);
     }
     top *= c1;
     if (__any(top > base + (kSlack - a.lift))) {
@@ -328,7 +335,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
 
   // ---- P from s, and its product with V
-  uint32_t p[P::PARTS][2][8];
+  uint32_t p[P::PARTS][P::KB][8];
   // Weights 2 j, 2 j + 1 of block k (of 16), about the base b0, f their scales.
   auto weight_pair = [&](const f32x16* s, int k, int j, float b0, float f0, float f1) RP_INLINE {
     float u = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][2 * j], c1, -b0));
@@ -359,7 +366,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   auto weights = [&](const f32x16* s, int buf) RP_INLINE {
     const float b0 = weight_base();
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
+    for (int g = 0; g < 4 * P::KB; ++g) {
       f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
       if constexpr (P::FP8) f = scales(buf, g);
       weight_pair(s, g / 4, 2 * (g % 4), b0, f[0], f[1]);
@@ -373,7 +380,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       lds_address(&sh.v[0][4 * h + (l16 >> 2)][(lane >> 4 & 1) * 16 + (l16 & 3) * 4]);
   auto v_frag = [&](int buf, int n) RP_INLINE -> u32x4 {
     const uint32_t at =
-        vlds + 2 * ((buf * kTile + 16 * (n / P::DB)) * P::LDV + 32 * (n % P::DB));
+        vlds + 2 * ((buf * P::TILE + 16 * (n / P::DB)) * P::LDV + 32 * (n % P::DB));
     const u32x2 lo = column4(at), hi = column4(at + 2 * 8 * P::LDV);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
   auto values = [&](int buf) RP_INLINE {
 #pragma unroll
-    for (int n = 0; n < 4 * P::DB; ++n) {
+    for (int n = 0; n < 2 * P::KB * P::DB; ++n) {
       const u32x4 f = v_frag(buf, n);
 #pragma unroll
       for (int e = 0; e < P::PARTS; ++e)
@@ -395,7 +402,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     for (int32_t at = pmin; at <= pmax; ++at) {
       const bool mine = pos == at;
 #pragma unroll
-      for (int n = 0; n < 4 * P::DB; ++n) {
+      for (int n = 0; n < 2 * P::KB * P::DB; ++n) {
         u32x4 f = v_frag(buf, n);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -419,27 +426,29 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   // scores: matrix instructions one by one, each with the LDS reads of the one
   // kAhead later and a share of the vector work, in the order written.
   auto fused = [&](const f32x16* s, f32x16* next, int buf) RP_INLINE {
-    constexpr int NK = 2 * P::QSTEPS, NV = 4 * P::DB;
-    u32x4 kf[kAhead], vf[kAhead], qf[2];
+    constexpr int NK = P::KB * P::QSTEPS, NV = 2 * P::KB * P::DB;
+    constexpr int QA = P::KB == 2 ? 2 : 4;               // Q's operands in registers
+    u32x4 kf[kAhead], vf[kAhead], qf[QA];
     f32x4 sf[2];
     const float b0 = weight_base();
     __builtin_amdgcn_s_setprio(1);                       // before the half that stages
     if constexpr (P::FP8) sf[0] = scales(buf, 0);
-    qf[0] = q_frag(0);
+#pragma unroll
+    for (int t = 0; t < QA - 1; ++t) qf[t] = q_frag(t);
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) kf[n] = k_frag(buf ^ 1, n);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) next[0][i] = next[1][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) next[0][i] = next[P::KB - 1][i] = 0.0f;
     // The pairs of weights evenly over the steps before the product that asks for
     // the last of them, each in time for its own.
     auto some_weights = [&](int step) RP_INLINE {
       constexpr int T = NK + 3 * NV / 4;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (2 * j * T / 33 != step) continue;
+      for (int j = 0; j < 8 * P::KB; ++j) {
+        if (2 * j * T / (16 * P::KB + 1) != step) continue;
         const int g = j / 2;
         if constexpr (P::FP8) {
-          if (j % 2 == 0 && g + 1 < 8) sf[(g + 1) % 2] = scales(buf, g + 1);
+          if (j % 2 == 0 && g + 1 < 4 * P::KB) sf[(g + 1) % 2] = scales(buf, g + 1);
         }
         const f32x4 f = P::FP8 ? sf[g % 2] : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
         weight_pair(s, j / 8, j % 8, b0, f[2 * (j % 2)], f[2 * (j % 2) + 1]);
@@ -449,8 +458,9 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-      if (n % 2 == 0 && n / 2 + 1 < P::QSTEPS) qf[(n / 2 + 1) % 2] = q_frag(n / 2 + 1);
-      next[n % 2] = mma32<P::QF16>(kf[n % kAhead], qf[n / 2 % 2], next[n % 2]);
+      const int t = n / P::KB, later = t + QA - 1;
+      if (n % P::KB == 0 && later < P::QSTEPS) qf[later % QA] = q_frag(later);
+      next[n % P::KB] = mma32<P::QF16>(kf[n % kAhead], qf[t % QA], next[n % P::KB]);
       if (n + kAhead < NK) kf[n % kAhead] = k_frag(buf ^ 1, n + kAhead);
       else vf[(n + kAhead - NK) % kAhead] = v_frag(buf, n + kAhead - NK);
       some_weights(n);
@@ -463,9 +473,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       if (n + kAhead < NV) vf[n % kAhead] = v_frag(buf, n + kAhead);
       if constexpr (!P::FP8) {
 #pragma unroll
-        for (int i = 16 * n / NV; i < 16 * (n + 1) / NV; ++i)
-          top = i == 0 ? __builtin_elementwise_maximum(next[0][0], next[1][0])
-                       : __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[0][i]), next[1][i]);
+        for (int i = 16 * n / NV; i < 16 * (n + 1) / NV; ++i) larger(next, i);
       }
       some_weights(NK + n);
     }
@@ -517,7 +525,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       store_k((tk - t0) & 1, here);
       store_v((tk - t0 + 1) & 1, before);
     };
-    f32x16 even[2], odd[2];                              // the tiles' scores in turn
+    f32x16 even[P::KB], odd[P::KB];                              // the tiles' scores in turn
     {
       page = page_of(t0, entry(t0));
       off = offset_of(t0, page);
@@ -583,7 +591,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       store_k(0, here);
       store_v(0, here);
       __syncthreads();
-      f32x16 s[2];
+      f32x16 s[P::KB];
       product(0, s);
       weigh(s, 0, keys.key(t), here, false);
       weights(s, 0);
