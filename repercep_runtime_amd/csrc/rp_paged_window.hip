@@ -83,8 +83,12 @@ constexpr int64_t kFewGroups = 512;
 constexpr int64_t kFewPartBytes = 128 << 10;
 
 // prompt_kernel: workgroups that fill the card (its LDS and registers hold one a
-// CU), and the keys that are worth a part of their own.
-constexpr int64_t kPromptGroups = 256, kPromptPartKeys = 1024;
+// CU), and the keys that are worth a part of their own: 256 where all rows see
+// nearly all of them, 512 where a prompt's tiles see from few to all.  64 tokens of
+// 2000 keys, 8 kv heads, 60 us in parts of 1024, 33 of 512, 28 of 256, 30 of 128;
+// prompts of 512 tokens 22 us unsplit, 32 in parts of 256; of 2048, 2 kv heads, 53,
+// 43 and 54 us in parts of 1024, 512 and 256.
+constexpr int64_t kPromptGroups = 256, kPromptPartKeys = 512, kAfterPartKeys = 256;
 
 struct Layout : WindowLaunch {
   int64_t tiles, splits, room;
@@ -131,8 +135,9 @@ inline Layout window_layout(int64_t B, int64_t H, int64_t S, const rp_paged_cach
   } else {
     // One workgroup a CU; two where tiles of a prompt see few keys and many: 4096
     // tokens on one kv head 113 us unsplit, 81 in four parts.
-    l.splits = keys >= 4 * S ? kPromptGroups / blocks : (2 * kPromptGroups + blocks - 1) / blocks;
-    l.splits = std::min(l.splits, keys / kPromptPartKeys);
+    l.splits = keys >= 4 * S
+        ? std::min(kPromptGroups / blocks, keys / kAfterPartKeys)
+        : std::min((2 * kPromptGroups + blocks - 1) / blocks, keys / kPromptPartKeys);
   }
   l.splits = std::max((int64_t)1, std::min(l.splits, kMaxSplits));
   const int64_t parts = l.splits > 1 ? B * H * S * l.splits : 0;

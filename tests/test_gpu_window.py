@@ -288,6 +288,18 @@ def test_row_tiles_of_long_sequences(D: int, S: int, G: int, kind: str, gpu: tor
     check(c, q, [n], [S - 1], gpu)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "bf16-e4m3", "fp16-e4m3"])
+@pytest.mark.parametrize("D", [32, 128, 256])
+def test_chunks_in_short_parts(D: int, kind: str, gpu: torch.device) -> None:
+    """A chunk after four parts' keys, beside a sequence that leaves parts empty;
+    a prompt of its own in two."""
+    dtype, cache = kind.split("-") if "-" in kind else (kind, kind)
+    c = _paged.Cache([1105, 90], 2, D, 16, cache, seed=D)
+    check(c, queries(2, 4, 70, D, dtype), [1105, 90], [70, 41], gpu)
+    check(c, queries(2, 4, 70, D, dtype), [1105, 90], [70, 41], gpu, window=700, sinks=33)
+    check(c, queries(2, 4, 280, D, dtype), [1105, 90], [280, 90], gpu)
+
+
 def test_one_token_as_decode(gpu: torch.device) -> None:
     """Without a window one token's attention is ``paged_attention_decode``'s, to rounding."""
     for kind in ("bf16", "fp16", "e4m3"):
