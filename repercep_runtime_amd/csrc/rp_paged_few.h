@@ -230,7 +230,7 @@ struct Few : StepRows<QT == kInF16, CT, D, STREAM> {
           }
       } else {
         // one token at a time, V as that token sees it
-        for (int32_t at = pmin; at <= pmax; ++at) {
+        for (int32_t at = max(0, pmin); at <= pmax; ++at) {
           uint32_t mask[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kFewThreads, D <= 128 ? 2 : 1) void few_kernel(Wind
   const Place pl(a, b);
   const int rows = pl.m * a.group, all = a.S * a.group;
   const int last = min(r0 + 16 * NQ, rows) - 1;
-  const int32_t pmin = pl.first + r0 / a.group;
+  const int32_t pmin = last >= r0 ? pl.first + r0 / a.group : 0x7fffffff;   // see prompt_kernel
   const int32_t pmax = last >= r0 ? max(-1, pl.first + last / a.group) : -1;
   const KeyTiles<kStep> keys = tile_keys<kStep>(a, c, pl, r0, 16 * NQ);
   W w(a, c, keys);

@@ -150,9 +150,11 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   const bool live = row < rows;
   const int64_t orow = ((int64_t)b * a.H + head) * a.S + token;
   const int32_t pos = live ? pl.first + token : -1;
-  // the wave's rows' first and last positions
+  // the wave's rows' first and last positions (no row: the largest number and -1,
+  // between which no pass over positions has a step)
   const int w0 = r0 + 32 * wave, w1 = min(w0 + 32, rows) - 1;
-  const int32_t pmin = pl.first + w0 / a.group, pmax = w1 >= w0 ? max(-1, pl.first + w1 / a.group) : -1;
+  const int32_t pmin = w1 >= w0 ? pl.first + w0 / a.group : 0x7fffffff;
+  const int32_t pmax = w1 >= w0 ? max(-1, pl.first + w1 / a.group) : -1;
   const KeyTiles<P::TILE> keys = tile_keys<P::TILE>(a, c, pl, r0, P::ROWS);
   const int t0 = (int)((int64_t)keys.count * split / a.splits);
   const int t1 = (int)((int64_t)keys.count * (split + 1) / a.splits);
@@ -399,7 +401,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
   // The same one token of the wave at a time, V as that token sees it.
   auto values_apart = [&](int buf, int32_t kb) RP_INLINE {
-    for (int32_t at = pmin; at <= pmax; ++at) {
+    for (int32_t at = max(0, pmin); at <= pmax; ++at) {
       const bool mine = pos == at;
 #pragma unroll
       for (int n = 0; n < 2 * P::KB * P::DB; ++n) {

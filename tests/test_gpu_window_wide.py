@@ -1,0 +1,26 @@
+"""Attention of long prompts over a paged cache, eight waves a workgroup, on the
+GPU against 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import _drafts
+import _paged
+import _wide
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("places", [64, 2048])
+@pytest.mark.parametrize("S", [3, 90])
+def test_not_finite_values_at_the_largest_lengths(S: int, places: int, gpu: torch.device) -> None:
+    """A NaN that is seen, beside rows of padding behind a sequence whose length
+    is the largest (their positions pass 32 bits), and tokens before a
+    sequence's first row."""
+    c = _wide.widen(_paged.Cache([64, 64, 64], 2, 64, 16, "bf16", seed=5), places)
+    for b in range(3):
+        c.v[int(c.table[b, 1]), 1, 3, 40] = float("nan")
+    _wide.check(c, _wide.queries(3, 4, S, 64, "bf16"), [2 ** 31 - 1, 30, 2 ** 31 - 1], [1, S, S],
+                gpu, exact=_drafts.window_attention)
