@@ -676,8 +676,9 @@ int rp_verify_drafts(const int64_t* tokens, const int32_t* lens, int64_t B, int6
  * by axis 1, ... (sections: host memory, `axes` of them, rot / 2 in all).
  * Angles are formed in 64 bits, all else in fp32, the result rounded once.
  *   q, k, q_out, k_out   strides sb, sh, ss in elements, unit stride along D,
- *            rows 16-byte aligned; an output may be its input (same strides),
- *            rows of an output do not overlap.  Hkv 0: no k
+ *            rows 16-byte aligned; an output may be its input (same strides)
+ *            and shares no memory with any other array, nor do its rows with
+ *            each other.  Hkv 0: no k
  *   weights  (D) of q's type, 16-byte aligned
  *   positions   int32, strides psa, psb, pss
  *   freq     (rot / 2) float, or double where freq_is_double

@@ -227,6 +227,85 @@ inline bool rows_apart(int64_t unit, const Dim (&dims)[N]) {
   return true;
 }
 
+// Rows of `unit` bytes at `at` and steps of up to three dimensions (in bytes).
+struct RowSet {
+  const void* at;
+  int64_t unit;
+  Dim dims[3];
+
+  bool same(const RowSet& o) const {
+    for (int i = 0; i < 3; ++i)
+      if (dims[i].size != o.dims[i].size || (dims[i].size > 1 && dims[i].stride != o.dims[i].stride))
+        return false;
+    return at == o.at && unit == o.unit;
+  }
+  // The first byte of its memory and the one behind its last.
+  void span(__int128* lo, __int128* hi) const {
+    *lo = reinterpret_cast<uintptr_t>(at);
+    *hi = *lo + unit;
+    for (const Dim& d : dims) *(d.stride < 0 ? lo : hi) += (__int128)(d.size - 1) * d.stride;
+  }
+};
+
+// Whether a row of x and one of y share memory: whether some sum of their steps
+// brings the two starts closer than a row.  Steps of one length count as one of
+// more places; from the longest on, only those are tried that the shorter ones
+// can still make up for, which for layouts that nest are one or two.  (Layouts
+// that ask for more than 4096 trials count as sharing.)
+inline bool rows_meet(const RowSet& x, const RowSet& y) {
+  struct Step {
+    __int128 size, lo, hi;
+  } steps[6];
+  for (const RowSet* r : {&x, &y}) {
+    if (!r->at || r->unit <= 0) return false;
+    for (const Dim& dim : r->dims)
+      if (dim.size <= 0) return false;
+  }
+  __int128 x0, x1, y0, y1;
+  x.span(&x0, &x1);
+  y.span(&y0, &y1);
+  if (x1 <= y0 || y1 <= x0) return false;
+  // the distance of two starts ranges over [d + lo, d + hi] of the steps
+  const __int128 d = (__int128)reinterpret_cast<uintptr_t>(x.at) - reinterpret_cast<uintptr_t>(y.at);
+  __int128 lo = 0, hi = 0;
+  int n = 0;
+  for (const RowSet* r : {&x, &y})
+    for (const Dim& dim : r->dims) {
+      if (dim.size == 1 || dim.stride == 0) continue;
+      const bool up = (dim.stride > 0) == (r == &x);
+      const __int128 size = dim.stride > 0 ? (__int128)dim.stride : -(__int128)dim.stride;
+      const __int128 most = dim.size - 1, a = up ? 0 : -most, b = up ? most : 0;
+      lo += a * size;
+      hi += b * size;
+      int i = 0;
+      while (i < n && steps[i].size > size) ++i;
+      if (i < n && steps[i].size == size) {
+        steps[i].lo += a;
+        steps[i].hi += b;
+        continue;
+      }
+      for (int j = n++; j > i; --j) steps[j] = steps[j - 1];
+      steps[i] = Step{size, a, b};
+    }
+  int trials = 0;
+  auto meet = [&](auto& self, int i, __int128 at, __int128 low, __int128 high) -> bool {
+    if (i == n) return -(__int128)x.unit < at && at < y.unit;
+    const Step& s = steps[i];
+    low -= s.lo * s.size;                               // what the shorter steps reach
+    high -= s.hi * s.size;
+    // -x.unit < at + z size + [low, high] < y.unit
+    const __int128 least = -(__int128)x.unit + 1 - high - at, most = y.unit - 1 - low - at;
+    __int128 z = least >= 0 ? (least + s.size - 1) / s.size : -(-least / s.size);
+    if (z < s.lo) z = s.lo;
+    for (; z <= s.hi && z * s.size <= most; ++z) {
+      if (++trials > 4096) return true;
+      if (self(self, i + 1, at + z * s.size, low, high)) return true;
+    }
+    return false;
+  };
+  return meet(meet, 0, d, lo, hi);
+}
+
 }  // namespace rp
 
 // Thread-local last-error message shared by all entry points.

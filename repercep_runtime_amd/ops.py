@@ -1550,7 +1550,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     over the batch.  ``inv_freq`` fp32 or fp64, a multiple of 8 long.  Angles
     are formed in 64 bits, so far positions lose nothing; all else is fp32,
     rounded once.  Returns (q, k) of q's dtype; ``out_q`` may be q itself, and
-    ``out_k`` k."""
+    ``out_k`` k; outputs that share memory in any other way are refused."""
     if q.dim() != 4:
         raise ValueError(f"q must be (B, H, S, D), got {tuple(q.shape)}")
     B, H, S, D = q.shape

@@ -1,0 +1,49 @@
+"""A drafted step's operators on the CPU: outputs that share memory with another
+array of the call are refused before any launch."""
+
+from __future__ import annotations
+
+import struct
+
+import pytest
+
+import test_drafts
+from repercep_runtime_amd import _capi
+
+A = test_drafts.FAKE                    # never read
+MB = 1 << 20
+
+
+def rope(**kw) -> int:
+    """2 sequences of 5 tokens, 4 + 2 heads of 128, each array in a MiB of its own."""
+    a = dict(q=A, k=A + MB, qo=A + 2 * MB, ko=A + 3 * MB, pos=A + 4 * MB, freq=A + 5 * MB,
+             qw=A + 6 * MB, kw=A + 7 * MB)
+    return test_drafts.rope(**{**a, **kw})
+
+
+@pytest.mark.parametrize("kw", [
+    dict(ko=A + 2 * MB),                                    # one place for both
+    dict(ko=A + 2 * MB + 256),                              # a row further
+    dict(qo=A + MB),                                        # the other's input
+    dict(ko=A),
+    dict(qo=A, qob=4 * 640, qoh=128, qos=512),              # its input in another order
+    dict(qo=A + 256),                                       # its input a row further
+    dict(qo=A + 16),                                        # half a row
+    dict(ko=A + MB - 240),                                  # into its input's first row
+    dict(q=A + 2 * MB + 4 * 640, qsb=0, qsh=0, qss=0),      # one row for all, among the outputs
+    dict(qo=A + 4 * MB), dict(ko=A + 5 * MB - 256), dict(qo=A + 6 * MB), dict(ko=A + 7 * MB),
+    dict(pos=A + 2 * MB + 252, psb=0, pss=0),               # the end of an output's first row
+    # slices of a projection with a row in common: q's heads 0 to 3, k's 3 and 4
+    dict(qsb=5 * 768, qsh=128, qss=768, k=A + 3 * 256, ksb=5 * 768, ksh=128, kss=768, qo=A,
+         qob=5 * 768, qoh=128, qos=768, ko=A + 3 * 256, kob=5 * 768, koh=128, kos=768),
+])
+def test_rotation(kw: dict) -> None:
+    assert rope(**kw) == 1
+    assert "shares memory" in _capi.lib().rp_last_error().decode()
+
+
+def test_rotation_of_several_axes() -> None:
+    """Positions of an axis that reach into an output."""
+    kw = dict(axes=2, sections=struct.pack("2q", 30, 34), psa=MB // 4)
+    assert rope(**kw, pos=A + MB + 2048) == 1
+    assert "shares memory" in _capi.lib().rp_last_error().decode()
