@@ -580,6 +580,7 @@ int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64
  *   lse_i = log(sum_j exp(s_j))                      (lse NULL: not written)
  * q (B, H, S, head_dim) with strides qsb, qsh, qss, out of q's type with
  * strides osb, osh, oss (no two rows of out share memory); lse float (B, H, S).
+ * out may be q (same strides); else out and lse share no memory with any array.
  * Types, heads, scale and cache as in rp_paged_attn_decode.  A token that sees
  * no row, or scores of -inf only, and a token i >= q_lens[b] get zeros and lse
  * -inf.  Sums are held in fp32; a weight enters the product with V rounded once

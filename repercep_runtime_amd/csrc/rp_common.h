@@ -306,6 +306,25 @@ inline bool rows_meet(const RowSet& x, const RowSet& y) {
   return meet(meet, 0, d, lo, hi);
 }
 
+// Memory without a gap.
+inline RowSet whole(const void* at, int64_t bytes) {
+  return RowSet{at, bytes, {{1, 0}, {1, 0}, {1, 0}}};
+}
+
+// Whether a call's outputs share memory with each other or with its inputs.  The
+// first `own` outputs may each lie where the input of the same index does, row
+// on row.
+template <int N, int M>
+inline bool outputs_meet(const RowSet (&to)[N], const RowSet (&in)[M], int own) {
+  for (int o = 0; o < N; ++o) {
+    for (int i = o + 1; i < N; ++i)
+      if (rows_meet(to[o], to[i])) return true;
+    for (int i = 0; i < M; ++i)
+      if (!(i == o && o < own && to[o].same(in[i])) && rows_meet(to[o], in[i])) return true;
+  }
+  return false;
+}
+
 }  // namespace rp
 
 // Thread-local last-error message shared by all entry points.

@@ -231,6 +231,27 @@ extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64
     rp_set_error("paged_attn_window: workspace of %zu bytes, 256-byte aligned, needed", l.total);
     return RP_ERR_WORKSPACE;
   }
+  // A row of q is read by the workgroup that writes its row of out, or before any
+  // is written, so out can take q's place.
+  const int64_t D = cache->head_dim, eb = cache_elem_bytes(cache->dtype);
+  const int64_t scales = fp8 ? 4 * cache->num_pages * cache->heads * cache->page_size : 0;
+  const Dim pages{cache->num_pages, cache->stride_page * eb},
+      heads{cache->heads, cache->stride_head * eb}, slots{cache->page_size, cache->stride_row * eb};
+  const RowSet in[] = {{q, 2 * D, {{B, 2 * qsb}, {H, 2 * qsh}, {S, 2 * qss}}},
+                       {cache->k, D * eb, {pages, heads, slots}},
+                       {cache->v, D * eb, {pages, heads, slots}},
+                       whole(cache->k_scale, scales),
+                       whole(cache->v_scale, scales),
+                       {cache->block_table, 4 * cache->max_pages, {{B, 4 * cache->table_stride}, {1, 0}, {1, 0}}},
+                       whole(seq_lens, 4 * B),
+                       whole(q_lens, 4 * B)};
+  const RowSet to[] = {{out, 2 * D, {{B, 2 * osb}, {H, 2 * osh}, {S, 2 * oss}}},
+                       whole(lse, 4 * B * H * S)};
+  if (outputs_meet(to, in, 1)) {
+    rp_set_error("paged_attn_window: an output shares memory with another array, or with q at "
+                 "other strides");
+    return RP_ERR_INVALID_ARGUMENT;
+  }
   char* ws = static_cast<char*>(workspace);
   WindowArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -265,7 +286,6 @@ extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64
   a.part = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float2*>(ws + l.ml);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t D = cache->head_dim;
   if (q_dtype == RP_DTYPE_F16) {
     if (fp8) launch_window<kInF16, RP_CACHE_E4M3>(a, c, D, l, st);
     else launch_window<kInF16, RP_CACHE_F16>(a, c, D, l, st);

@@ -297,16 +297,13 @@ extern "C" int rp_qk_norm_rope(const void* q, const void* k, int dtype, int64_t 
   // read by the lanes that write it, so an output can take its own input's place.
   const RowSet in[] = {{q, 2 * D, {{B, 2 * qsb}, {H, 2 * qsh}, {S, 2 * qss}}},
                        {k, 2 * D, {{B, 2 * ksb}, {Hkv, 2 * ksh}, {S, 2 * kss}}},
-                       {q_weight, 2 * D, {{1, 0}, {1, 0}, {1, 0}}},
-                       {k_weight, 2 * D, {{1, 0}, {1, 0}, {1, 0}}},
+                       whole(q_weight, 2 * D),
+                       whole(k_weight, 2 * D),
                        {positions, 4, {{axes, 4 * psa}, {B, 4 * psb}, {S, 4 * pss}}},
-                       {freq, (freq_is_double ? 4 : 2) * rot, {{1, 0}, {1, 0}, {1, 0}}}};
+                       whole(freq, (freq_is_double ? 4 : 2) * rot)};
   const RowSet to[] = {{q_out, 2 * D, {{B, 2 * qob}, {H, 2 * qoh}, {S, 2 * qos}}},
                        {k_out, 2 * D, {{B, 2 * kob}, {Hkv, 2 * koh}, {S, 2 * kos}}}};
-  bool meet = rows_meet(to[0], to[1]);
-  for (int o = 0; o < 2; ++o)
-    for (int i = 0; i < 6; ++i) meet |= !(i == o && to[o].same(in[i])) && rows_meet(to[o], in[i]);
-  if (meet) {
+  if (outputs_meet(to, in, 2)) {
     rp_set_error("qk_norm_rope: an output shares memory with another array, or with its input at "
                  "other strides");
     return RP_ERR_INVALID_ARGUMENT;

@@ -1268,10 +1268,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     and the first ``sinks`` ones.  Pages that no token sees any more may be
     given away and their table entries set to -1.
 
-    Caches, heads, ``scale``, ``max_seq_len``, ``out`` as in
-    ``paged_attention_decode``.  Returns out (B, H, S, D) in q's dtype, or (out,
-    lse) with ``return_lse``, lse (B, H, S) fp32.  A token that sees no row and
-    the rows past q_lens give zeros and -inf."""
+    Caches, heads, ``scale``, ``max_seq_len`` as in ``paged_attention_decode``;
+    ``out`` too, which may be q itself and shares no other memory.  Returns out
+    (B, H, S, D) in q's dtype, or (out, lse) with ``return_lse``, lse (B, H, S)
+    fp32.  A token that sees no row and the rows past q_lens give zeros and
+    -inf."""
     if q.dim() != 4:
         raise ValueError(f"q must be (B, H, S, D), got {tuple(q.shape)}")
     B, H, S, D = q.shape

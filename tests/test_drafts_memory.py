@@ -8,6 +8,7 @@ import struct
 import pytest
 
 import test_drafts
+import test_paged
 from repercep_runtime_amd import _capi
 
 A = test_drafts.FAKE                    # never read
@@ -46,4 +47,24 @@ def test_rotation_of_several_axes() -> None:
     """Positions of an axis that reach into an output."""
     kw = dict(axes=2, sections=struct.pack("2q", 30, 34), psa=MB // 4)
     assert rope(**kw, pos=A + MB + 2048) == 1
+    assert "shares memory" in _capi.lib().rp_last_error().decode()
+
+
+def window(**kw) -> int:
+    """2 sequences of 3 tokens, 4 heads of 128, each array in a MiB of its own."""
+    c = test_paged.cache(k=A + MB, v=A + 2 * MB, block_table=A + 3 * MB)
+    a = dict(q=A, out=A + 4 * MB, lse=A + 5 * MB, lens=A + 6 * MB, qlens=A + 7 * MB, ws=A + 8 * MB)
+    return test_drafts.window(c, **{**a, **kw})
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=A, osb=4 * 3 * 128, osh=128, oss=512),         # q in another order
+    dict(out=A + 256), dict(out=A + 8),                     # a row further, a part of one
+    dict(out=A + MB), dict(out=A + 2 * MB + 1024),          # the cache's rows
+    dict(out=A + 3 * MB - 64), dict(out=A + 6 * MB), dict(out=A + 7 * MB - 8),
+    dict(lse=A), dict(lse=A + 4 * MB), dict(lse=A + MB), dict(lse=A + 6 * MB),
+    dict(q=A + 4 * MB + 2560, qsb=0, qsh=0, qss=0),         # one row for all, among out's
+])
+def test_attention(kw: dict) -> None:
+    assert window(**kw) == 1
     assert "shares memory" in _capi.lib().rp_last_error().decode()

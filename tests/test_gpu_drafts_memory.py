@@ -6,7 +6,10 @@ from __future__ import annotations
 import pytest
 import torch
 
+import _paged
+import _wide
 import test_gpu_rope as rope
+from repercep_runtime_amd import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +31,34 @@ def test_rotation(gpu: torch.device) -> None:
         q.copy_(c["q"])
         k.copy_(c["k"])
         rope.check(c, rope.call(c, gpu, "half", 1e-6, q=q, k=k, **kw), "half", 1e-6)
+
+
+@pytest.mark.parametrize("S,places", [(1, 64), (3, 64), (3, 4096), (90, 64), (90, 2048), (90, 150000)])
+def test_attention(S: int, places: int, gpu: torch.device) -> None:
+    """The queries' own place, in one part and in several; slices of a projection."""
+    B, H, Hkv, D = 2, 4, 2, 64
+    c = _wide.widen(_paged.Cache([190, 90], Hkv, D, 16, "bf16", seed=3), places)
+    x = torch.zeros((B, S, (H + Hkv) * D), dtype=torch.bfloat16, device=gpu)
+    heads = x.view(B, S, H + Hkv, D).permute(0, 2, 1, 3)
+    q = _wide.queries(B, H, S, D, "bf16")
+    heads[:, :H].copy_(q)
+    for out in (heads[:, 1:1 + H], heads[:, 2:]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            _wide.call(c, q, [190, 90], None, gpu, qview=heads[:, :H], out=out)
+    _wide.check(c, q, [190, 90], [S, 1], gpu, 70, 3, qview=heads[:, :H], out=heads[:, :H])
+    assert bool((heads[:, H:] == 0).all())
+    # between the rows of another tensor
+    y = torch.zeros((B, S, 2 * H, D), dtype=torch.bfloat16, device=gpu).permute(0, 2, 1, 3)
+    y[:, ::2].copy_(q)
+    _wide.check(c, q, [190, 90], None, gpu, qview=y[:, ::2], out=y[:, 1::2])
+    assert torch.equal(y[:, ::2].cpu(), q)
+
+
+def test_attention_into_the_cache(gpu: torch.device) -> None:
+    c = _paged.Cache([20], 4, 64, 16, "bf16")
+    f = c.to(gpu)
+    q = torch.zeros((1, 4, 16, 64), dtype=torch.bfloat16, device=gpu)
+    lens = torch.tensor([20], dtype=torch.int32, device=gpu)
+    for name in ("k_cache", "v_cache"):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.paged_attention(q, seq_lens=lens, out=f[name][1:2], **f)
