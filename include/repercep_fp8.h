@@ -657,7 +657,8 @@ int rp_token_logprobs(const void* logits, int logits_dtype, int64_t N, int64_t V
  *            draft NULL: the drafts were certain, q_i(d_i) = 1 and 0 elsewhere
  *   u        (B, N + 1) in [0, 1)
  *   out      (B, N + 1): the accepted drafts, the drawn token (-1 where every
- *            w is 0), then -1; accepted (B): m
+ *            w is 0), then -1; accepted (B): m.  Neither shares memory with
+ *            another array
  * N may be 0 (a draw from p_0).  V up to 2^22.  Equal calls give equal tokens.
  * workspace: rp_verify_drafts_workspace_bytes, 256-byte aligned (may be NULL
  * where that is 0).  No counterpart in the reference. */

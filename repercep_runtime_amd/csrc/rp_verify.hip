@@ -378,7 +378,7 @@ extern "C" int rp_verify_drafts(const int64_t* tokens, const int32_t* lens, int6
     rp_set_error("verify_drafts: too many sequences, drafts or tokens");
     return RP_ERR_UNSUPPORTED;
   }
-  const int eb = dtype == RP_OUT_F32 ? 4 : 2;
+  const int64_t eb = dtype == RP_OUT_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(target) % eb != 0 || reinterpret_cast<uintptr_t>(draft) % eb != 0) {
     rp_set_error("verify_drafts: probabilities must be aligned to their type");
     return RP_ERR_INVALID_ARGUMENT;
@@ -389,6 +389,17 @@ extern "C" int rp_verify_drafts(const int64_t* tokens, const int32_t* lens, int6
     rp_set_error("verify_drafts: workspace of %zu bytes, 256-byte aligned, needed",
                  (size_t)(B * parts * 16));
     return RP_ERR_WORKSPACE;
+  }
+  // a block's waves write out while others still read the drafts
+  const RowSet in[] = {whole(tokens, 8 * B * N),
+                       whole(lens, 4 * B),
+                       whole(u, 4 * B * (N + 1)),
+                       {target, eb * V, {{B, eb * tsb}, {N + 1, eb * tsn}, {1, 0}}},
+                       {draft, eb * V, {{B, eb * dsb}, {N, eb * dsn}, {1, 0}}}};
+  const RowSet to[] = {whole(out, 8 * B * (N + 1)), whole(accepted, 4 * B)};
+  if (outputs_meet(to, in, 0)) {
+    rp_set_error("verify_drafts: an output shares memory with another array");
+    return RP_ERR_INVALID_ARGUMENT;
   }
   const VerifyArgs a{static_cast<const char*>(target), static_cast<const char*>(draft), tsb, tsn,
                      dsb, dsn, tokens, u, lens, (int32_t)N, (int32_t)V, (int32_t)parts, out,

@@ -68,3 +68,19 @@ def window(**kw) -> int:
 def test_attention(kw: dict) -> None:
     assert window(**kw) == 1
     assert "shares memory" in _capi.lib().rp_last_error().decode()
+
+
+@pytest.mark.parametrize("V", [100, 50000])
+@pytest.mark.parametrize("kw", [
+    dict(out=A), dict(out=A + 40), dict(accepted=A + 16), dict(out=A + MB - 56),
+    dict(accepted=A + MB), dict(out=A + 2 * MB + 4), dict(out=A + 3 * MB), dict(accepted=A + 4 * MB),
+    dict(out=A + 5 * MB), dict(accepted=A + 5 * MB + 56)])
+def test_verdict(V: int, kw: dict) -> None:
+    """2 sequences of 3 drafts, each array in a MiB of its own."""
+    a = dict(tokens=A, lens=A + MB, u=A + 2 * MB, target=A + 3 * MB, draft=A + 4 * MB,
+             out=A + 5 * MB, accepted=A + 6 * MB, V=V, tsn=V, dsn=V, tsb=0, dsb=0)
+    a.update(kw)
+    if "accepted" not in kw and kw["out"] == A + 5 * MB:
+        a["accepted"] = A + 5 * MB + 32
+    assert test_drafts.verify(**a) == 1
+    assert "shares memory" in _capi.lib().rp_last_error().decode()
