@@ -1305,12 +1305,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, H, S), dtype=torch.float32) if return_lse else None
     if B > 0 and S > 0 and H > 0:
-        hint = max_seq_len if max_seq_len is not None else 0
-        n = C.lib().rp_paged_window_workspace_bytes(B, H, S, cache, window or 0, sinks, hint)
+        # no position passes 31 bits, and ctypes would cut a number of more than 64
+        window, sinks, hint = (min(x or 0, 0x7fffffff) for x in (window, sinks, max_seq_len))
+        n = C.lib().rp_paged_window_workspace_bytes(B, H, S, cache, window, sinks, hint)
         ws = q.new_empty(n, dtype=torch.uint8) if n else None
         rc = _on_device(
             dev, C.lib().rp_paged_attn_window, q.data_ptr(), dt, B, H, S, *_strides(q, 3), cache,
-            seq_lens.data_ptr(), q_lens.data_ptr() if q_lens is not None else None, window or 0,
+            seq_lens.data_ptr(), q_lens.data_ptr() if q_lens is not None else None, window,
             sinks, 1.0 / math.sqrt(D) if scale is None else float(scale), out.data_ptr(),
             *_strides(out, 3), lse.data_ptr() if return_lse else None, hint,
             ws.data_ptr() if n else None, n, _stream(q))

@@ -67,7 +67,7 @@ def definition(q: torch.Tensor, rows: list[tuple[torch.Tensor, torch.Tensor]], l
         j = torch.arange(k.shape[1])[None]
         seen = j <= p
         if window is not None:
-            seen &= (p - j < window) | (j < sinks)
+            seen &= (p - j < min(window, 2 ** 62)) | (j < min(sinks, 2 ** 62))
         kt = k.transpose(1, 2).contiguous()
         qb = q[b, :, :m].double()
         s = torch.matmul(qb, kt) * scale

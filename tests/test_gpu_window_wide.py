@@ -24,3 +24,11 @@ def test_not_finite_values_at_the_largest_lengths(S: int, places: int, gpu: torc
         c.v[int(c.table[b, 1]), 1, 3, 40] = float("nan")
     _wide.check(c, _wide.queries(3, 4, S, 64, "bf16"), [2 ** 31 - 1, 30, 2 ** 31 - 1], [1, S, S],
                 gpu, exact=_drafts.window_attention)
+
+
+@pytest.mark.parametrize("S", [3, 90])
+def test_windows_and_sinks_past_64_bits(S: int, gpu: torch.device) -> None:
+    c = _paged.Cache([200], 2, 64, 16, "bf16", seed=6)
+    q = _wide.queries(1, 4, S, 64, "bf16")
+    for window, sinks in ((2 ** 64 + 3, 0), (5, 2 ** 64), (2 ** 63, 2 ** 63)):
+        _wide.check(c, q, [200], None, gpu, window, sinks, max_seq_len=2 ** 64 + 16)
