@@ -585,9 +585,11 @@ int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64
  * no row, or scores of -inf only, and a token i >= q_lens[b] get zeros and lse
  * -inf.  Sums are held in fp32; a weight enters the product with V rounded once
  * to 16 bits or more (the type of out at least), and out is rounded once.
- * Values up to the type's largest do not overflow on the way.  Infinities and
- * NaNs in rows of V reach the tokens that see them and no others (a weight
- * below 2^-31 of the largest may count as 0 beside an infinity: NaN).
+ * Values up to the type's largest do not overflow on the way, nor do small ones
+ * vanish (but for a weight times its e4m3fn row's scale below 2^-126, of which
+ * bits may be lost).  Infinities and NaNs in rows of V reach the tokens that see
+ * them and no others (a weight below 2^-31 of the largest may count as 0 beside
+ * an infinity: NaN).
  * max_seq_len (0: unknown) as in rp_paged_attn_decode.
  * workspace: rp_paged_window_workspace_bytes of the same arguments, 256-byte
  * aligned (may be NULL where that is 0). */

@@ -118,6 +118,7 @@ struct Few : StepRows<QT == kInF16, CT, D, STREAM> {
   template <bool CAREFUL>
   __device__ __forceinline__ void step(int u, bool more) {
     const int k = keys.key(u);
+    const float lift = base_lift<VF16, CAREFUL>(a);
     f32x4 s[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -169,10 +170,10 @@ struct Few : StepRows<QT == kInF16, CT, D, STREAM> {
       }
       float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
                         fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      if (__any(top > base[n] + (kSlack - a.lift))) {
+      if (__any(top > base[n] + (kSlack - lift))) {
         top = fmaxf(top, __shfl_xor(top, 16, kWave));
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float next = fmaxf(base[n], top + a.lift);
+        const float next = fmaxf(base[n], top + lift);
         const float r = next == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(base[n] - next);
         sum[n] *= r;
 #pragma unroll

@@ -13,10 +13,12 @@
 //   P never leaves the lane.
 // * The running maximum is lazy: rows are weighed about their base, which is
 //   only moved, and the sums rescaled, when a score exceeds it by 2^kSlack.
-//   A bf16 P is weighed about a base so high that a row's weights add up to
-//   less than 1, so sums of values near fp32's largest cannot overflow; an fp16
-//   P about one below the largest score, so that weights down to 2^-21 of the
-//   largest keep their 11 bits, and smaller ones 2^-31 of it.
+//   A bf16 P is weighed about the largest score, and again, token by token as
+//   below, if a sum of values near the type's largest overflows: then about a base
+//   so high that a row's weights add up to less than 1 (always there, products with
+//   values below 2^-100 lost bits).  An fp16 P is weighed about a base below the
+//   largest score, so that weights down to 2^-21 of the largest keep their 11 bits,
+//   and smaller ones 2^-31 of it.
 // * P enters the second product rounded once to 16 bits, as precise as the
 //   output.  For an e4m3fn cache, whose row scales can be of any size, it is
 //   bf16; an fp16 output then takes it as the sum of two bf16 numbers.
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
 
   f32x16 acc[P::DB];
-  float base, sum;
+  float base, sum, lift;
 
   // ---- staging: lane l's page entry says where key l of a tile lies; a thread
   // brings chunks of 16 bytes, a row's by threads next to each other
@@ -325,9 +327,9 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
       for (int i = 0; i < 16; ++i) larger(s, i);
     }
     top *= c1;
-    if (__any(top > base + (kSlack - a.lift))) {
+    if (__any(top > base + (kSlack - lift))) {
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      const float next = fmaxf(base, top + a.lift);
+      const float next = fmaxf(base, top + lift);
       const float r = next == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(base - next);
       sum *= r;
 #pragma unroll
@@ -485,7 +487,8 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
     if constexpr (!P::FP8) asm volatile("" : "+v"(top));
   };
 
-  auto reset = [&]() RP_INLINE {
+  auto reset = [&](float to) RP_INLINE {
+    lift = to;
     base = neg_inf();
     sum = 0.0f;
 #pragma unroll
@@ -501,7 +504,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   //   first half   fused(t) | mask t + 1, store K t + 2 and V t + 1 | fused(t + 1)
   //   second half  store K t + 2 and V t + 1 | fused(t) | mask t + 1, store t + 3 and t + 2
   auto run = [&]() RP_INLINE {
-    reset();
+    reset(base_lift<P::VF16, false>(a));
     if (t0 >= t1) return;
     const bool second = NW == 8 && wave >= 4;
     uint64_t q0, q1 = 0, q2 = 0;                         // the tiles' keys that are there, t + 1 on
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(NW* kWave) void prompt_kernel(WindowArgs a, PagedVi
   };
   // The same a tile after the other, each token's part of V by itself.
   auto run_apart = [&]() RP_INLINE {
-    reset();
+    reset(base_lift<P::VF16, true>(a));
     for (int t = t0; t < t1; ++t) {
       const int32_t page = page_of(t, entry(t));
       const int64_t off = offset_of(t, page);

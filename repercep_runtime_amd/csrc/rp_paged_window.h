@@ -19,7 +19,7 @@ struct WindowArgs {
   const int32_t* qlens;          // or null: S each
   float c;                       // |sm_scale| * log2(e)
   uint32_t flip;                 // the sign of sm_scale, for a pair of q's values
-  float lift;                    // how far bases lie above the scores, in powers of two
+  float lift;                    // see base_lift
   int32_t window, sinks;         // window: 0x7fffffff where there is none
   uint16_t* out;
   int64_t osb, osh, oss;
@@ -48,6 +48,13 @@ void launch_window(const WindowArgs& a, const PagedView& c, int64_t D, const Win
 namespace {
 
 constexpr float kSlack = 8.0f;                  // powers of two, see rp_paged_prompt.h
+
+// How far bases lie above the scores, in powers of two: of fp16 weights as far as
+// their range asks (F16), of bf16 ones not at all, unless sums overflowed (AGAIN).
+template <bool F16, bool AGAIN>
+__device__ __forceinline__ float base_lift(const WindowArgs& a) {
+  return F16 || AGAIN ? a.lift : 0.0f;
+}
 
 // A sequence's place: its length, its new tokens, the first one's position.
 struct Place {

@@ -264,8 +264,8 @@ extern "C" int rp_paged_attn_window(const void* q, int q_dtype, int64_t B, int64
   // is less than 2^-21
   a.c = c2 == 0.0f ? 0x1p-149f : c2 < 0.0f ? -c2 : c2;
   a.flip = c2 < 0.0f ? 0x80008000u : 0u;
-  // bf16 weights: of at most as many keys as the table has places, 1 in all;
-  // fp16 ones: up to 2^15
+  // bf16 weights where sums overflow: of at most as many keys as the table has
+  // places, 1 in all; fp16 ones: up to 2^15
   a.lift = cache->dtype == RP_CACHE_F16
       ? kSlack - 15.0f
       : kSlack + (float)(64 - __builtin_clzll((unsigned long long)c.capacity()));
