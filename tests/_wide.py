@@ -49,9 +49,10 @@ def held(c: _paged.Cache, n: list[int]) -> list[tuple[torch.Tensor, torch.Tensor
 
 def definition(q: torch.Tensor, rows: list[tuple[torch.Tensor, torch.Tensor]], lens: list[int],
                qlens: list[int], window: int | None, sinks: int, scale: float,
-               weight_half: float) -> tuple[torch.Tensor, ...]:
+               weight_half: float, gone: tuple[int, ...] = ()) -> tuple[torch.Tensor, ...]:
     """``_drafts.window_attention`` of rows that are finite, all tokens of a
-    sequence at a time (a masked weight of 0 meets no infinity)."""
+    sequence at a time (a masked weight of 0 meets no infinity); the positions
+    ``gone`` are no rows."""
     B, H, S, D = q.shape
     u = _drafts.U32
     out = torch.zeros((B, H, S, D), dtype=torch.float64)
@@ -68,6 +69,7 @@ def definition(q: torch.Tensor, rows: list[tuple[torch.Tensor, torch.Tensor]], l
         seen = j <= p
         if window is not None:
             seen &= (p - j < min(window, 2 ** 62)) | (j < min(sinks, 2 ** 62))
+        seen[:, [at for at in gone if at < k.shape[1]]] = False
         kt = k.transpose(1, 2).contiguous()
         qb = q[b, :, :m].double()
         s = torch.matmul(qb, kt) * scale
