@@ -1,5 +1,5 @@
-"""Attention of long prompts over a paged cache, eight waves a workgroup, on the
-GPU against 64 bits."""
+"""Attention of long prompts over a paged cache, eight waves a workgroup (at 256
+dims four), on the GPU against 64 bits."""
 
 from __future__ import annotations
 
@@ -29,6 +29,9 @@ CASES = [  # B, H, Hkv, D, S, lens, qlens, window, sinks, page
     (2, 4, 2, 64, 100, [100, 300], [100, 7], None, 0, 16),
     (1, 2, 1, 128, 280, [1105], None, None, 0, 16),
     (1, 2, 1, 64, 600, [2111], [599], None, 0, 64),
+    # four waves, tiles of 32 keys
+    (2, 4, 2, 256, 150, [400, 90], [150, 33], 70, 40, 16),
+    (1, 2, 1, 256, 140, [1105], None, None, 0, 32),
 ]
 
 
@@ -45,10 +48,10 @@ def test_matches_definition(case: tuple, kind: str, gpu: torch.device) -> None:
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_every_number_of_key_tiles(D: int, kind: str, gpu: torch.device) -> None:
-    """136 workgroups, too many to be split: sequences of one tile of 64 keys to
-    six, some with fewer rows than tokens; then as many over a narrow table."""
+    """136 workgroups or more, too many to be split: sequences of one tile of 64 keys
+    to six, some with fewer rows than tokens; then as many over a narrow table."""
     dtype, cache = _wide.kinds(kind)
     lens = [1 + 20 * i for i in range(17)]
     lens[3], lens[6] = 64, 128
@@ -65,7 +68,7 @@ def test_every_number_of_key_tiles(D: int, kind: str, gpu: torch.device) -> None
 
 @pytest.mark.parametrize("page", [1, 2, 8, 256])
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_page_sizes(D: int, kind: str, page: int, gpu: torch.device) -> None:
     """Pages smaller than the rows that a wave brings at a time."""
     dtype, cache = _wide.kinds(kind)
@@ -142,7 +145,7 @@ def test_given_away_pages(kind: str, gpu: torch.device) -> None:
 
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("D,window", [(32, None), (64, 40), (128, 40), (128, None)])
+@pytest.mark.parametrize("D,window", [(32, None), (64, 40), (128, 40), (128, None), (256, 40)])
 def test_infinite_values(D: int, window: int | None, kind: str, value: float,
                          gpu: torch.device) -> None:
     """An infinity or NaN in V reaches the tokens that see its row, in its
