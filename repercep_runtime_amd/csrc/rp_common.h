@@ -316,12 +316,15 @@ inline RowSet whole(const void* at, int64_t bytes) {
 // on row.
 template <int N, int M>
 inline bool outputs_meet(const RowSet (&to)[N], const RowSet (&in)[M], int own) {
-  for (int o = 0; o < N; ++o) {
-    for (int i = o + 1; i < N; ++i)
-      if (rows_meet(to[o], to[i])) return true;
-    for (int i = 0; i < M; ++i)
-      if (!(i == o && o < own && to[o].same(in[i])) && rows_meet(to[o], in[i])) return true;
-  }
+  __int128 lo[N + M], hi[N + M];                        // most arrays' spans lie apart
+  for (int i = 0; i < N + M; ++i) (i < N ? to[i] : in[i - N]).span(&lo[i], &hi[i]);
+  for (int o = 0; o < N; ++o)
+    for (int i = o + 1; i < N + M; ++i) {
+      const RowSet& other = i < N ? to[i] : in[i - N];
+      if (hi[o] <= lo[i] || hi[i] <= lo[o]) continue;
+      if (i == N + o && o < own && to[o].same(other)) continue;
+      if (rows_meet(to[o], other)) return true;
+    }
   return false;
 }
 
