@@ -589,7 +589,7 @@ int rp_paged_attn_decode(const void* q, int q_dtype, int64_t B, int64_t H, int64
  * vanish (but for a weight times its e4m3fn row's scale below 2^-126, of which
  * bits may be lost).  Infinities and NaNs in rows of V reach the tokens that see
  * them and no others (a weight below 2^-31 of the largest may count as 0 beside
- * an infinity: NaN).
+ * an infinity: NaN; so may an infinite scale of an RP_CACHE_E4M3 row come out).
  * max_seq_len (0: unknown) as in rp_paged_attn_decode.
  * workspace: rp_paged_window_workspace_bytes of the same arguments, 256-byte
  * aligned (may be NULL where that is 0). */

@@ -15,9 +15,10 @@
 // and what infinities in V ask for: rp_paged_prompt.h.
 //
 // One token of 32 sequences in a window of 1024, 32 heads on 8 of 128, bf16, takes
-// 27 us (4.9 TB/s); 1 to 6 tokens of 16 sequences of 640 to 8000 e4m3fn keys 46
-// (3.2 TB/s: their conversion and a workgroup's first loads beside 10 steps a
-// wave), 8 tokens after 131063 fp16 keys of 8 heads 130 (4.1 TB/s, two row tiles).
+// 27 us (4.9 TB/s), 8 tokens after 131063 fp16 keys of 8 heads 124 (4.3 TB/s, two row
+// tiles).  1 to 6 tokens of 16 sequences of 640 to 8000 e4m3fn keys take 42 (3.5
+// TB/s): a wave lives 65k cycles, about 30 of those us; 39% of them it waits for
+// rows, 42% it issues, three quarters of that vector work.
 // Two columns of 16 rows fit 256 registers, two waves a SIMD; four took 512 and
 // lost on e4m3fn caches (64 rows of 8000 keys, 16 sequences, 114 us; two tiles of
 // two 100), and won on 16-bit ones (130 against 137).

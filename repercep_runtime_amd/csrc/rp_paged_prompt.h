@@ -25,20 +25,21 @@
 // * A row of V that only some of a wave's rows see may hold infinities or NaNs,
 //   which 0 P does not silence.  Sums that come out infinite or NaN are taken
 //   again token by token, V masked for each.
-// * A tile takes a wave 32 matrix instructions (1024 cycles) and about 160 vector
+// * A tile takes a wave 32 matrix instructions (1024 cycles) and about 200 vector
 //   ones; one after the other they took 3000 cycles.  So a tile's weights and
 //   product with V run beside the next tile's scores (fused), in an order that is
 //   written out, since the compiler's own put the LDS reads right before their
 //   uses; and the two waves of a SIMD take turns at that and at staging.  What
 //   each brought, a prompt of 16384 tokens, 32 heads on 8 of 128, bf16:
 //   one phase after the other 2.59 ms, side by side 2.41, in written order 2.22,
-//   in turns and weights spread evenly 2.11-2.20, the rows of the tile after the
-//   next stored and asked for before the next tile's scores are weighed 2.06-2.12.
+//   in turns and weights spread evenly 2.17, the rows of the tile after the
+//   next stored and asked for before the next tile's scores are weighed 2.12.
 //
-// That is 1.04 to 1.07 PFLOP/s; a library product of 16384^2 reaches 1.39 on this
-// card.  Matrix cores 48% busy, the VALU 51%, no LDS conflicts: what is left are the
-// barriers, at which the halves wait for each other, and a fused phase of 1800
-// cycles.  256 dims, four waves a workgroup and so one a SIMD, take 6.4 ms (0.68
+// That prompt takes 2.11 to 2.18 ms, 1.01 to 1.04 PFLOP/s, where a library product of
+// 16384^2 reaches 1.38 (2.56 ms on a card where that reaches 1.21); fp16 2.25, bf16
+// over e4m3fn rows 2.45.  Matrix cores 48% busy, the VALU 51%, no LDS conflicts;
+// waves spend 27% of their cycles at barriers and counters, 28% without an issue
+// slot.  256 dims, four waves a workgroup and so one a SIMD, take 6.5 ms (0.68
 // PFLOP/s).
 
 #pragma once
@@ -97,7 +98,7 @@ struct Prompt {
   static constexpr int QSTEPS = D / 16, DB = D / 32;
   // Keys a tile, up to one page entry a lane, in blocks of 32.  At 256 dims a wave's
   // sums and Q leave no registers, and LDS no room, for 64: Q spilled, and 16384
-  // tokens took 9.5 ms, with 32 6.4.
+  // tokens took 9.5 ms, with 32 6.5.
   static constexpr int TILE = D == 256 ? 32 : 64, KB = TILE / 32;
   static constexpr uint64_t ALL = ~0ull >> (64 - TILE);
   // Rows of LDS, without bank conflicts: eight rows of K at one column are read
@@ -110,8 +111,8 @@ struct Prompt {
 
   // Q in LDS: 256 registers a lane, two waves a SIMD, hold it barely or not, read
   // back from scratch they wait for the staged loads, which the same counter counts.
-  // 16384 tokens of 16-bit rows 2.24 ms with Q in LDS or in registers, of e4m3fn rows
-  // 2.59 and 3.02.
+  // 16384 tokens with Q in LDS and in registers: bf16 2.15 and 2.12 ms, fp16 2.27 and
+  // 2.32, bf16 over e4m3fn rows 2.49 and 2.90, fp16 over those 3.19 and 3.21.
   static constexpr bool QLDS = D == 256 || (D == 128 && NW == 8);
 
   struct alignas(16) Shared {

@@ -1272,7 +1272,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``out`` too, which may be q itself and shares no other memory.  Returns out
     (B, H, S, D) in q's dtype, or (out, lse) with ``return_lse``, lse (B, H, S)
     fp32.  A token that sees no row and the rows past q_lens give zeros and
-    -inf."""
+    -inf.  A call is split over its keys by S and max_seq_len: sequences of few
+    new tokens after long contexts are better a call of their own than beside
+    one of many."""
     if q.dim() != 4:
         raise ValueError(f"q must be (B, H, S, D), got {tuple(q.shape)}")
     B, H, S, D = q.shape
